@@ -54,6 +54,8 @@ typedef enum lcpp_dtype {
     LCPP_F64 = 5,
     LCPP_U8 = 6,    /* 1-byte (bool) selection flags of DeviceSelect /
                        DevicePartition only; every other entry point rejects it */
+    LCPP_F16 = 7,   /* half and bfloat16: logits and token rows of */
+    LCPP_BF16 = 8,  /* lcpp_b200_model.h only; every other entry point rejects them */
     LCPP_NONE = 255 /* "no values" (keys-only) */
 } lcpp_dtype;
 

@@ -26,7 +26,10 @@ typedef enum lcpp_kernel_kind {
     LCPP_KERNEL_MERGE = 5,          /* merge path (lcpp_dist_merge_sorted*) */
     LCPP_KERNEL_ARG_REDUCE = 6,     /* ArgMin / ArgMax */
     LCPP_KERNEL_BY_KEY = 7,         /* by-key scans and ReduceByKey */
-    LCPP_KERNEL_SELECT = 8          /* DeviceSelect / DevicePartition */
+    LCPP_KERNEL_SELECT = 8,         /* DeviceSelect / DevicePartition */
+    LCPP_KERNEL_BLOCK_TABLE = 9,    /* DeviceBlockTable (lcpp_b200_model.h) */
+    LCPP_KERNEL_ROUTER = 10,        /* DeviceRouter */
+    LCPP_KERNEL_DISPATCH = 11       /* DeviceDispatch */
 } lcpp_kernel_kind;
 
 typedef struct lcpp_kernel_time {

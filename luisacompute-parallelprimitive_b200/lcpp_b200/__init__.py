@@ -25,6 +25,9 @@ ERR_CUDA, ERR_LOOKBACK_TIMEOUT, ERR_COMM, ERR_INTERNAL = 4, 5, 6, 7
 # lcpp_dtype
 U32, I32, F32, U64, I64, F64, NONE = 0, 1, 2, 3, 4, 5, 255
 U8 = 6  # 1-byte (bool) selection flags only
+F16, BF16 = 7, 8  # logits and token rows of the model-step operators only
+# lcpp_router_score
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 # lcpp_op
 OP_SUM, OP_MIN, OP_MAX = 0, 1, 2
 # lcpp_testgen_dist
@@ -38,6 +41,7 @@ KERNEL_MERGE = 5
 KERNEL_ARG_REDUCE = 6
 KERNEL_BY_KEY = 7
 KERNEL_SELECT = 8
+KERNEL_BLOCK_TABLE, KERNEL_ROUTER, KERNEL_DISPATCH = 9, 10, 11
 
 _lib = None
 
@@ -52,6 +56,23 @@ class DistSortTimes(ctypes.Structure):
                 ("host_wait_ms", ctypes.c_float), ("exchange_merge_ms", ctypes.c_float),
                 ("local_merge_ms", ctypes.c_float), ("total_ms", ctypes.c_float), ("host_ms", ctypes.c_float),
                 ("peer_exchange", ctypes.c_int)]
+
+
+class BlockTableArgs(ctypes.Structure):
+    """lcpp_block_table_args (include/lcpp_b200_model.h)."""
+    _fields_ = [("context_lens", ctypes.c_void_p), ("new_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_uint64), ("table_width", ctypes.c_uint32),
+                ("num_requests", ctypes.c_uint32), ("block_size", ctypes.c_uint32), ("num_free", ctypes.c_uint32),
+                ("free_blocks", ctypes.c_void_p), ("free_used", ctypes.c_void_p), ("free_used_out", ctypes.c_void_p),
+                ("seq_lens_out", ctypes.c_void_p), ("query_starts_out", ctypes.c_void_p),
+                ("slots_out", ctypes.c_void_p), ("positions_out", ctypes.c_void_p),
+                ("token_request_out", ctypes.c_void_p), ("max_tokens", ctypes.c_uint64)]
+
+
+class RouterConfig(ctypes.Structure):
+    """lcpp_router_config (include/lcpp_b200_model.h)."""
+    _fields_ = [("num_experts", ctypes.c_uint32), ("top_k", ctypes.c_uint32), ("score", ctypes.c_int32),
+                ("renormalize", ctypes.c_int32), ("weight_scale", ctypes.c_float), ("loss_coef", ctypes.c_float)]
 
 
 class LcppError(RuntimeError):
@@ -75,6 +96,7 @@ def lib() -> ctypes.CDLL:
     szp = ctypes.POINTER(ctypes.c_size_t)
     ip = ctypes.POINTER(ctypes.c_int)
     vpa = ctypes.c_void_p * 2
+    u32, cfg = ctypes.c_uint32, ctypes.POINTER(RouterConfig)
     sigs = {
         "lcpp_status_string": ([i], ctypes.c_char_p),
         "lcpp_version": ([], i),
@@ -160,6 +182,18 @@ def lib() -> ctypes.CDLL:
         "lcpp_dist_exclusive_sum": ([vp, vp, sz, vp, vp, u64, i, vp], i),
         "lcpp_dist_reduce_temp_bytes": ([vp, i, u64, szp], i),
         "lcpp_dist_reduce": ([vp, vp, sz, vp, vp, u64, i, vp, i, vp], i),
+        "lcpp_block_table_temp_bytes": ([u64, u64, szp], i),
+        "lcpp_block_table_extend": ([vp, sz, ctypes.POINTER(BlockTableArgs), vp], i),
+        "lcpp_router_temp_bytes": ([u64, u32, szp], i),
+        "lcpp_router_forward": ([vp, sz, vp, u64, i, vp, vp, vp, vp, vp, vp, vp, u64, cfg, vp], i),
+        "lcpp_router_backward": ([vp, u64, i, vp, vp, vp, vp, vp, vp, u64, u64, cfg, vp], i),
+        "lcpp_dispatch_temp_bytes": ([u64, u32, u32, szp], i),
+        "lcpp_dispatch_max_rows": ([u64, u32, u32, u32, ctypes.POINTER(u64)], i),
+        "lcpp_dispatch_plan": ([vp, sz, vp, vp, vp, vp, u64, u32, u32, u32, u64, vp], i),
+        "lcpp_dispatch_gather": ([vp, u64, vp, vp, vp, vp, u64, u64, u32, u32, u64, u64, i, vp], i),
+        "lcpp_dispatch_combine": ([vp, u64, vp, vp, vp, u64, u64, u32, u64, u64, i, vp], i),
+        "lcpp_dispatch_combine_backward": ([vp, u64, vp, u64, vp, vp, vp, vp, vp, u64, vp, u64, u32, u32, u64, u64,
+                                            i, vp], i),
         "lcpp_diag_timing_enable": ([i], i),
         "lcpp_diag_wait_timeout_probe": ([vp, sz, u64, vp], i),
         "lcpp_diag_timing_read": ([ctypes.POINTER(KernelTime), i, ip], i),
@@ -835,3 +869,185 @@ class DevicePartition:
                                                 _ptr(d_second_out), _ptr(d_unselected_out),
                                                 _ptr(d_num_selected_out), num_items, code, a1, n1, a2, n2,
                                                 _stream(stream)), "IfThreeWay")
+
+
+# ---------------------------------------------------------------------------
+# Operators of one language-model step (include/lcpp_b200_model.h)
+# ---------------------------------------------------------------------------
+_ROW_CODES = None
+
+
+def _row_code(t) -> int:
+    """dtype code of logits or token rows."""
+    global _ROW_CODES
+    if _ROW_CODES is None:
+        torch = _torch()
+        _ROW_CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    code = _ROW_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    return code
+
+
+def _flat(t, dtype, count, name):
+    """Pointer of a contiguous tensor of `dtype` with at least `count` elements (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or not t.is_contiguous() or t.numel() < count:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: contiguous {dtype} with at least {count} elements")
+    return t.data_ptr()
+
+
+def _rows(t, rows, columns, code, name):
+    """(pointer, row stride) of a 2-D tensor of at least rows x columns with unit column stride."""
+    if _row_code(t) != code or t.dim() != 2 or t.shape[0] < rows or t.shape[1] < columns or \
+            (t.stride(1) != 1 and t.shape[1] > 1 and t.shape[0]):
+        raise LcppError(ERR_INVALID_ARG, f"{name}: rows of one dtype, at least {rows} x {columns}, columns adjacent")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), columns))
+
+
+class DeviceBlockTable:
+    """Block tables and slot maps of a paged cache, from request lengths."""
+
+    @staticmethod
+    def GetTempStorageBytes(num_requests: int, max_tokens: int) -> int:
+        out = ctypes.c_size_t()
+        check(lib().lcpp_block_table_temp_bytes(num_requests, max_tokens, ctypes.byref(out)), "GetTempStorageBytes")
+        return out.value
+
+    def Extend(self, temp, d_context_lens, d_new_lens, d_block_table, d_free_blocks, d_free_used, d_free_used_out,
+               d_seq_lens_out, d_query_starts_out, d_slots_out, d_positions_out, d_token_request_out, num_requests,
+               block_size, stream=None):
+        """Gives the step's tokens their pages and slots (lcpp_block_table_extend).
+
+        d_block_table [num_requests, width] is extended in place; d_new_lens None
+        adds one token to each request; d_free_used, d_positions_out and
+        d_token_request_out may be None.  All tensors int32, d_slots_out int64;
+        its length is the number of tokens laid out, padding included."""
+        torch = _torch()
+        i32, n, tokens = torch.int32, num_requests, d_slots_out.numel()
+        if d_block_table.dtype != i32 or d_block_table.dim() != 2 or d_block_table.shape[0] < n or \
+                (d_block_table.stride(1) != 1 and d_block_table.shape[1] > 1 and n):
+            raise LcppError(ERR_INVALID_ARG, "d_block_table: int32 [num_requests, width], columns adjacent")
+        width = d_block_table.shape[1]
+        args = BlockTableArgs(
+            _flat(d_context_lens, i32, n, "d_context_lens"), _flat(d_new_lens, i32, n, "d_new_lens"),
+            d_block_table.data_ptr(), max(d_block_table.stride(0), width), width, n, block_size,
+            d_free_blocks.numel(), _flat(d_free_blocks, i32, 0, "d_free_blocks"),
+            _flat(d_free_used, i32, 1, "d_free_used"), _flat(d_free_used_out, i32, 1, "d_free_used_out"),
+            _flat(d_seq_lens_out, i32, n, "d_seq_lens_out"),
+            _flat(d_query_starts_out, i32, n + 1, "d_query_starts_out"),
+            _flat(d_slots_out, torch.int64, tokens, "d_slots_out"),
+            _flat(d_positions_out, i32, tokens, "d_positions_out"),
+            _flat(d_token_request_out, i32, tokens, "d_token_request_out"), tokens)
+        check(lib().lcpp_block_table_extend(_ptr(temp), _tb(temp), args, _stream(stream)), "Extend")
+
+
+class DeviceRouter:
+    """Experts of each token, their weights, per-expert counts and the balance loss, with the gradient."""
+
+    @staticmethod
+    def GetTempStorageBytes(num_tokens: int, num_experts: int) -> int:
+        out = ctypes.c_size_t()
+        check(lib().lcpp_router_temp_bytes(num_tokens, num_experts, ctypes.byref(out)), "GetTempStorageBytes")
+        return out.value
+
+    def Forward(self, temp, d_logits, d_weights_out, d_experts_out, d_counts_out, d_num_routed_out, d_loss_out,
+                num_tokens, num_experts, top_k, score=SCORE_SOFTMAX, renormalize=True, weight_scale=1.0,
+                loss_coef=1.0, d_bias=None, d_token_request=None, stream=None):
+        """lcpp_router_forward: d_logits [num_tokens, num_experts] float32, float16 or bfloat16;
+        weights float32 and experts int32 [num_tokens, top_k], counts int32 [num_experts]."""
+        torch = _torch()
+        i32, f32, pairs, code = torch.int32, torch.float32, num_tokens * top_k, _row_code(d_logits)
+        logits, stride = _rows(d_logits, num_tokens, num_experts, code, "d_logits")
+        check(lib().lcpp_router_forward(
+            _ptr(temp), _tb(temp), logits, stride, code, _flat(d_bias, f32, num_experts, "d_bias"),
+            _flat(d_token_request, i32, num_tokens, "d_token_request"),
+            _flat(d_weights_out, f32, pairs, "d_weights_out"), _flat(d_experts_out, i32, pairs, "d_experts_out"),
+            _flat(d_counts_out, i32, num_experts, "d_counts_out"),
+            _flat(d_num_routed_out, i32, 1, "d_num_routed_out"), _flat(d_loss_out, f32, 1, "d_loss_out"), num_tokens,
+            RouterConfig(num_experts, top_k, score, int(renormalize), weight_scale, loss_coef), _stream(stream)),
+            "Forward")
+
+    def Backward(self, d_logits, d_experts, d_counts, d_num_routed, d_grad_weights, d_grad_loss, d_grad_logits_out,
+                 num_tokens, num_experts, top_k, score=SCORE_SOFTMAX, renormalize=True, weight_scale=1.0,
+                 loss_coef=1.0, stream=None):
+        """lcpp_router_backward: experts, counts and num_routed as Forward wrote them;
+        d_grad_weights and d_grad_loss may be None."""
+        torch = _torch()
+        i32, f32, pairs, code = torch.int32, torch.float32, num_tokens * top_k, _row_code(d_logits)
+        logits, stride = _rows(d_logits, num_tokens, num_experts, code, "d_logits")
+        grad, grad_stride = _rows(d_grad_logits_out, num_tokens, num_experts, code, "d_grad_logits_out")
+        check(lib().lcpp_router_backward(
+            logits, stride, code, _flat(d_experts, i32, pairs, "d_experts"),
+            _flat(d_counts, i32, num_experts, "d_counts"), _flat(d_num_routed, i32, 1, "d_num_routed"),
+            _flat(d_grad_weights, f32, pairs, "d_grad_weights"), _flat(d_grad_loss, f32, 1, "d_grad_loss"), grad,
+            grad_stride, num_tokens,
+            RouterConfig(num_experts, top_k, score, int(renormalize), weight_scale, loss_coef), _stream(stream)),
+            "Backward")
+
+
+class DeviceDispatch:
+    """Token rows grouped by expert and summed back, with the gradients."""
+
+    @staticmethod
+    def GetTempStorageBytes(num_tokens: int, top_k: int, num_experts: int) -> int:
+        out = ctypes.c_size_t()
+        check(lib().lcpp_dispatch_temp_bytes(num_tokens, top_k, num_experts, ctypes.byref(out)),
+              "GetTempStorageBytes")
+        return out.value
+
+    @staticmethod
+    def MaxRows(num_tokens: int, top_k: int, num_experts: int, row_align: int = 1) -> int:
+        """Rows that hold any choice when segments start at multiples of row_align."""
+        out = ctypes.c_uint64()
+        check(lib().lcpp_dispatch_max_rows(num_tokens, top_k, num_experts, row_align, ctypes.byref(out)), "MaxRows")
+        return out.value
+
+    def Plan(self, temp, d_experts, d_expert_starts_out, d_row_of_out, d_pair_of_out, num_tokens, top_k, num_experts,
+             row_align=1, stream=None):
+        """Groups the pairs by expert (lcpp_dispatch_plan); d_pair_of_out's length is max_rows.  All int32."""
+        i32, pairs = _torch().int32, num_tokens * top_k
+        check(lib().lcpp_dispatch_plan(
+            _ptr(temp), _tb(temp), _flat(d_experts, i32, pairs, "d_experts"),
+            _flat(d_expert_starts_out, i32, num_experts + 1, "d_expert_starts_out"),
+            _flat(d_row_of_out, i32, pairs, "d_row_of_out"), _flat(d_pair_of_out, i32, 0, "d_pair_of_out"),
+            num_tokens, top_k, num_experts, row_align, d_pair_of_out.numel(), _stream(stream)), "Plan")
+
+    def Gather(self, d_x, d_row_of, d_pair_of, d_expert_starts, d_rows_out, num_tokens, top_k, num_experts,
+               stream=None):
+        """Token rows to their experts' rows (lcpp_dispatch_gather); d_rows_out has a row per entry of d_pair_of."""
+        i32, code, hidden, rows = _torch().int32, _row_code(d_x), d_x.shape[1], d_pair_of.numel()
+        x, x_stride = _rows(d_x, num_tokens, hidden, code, "d_x")
+        out, out_stride = _rows(d_rows_out, rows, hidden, code, "d_rows_out")
+        check(lib().lcpp_dispatch_gather(
+            x, x_stride, _flat(d_row_of, i32, num_tokens * top_k, "d_row_of"), _flat(d_pair_of, i32, 0, "d_pair_of"),
+            _flat(d_expert_starts, i32, num_experts + 1, "d_expert_starts"), out, out_stride, num_tokens, top_k,
+            num_experts, rows, hidden, code, _stream(stream)), "Gather")
+
+    def Combine(self, d_rows, d_row_of, d_weights, d_out, num_tokens, top_k, stream=None):
+        """Sums of the tokens' rows, weighted unless d_weights is None (lcpp_dispatch_combine)."""
+        torch = _torch()
+        code, hidden, pairs = _row_code(d_rows), d_out.shape[1], num_tokens * top_k
+        rows, rows_stride = _rows(d_rows, 0, hidden, code, "d_rows")
+        out, out_stride = _rows(d_out, num_tokens, hidden, code, "d_out")
+        check(lib().lcpp_dispatch_combine(
+            rows, rows_stride, _flat(d_row_of, torch.int32, pairs, "d_row_of"),
+            _flat(d_weights, torch.float32, pairs, "d_weights"), out, out_stride, num_tokens, top_k,
+            d_rows.shape[0], hidden, code, _stream(stream)), "Combine")
+
+    def CombineBackward(self, d_grad_out, d_rows, d_row_of, d_pair_of, d_expert_starts, d_weights, d_grad_rows_out,
+                        d_grad_weights_out, num_tokens, top_k, num_experts, stream=None):
+        """Gradients of Combine with weights (lcpp_dispatch_combine_backward)."""
+        torch = _torch()
+        i32, f32, pairs, max_rows = torch.int32, torch.float32, num_tokens * top_k, d_pair_of.numel()
+        code, hidden = _row_code(d_grad_out), d_grad_out.shape[1]
+        grad, grad_stride = _rows(d_grad_out, num_tokens, hidden, code, "d_grad_out")
+        rows, rows_stride = _rows(d_rows, max_rows, hidden, code, "d_rows")
+        out, out_stride = _rows(d_grad_rows_out, max_rows, hidden, code, "d_grad_rows_out")
+        check(lib().lcpp_dispatch_combine_backward(
+            grad, grad_stride, rows, rows_stride, _flat(d_row_of, i32, pairs, "d_row_of"),
+            _flat(d_pair_of, i32, 0, "d_pair_of"), _flat(d_expert_starts, i32, num_experts + 1, "d_expert_starts"),
+            _flat(d_weights, f32, pairs, "d_weights"), out, out_stride,
+            _flat(d_grad_weights_out, f32, pairs, "d_grad_weights_out"), num_tokens, top_k, num_experts, max_rows,
+            hidden, code, _stream(stream)), "CombineBackward")
