@@ -27,7 +27,7 @@ extern "C" {
  * ------------------------------------------------------------------------ */
 
 /* Largest num_requests of lcpp_block_table_extend. */
-#define LCPP_MAX_REQUESTS (1u << 24)
+#define LCPP_MAX_REQUESTS (1u << 20)
 
 typedef struct lcpp_block_table_args {
     const int32_t* context_lens;  /* [num_requests] tokens already in the cache (below 0: 0) */
@@ -46,7 +46,7 @@ typedef struct lcpp_block_table_args {
     int64_t* slots_out;           /* [max_tokens] page id * block_size + offset in the page */
     int32_t* positions_out;       /* [max_tokens] position in the request's sequence, or NULL */
     int32_t* token_request_out;   /* [max_tokens] request of the token, or NULL */
-    uint64_t max_tokens;          /* entries of the three arrays above, below 2^31 */
+    uint64_t max_tokens;          /* entries of the three arrays above, below 2^31 - 1 */
 } lcpp_block_table_args;
 
 lcpp_status lcpp_block_table_temp_bytes(uint64_t num_requests, uint64_t max_tokens, size_t* temp_bytes);

@@ -12,8 +12,8 @@
 // Up to kFusedRequests requests one launch does all: every block sums the
 // lengths itself (they come from L2; 8 bytes per request) and then lays out
 // its own range of tokens from the sums in shared memory.  Beyond that, the
-// sums take two small launches (tile totals, then each tile's scan on top of
-// the totals before it) and the third lays out the tokens.
+// sums take two small launches (totals of 512 requests, then each 512's scan on
+// top of the totals before it) and the third lays out the tokens.
 #include "model.cuh"
 
 using namespace lcpp;
@@ -23,10 +23,10 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / kWarp;
-constexpr int kItems = 8;                      // requests per thread of one scan tile
-constexpr int kTile = kThreads * kItems;       // requests of one scan tile
-constexpr uint32_t kFusedRequests = kTile;
-constexpr uint32_t kMaxStart = 0x7fffffffu;    // starts saturate here, past any token
+constexpr int kItems = 8;                      // requests per thread of the fused kernel, at most
+constexpr uint32_t kFusedRequests = kThreads * kItems;
+constexpr uint32_t kWindow = 1024;             // requests of a block's tokens held in shared memory
+constexpr uint32_t kMost = 0x7fffffffu;        // sums saturate here, past every token and page
 
 struct Params {
     const int32_t* context;
@@ -48,7 +48,8 @@ struct Params {
     uint32_t tokens;        // entries of slots
     uint32_t div_mul;       // p / block_size == (p * div_mul) >> div_shift for p < 2^31
     uint32_t div_shift;
-    uint32_t tokens_per_warp;
+    uint32_t tokens_per_block;
+    uint32_t wide;          // token arrays start on 16-byte boundaries
     uint32_t* ctrl;
 };
 
@@ -81,39 +82,41 @@ __device__ __forceinline__ Request request_at(const Params& p, uint32_t r)
     return q;
 }
 
-// Inclusive sums of two counts over the block, per thread.
+// Tokens and pages, added up to at most kMost: what saturates is past every
+// array, and saturating sums may be taken in any order.
 struct Sums {
-    uint64_t tokens, pages;
+    uint32_t tokens, pages;
 };
 
-__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {a.tokens + b.tokens, a.pages + b.pages}; }
-
-__device__ __forceinline__ Sums shfl_up(Sums v, int d)
+__device__ __forceinline__ Sums operator+(Sums a, Sums b)
 {
-    return {__shfl_up_sync(~0u, v.tokens, d), __shfl_up_sync(~0u, v.pages, d)};
+    return {min(a.tokens + b.tokens, kMost), min(a.pages + b.pages, kMost)};
 }
 
-// Exclusive sum of `mine` over the block's threads; `total` over all of them.
-__device__ Sums block_exclusive(Sums mine, Sums* warp_sums, Sums& total)
+// Sum of the values of the lanes before this one, and of all lanes.
+__device__ __forceinline__ Sums warp_exclusive(Sums v, Sums& total)
 {
-    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-    Sums inc = mine;
+    const int lane = threadIdx.x % kWarp;
+    Sums inc = v;
 #pragma unroll
     for (int d = 1; d < kWarp; d *= 2) {
-        const Sums o = shfl_up(inc, d);
+        const Sums o{__shfl_up_sync(~0u, inc.tokens, d), __shfl_up_sync(~0u, inc.pages, d)};
         if (lane >= d) inc = inc + o;
     }
-    if (lane == kWarp - 1) warp_sums[warp] = inc;
+    total = {__shfl_sync(~0u, inc.tokens, kWarp - 1), __shfl_sync(~0u, inc.pages, kWarp - 1)};
+    const Sums before{__shfl_up_sync(~0u, inc.tokens, 1), __shfl_up_sync(~0u, inc.pages, 1)};
+    return lane ? before : Sums{0, 0};
+}
+
+// Sum of the warps' values before this warp, and of all warps.
+__device__ __forceinline__ Sums warps_exclusive(Sums of_warp, Sums* shared, Sums& total)
+{
+    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+    if (lane == 0) shared[warp] = of_warp;
     __syncthreads();
-    Sums before{0, 0};
-    total = {0, 0};
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w == warp) before = total;
-        total = total + warp_sums[w];
-    }
+    const Sums before = warp_exclusive(lane < kWarps ? shared[lane] : Sums{0, 0}, total);
     __syncthreads();
-    return {before.tokens + inc.tokens - mine.tokens, before.pages + inc.pages - mine.pages};
+    return {__shfl_sync(~0u, before.tokens, warp), __shfl_sync(~0u, before.pages, warp)};
 }
 
 __device__ __forceinline__ uint32_t used_before(const Params& p) { return p.free_used ? uint32_t(max(*p.free_used, 0)) : 0u; }
@@ -127,155 +130,186 @@ struct Plan {
     uint32_t* free_base;
 };
 
-// Scans one tile of requests on top of `before` into the plan (indexed from
-// the tile's first request) and, where `write`, the outputs.  Returns the pages
-// in use after the thread's last request that was served with new ones.
+// Scans the block's ITEMS * kThreads requests from `first` on, on top of
+// `before`, into the plan (indexed from `first`).  Each warp has ITEMS * 32 of
+// them in a row and takes 32 at a time, so that all accesses are coalesced.
+// Returns the pages in use after the last request that this thread saw served
+// with new ones; `total` includes `before`.
 template <int ITEMS>
-__device__ uint64_t scan_tile(const Params& p, uint32_t first, Sums before, Plan plan, bool write, Sums* warp_sums,
-                              Sums& total)
+__device__ uint32_t scan_tile(const Params& p, uint32_t first, Sums before, Plan plan, Sums* shared, Sums& total)
 {
+    const uint32_t lane = threadIdx.x % kWarp, slot0 = threadIdx.x / kWarp * kWarp * ITEMS + lane;
     Request q[ITEMS];
-    Sums mine{0, 0};
-    const uint32_t r0 = first + threadIdx.x * ITEMS;
+    Sums at[ITEMS], of_warp{0, 0};
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) q[i] = request_at(p, first + slot0 + i * kWarp);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        q[i] = request_at(p, r0 + i);
-        mine = mine + Sums{q[i].fresh, q[i].need};
+        Sums of_row;
+        at[i] = of_warp + warp_exclusive(Sums{q[i].fresh, q[i].need}, of_row);
+        of_warp = of_warp + of_row;
     }
-    Sums at = before + block_exclusive(mine, warp_sums, total);
-    const uint64_t used = used_before(p);
-    uint64_t used_after = 0;
+    const Sums base = before + warps_exclusive(of_warp, shared, total);
+    total = before + total;
+    const uint32_t used = used_before(p);
+    uint32_t used_after = 0;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const uint32_t r = r0 + i;
-        if (r < p.requests) {
-            const Sums end = at + Sums{q[i].fresh, q[i].need};
+        const uint32_t slot = slot0 + i * kWarp;
+        if (first + slot < p.requests) {
+            const Sums start = base + at[i], end = start + Sums{q[i].fresh, q[i].need};
             const bool fits = q[i].in_row && end.tokens <= p.tokens &&
-                              (q[i].need == 0 || used + end.pages <= p.num_free);
-            const uint32_t start = uint32_t(min(at.tokens, uint64_t(kMaxStart)));
-            const uint32_t slot = r - first;
-            plan.start[slot] = start;
+                              (q[i].need == 0 || (used <= p.num_free && end.pages <= p.num_free - used));
+            plan.start[slot] = start.tokens;
             plan.context[slot] = fits ? int32_t(q[i].context) : -1;
-            plan.free_base[slot] = uint32_t(used + at.pages) - q[i].held;
-            if (write) {
-                p.starts[r] = int32_t(start);
-                if (r == p.requests - 1) p.starts[r + 1] = int32_t(min(end.tokens, uint64_t(kMaxStart)));
-                p.seq_lens[r] = int32_t(fits ? q[i].context + q[i].fresh : q[i].context);
-                if (fits && q[i].need) used_after = used + end.pages;
-            }
-            at = end;
+            plan.free_base[slot] = used + start.pages - q[i].held;
+            if (fits && q[i].need) used_after = used + end.pages;
         }
     }
     return used_after;
 }
 
-// Last request of [lo, hi] that starts at or before token t; start[lo] <= t.
-__device__ __forceinline__ uint32_t find(const uint32_t* start, uint32_t lo, uint32_t hi, uint32_t t)
+// The outputs by request: i of the plan is request `first` + i.
+__device__ __forceinline__ void write_request(const Params& p, const Plan& plan, uint32_t first, uint32_t i)
 {
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1) / 2;
-        if (start[mid] <= t) lo = mid;
-        else hi = mid - 1;
+    const uint32_t r = first + i;
+    p.starts[r] = int32_t(plan.start[i]);
+    const Request q = request_at(p, r);
+    p.seq_lens[r] = int32_t(plan.context[i] < 0 ? q.context : q.context + q.fresh);
+}
+
+// Number of the first `n` starts at or below t, found by all threads of the
+// block together: each round narrows the range kThreads-fold.
+__device__ uint32_t block_count_starts(const uint32_t* start, uint32_t n, uint32_t t)
+{
+    uint32_t lo = 0;  // starts known to be at or below t
+    while (n > 0) {
+        const uint32_t step = (n + kThreads - 1) / kThreads;
+        const uint32_t at = threadIdx.x * step + step - 1;  // last of the thread's stretch
+        const uint32_t whole = uint32_t(__syncthreads_count(at < n && start[lo + at] <= t));
+        lo += whole * step;
+        if (step == 1) break;
+        n = min(step - 1, n - whole * step);
     }
     return lo;
 }
 
-// Lays out tokens [first, last) of the warp.  `plan` is indexed from request
-// `base`; `end` is the step's token count.  Tokens go 32 at a time; where one
-// request covers all 32 (prompts) nothing is searched, else each lane searches
-// between the group's first request and the warp's last.
-__device__ void lay_out(const Params& p, const Plan& plan, uint32_t base, uint32_t lo, uint32_t hi, uint32_t first,
+// Last request of the plan's first `window` that starts at or before token t
+// (the first one does).
+__device__ __forceinline__ uint32_t request_of(const Plan& plan, uint32_t window, uint32_t t)
+{
+    uint32_t r = 0;
+    for (uint32_t half = 1u << (31 - __clz(max(window, 2u) - 1)); half > 0; half /= 2) {
+        const uint32_t at = r + half;
+        if (at < window && plan.start[at] <= t) r = at;
+    }
+    return r;
+}
+
+// The G tokens from t on of request r, all of them served or none.  They lie in
+// one page or two: G is 1 or at most the page size.
+template <int G>
+__device__ __forceinline__ void lay_out_run(const Params& p, const Plan& plan, uint32_t base, uint32_t r, bool in_step,
+                                            uint32_t t)
+{
+    const int32_t context = in_step ? plan.context[r] : -1;
+    const bool served = context >= 0;
+    uint32_t position = 0;
+    int64_t slot[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) slot[i] = -1;
+    if (served) {
+        position = uint32_t(context) + (t - plan.start[r]);
+        const uint32_t page = divide(p, position), offset = position - page * p.block_size;
+        const bool two = G > 1 && offset + G > p.block_size;
+        // pages the row did not hold come from the free list
+        const bool fresh0 = page * p.block_size >= uint32_t(context);
+        const bool fresh1 = two && (page + 1) * p.block_size >= uint32_t(context);
+        int32_t* row = p.table + uint64_t(base + r) * p.table_stride + page;
+        const uint32_t at0 = plan.free_base[r] + page, at1 = at0 + 1;  // modulo 2^32, before they index
+        const int32_t id0 = fresh0 ? p.free_blocks[at0] : row[0];
+        const int32_t id1 = two ? (fresh1 ? p.free_blocks[at1] : row[1]) : -1;
+        if (fresh0 && offset == 0) row[0] = id0;
+        if (fresh1) row[1] = id1;
+        const int64_t slot0 = int64_t(id0) * p.block_size + offset;
+        const int64_t slot1 = (int64_t(id1) - 1) * p.block_size + offset;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            const bool second = G > 1 && offset + i >= p.block_size;
+            if ((second ? id1 : id0) >= 0) slot[i] = (second ? slot1 : slot0) + i;
+        }
+    }
+    const int32_t request = served ? int32_t(base + r) : -1;
+    if (G == 4 && p.wide) {
+        longlong2* s = reinterpret_cast<longlong2*>(p.slots + t);
+        s[0] = make_longlong2(slot[0], slot[1 % G]);
+        s[1] = make_longlong2(slot[2 % G], slot[3 % G]);
+        const int32_t q = int32_t(position);
+        if (p.positions)
+            *reinterpret_cast<int4*>(p.positions + t) = served ? make_int4(q, q + 1, q + 2, q + 3) : make_int4(0, 0, 0, 0);
+        if (p.token_request) *reinterpret_cast<int4*>(p.token_request + t) = make_int4(request, request, request, request);
+    } else {
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            p.slots[t + i] = slot[i];
+            if (p.positions) p.positions[t + i] = served ? int32_t(position + i) : 0;
+            if (p.token_request) p.token_request[t + i] = request;
+        }
+    }
+}
+
+// Lays out tokens [first, last) of the block, whose requests are among
+// [0, window) of the plan, the first of them numbered `base`; `end` is the
+// step's token count.  A thread takes G tokens at a time: where one request has
+// them all they cost one search, one division and, mostly, one page.
+template <int G>
+__device__ void lay_out(const Params& p, const Plan& plan, uint32_t base, uint32_t window, uint32_t first,
                         uint32_t last, uint32_t end)
 {
-    const uint32_t lane = threadIdx.x % kWarp;
-    const uint32_t inside = min(last, end);
-    uint32_t r = lo;
-    if (first < inside) {
-        r = find(plan.start, lo, hi, first);
-        hi = find(plan.start, r, hi, inside - 1);
-    }
-    for (uint32_t t0 = first; t0 < last; t0 += kWarp) {
-        const uint32_t t = t0 + lane;
-        if (t0 < inside) {
-            const uint32_t t_last = min(t0 + kWarp, inside) - 1;
-            uint32_t mine = r;
-            if (r < hi && plan.start[r + 1] <= t_last) mine = find(plan.start, r, hi, min(t, t_last));
-            r = __shfl_sync(~0u, mine, kWarp - 1);
-            if (t >= last) continue;
-            const int32_t context = plan.context[mine];
-            if (t < inside && context >= 0) {
-                const uint32_t position = uint32_t(context) + (t - plan.start[mine]);
-                const uint32_t page = divide(p, position);
-                const uint32_t offset = position - page * p.block_size;
-                const uint64_t row = uint64_t(base + mine) * p.table_stride;
-                int32_t id;
-                if (page * p.block_size >= uint32_t(context)) {  // a page the row did not hold
-                    id = p.free_blocks[plan.free_base[mine] + page];
-                    if (offset == 0) p.table[row + page] = id;
-                } else {
-                    id = p.table[row + page];
-                }
-                p.slots[t] = id < 0 ? -1 : int64_t(id) * p.block_size + offset;
-                if (p.positions) p.positions[t] = int32_t(position);
-                if (p.token_request) p.token_request[t] = int32_t(base + mine);
-                continue;
-            }
-        }
-        if (t < last) {
-            p.slots[t] = -1;
-            if (p.positions) p.positions[t] = 0;
-            if (p.token_request) p.token_request[t] = -1;
+    for (uint32_t t = first + threadIdx.x * G; t < last; t += kThreads * G) {
+        const uint32_t r = request_of(plan, window, t);
+        const uint32_t next = r + 1 < window ? min(plan.start[r + 1], end) : end;
+        if (G == 1 || (t + G <= last && (t + G <= next || t >= end))) {
+            lay_out_run<G>(p, plan, base, r, t < end, t);
+        } else {
+            for (uint32_t i = t; i < min(t + G, last); ++i)
+                lay_out_run<1>(p, plan, base, i == t ? r : request_of(plan, window, i), i < end, i);
         }
     }
 }
 
-__device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* shared)
-{
-    if (threadIdx.x == 0) *shared = 0;
-    __syncthreads();
-    if (v) atomicMax(reinterpret_cast<unsigned long long*>(shared), static_cast<unsigned long long>(v));
-    __syncthreads();
-    return *shared;
-}
-
-template <int ITEMS>
+template <int ITEMS, int G>
 __global__ void __launch_bounds__(kThreads) fused_kernel(const Params p)
 {
-    __shared__ Sums warp_sums[kWarps];
-    __shared__ uint64_t top;
+    __shared__ Sums shared[kWarps];
+    __shared__ uint32_t used_after;
     extern __shared__ uint32_t dynamic[];
     const uint32_t n = p.requests;
     const Plan plan{dynamic, reinterpret_cast<int32_t*>(dynamic) + n, dynamic + 2 * n};
+    if (threadIdx.x == 0) used_after = used_before(p);
     Sums total;
-    const bool writer = blockIdx.x == 0;
-    const uint64_t used_after = scan_tile<ITEMS>(p, 0, Sums{0, 0}, plan, writer, warp_sums, total);
-    if (writer) {
-        const uint64_t most = block_max(used_after, &top);
-        if (threadIdx.x == 0) {
-            *p.free_used_out = int32_t(max(most, uint64_t(used_before(p))));
-            p.ctrl[0] = p.ctrl[1] = 0;
-        }
-    }
+    const uint32_t used = scan_tile<ITEMS>(p, 0, Sums{0, 0}, plan, shared, total);
+    if (used) atomicMax(&used_after, used);
     __syncthreads();
-    const uint32_t warp = blockIdx.x * kWarps + threadIdx.x / kWarp;
-    const uint64_t first = uint64_t(warp) * p.tokens_per_warp;
-    if (first >= p.tokens) return;
-    lay_out(p, plan, 0, 0, n - 1, uint32_t(first), uint32_t(min(first + p.tokens_per_warp, uint64_t(p.tokens))),
-            uint32_t(min(total.tokens, uint64_t(kMaxStart))));
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *p.free_used_out = int32_t(used_after);
+        p.starts[n] = int32_t(total.tokens);
+        p.ctrl[0] = p.ctrl[1] = 0;
+    }
+    for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < n; i += gridDim.x * kThreads)
+        write_request(p, plan, 0, i);
+    const uint32_t first = min(blockIdx.x * p.tokens_per_block, p.tokens);
+    lay_out<G>(p, plan, 0, n, first, min(first + p.tokens_per_block, p.tokens), total.tokens);
 }
 
 // The three launches for many requests.
 __global__ void __launch_bounds__(kThreads) totals_kernel(const Params p, Sums* tile_sums)
 {
-    __shared__ Sums warp_sums[kWarps];
-    Sums mine{0, 0}, total;
-    // the tile's sums only: lane-consecutive requests, so that loads coalesce
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-        const Request q = request_at(p, blockIdx.x * kTile + i * kThreads + threadIdx.x);
-        mine = mine + Sums{q.fresh, q.need};
-    }
-    block_exclusive(mine, warp_sums, total);
+    __shared__ Sums shared[kWarps];
+    const Request q = request_at(p, blockIdx.x * kThreads + threadIdx.x);
+    Sums of_warp, total;
+    warp_exclusive(Sums{q.fresh, q.need}, of_warp);
+    warps_exclusive(of_warp, shared, total);
     if (threadIdx.x == 0) {
         tile_sums[blockIdx.x] = total;
         if (blockIdx.x == 0) {
@@ -285,27 +319,49 @@ __global__ void __launch_bounds__(kThreads) totals_kernel(const Params p, Sums* 
     }
 }
 
-__global__ void __launch_bounds__(kThreads) starts_kernel(const Params p, const Sums* tile_sums, Plan plan)
+__global__ void __launch_bounds__(kThreads) starts_kernel(const Params p, const Sums* tile_sums, const Plan all)
 {
-    __shared__ Sums warp_sums[kWarps];
-    __shared__ uint64_t top;
-    Sums before{0, 0}, mine{0, 0}, total;
+    __shared__ Sums shared[kWarps];
+    __shared__ uint32_t used_after;
+    if (threadIdx.x == 0) used_after = 0;
+    Sums mine{0, 0}, of_warp, before, total;
     for (uint32_t i = threadIdx.x; i < blockIdx.x; i += kThreads) mine = mine + tile_sums[i];
-    block_exclusive(mine, warp_sums, before);
-    const uint32_t first = blockIdx.x * kTile;
-    const Plan here{plan.start + first, plan.context + first, plan.free_base + first};
-    const uint64_t used_after = scan_tile<kItems>(p, first, before, here, true, warp_sums, total);
-    const uint64_t most = block_max(used_after, &top);
-    if (threadIdx.x == 0 && most) atomicMax(p.free_used_out, int32_t(most));
+    warp_exclusive(mine, of_warp);
+    warps_exclusive(of_warp, shared, before);
+    const uint32_t first = blockIdx.x * kThreads;
+    const Plan plan{all.start + first, all.context + first, all.free_base + first};
+    const uint32_t used = scan_tile<1>(p, first, before, plan, shared, total);
+    if (used) atomicMax(&used_after, used);
+    if (first + threadIdx.x < p.requests) write_request(p, plan, first, threadIdx.x);  // what this thread planned
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        if (used_after) atomicMax(p.free_used_out, int32_t(used_after));
+        if (blockIdx.x == gridDim.x - 1) p.starts[p.requests] = int32_t(total.tokens);
+    }
 }
 
-__global__ void __launch_bounds__(kThreads) tokens_kernel(const Params p, const Plan plan)
+// The requests of the block's tokens come into shared memory where they fit
+// (a window has at least one token per request that is not empty).
+template <int G>
+__global__ void __launch_bounds__(kThreads) tokens_kernel(const Params p, const Plan all)
 {
-    const uint32_t warp = blockIdx.x * kWarps + threadIdx.x / kWarp;
-    const uint64_t first = uint64_t(warp) * p.tokens_per_warp;
-    if (first >= p.tokens) return;
-    lay_out(p, plan, 0, 0, p.requests - 1, uint32_t(first),
-            uint32_t(min(first + p.tokens_per_warp, uint64_t(p.tokens))), uint32_t(p.starts[p.requests]));
+    __shared__ uint32_t start[kWindow], free_base[kWindow];
+    __shared__ int32_t context[kWindow];
+    const uint32_t first = blockIdx.x * p.tokens_per_block, last = min(first + p.tokens_per_block, p.tokens);
+    const uint32_t end = uint32_t(p.starts[p.requests]);
+    const uint32_t lo = block_count_starts(all.start, p.requests, first) - 1;  // the first starts at 0
+    const uint32_t window = block_count_starts(all.start + lo, p.requests - lo, last - 1);
+    Plan plan{all.start + lo, all.context + lo, all.free_base + lo};
+    if (window <= kWindow) {
+        for (uint32_t i = threadIdx.x; i < window; i += kThreads) {
+            start[i] = plan.start[i];
+            context[i] = plan.context[i];
+            free_base[i] = plan.free_base[i];
+        }
+        plan = Plan{start, context, free_base};
+        __syncthreads();
+    }
+    lay_out<G>(p, plan, lo, window, first, last, end);
 }
 
 // No requests: one start and marked entries.
@@ -338,7 +394,7 @@ Layout layout(uint64_t requests)
         l.bytes += align_up(bytes, kTempAlign);
         return at;
     };
-    l.sums = take(ceil_div(requests, kTile) * sizeof(Sums));
+    l.sums = take(ceil_div(requests, kThreads) * sizeof(Sums));
     l.start = take(requests * 4);
     l.context = take(requests * 4);
     l.free_base = take(requests * 4);
@@ -347,7 +403,7 @@ Layout layout(uint64_t requests)
 
 lcpp_status run(void* temp, size_t temp_bytes, const lcpp_block_table_args* a, cudaStream_t s)
 {
-    if (!a || !a->block_size || a->max_tokens >> 31 || a->num_requests > LCPP_MAX_REQUESTS ||
+    if (!a || !a->block_size || a->max_tokens >= kMost || a->num_requests > LCPP_MAX_REQUESTS ||
         a->table_stride < a->table_width)
         return LCPP_ERR_INVALID_ARG;
     const uint64_t n = a->num_requests;
@@ -379,8 +435,7 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_block_table_args* a, c
     p.width = a->table_width;
     p.requests = a->num_requests;
     p.block_size = a->block_size;
-    // num_free past 2^31 - 1 cannot be counted in free_used; the rest is not used
-    p.num_free = std::min(a->num_free, 0x7fffffffu);
+    p.num_free = std::min(a->num_free, kMost - 1);  // free_used counts no further
     p.free_blocks = a->free_blocks;
     p.free_used = a->free_used;
     p.free_used_out = a->free_used_out;
@@ -404,15 +459,23 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_block_table_args* a, c
         empty_kernel<<<unsigned(std::max<uint64_t>(1, ceil_div(p.tokens, kThreads))), kThreads, 0, s>>>(p);
         return launched();
     }
-    // tokens in equal contiguous runs over the warps of at most three blocks per SM
-    const uint64_t most_warps = uint64_t(device_sm_count()) * 3 * kWarps;
-    p.tokens_per_warp = uint32_t(align_up(ceil_div(std::max(p.tokens, 1u), most_warps), kWarp));
-    const unsigned grid = unsigned(std::max<uint64_t>(1, ceil_div(ceil_div(p.tokens, p.tokens_per_warp), kWarps)));
+    // four tokens to a thread where every SM has work for a block of such threads
+    // and four tokens lie in two pages at most
+    const bool many = p.tokens >= uint64_t(device_sm_count()) * kThreads * 4 && p.block_size >= 4;
+    p.wide = !(misaligned(p.slots, 16) || misaligned(p.positions, 16) || misaligned(p.token_request, 16));
+    // tokens in equal contiguous runs over the resident blocks
+    const auto grid_of = [&](const void* kernel, size_t smem) {
+        const uint64_t most = uint64_t(device_sm_count()) * resident_blocks(kernel, kThreads, smem);
+        p.tokens_per_block = uint32_t(align_up(std::max<uint64_t>(ceil_div(p.tokens, most), 1), kThreads * (many ? 4 : 1)));
+        return unsigned(std::max<uint64_t>(1, ceil_div(p.tokens, p.tokens_per_block)));
+    };
     if (n <= kFusedRequests) {
         const size_t smem = n * 12;
-        auto kernel = n <= kThreads ? fused_kernel<1> : n <= 2 * kThreads ? fused_kernel<2> : fused_kernel<kItems>;
+        auto kernel = many ? (n <= kThreads ? fused_kernel<1, 4> : n <= 2 * kThreads ? fused_kernel<2, 4> : fused_kernel<kItems, 4>)
+                           : (n <= kThreads ? fused_kernel<1, 1> : n <= 2 * kThreads ? fused_kernel<2, 1> : fused_kernel<kItems, 1>);
         if (n > 2 * kThreads)  // up to 48 KB beside the static arrays
             set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), size_t(kFusedRequests) * 12);
+        const unsigned grid = grid_of(reinterpret_cast<const void*>(kernel), smem);
         kernel<<<grid, kThreads, smem, s>>>(p);
         return launched();
     }
@@ -420,10 +483,14 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_block_table_args* a, c
     const Plan plan{reinterpret_cast<uint32_t*>(t + l.start), reinterpret_cast<int32_t*>(t + l.context),
                     reinterpret_cast<uint32_t*>(t + l.free_base)};
     Sums* sums = reinterpret_cast<Sums*>(t + l.sums);
-    const unsigned tiles = unsigned(ceil_div(n, kTile));
+    const unsigned tiles = unsigned(ceil_div(n, kThreads));
     totals_kernel<<<tiles, kThreads, 0, s>>>(p, sums);
     starts_kernel<<<tiles, kThreads, 0, s>>>(p, sums, plan);
-    tokens_kernel<<<grid, kThreads, 0, s>>>(p, plan);
+    if (p.tokens) {
+        auto kernel = many ? tokens_kernel<4> : tokens_kernel<1>;
+        const unsigned grid = grid_of(reinterpret_cast<const void*>(kernel), 0);
+        kernel<<<grid, kThreads, 0, s>>>(p, plan);
+    }
     return launched();
 }
 
@@ -433,7 +500,7 @@ extern "C" {
 
 lcpp_status lcpp_block_table_temp_bytes(uint64_t num_requests, uint64_t max_tokens, size_t* temp_bytes)
 {
-    if (!temp_bytes || num_requests > LCPP_MAX_REQUESTS || max_tokens >> 31) return LCPP_ERR_INVALID_ARG;
+    if (!temp_bytes || num_requests > LCPP_MAX_REQUESTS || max_tokens >= kMost) return LCPP_ERR_INVALID_ARG;
     *temp_bytes = layout(num_requests).bytes;
     return LCPP_OK;
 }

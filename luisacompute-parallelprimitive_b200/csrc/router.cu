@@ -9,6 +9,13 @@ namespace {
 
 size_t temp_size(uint32_t experts) { return align_up(router::cleared_bytes(experts), kTempAlign); }
 
+// Bytes of the widest copy that every row's start and length are a multiple of.
+uint32_t copy_unit(const void* logits, uint64_t stride, uint32_t experts, int size)
+{
+    const uint64_t bits = reinterpret_cast<uintptr_t>(logits) | stride * size | uint64_t(experts) * size | 16;
+    return uint32_t(bits & (~bits + 1));
+}
+
 lcpp_status check_config(const lcpp_router_config* c, uint64_t tokens, uint64_t stride)
 {
     if (!c || !c->num_experts || c->num_experts > LCPP_MAX_EXPERTS || !c->top_k || c->top_k > c->num_experts ||
@@ -55,7 +62,7 @@ lcpp_status forward(void* temp, size_t temp_bytes, const void* logits, uint64_t 
     p.renormalize = c->renormalize != 0;
     p.weight_scale = c->weight_scale;
     p.loss_coef = c->loss_coef;
-    p.aligned = rows_16b(logits, stride, size);
+    p.unit = copy_unit(logits, stride, c->num_experts, size);
     p.ctrl = reinterpret_cast<uint32_t*>(t);
     p.share_total = reinterpret_cast<unsigned long long*>(t + router::kShareOffset);
     p.count_total = reinterpret_cast<uint32_t*>(p.share_total + c->num_experts);
@@ -106,7 +113,8 @@ lcpp_status backward(const void* logits, uint64_t stride, lcpp_dtype dtype, cons
     p.renormalize = c->renormalize != 0;
     p.weight_scale = c->weight_scale;
     p.loss_coef = c->loss_coef;
-    p.aligned = uint32_t(rows_16b(logits, stride, size)) | uint32_t(rows_16b(grad_logits, grad_stride, size)) << 1;
+    p.unit = copy_unit(logits, stride, c->num_experts, size);
+    p.wide_stores = rows_16b(grad_logits, grad_stride, size);
     const bool sigmoid = c->score == LCPP_SCORE_SIGMOID;
     diag::KernelTimer timer(kTimerRouter, tokens * c->num_experts, s);
     switch (dtype) {

@@ -900,10 +900,39 @@ def _flat(t, dtype, count, name):
 
 def _rows(t, rows, columns, code, name):
     """(pointer, row stride) of a 2-D tensor of at least rows x columns with unit column stride."""
-    if _row_code(t) != code or t.dim() != 2 or t.shape[0] < rows or t.shape[1] < columns or \
-            (t.stride(1) != 1 and t.shape[1] > 1 and t.shape[0]):
-        raise LcppError(ERR_INVALID_ARG, f"{name}: rows of one dtype, at least {rows} x {columns}, columns adjacent")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), columns))
+    shape = t.shape
+    if _row_code(t) != code or len(shape) != 2 or shape[0] < rows or shape[1] < columns:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: rows of one dtype, at least {rows} x {columns}")
+    stride = t.stride()
+    if stride[1] != 1 and shape[1] > 1 and shape[0]:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a row's columns have to be adjacent")
+    return t.data_ptr(), (stride[0] if shape[0] > 1 else max(stride[0], columns))
+
+
+def _queue(stream):
+    """Handle of the stream to enqueue on: the one given, else torch's current one."""
+    if stream is not None:
+        return stream.cuda_stream
+    cuda = _torch().cuda
+    return cuda.current_stream(cuda.current_device()).cuda_stream
+
+
+def _scratch(temp):
+    """(pointer, bytes) of temp storage."""
+    return (None, 0) if temp is None else (temp.data_ptr(), temp.numel() * temp.element_size())
+
+
+_router_configs = {}
+
+
+def _router_config(*fields):
+    """The lcpp_router_config of these settings; a program uses few, so they are kept."""
+    config = _router_configs.get(fields)
+    if config is None:
+        if len(_router_configs) >= 256:
+            _router_configs.clear()
+        config = _router_configs[fields] = RouterConfig(*fields)
+    return config
 
 
 class DeviceBlockTable:
@@ -940,7 +969,7 @@ class DeviceBlockTable:
             _flat(d_slots_out, torch.int64, tokens, "d_slots_out"),
             _flat(d_positions_out, i32, tokens, "d_positions_out"),
             _flat(d_token_request_out, i32, tokens, "d_token_request_out"), tokens)
-        check(lib().lcpp_block_table_extend(_ptr(temp), _tb(temp), args, _stream(stream)), "Extend")
+        check(lib().lcpp_block_table_extend(*_scratch(temp), args, _queue(stream)), "Extend")
 
 
 class DeviceRouter:
@@ -961,12 +990,12 @@ class DeviceRouter:
         i32, f32, pairs, code = torch.int32, torch.float32, num_tokens * top_k, _row_code(d_logits)
         logits, stride = _rows(d_logits, num_tokens, num_experts, code, "d_logits")
         check(lib().lcpp_router_forward(
-            _ptr(temp), _tb(temp), logits, stride, code, _flat(d_bias, f32, num_experts, "d_bias"),
+            *_scratch(temp), logits, stride, code, _flat(d_bias, f32, num_experts, "d_bias"),
             _flat(d_token_request, i32, num_tokens, "d_token_request"),
             _flat(d_weights_out, f32, pairs, "d_weights_out"), _flat(d_experts_out, i32, pairs, "d_experts_out"),
             _flat(d_counts_out, i32, num_experts, "d_counts_out"),
             _flat(d_num_routed_out, i32, 1, "d_num_routed_out"), _flat(d_loss_out, f32, 1, "d_loss_out"), num_tokens,
-            RouterConfig(num_experts, top_k, score, int(renormalize), weight_scale, loss_coef), _stream(stream)),
+            _router_config(num_experts, top_k, score, int(renormalize), weight_scale, loss_coef), _queue(stream)),
             "Forward")
 
     def Backward(self, d_logits, d_experts, d_counts, d_num_routed, d_grad_weights, d_grad_loss, d_grad_logits_out,
@@ -983,7 +1012,7 @@ class DeviceRouter:
             _flat(d_counts, i32, num_experts, "d_counts"), _flat(d_num_routed, i32, 1, "d_num_routed"),
             _flat(d_grad_weights, f32, pairs, "d_grad_weights"), _flat(d_grad_loss, f32, 1, "d_grad_loss"), grad,
             grad_stride, num_tokens,
-            RouterConfig(num_experts, top_k, score, int(renormalize), weight_scale, loss_coef), _stream(stream)),
+            _router_config(num_experts, top_k, score, int(renormalize), weight_scale, loss_coef), _queue(stream)),
             "Backward")
 
 
@@ -1009,10 +1038,10 @@ class DeviceDispatch:
         """Groups the pairs by expert (lcpp_dispatch_plan); d_pair_of_out's length is max_rows.  All int32."""
         i32, pairs = _torch().int32, num_tokens * top_k
         check(lib().lcpp_dispatch_plan(
-            _ptr(temp), _tb(temp), _flat(d_experts, i32, pairs, "d_experts"),
+            *_scratch(temp), _flat(d_experts, i32, pairs, "d_experts"),
             _flat(d_expert_starts_out, i32, num_experts + 1, "d_expert_starts_out"),
             _flat(d_row_of_out, i32, pairs, "d_row_of_out"), _flat(d_pair_of_out, i32, 0, "d_pair_of_out"),
-            num_tokens, top_k, num_experts, row_align, d_pair_of_out.numel(), _stream(stream)), "Plan")
+            num_tokens, top_k, num_experts, row_align, d_pair_of_out.numel(), _queue(stream)), "Plan")
 
     def Gather(self, d_x, d_row_of, d_pair_of, d_expert_starts, d_rows_out, num_tokens, top_k, num_experts,
                stream=None):
@@ -1023,7 +1052,7 @@ class DeviceDispatch:
         check(lib().lcpp_dispatch_gather(
             x, x_stride, _flat(d_row_of, i32, num_tokens * top_k, "d_row_of"), _flat(d_pair_of, i32, 0, "d_pair_of"),
             _flat(d_expert_starts, i32, num_experts + 1, "d_expert_starts"), out, out_stride, num_tokens, top_k,
-            num_experts, rows, hidden, code, _stream(stream)), "Gather")
+            num_experts, rows, hidden, code, _queue(stream)), "Gather")
 
     def Combine(self, d_rows, d_row_of, d_weights, d_out, num_tokens, top_k, stream=None):
         """Sums of the tokens' rows, weighted unless d_weights is None (lcpp_dispatch_combine)."""
@@ -1034,7 +1063,7 @@ class DeviceDispatch:
         check(lib().lcpp_dispatch_combine(
             rows, rows_stride, _flat(d_row_of, torch.int32, pairs, "d_row_of"),
             _flat(d_weights, torch.float32, pairs, "d_weights"), out, out_stride, num_tokens, top_k,
-            d_rows.shape[0], hidden, code, _stream(stream)), "Combine")
+            d_rows.shape[0], hidden, code, _queue(stream)), "Combine")
 
     def CombineBackward(self, d_grad_out, d_rows, d_row_of, d_pair_of, d_expert_starts, d_weights, d_grad_rows_out,
                         d_grad_weights_out, num_tokens, top_k, num_experts, stream=None):
@@ -1050,4 +1079,4 @@ class DeviceDispatch:
             _flat(d_pair_of, i32, 0, "d_pair_of"), _flat(d_expert_starts, i32, num_experts + 1, "d_expert_starts"),
             _flat(d_weights, f32, pairs, "d_weights"), out, out_stride,
             _flat(d_grad_weights_out, f32, pairs, "d_grad_weights_out"), num_tokens, top_k, num_experts, max_rows,
-            hidden, code, _stream(stream)), "CombineBackward")
+            hidden, code, _queue(stream)), "CombineBackward")

@@ -24,7 +24,7 @@ def table_args(lcpp, **changes):
 
 
 @pytest.mark.parametrize("change", [
-    {"block_size": 0}, {"max_tokens": 1 << 31}, {"num_requests": (1 << 24) + 1}, {"table_stride": 7},
+    {"block_size": 0}, {"max_tokens": (1 << 31) - 1}, {"num_requests": (1 << 20) + 1}, {"table_stride": 7},
     {"context_lens": None}, {"block_table": None}, {"free_blocks": None}, {"free_used_out": None},
     {"seq_lens_out": None}, {"query_starts_out": None}, {"slots_out": None},
     {"slots_out": 0x9000004}, {"positions_out": 0xA000002}, {"new_lens": 0x2000001},
@@ -45,7 +45,7 @@ def test_block_table_refuses_temp(lcpp):
     need = lcpp.DeviceBlockTable.GetTempStorageBytes(5000, 32)
     many = table_args(lcpp, num_requests=5000)
     assert lib.lcpp_block_table_extend(p(0), need - 1, many, None) == lcpp.ERR_TEMP_TOO_SMALL
-    for n, tokens in (((1 << 24) + 1, 1), (1, 1 << 31)):
+    for n, tokens in (((1 << 20) + 1, 1), (1, (1 << 31) - 1)):
         with pytest.raises(lcpp.LcppError):
             lcpp.DeviceBlockTable.GetTempStorageBytes(n, tokens)
 

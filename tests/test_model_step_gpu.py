@@ -99,6 +99,32 @@ def test_extend_one_token_each(lcpp, n):
     check_extend(lcpp, context, None, table, 8, free, None, n, 16, optional=False)
 
 
+@pytest.mark.parametrize("n", [3, 700, 4000, 5000])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_extend_many_tokens(lcpp, n, offset):
+    """Enough tokens for four to a thread, in arrays that start on a vector boundary or off it: long prompts,
+    single tokens and idle requests side by side."""
+    rng = np.random.default_rng(n)
+    context, new = rng.integers(0, 50, n).astype(np.int32), np.ones(n, np.int32)
+    new[rng.random(n) < 0.2] = 0
+    long = rng.choice(n, 3, replace=False)
+    new[long] = rng.integers(100_000, 130_000, 3)
+    block, width = 24, 5500
+    table = rng.permutation(n * 3).astype(np.int32).reshape(n, 3)
+    table = np.concatenate([table, np.full((n, width - 3), -1, np.int32)], 1)
+    free = (n * 3 + rng.permutation(20_000)).astype(np.int32)
+    tokens = int(new.sum()) + 13
+    expect = ref.extend(context, new, table, width, free, 0, tokens, block)
+    slots = torch.full((tokens + offset,), -9, dtype=torch.int64, device="cuda")[offset:]
+    positions, requests = i32(tokens + offset)[offset:], i32(tokens + offset)[offset:]
+    d_table, starts, seq, used = cuda(table), i32(n + 1), i32(n), i32(1)
+    temp = lcpp.alloc_temp(lcpp.DeviceBlockTable.GetTempStorageBytes(n, tokens))
+    lcpp.DeviceBlockTable().Extend(temp, cuda(context), cuda(new), d_table, cuda(free), None, used, seq, starts, slots,
+                                   positions, requests, n, block)
+    for got, want in zip((d_table, slots, positions, requests, starts, seq, used), expect):
+        np.testing.assert_array_equal(host(got), want)
+
+
 @pytest.mark.parametrize("n,seed", [(40, 0), (40, 1), (700, 2), (6000, 3)])
 def test_extend_refuses(lcpp, n, seed):
     """Free pages that end early, rows that are too narrow, arrays that are too short: what does not fit
