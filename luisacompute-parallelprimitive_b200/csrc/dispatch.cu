@@ -6,10 +6,10 @@
 // counts the experts of its own run of pairs in shared memory; sums of the
 // counts over the warps before it, the blocks before it and the experts
 // before it give each (warp, expert) its first row, and a second walk over the
-// run ranks each 32 pairs with match.any.  Up to kSmallPairs pairs one block
-// does all; beyond that one block per SM counts its tile in a first launch,
-// and in a second one every block adds up all tiles' counts itself (a few
-// hundred KB from L2) before it ranks its tile.
+// run ranks each 32 pairs by ballots.  Up to kSmallPairs pairs one block
+// does all; beyond that up to one block per SM counts its tile in a first
+// launch, and in a second one every block adds up all tiles' counts itself (a
+// few hundred KB from L2) before it ranks its tile.
 //
 // The row kernels work by token: x (or its gradient) is read once and goes to,
 // or comes from, the token's rows, so nothing but those rows is read or
@@ -23,9 +23,10 @@ using namespace lcpp::model;
 namespace {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanWarps = kPlanThreads / kWarp;
-constexpr uint64_t kSmallPairs = 16384;  // one block ranks these
-constexpr uint64_t kTilePairs = 4096;    // fewest pairs worth a block of their own
+constexpr int kFewThreads = 256;
+constexpr uint64_t kFewPairs = 1024;    // these, of at most kFewThreads experts, take a block of kFewThreads
+constexpr uint64_t kSmallPairs = 2048;  // these take one block
+constexpr uint64_t kTilePairs = 1024;   // fewest pairs of a block among several
 
 struct PlanParams {
     const int32_t* experts;
@@ -39,12 +40,15 @@ struct PlanParams {
     uint32_t tile;      // pairs of a block
     uint32_t per_warp;  // pairs of a warp, a multiple of 32
     uint32_t* ctrl;
-    uint32_t* table;    // [tiles][num_experts]
+    uint32_t* table;    // [tiles][table_pitch]
+    uint32_t table_pitch;  // num_experts, rounded up to 4
 };
 
 // Exclusive sum over the block of one value per thread.
+template <int THREADS>
 __device__ uint32_t block_exclusive(uint32_t v, uint32_t* warp_sums)
 {
+    constexpr int kWarps = THREADS / kWarp;
     const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
     uint32_t inc = v;
 #pragma unroll
@@ -55,13 +59,13 @@ __device__ uint32_t block_exclusive(uint32_t v, uint32_t* warp_sums)
     if (lane == kWarp - 1) warp_sums[warp] = inc;
     __syncthreads();
     if (warp == 0) {
-        uint32_t w = warp_sums[lane];
+        uint32_t w = lane < kWarps ? warp_sums[lane] : 0;
 #pragma unroll
-        for (int d = 1; d < kWarp; d *= 2) {
+        for (int d = 1; d < kWarps; d *= 2) {
             const uint32_t o = __shfl_up_sync(~0u, w, d);
             if (lane >= d) w += o;
         }
-        warp_sums[lane] = w;
+        if (lane < kWarps) warp_sums[lane] = w;
     }
     __syncthreads();
     const uint32_t before = warp ? warp_sums[warp - 1] : 0;
@@ -80,59 +84,68 @@ __global__ void __launch_bounds__(kPlanThreads) count_kernel(const PlanParams p)
         if (e < p.num_experts) atomicAdd(count + e, 1u);
     }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < p.num_experts; e += kPlanThreads)
-        p.table[uint64_t(blockIdx.x) * p.num_experts + e] = count[e];
+    for (uint32_t e = threadIdx.x; e < p.table_pitch; e += kPlanThreads)
+        p.table[blockIdx.x * p.table_pitch + e] = e < p.num_experts ? count[e] : 0;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p)
 {
+    constexpr int kWarps = THREADS / kWarp;
     const uint32_t n = p.num_experts;
     extern __shared__ uint32_t dynamic[];
-    uint32_t* counter = dynamic;                  // [kPlanWarps][n], then each (warp, expert)'s next row
-    uint32_t* earlier = counter + kPlanWarps * n; // [n] pairs of earlier tiles
+    uint32_t* counter = dynamic;                  // [kWarps][n], then each (warp, expert)'s next row
+    uint32_t* earlier = counter + kWarps * n; // [n] pairs of earlier tiles
     uint32_t* total = earlier + n;                // [n] pairs of all tiles
-    __shared__ uint32_t warp_sums[kPlanWarps];
+    __shared__ uint32_t warp_sums[kWarps];
     const uint32_t lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
     const uint32_t tile_first = blockIdx.x * p.tile, tile_last = min(tile_first + p.tile, p.pairs);
     const uint32_t first = min(tile_first + warp * p.per_warp, tile_last), last = min(first + p.per_warp, tile_last);
     uint32_t* mine = counter + warp * n;
 
-    for (uint32_t i = threadIdx.x; i < (kPlanWarps + 2) * n; i += kPlanThreads) counter[i] = 0;
+    for (uint32_t i = threadIdx.x; i < (kWarps + 2) * n; i += THREADS) counter[i] = 0;
     __syncthreads();
     for (uint32_t i = first + lane; i < last; i += kWarp) {
         const uint32_t e = uint32_t(p.experts[i]);
         if (e < n) atomicAdd(mine + e, 1u);
     }
     if (gridDim.x > 1) {
-        // threads in groups of one per expert, each group a share of the tiles
-        const uint32_t groups = max(1u, kPlanThreads / n), group = threadIdx.x / n;
+        // Threads in groups of one per four experts, each group a share of the
+        // tiles (at most kMaxTiles): a thread's loads are all in flight at once.
+        const uint32_t quads = p.table_pitch / 4, groups = THREADS / quads, group = threadIdx.x / quads;
+        const uint32_t quad = threadIdx.x - group * quads;
         if (group < groups) {
-            for (uint32_t e = threadIdx.x - group * n; e < n; e += kPlanThreads) {
-                uint32_t before = 0, all = 0;
+            uint4 before{0, 0, 0, 0}, all{0, 0, 0, 0};
 #pragma unroll 8
-                for (uint32_t b = group; b < gridDim.x; b += groups) {
-                    const uint32_t c = p.table[uint64_t(b) * n + e];
-                    all += c;
-                    before += b < blockIdx.x ? c : 0;
-                }
-                if (all) atomicAdd(total + e, all);
-                if (before) atomicAdd(earlier + e, before);
+            for (uint32_t b = group; b < gridDim.x; b += groups) {
+                const uint4 c = reinterpret_cast<const uint4*>(p.table + b * p.table_pitch)[quad];
+                const bool is = b < blockIdx.x;
+                all = uint4{all.x + c.x, all.y + c.y, all.z + c.z, all.w + c.w};
+                before = uint4{before.x + (is ? c.x : 0), before.y + (is ? c.y : 0), before.z + (is ? c.z : 0),
+                               before.w + (is ? c.w : 0)};
+            }
+            const uint32_t alls[4] = {all.x, all.y, all.z, all.w}, befores[4] = {before.x, before.y, before.z, before.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t e = quad * 4 + i;
+                if (e < n && alls[i]) atomicAdd(total + e, alls[i]);
+                if (e < n && befores[i]) atomicAdd(earlier + e, befores[i]);
             }
         }
     }
     __syncthreads();
-    // one thread per expert (n <= kPlanThreads): its segment, then its row for every warp
+    // one thread per expert (n <= THREADS): its segment, then its row for every warp
     uint32_t count = 0, segment = 0;
     if (threadIdx.x < n) {
         uint32_t in_block = 0;
-        for (int w = 0; w < kPlanWarps; ++w) in_block += counter[w * n + threadIdx.x];
+        for (int w = 0; w < kWarps; ++w) in_block += counter[w * n + threadIdx.x];
         count = gridDim.x > 1 ? total[threadIdx.x] : in_block;
         segment = (count + p.align - 1) / p.align * p.align;
     }
-    const uint32_t start = block_exclusive(segment, warp_sums);
+    const uint32_t start = block_exclusive<THREADS>(segment, warp_sums);
     if (threadIdx.x < n) {
         uint32_t row = start + earlier[threadIdx.x];
-        for (int w = 0; w < kPlanWarps; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
             const uint32_t c = counter[w * n + threadIdx.x];
             counter[w * n + threadIdx.x] = row;
             row += c;
@@ -151,7 +164,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p)
         const uint32_t i = i0 + lane;
         const uint32_t e = i < last ? uint32_t(p.experts[i]) : ~0u;
         const bool valid = e < n;
-        const uint32_t peers = __match_any_sync(~0u, valid ? e : ~0u);
+        // lanes with the same expert, by its bits
+        uint32_t peers = __ballot_sync(~0u, valid);
+        for (uint32_t b = 1; b < n; b *= 2) {
+            const uint32_t ones = __ballot_sync(~0u, e & b);
+            peers &= e & b ? ones : ~ones;
+        }
         const uint32_t rank = __popc(peers & lanemask_lt());
         uint32_t row = ~0u;
         if (valid) row = mine[e] + rank;
@@ -164,10 +182,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p)
         }
     }
     // rows without a pair
-    for (uint32_t e = blockIdx.x * kPlanWarps + warp; e < n; e += gridDim.x * kPlanWarps)
+    for (uint32_t e = blockIdx.x * kWarps + warp; e < n; e += gridDim.x * kWarps)
         for (uint32_t r = earlier[e] + lane; r < min(total[e], p.max_rows); r += kWarp) p.pair_of[r] = -1;
-    for (uint64_t r = uint64_t(total[n - 1]) + blockIdx.x * kPlanThreads + threadIdx.x; r < p.max_rows;
-         r += uint64_t(gridDim.x) * kPlanThreads)
+    for (uint64_t r = uint64_t(total[n - 1]) + blockIdx.x * THREADS + threadIdx.x; r < p.max_rows;
+         r += uint64_t(gridDim.x) * THREADS)
         p.pair_of[r] = -1;
 }
 
@@ -176,8 +194,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p)
 // of two) share a token.
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
-constexpr int kPadRows = 64;   // rows a block looks through for padding
-constexpr int kUnroll = 8;     // expert rows in flight per thread
+constexpr int kPadRows = 64;   // most rows a block looks through for padding
 
 template <int UB>
 struct Unit;
@@ -205,17 +222,19 @@ struct RowParams {
     uint32_t units;
     uint32_t lanes_log2;
     uint32_t pad_blocks;
+    uint32_t pad_rows;           // rows of a padding block
     uint32_t chunks;             // column chunks of a token
+    uint32_t rows_per_pass;      // expert rows of a token taken together
 };
 
-// Zeros in the padding rows among this block's kPadRows rows.
+// Zeros in the padding rows among this block's pad_rows rows.
 template <int UB>
 __device__ void clear_padding(const RowParams& p, uint32_t block)
 {
     using U = typename Unit<UB>::type;
     __shared__ uint32_t masks[kPadRows / kWarp];
-    const uint32_t first = block * kPadRows;
-    const uint32_t end = min(uint32_t(p.starts[p.num_experts]), p.max_rows);
+    const uint32_t first = block * p.pad_rows;
+    const uint32_t end = min(min(uint32_t(p.starts[p.num_experts]), p.max_rows), first + p.pad_rows);
     if (threadIdx.x < kPadRows) {
         const uint32_t r = first + threadIdx.x;
         const uint32_t m = __ballot_sync(~0u, r < end && p.pair_of[r] < 0);
@@ -230,26 +249,25 @@ __device__ void clear_padding(const RowParams& p, uint32_t block)
     }
 }
 
-// Tokens' rows copied to their experts' rows.  Blocks: first the padding's.
-template <int UB>
+// Tokens' rows copied to their experts' rows, N accesses per thread.  Blocks:
+// first the padding's.
+template <int UB, int N>
 __global__ void __launch_bounds__(kRowThreads) gather_kernel(const RowParams p)
 {
     using U = typename Unit<UB>::type;
-    constexpr int kUnits = 2;
     if (blockIdx.x < p.pad_blocks) {
         clear_padding<UB>(p, blockIdx.x);
         return;
     }
     const uint32_t block = blockIdx.x - p.pad_blocks;
     const uint32_t lanes = 1u << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const uint32_t chunk = block % p.chunks;
     const uint32_t t = (block / p.chunks) * (kRowThreads >> p.lanes_log2) + (threadIdx.x >> p.lanes_log2);
     if (t >= p.tokens) return;
     const U* x = reinterpret_cast<const U*>(p.x + uint64_t(t) * p.x_pitch);
-    const uint32_t u0 = chunk * lanes * kUnits + lane;
-    U v[kUnits];
+    const uint32_t u0 = (block % p.chunks) * lanes * N + lane;
+    U v[N];
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i)
+    for (int i = 0; i < N; ++i)
         if (u0 + i * lanes < p.units) v[i] = x[u0 + i * lanes];
     const int32_t* row_of = p.row_of + uint64_t(t) * p.top_k;
 #pragma unroll 4
@@ -258,7 +276,7 @@ __global__ void __launch_bounds__(kRowThreads) gather_kernel(const RowParams p)
         if (r >= p.max_rows) continue;
         U* row = reinterpret_cast<U*>(p.out + uint64_t(r) * p.out_pitch);
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i)
+        for (int i = 0; i < N; ++i)
             if (u0 + i * lanes < p.units) row[u0 + i * lanes] = v[i];
     }
 }
@@ -281,55 +299,67 @@ __device__ __forceinline__ typename Unit<UB>::type pack(const float (&in)[UB / s
     return raw;
 }
 
-// out[t] = sum_j w[t][j] rows[row_of[t][j]], kUnroll rows in flight per thread.
-template <typename T, int UB>
-__global__ void __launch_bounds__(kRowThreads) combine_kernel(const RowParams p)
+// out[t] = sum_j w[t][j] rows[row_of[t][j]]: N accesses per thread of R rows at
+// a time, all in flight before the first is used.
+template <typename T, int UB, int R, int N>
+__global__ void __launch_bounds__(kRowThreads, 4) combine_kernel(const RowParams p)
 {
     using U = typename Unit<UB>::type;
     constexpr int kN = UB / int(sizeof(T));
     const uint32_t lanes = 1u << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const uint32_t chunk = blockIdx.x % p.chunks;
     const uint32_t t = (blockIdx.x / p.chunks) * (kRowThreads >> p.lanes_log2) + (threadIdx.x >> p.lanes_log2);
-    const uint32_t u = chunk * lanes + lane;
-    if (t >= p.tokens || u >= p.units) return;
+    const uint32_t u0 = (blockIdx.x % p.chunks) * lanes * N + lane;
+    if (t >= p.tokens || u0 >= p.units) return;
     const int32_t* row_of = p.row_of + uint64_t(t) * p.top_k;
     const float* weights = p.weights ? p.weights + uint64_t(t) * p.top_k : nullptr;
-    float acc[kN];
+    float acc[N][kN];
 #pragma unroll
-    for (int i = 0; i < kN; ++i) acc[i] = 0.f;
-    for (uint32_t j0 = 0; j0 < p.top_k; j0 += kUnroll) {
-        U raw[kUnroll];
-        float w[kUnroll];
-        bool has[kUnroll];
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) {
-            const uint32_t r = j0 + j < p.top_k ? uint32_t(row_of[j0 + j]) : ~0u;
+        for (int e = 0; e < kN; ++e) acc[i][e] = 0.f;
+    for (uint32_t j0 = 0; j0 < p.top_k; j0 += p.rows_per_pass) {
+        const uint32_t j1 = min(j0 + p.rows_per_pass, p.top_k);
+        U raw[R][N];
+        float w[R];
+        bool has[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const uint32_t r = j0 + j < j1 ? uint32_t(row_of[j0 + j]) : ~0u;
             has[j] = r < p.max_rows;
             w[j] = has[j] && weights ? weights[j0 + j] : 1.f;
-            if (has[j]) raw[j] = reinterpret_cast<const U*>(p.rows + uint64_t(r) * p.rows_pitch)[u];
+            const U* row = reinterpret_cast<const U*>(p.rows + uint64_t(has[j] ? r : 0) * p.rows_pitch);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (has[j] && u0 + i * lanes < p.units) raw[j][i] = row[u0 + i * lanes];
         }
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) {
+        for (int j = 0; j < R; ++j) {
             if (!has[j]) continue;
-            float v[kN];
-            unpack<T, UB>(raw[j], v);
 #pragma unroll
-            for (int i = 0; i < kN; ++i) acc[i] = fmaf(w[j], v[i], acc[i]);
+            for (int i = 0; i < N; ++i) {
+                float v[kN];
+                unpack<T, UB>(raw[j][i], v);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) acc[i][e] = fmaf(w[j], v[e], acc[i][e]);
+            }
         }
     }
-    reinterpret_cast<U*>(p.out + uint64_t(t) * p.out_pitch)[u] = pack<T, UB>(acc);
+    U* out = reinterpret_cast<U*>(p.out + uint64_t(t) * p.out_pitch);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (u0 + i * lanes < p.units) out[u0 + i * lanes] = pack<T, UB>(acc[i]);
 }
 
 // out[row] = w dy and grad_w = <rows[row], dy>, a token's lanes walking its
-// columns once per kUnroll experts; the dot products are summed over a warp
-// by shuffles and over a token's warps in order.
-template <typename T, int UB>
-__global__ void __launch_bounds__(kRowThreads) combine_backward_kernel(const RowParams p)
+// columns once per pass of up to R experts; the dot products are summed over a
+// warp by shuffles and over a token's warps in order.
+template <typename T, int UB, int R, int N>
+__global__ void __launch_bounds__(kRowThreads, 3) combine_backward_kernel(const RowParams p)
 {
     using U = typename Unit<UB>::type;
     constexpr int kN = UB / int(sizeof(T));
     constexpr int kRowWarps = kRowThreads / kWarp;
-    __shared__ float part[kRowWarps][kUnroll];
+    __shared__ float part[kRowWarps][R];
     if (blockIdx.x < p.pad_blocks) {
         clear_padding<UB>(p, blockIdx.x);
         return;
@@ -341,49 +371,61 @@ __global__ void __launch_bounds__(kRowThreads) combine_backward_kernel(const Row
     const U* dy = reinterpret_cast<const U*>(p.x + uint64_t(inside ? t : 0) * p.x_pitch);
     const int32_t* row_of = p.row_of + uint64_t(t) * p.top_k;
     const float* weights = p.weights + uint64_t(t) * p.top_k;
-    for (uint32_t j0 = 0; j0 < p.top_k; j0 += kUnroll) {
-        uint32_t row[kUnroll];
-        float w[kUnroll], dot[kUnroll];
+    for (uint32_t j0 = 0; j0 < p.top_k; j0 += p.rows_per_pass) {
+        const uint32_t j1 = min(j0 + p.rows_per_pass, p.top_k);
+        uint32_t row[R];
+        float w[R], dot[R];
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) {
-            const bool is = inside && j0 + j < p.top_k;
+        for (int j = 0; j < R; ++j) {
+            const bool is = inside && j0 + j < j1;
             row[j] = is ? uint32_t(row_of[j0 + j]) : ~0u;
             w[j] = is ? weights[j0 + j] : 0.f;
             dot[j] = 0.f;
         }
-        for (uint32_t u = lane; u < p.units; u += lanes) {
-            float g[kN];
-            unpack<T, UB>(dy[u], g);
-            U raw[kUnroll];
+        for (uint32_t u0 = lane; u0 < p.units; u0 += lanes * N) {
+            U own[N], raw[R][N];
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j)
-                if (row[j] < p.max_rows)
-                    raw[j] = reinterpret_cast<const U*>(p.rows + uint64_t(row[j]) * p.rows_pitch)[u];
+            for (int i = 0; i < N; ++i)
+                if (u0 + i * lanes < p.units) own[i] = dy[u0 + i * lanes];
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j) {
+            for (int j = 0; j < R; ++j) {
                 if (row[j] >= p.max_rows) continue;
-                float v[kN];
-                unpack<T, UB>(raw[j], v);
+                const U* from = reinterpret_cast<const U*>(p.rows + uint64_t(row[j]) * p.rows_pitch);
 #pragma unroll
-                for (int i = 0; i < kN; ++i) {
-                    dot[j] = fmaf(v[i], g[i], dot[j]);
-                    v[i] = w[j] * g[i];
+                for (int i = 0; i < N; ++i)
+                    if (u0 + i * lanes < p.units) raw[j][i] = from[u0 + i * lanes];
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (u0 + i * lanes >= p.units) continue;
+                float g[kN];
+                unpack<T, UB>(own[i], g);
+#pragma unroll
+                for (int j = 0; j < R; ++j) {
+                    if (row[j] >= p.max_rows) continue;
+                    float v[kN];
+                    unpack<T, UB>(raw[j][i], v);
+#pragma unroll
+                    for (int e = 0; e < kN; ++e) {
+                        dot[j] = fmaf(v[e], g[e], dot[j]);
+                        v[e] = w[j] * g[e];
+                    }
+                    reinterpret_cast<U*>(p.out + uint64_t(row[j]) * p.out_pitch)[u0 + i * lanes] = pack<T, UB>(v);
                 }
-                reinterpret_cast<U*>(p.out + uint64_t(row[j]) * p.out_pitch)[u] = pack<T, UB>(v);
             }
         }
         const uint32_t in_warp = min(lanes, uint32_t(kWarp));
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j)
+        for (int j = 0; j < R; ++j)
             for (uint32_t d = in_warp / 2; d > 0; d /= 2) dot[j] += __shfl_xor_sync(~0u, dot[j], d);
         if (lanes > kWarp) {
             const uint32_t warp = threadIdx.x / kWarp, token_warps = lanes / kWarp;
             if (threadIdx.x % kWarp == 0) {
 #pragma unroll
-                for (int j = 0; j < kUnroll; ++j) part[warp][j] = dot[j];
+                for (int j = 0; j < R; ++j) part[warp][j] = dot[j];
             }
             __syncthreads();
-            if (inside && lane < kUnroll && j0 + lane < p.top_k) {
+            if (inside && lane < R && j0 + lane < j1) {
                 float sum = 0.f;
                 for (uint32_t i = 0; i < token_warps; ++i) sum += part[warp + i][lane];
                 p.grad_weights[uint64_t(t) * p.top_k + j0 + lane] = sum;
@@ -391,8 +433,8 @@ __global__ void __launch_bounds__(kRowThreads) combine_backward_kernel(const Row
             __syncthreads();
         } else if (inside && lane == 0) {
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j)
-                if (j0 + j < p.top_k) p.grad_weights[uint64_t(t) * p.top_k + j0 + j] = dot[j];
+            for (int j = 0; j < R; ++j)
+                if (j0 + j < j1) p.grad_weights[uint64_t(t) * p.top_k + j0 + j] = dot[j];
         }
     }
 }
@@ -413,7 +455,7 @@ constexpr uint64_t kMaxTiles = 256;
 size_t plan_bytes(uint64_t pairs, uint32_t experts)
 {
     if (pairs <= kSmallPairs) return kTempAlign;
-    return kTempAlign + align_up(std::min(kMaxTiles, ceil_div(pairs, kTilePairs)) * experts * 4, kTempAlign);
+    return kTempAlign + align_up(std::min(kMaxTiles, ceil_div(pairs, kTilePairs)) * align_up(experts, 4) * 4, kTempAlign);
 }
 
 bool counts_ok(uint64_t tokens, uint32_t top_k, uint32_t experts, uint64_t max_rows)
@@ -454,16 +496,24 @@ lcpp_status plan(void* temp, size_t temp_bytes, const int32_t* experts, int32_t*
     p.num_experts = num_experts;
     p.align = align;
     p.max_rows = uint32_t(max_rows);
-    p.per_warp = uint32_t(align_up(ceil_div(ceil_div(pairs, tiles), kPlanWarps), kWarp));
-    p.tile = p.per_warp * kPlanWarps;
+    const bool few = pairs <= kFewPairs && num_experts <= uint32_t(kFewThreads);
+    const int threads = few ? kFewThreads : kPlanThreads, warps = threads / kWarp;
+    p.per_warp = uint32_t(align_up(ceil_div(ceil_div(pairs, tiles), warps), kWarp));
+    p.tile = p.per_warp * warps;
     p.ctrl = static_cast<uint32_t*>(temp);
     p.table = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(temp) + kTempAlign);
+    p.table_pitch = uint32_t(align_up(num_experts, 4));
     const unsigned grid = unsigned(std::max<uint64_t>(1, pairs ? ceil_div(pairs, p.tile) : 1));
-    const size_t smem = size_t(kPlanWarps + 2) * num_experts * 4;
-    set_max_dynamic_smem(reinterpret_cast<const void*>(plan_kernel), size_t(kPlanWarps + 2) * LCPP_MAX_EXPERTS * 4);
+    const size_t smem = size_t(warps + 2) * num_experts * 4;
     diag::KernelTimer timer(kTimerDispatch, pairs, s);
+    if (few) {
+        plan_kernel<kFewThreads><<<1, threads, smem, s>>>(p);
+        return launched();
+    }
+    set_max_dynamic_smem(reinterpret_cast<const void*>(plan_kernel<kPlanThreads>),
+                         size_t(kPlanThreads / kWarp + 2) * LCPP_MAX_EXPERTS * 4);
     if (grid > 1) count_kernel<<<grid, kPlanThreads, num_experts * 4, s>>>(p);
-    plan_kernel<<<grid, kPlanThreads, smem, s>>>(p);
+    plan_kernel<kPlanThreads><<<grid, threads, smem, s>>>(p);
     return launched();
 }
 
@@ -492,12 +542,33 @@ lcpp_status with_unit(int bytes, F&& fn)
     }
 }
 
-uint32_t lanes_log2_for(uint64_t units)
+// Padding is looked for by up to four blocks per SM.
+void set_padding(RowParams& p)
 {
-    uint32_t log = 0;
-    while (log < 8 && (uint64_t(1) << log) < units) ++log;  // at most kRowThreads
-    return log;
+    p.pad_rows = uint32_t(std::min<uint64_t>(kPadRows, std::max<uint64_t>(1, ceil_div(p.max_rows, uint64_t(device_sm_count()) * 4))));
+    p.pad_blocks = uint32_t(ceil_div(p.max_rows, p.pad_rows));
 }
+
+// Threads per token: of 32 to kRowThreads the power of two that leaves the
+// fewest idle in the last chunk (the larger of equals), fewer for short rows.
+uint32_t lanes_log2_for(uint64_t units, int per_thread)
+{
+    uint32_t best = 0;
+    while (best < 5 && (uint64_t(per_thread) << best) < units) ++best;
+    if (best < 5) return best;
+    uint64_t best_slots = ~0ull;
+    for (uint32_t log = 5; (1 << log) <= kRowThreads; ++log) {
+        const uint64_t slots = align_up(units, uint64_t(per_thread) << log);
+        if (slots <= best_slots) {
+            best = log;
+            best_slots = slots;
+        }
+    }
+    return best;
+}
+
+// top_k rows in equal passes of at most `most`.
+uint32_t rows_per_pass_for(uint32_t top_k, int most) { return uint32_t(ceil_div(top_k, ceil_div(top_k, most))); }
 
 bool strides_ok(uint64_t hidden, std::initializer_list<uint64_t> strides)
 {
@@ -537,14 +608,15 @@ lcpp_status gather(const void* x, uint64_t x_stride, const int32_t* row_of, cons
     const Access accesses[] = {{x, p.x_pitch}, {rows, p.out_pitch}};
     const int ub = unit_bytes(accesses, hidden * size);
     p.units = uint32_t(hidden * size / ub);
-    p.lanes_log2 = lanes_log2_for(ceil_div(p.units, 2));
-    p.chunks = uint32_t(ceil_div(p.units, uint64_t(2) << p.lanes_log2));
-    p.pad_blocks = uint32_t(ceil_div(max_rows, kPadRows));
-    const uint64_t grid = p.pad_blocks + ceil_div(tokens, kRowThreads >> p.lanes_log2) * p.chunks;
-    if (grid >> 31) return LCPP_ERR_INVALID_ARG;
-    diag::KernelTimer timer(kTimerDispatch, tokens * top_k, s);
     return with_unit(ub, [&](auto unit) {
-        gather_kernel<decltype(unit)::value><<<unsigned(grid), kRowThreads, 0, s>>>(p);
+        constexpr int kUb = decltype(unit)::value, kN = std::min(8, 32 / kUb);
+        p.lanes_log2 = lanes_log2_for(p.units, kN);
+        p.chunks = uint32_t(ceil_div(p.units, uint64_t(kN) << p.lanes_log2));
+        set_padding(p);
+        const uint64_t grid = p.pad_blocks + ceil_div(tokens, kRowThreads >> p.lanes_log2) * p.chunks;
+        if (grid >> 31) return LCPP_ERR_INVALID_ARG;
+        diag::KernelTimer timer(kTimerDispatch, tokens * top_k, s);
+        gather_kernel<kUb, kN><<<unsigned(grid), kRowThreads, 0, s>>>(p);
         return launched();
     });
 }
@@ -576,18 +648,23 @@ lcpp_status combine(const void* rows, uint64_t rows_stride, const int32_t* row_o
     const Access accesses[] = {{rows, p.rows_pitch}, {out, p.out_pitch}};
     const int ub = unit_bytes(accesses, hidden * size);
     p.units = uint32_t(hidden * size / ub);
-    p.lanes_log2 = lanes_log2_for(p.units);
-    p.chunks = uint32_t(ceil_div(p.units, uint64_t(1) << p.lanes_log2));
-    const uint64_t grid = ceil_div(tokens, kRowThreads >> p.lanes_log2) * p.chunks;
-    if (grid >> 31) return LCPP_ERR_INVALID_ARG;
-    diag::KernelTimer timer(kTimerDispatch, tokens * top_k, s);
     return with_row_type(dtype, [&](auto t) {
         using T = decltype(t);
         return with_unit(ub, [&](auto unit) {
             constexpr int kUb = decltype(unit)::value;
-            if constexpr (kUb >= int(sizeof(T)))
-                combine_kernel<T, kUb><<<unsigned(grid), kRowThreads, 0, s>>>(p);
-            return launched();
+            const auto go = [&](auto kernel, int rows_most, int per_thread) -> lcpp_status {
+                p.rows_per_pass = rows_per_pass_for(top_k, rows_most);
+                p.lanes_log2 = lanes_log2_for(p.units, per_thread);
+                p.chunks = uint32_t(ceil_div(p.units, uint64_t(per_thread) << p.lanes_log2));
+                const uint64_t grid = ceil_div(tokens, kRowThreads >> p.lanes_log2) * p.chunks;
+                if (grid >> 31) return LCPP_ERR_INVALID_ARG;
+                diag::KernelTimer timer(kTimerDispatch, tokens * top_k, s);
+                kernel<<<unsigned(grid), kRowThreads, 0, s>>>(p);
+                return launched();
+            };
+            if constexpr (kUb < int(sizeof(T))) return LCPP_ERR_INTERNAL;  // rows are aligned to their elements
+            else if constexpr (kUb < 16) return go(combine_kernel<T, kUb, 2, 32 / kUb>, 2, 32 / kUb);
+            else return go(combine_kernel<T, kUb, 4, 2>, 4, 2);
         });
     });
 }
@@ -635,19 +712,28 @@ lcpp_status combine_backward(const void* grad_out, uint64_t grad_out_stride, con
     const Access accesses[] = {{grad_out, p.x_pitch}, {rows, p.rows_pitch}, {grad_rows, p.out_pitch}};
     const int ub = unit_bytes(accesses, hidden * size);
     p.units = uint32_t(hidden * size / ub);
-    p.lanes_log2 = lanes_log2_for(p.units);
-    p.pad_blocks = uint32_t(ceil_div(max_rows, kPadRows));
-    const uint64_t grid = p.pad_blocks + ceil_div(tokens, kRowThreads >> p.lanes_log2);
-    if (!grid) return LCPP_OK;
-    if (grid >> 31) return LCPP_ERR_INVALID_ARG;
-    diag::KernelTimer timer(kTimerDispatch, tokens * top_k, s);
     return with_row_type(dtype, [&](auto t) {
         using T = decltype(t);
         return with_unit(ub, [&](auto unit) {
             constexpr int kUb = decltype(unit)::value;
-            if constexpr (kUb >= int(sizeof(T)))
-                combine_backward_kernel<T, kUb><<<unsigned(grid), kRowThreads, 0, s>>>(p);
-            return launched();
+            const auto go = [&](auto kernel, int rows_most, int per_thread) -> lcpp_status {
+                p.rows_per_pass = rows_per_pass_for(top_k, rows_most);
+                // Twice a thread's accesses or more, to share the cost of the sums
+                // over a token's lanes, where that still fills the SMs twice.
+                const uint64_t wide = uint64_t(per_thread) * kRowThreads * device_sm_count() * 4;
+                p.lanes_log2 = lanes_log2_for(p.units, tokens * p.units >= wide ? 2 * per_thread : per_thread);
+                set_padding(p);
+                const uint64_t grid = p.pad_blocks + ceil_div(tokens, kRowThreads >> p.lanes_log2);
+                if (!grid) return LCPP_OK;
+                if (grid >> 31) return LCPP_ERR_INVALID_ARG;
+                diag::KernelTimer timer(kTimerDispatch, tokens * top_k, s);
+                kernel<<<unsigned(grid), kRowThreads, 0, s>>>(p);
+                return launched();
+            };
+            if constexpr (kUb < int(sizeof(T))) return LCPP_ERR_INTERNAL;  // rows are aligned to their elements
+            else if constexpr (kUb < 16) return go(combine_backward_kernel<T, kUb, 2, std::min(8, 32 / kUb)>, 2, std::min(8, 32 / kUb));
+            else if (top_k <= 2) return go(combine_backward_kernel<T, kUb, 2, 4>, 2, 4);
+            else return go(combine_backward_kernel<T, kUb, 4, 2>, 4, 2);
         });
     });
 }
