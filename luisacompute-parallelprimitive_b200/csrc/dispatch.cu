@@ -609,7 +609,7 @@ lcpp_status gather(const void* x, uint64_t x_stride, const int32_t* row_of, cons
     const int ub = unit_bytes(accesses, hidden * size);
     p.units = uint32_t(hidden * size / ub);
     return with_unit(ub, [&](auto unit) {
-        constexpr int kUb = decltype(unit)::value, kN = std::min(8, 32 / kUb);
+        constexpr int kUb = decltype(unit)::value, kN = std::min(8, 16 / kUb);
         p.lanes_log2 = lanes_log2_for(p.units, kN);
         p.chunks = uint32_t(ceil_div(p.units, uint64_t(kN) << p.lanes_log2));
         set_padding(p);

@@ -5,6 +5,18 @@
 using namespace lcpp;
 using namespace lcpp::model;
 
+namespace lcpp {
+namespace router {
+
+__global__ void __launch_bounds__(kThreads) clear_kernel(uint32_t* words, uint32_t n)
+{
+    asm volatile("griddepcontrol.launch_dependents;");
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) words[i] = 0;
+}
+
+}  // namespace router
+}  // namespace lcpp
+
 namespace {
 
 size_t temp_size(uint32_t experts) { return align_up(router::cleared_bytes(experts), kTempAlign); }

@@ -24,9 +24,10 @@
 // two words come from one 32-bit register in five instructions, the first
 // round's winner is the row's maximum, and a chosen word holds its own logit.
 // For the others the dropped bits matter only where two of the first top_k + 1
-// words agree in all kept bits and their sums do not; a row whose choice could
-// depend on them is chosen again from the full values (rows of continuous
-// 32-bit logits: about one in a thousand at 256 experts).
+// words agree in all kept bits and their sums do not; such a row's words (and
+// those past them that agree too) are put in the order of their full values
+// (about one row in 300 of continuous 32-bit logits at 256 experts); only where
+// more than kMoreRounds agree is the row chosen again from the full values.
 #pragma once
 
 #include "model.cuh"
@@ -44,6 +45,7 @@ constexpr float kNegInf = -INFINITY;
 constexpr float kDeepSigmoid = 1e-20f;
 constexpr float kDeepLogit = -60.f;  // the same for the largest chosen logit
 constexpr int kHeads = 4;
+constexpr int kMoreRounds = 8;  // words past top_k that a tie is followed for
 
 struct Params {
     const void* logits;
@@ -100,6 +102,15 @@ __device__ __forceinline__ void copy_async(void* to, const void* from)
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem), "l"(from), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Read each time it is used: loop-invariant values would fill the registers.
+__device__ __forceinline__ float4 shared_load4(const float* from)
+{
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(uint32_t(__cvta_generic_to_shared(from))));
+    return v;
+}
 // All but the newest group of this thread's copies have landed.
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 
@@ -140,23 +151,21 @@ struct Tile {
     static __device__ __forceinline__ void fetch(uint4* tile, const T* row, int wl, uint32_t n, uint32_t unit)
     {
         const int lane = wl % LANES;
+        if (unit == 16) {
 #pragma unroll
+            for (int v = 0; v < kVecs; ++v)
+                if (expert(lane, v * kV) < n) copy_async<16>(tile + v * kWarp + wl, row + expert(lane, v * kV));
+            return;
+        }
+#pragma unroll 1
         for (int v = 0; v < kVecs; ++v) {
             const uint32_t e0 = expert(lane, v * kV);
-            uint4* slot = tile + v * kWarp + wl;
-            if (unit == 16) {
-                if (e0 < n) copy_async<16>(slot, row + e0);
-            } else if (unit >= 4) {
-#pragma unroll
-                for (int b = 0; b < 16; b += 4) {
-                    if (e0 + b / int(sizeof(T)) >= n) break;
-                    if (unit == 8 && b % 8 == 0) copy_async<8>(reinterpret_cast<char*>(slot) + b, row + e0 + b / sizeof(T));
-                    if (unit == 4) copy_async<4>(reinterpret_cast<char*>(slot) + b, row + e0 + b / sizeof(T));
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kV; ++i)
-                    if (e0 + i < n) reinterpret_cast<T*>(slot)[i] = row[e0 + i];
+            T* slot = reinterpret_cast<T*>(tile + v * kWarp + wl);
+            const uint32_t step = unit >= 4 ? unit / sizeof(T) : 1;
+            for (uint32_t i = 0; i < kV && e0 + i < n; i += step) {
+                if (unit == 8) copy_async<8>(slot + i, row + e0 + i);
+                else if (unit == 4) copy_async<4>(slot + i, row + e0 + i);
+                else slot[i] = row[e0 + i];
             }
         }
     }
@@ -258,15 +267,22 @@ __device__ __forceinline__ float word_value(uint32_t word)
     return Packed<T>::value(o & 0x8000u ? o ^ 0x8000u : ~o & 0xffffu);
 }
 
-// exp(x) for x <= 0 and its sigmoid; results below 2^-126 become 0.
-__device__ __forceinline__ float exp_of(float x)
+// 2^x and exp(x); results below 2^-126 become 0.
+constexpr float kLog2E = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_of(float x)
 {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ float exp_of(float x) { return exp2_of(x * kLog2E); }
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + exp_of(-x)); }
+__device__ __forceinline__ float sigmoid(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + exp_of(-x)));
+    return r;
+}
 
 template <int C>
 __device__ __forceinline__ float lane_max(const float (&x)[C])
@@ -277,27 +293,56 @@ __device__ __forceinline__ float lane_max(const float (&x)[C])
     return m;
 }
 
+// What a row's softmax scores are taken relative to: exp(x - top), as one
+// multiply-add and 2^x where `top` is of ordinary size.  The rounding of
+// top log2(e) is then a factor common to all scores of the row, which are only
+// used as quotients; past 10^6 the factor itself could overflow.
+struct Reference {
+    float top, scaled;
+    bool wide;  // of any row of the warp
+    __device__ __forceinline__ explicit Reference(float t) : top(t), scaled(t * -kLog2E), wide(__any_sync(~0u, !(fabsf(t) < 1e6f))) {}
+    __device__ __forceinline__ float score(float x) const
+    {
+        return wide ? exp_of(x - top) : exp2_of(fmaf(x, kLog2E, scaled));
+    }
+};
+
 // x (in place) becomes the lane's scores; returns their sum over the lane.
-// Softmax scores are taken relative to `top`, as are sigmoids of a deep row.
-template <bool SIGMOID, int C>
-__device__ __forceinline__ float scores(float (&x)[C], float top, bool deep)
+template <int C>
+__device__ __forceinline__ float softmax_scores(float (&x)[C], const Reference& ref)
+{
+    float z[2] = {0.f, 0.f};
+    if (ref.wide) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) x[i] = exp_of(x[i] - ref.top);
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i) x[i] = exp2_of(fmaf(x[i], kLog2E, ref.scaled));
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) z[i % 2] += x[i];
+    return z[0] + z[1];
+}
+
+// The same for sigmoids; where `deep`, exp(x - top).
+template <int C>
+__device__ __forceinline__ float sigmoid_scores(float (&x)[C], float top, bool deep)
 {
     float z[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-        x[i] = SIGMOID && !deep ? sigmoid(x[i]) : exp_of(x[i] - top);
+        x[i] = deep ? exp_of(x[i] - top) : sigmoid(x[i]);
         z[i % 2] += x[i];
     }
     return z[0] + z[1];
 }
 
-// The score that a chosen expert's weight is made of, `most` being the largest
-// chosen logit where weights are renormalised and the row's largest otherwise.
+// What a chosen expert's renormalised weight is made of, `most` being the
+// largest chosen logit.
 template <bool SIGMOID>
-__device__ __forceinline__ float weight_score(float x, float most, bool renormalize)
+__device__ __forceinline__ float weight_score(float x, float most)
 {
-    if (SIGMOID) return renormalize && most < kDeepLogit ? exp_of(x - most) : sigmoid(x);
-    return exp_of(x - most);
+    return SIGMOID && !(most < kDeepLogit) ? sigmoid(x) : exp_of(x - most);
 }
 
 // The exact choice of a warp's rows from the full values, one composite word
@@ -375,58 +420,66 @@ __device__ void finish(const Params& p, uint32_t routed_tokens, bool broken, dou
 }
 
 template <typename T, int LANES, int C, bool SIGMOID, bool BIAS>
-__global__ void __launch_bounds__(kThreads, C > 16 ? 2 : C > 8 ? 3 : 5) forward_kernel(const Params p)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) forward_kernel(const Params p)
 {
     using L = Tile<T, LANES, C>;
     constexpr uint32_t kMask = L::kMask;
     constexpr bool kExact = sizeof(T) == 2 && !BIAS;  // words hold all of a logit
+    constexpr int kPlaces = LCPP_MAX_TOP_K / LANES;   // of a lane's entries
     constexpr uint32_t kLowest = kExact ? Packed<T>::kLowestChoice : 0x00800000u;
     const uint32_t n = p.num_experts, k = p.top_k;
     const int warp = threadIdx.x / kWarp, wl = threadIdx.x % kWarp, lane = wl % LANES, sub = wl / LANES;
 
-    // the warps' two tiles; after the last row the shares' sums of every warp
+    // The warps' two tiles, and every lane's sums of its experts' shares: they
+    // are touched once a row, and in registers they would cost a third of the
+    // resident warps.
     extern __shared__ uint4 dynamic[];
     uint4* tiles = dynamic + warp * 2 * L::kSlots;
-    float* share_sum = reinterpret_cast<float*>(dynamic);                              // [kWarps][n]
-    uint32_t* count = reinterpret_cast<uint32_t*>(dynamic + kWarps * 2 * L::kSlots);   // [n]
-    float* bias = reinterpret_cast<float*>(count + n);                                 // [n]
-    static_assert(2 * L::kSlots * 16 >= L::kSpan * 4, "the sums fit in the tiles");
-    __shared__ uint32_t chosen_all[kWarps][L::kRows][LCPP_MAX_TOP_K];
-    __shared__ float value_all[kWarps][L::kRows][LCPP_MAX_TOP_K];
+    float4* all_sums = reinterpret_cast<float4*>(dynamic + kWarps * 2 * L::kSlots);    // [kWarps][C / 4][32]
+    float4* sums = all_sums + warp * (C / 4) * kWarp + wl;
+    float* bias = reinterpret_cast<float*>(all_sums + kWarps * (C / 4) * kWarp);  // [kSpan]
+    uint32_t* count = reinterpret_cast<uint32_t*>(bias + (BIAS ? L::kSpan : 0));   // [n]
+    __shared__ uint32_t chosen_all[kExact ? 1 : kWarps][L::kRows][LCPP_MAX_TOP_K];
+    __shared__ uint64_t lists[kExact ? 1 : kWarps][kExact ? 1 : L::kRows][LCPP_MAX_TOP_K + kMoreRounds];
     __shared__ double scratch[kThreads];
     __shared__ uint32_t routed_block;
     __shared__ bool is_last;
-    uint32_t* chosen = chosen_all[warp][sub];
-    float* value = value_all[warp][sub];
-    for (uint32_t e = threadIdx.x; e < n; e += kThreads) {
-        count[e] = 0;
+    uint32_t* chosen = chosen_all[kExact ? 0 : warp][sub];
+    for (uint32_t e = threadIdx.x; e < n; e += kThreads) count[e] = 0;
+    if (BIAS) {
         // finite, so that a logit of -inf stays -inf; NaN counts as the largest too
-        if (BIAS) bias[e] = fminf(p.bias[e], 3.402823466e38f);
+        for (uint32_t e = threadIdx.x; e < L::kSpan; e += kThreads) bias[e] = e < n ? fminf(p.bias[e], 3.402823466e38f) : 0.f;
     }
     if (threadIdx.x == 0) routed_block = 0;
     L::clear(tiles, wl);
     L::clear(tiles + L::kSlots, wl);
     __syncthreads();
 
-    float acc[C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) acc[i] = 0.f;
+    for (int q = 0; q < C / 4; ++q) sums[q * kWarp] = float4{0.f, 0.f, 0.f, 0.f};
     uint32_t routed = 0;
 
-    // lanes past the last token work on its row and write nothing
-    const T* logits = static_cast<const T*>(p.logits);
+    // a row past the last token works on what its tile holds and writes nothing
     const uint32_t tokens = uint32_t(p.tokens), step = gridDim.x * kWarps * L::kRows;
-    uint32_t t0 = (blockIdx.x * kWarps + warp) * L::kRows;
-    if (t0 < tokens) L::fetch(tiles, logits + min(t0 + sub, tokens - 1) * p.stride, wl, n, p.unit);
+    uint32_t t = (blockIdx.x * kWarps + warp) * L::kRows + sub;
+    const T* row = static_cast<const T*>(p.logits) + t * p.stride;
+    const uint64_t row_step = step * p.stride;
+    int32_t request = 0, request_ahead = 0;
+    if (t < tokens) {
+        L::fetch(tiles, row, wl, n, p.unit);
+        if (p.token_request) request_ahead = p.token_request[t];
+    }
     copies_commit();
-    for (int stage = 0; t0 < tokens; t0 += step, stage ^= 1) {
-        const uint32_t t = t0 + sub;
+    for (int stage = 0; t - sub < tokens; t += step, stage ^= 1) {
         const bool inside = t < tokens;
         uint4* tile = tiles + stage * L::kSlots;
-        if (t0 + step < tokens)
-            L::fetch(tiles + (stage ^ 1) * L::kSlots, logits + min(t + step, tokens - 1) * p.stride, wl, n, p.unit);
+        row += row_step;
+        request = request_ahead;
+        if (t + step < tokens) {
+            L::fetch(tiles + (stage ^ 1) * L::kSlots, row, wl, n, p.unit);
+            if (p.token_request) request_ahead = p.token_request[t + step];
+        }
         copies_commit();
-        const bool wanted = inside && (!p.token_request || p.token_request[t] >= 0);
         copies_wait();
 
         uint32_t word[C], low = 0;
@@ -447,12 +500,15 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : C > 8 ? 3 : 5) forward_
             float x[C];
             L::unpack(tile, wl, x);
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                float f = x[i];
-                // read where it is used: the biases would fill the registers otherwise
-                if (BIAS) f += *static_cast<const volatile float*>(bias + min(L::expert(lane, i), n - 1));
-                low |= __float_as_uint(f);
-                word[i] = (ordered(f) & ~kMask) | L::register_bits(i);
+            for (int q = 0; q < C; q += 4) {
+                float4 b{0.f, 0.f, 0.f, 0.f};
+                if (BIAS) b = shared_load4(bias + L::expert(lane, q));
+                const float f[4] = {x[q] + b.x, x[q + 1] + b.y, x[q + 2] + b.z, x[q + 3] + b.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    low |= __float_as_uint(f[i]);
+                    word[q + i] = (ordered(f[i]) & ~kMask) | L::register_bits(q + i);
+                }
             }
         }
         // The lane's largest words, then the row's: words below kLowest are
@@ -464,79 +520,145 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : C > 8 ? 3 : 5) forward_
             head[h] = 0;
             if (uint32_t(h) < rounds) head[h] = tail = largest_below(word, tail);
         }
+        // each lane keeps those of its places j = lane, lane + LANES, ...
         const uint32_t lane_bits = L::lane_bits(lane);
-        uint32_t best = 0, handed = 0;
-        bool found = false, unsure = false;
-        for (uint32_t j = 0; j < rounds; ++j) {
-            const uint32_t mine = head[0] + lane_bits;
-            const uint32_t next = row_all<LANES>(mine, Max{});
-            if (!kExact) unsure |= j && next >= kLowest && (next & ~kMask) == (best & ~kMask);
-            best = next;
-            if (j == 0) found = best >= kLowest;
-            if (j < k && lane == 0) chosen[j] = best;
+        uint32_t picked[kPlaces + 1], best = 0, handed = 0;
+        bool unsure = false, tie = false;
+        // the row's largest head; `refill`: a lane may have handed out all it had
+        const auto hand_out = [&](bool refill) {
+            const uint32_t mine = head[0] + lane_bits, next = row_all<LANES>(mine, Max{});
             const bool out = mine == next;
 #pragma unroll
             for (int h = 0; h + 1 < kHeads; ++h) head[h] = out ? head[h + 1] : head[h];
             if (out) head[kHeads - 1] = 0;
             handed += out;
-            const bool empty = head[0] == 0 && handed < C;
-            if (__any_sync(~0u, empty) && j + 1 < rounds) {
-                const uint32_t more = largest_below(word, tail);
-                if (empty) head[0] = tail = more;
+            if (refill) {
+                const bool empty = head[0] == 0 && handed < C;
+                if (__any_sync(~0u, empty)) {
+                    const uint32_t more = largest_below(word, tail);
+                    if (empty) head[0] = tail = more;
+                }
+            }
+            return next;
+        };
+#pragma unroll
+        for (int s = 0; s <= kPlaces; ++s) {
+            picked[s] = 0;
+            if (uint32_t(s * LANES) >= rounds) break;
+            for (uint32_t i = 0, j = s * LANES; i < LANES && j < rounds; ++i, ++j) {
+                const uint32_t next = hand_out(j + 1 < rounds && j + 1 >= kHeads);
+                tie = next >= kLowest && (next & ~kMask) == (best & ~kMask);
+                unsure |= tie;
+                best = next;
+                if (uint32_t(lane) == i) picked[s] = next;
             }
         }
-        __syncwarp();
         if (!kExact) {
             // logits whose dropped bits are all zero were compared in full
             low = row_all<LANES>(low & kMask, Or{});
-            unsure = unsure && low;
-            if (__any_sync(~0u, unsure)) choose_exactly<T, LANES, C>(tile, BIAS ? bias : nullptr, wl, n, k, chosen);
+            if (__any_sync(~0u, unsure && low)) {
+                // Words that tie with the last one are handed out too, then all
+                // are put in the order of their full values.
+                uint64_t* list = lists[warp][sub];
+                const auto full = [&](uint32_t w) -> uint64_t {
+                    if (w < kLowest) return 0;
+                    const uint32_t e = kMask - (w & kMask);
+                    const float v = to_float(*L::element(tile, sub, e));
+                    return uint64_t(ordered(BIAS ? v + bias[e] : v)) << 32 | (0xffffffffu - e);
+                };
+                __syncwarp();
+#pragma unroll
+                for (int s = 0; s <= kPlaces; ++s)
+                    if (uint32_t(s * LANES + lane) < rounds) list[s * LANES + lane] = full(picked[s]);
+                uint32_t m = rounds;
+                for (; m < min(n, k + kMoreRounds) && __any_sync(~0u, tie); ++m) {
+                    const uint32_t next = hand_out(true);
+                    tie = next >= kLowest && (next & ~kMask) == (best & ~kMask);
+                    best = next;
+                    if (lane == 0) list[m] = full(next);
+                }
+                for (uint32_t j = lane; j < k; j += LANES) chosen[j] = 0;
+                __syncwarp();
+                if (__any_sync(~0u, tie && m < n)) {
+                    choose_exactly<T, LANES, C>(tile, BIAS ? bias : nullptr, wl, n, k, chosen);
+                } else {
+                    for (uint32_t j = lane; j < m; j += LANES) {
+                        const uint64_t mine = list[j];
+                        uint32_t rank = 0;
+                        for (uint32_t i = 0; i < m; ++i) rank += list[i] > mine;
+                        if (mine && rank < k) chosen[rank] = ~kMask | (uint32_t(mine) & kMask);
+                    }
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int s = 0; s < kPlaces; ++s)
+                    if (uint32_t(s * LANES + lane) < k) picked[s] = chosen[s * LANES + lane];
+            }
         }
-        const bool live = wanted && found;
+        const uint32_t first = __shfl_sync(~0u, picked[0], sub * LANES);
+        const bool live = inside && request >= 0 && first >= kLowest;
 
         float x[C], top = 0.f;
         L::unpack(tile, wl, x);
-        if (!SIGMOID) top = kExact ? word_value<T>(chosen[0]) : row_all<LANES>(lane_max(x), Max{});
-        float sum = row_all<LANES>(scores<SIGMOID>(x, top, false), Add{});
+        if (!SIGMOID) top = kExact ? word_value<T>(first) : row_all<LANES>(lane_max(x), Max{});
+        const Reference ref(top);
+        float sum = row_all<LANES>(SIGMOID ? sigmoid_scores(x, 0.f, false) : softmax_scores(x, ref), Add{});
         if (SIGMOID) {
             const bool deep = sum < kDeepSigmoid;
             if (__any_sync(~0u, deep)) {
                 L::unpack(tile, wl, x);
                 top = row_all<LANES>(lane_max(x), Max{});
-                sum = row_all<LANES>(scores<SIGMOID>(x, top, deep), Add{});
+                sum = row_all<LANES>(sigmoid_scores(x, top, deep), Add{});
             }
         }
         const float inv = live ? __fdividef(1.f, sum) : 0.f;
         if (live) {
 #pragma unroll
-            for (int i = 0; i < C; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
+            for (int q = 0; q < C / 4; ++q) {
+                float4 v = sums[q * kWarp];
+                v.x = fmaf(x[4 * q], inv, v.x);
+                v.y = fmaf(x[4 * q + 1], inv, v.y);
+                v.z = fmaf(x[4 * q + 2], inv, v.z);
+                v.w = fmaf(x[4 * q + 3], inv, v.w);
+                sums[q * kWarp] = v;
+            }
         }
 
         // weights of the chosen
-        float most = kNegInf;
-        for (uint32_t j = lane; j < k; j += LANES) {
-            const uint32_t w = chosen[j], e = kMask - (w & kMask);
-            const float v = w < kLowest ? kNegInf : kExact ? word_value<T>(w) : to_float(*L::element(tile, sub, e));
-            value[j] = v;
-            most = fmaxf(most, v);
+        float value[kPlaces], most = kNegInf, total = 0.f;
+#pragma unroll
+        for (int s = 0; s < kPlaces; ++s) {
+            if (uint32_t(s * LANES) >= k) break;
+            if (uint32_t(s * LANES + lane) >= k) picked[s] = 0;
+            const uint32_t w = picked[s];
+            value[s] = kNegInf;
+            if (w >= kLowest) value[s] = kExact ? word_value<T>(w) : to_float(*L::element(tile, sub, kMask - (w & kMask)));
+            most = fmaxf(most, value[s]);
         }
         if (p.renormalize) most = row_all<LANES>(most, Max{});
-        else most = top;
-        float total = 0.f;
-        for (uint32_t j = lane; j < k; j += LANES) {
-            const float s = chosen[j] >= kLowest ? weight_score<SIGMOID>(value[j], most, p.renormalize) : 0.f;
-            value[j] = s;
-            total += s;
+#pragma unroll
+        for (int s = 0; s < kPlaces; ++s) {
+            if (uint32_t(s * LANES) >= k) break;
+            float v = 0.f;
+            if (picked[s] >= kLowest) {
+                if (p.renormalize) v = weight_score<SIGMOID>(value[s], most);
+                else v = SIGMOID ? sigmoid(value[s]) : ref.score(value[s]);
+            }
+            value[s] = v;
+            total += v;
         }
         float scale = p.weight_scale;
         if (p.renormalize) scale = __fdividef(scale, row_all<LANES>(total, Add{}));
         else if (!SIGMOID) scale = __fdividef(scale, sum);
-        if (inside) {
-            for (uint32_t j = lane; j < k; j += LANES) {
-                const uint32_t w = chosen[j], e = kMask - (w & kMask);
-                const bool is = live && w >= kLowest;
-                p.weights[uint64_t(t) * k + j] = is ? value[j] * scale : 0.f;
-                p.experts[uint64_t(t) * k + j] = is ? int32_t(e) : -1;
+        const uint32_t at = t * k + lane;
+#pragma unroll
+        for (int s = 0; s < kPlaces; ++s) {
+            if (uint32_t(s * LANES) >= k) break;
+            if (inside && uint32_t(s * LANES + lane) < k) {
+                const bool is = live && picked[s] >= kLowest;
+                const uint32_t e = kMask - (picked[s] & kMask);
+                p.weights[at + s * LANES] = is ? value[s] * scale : 0.f;
+                p.experts[at + s * LANES] = is ? int32_t(e) : -1;
                 if (is) atomicAdd(count + e, 1u);
             }
         }
@@ -544,21 +666,16 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : C > 8 ? 3 : 5) forward_
         __syncwarp();
     }
 
-    // the block's sums, in the tiles' memory
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-#pragma unroll
-        for (int d = LANES; d < kWarp; d *= 2) acc[i] += __shfl_xor_sync(~0u, acc[i], d);
-        const uint32_t e = L::expert(lane, i);
-        if (sub == 0 && e < n) share_sum[warp * n + e] = acc[i];
-    }
     if (routed) atomicAdd(&routed_block, uint32_t(routed));
     __syncthreads();
+    // an expert's sum over the block: its register of its lane in every row of every warp
     const auto block_share = [&](uint32_t e) {
+        const uint32_t vec = e / L::kV, of_lane = vec % LANES, i = vec / LANES * L::kV + e % L::kV;
+        const float* at = reinterpret_cast<const float*>(all_sums + (i / 4) * kWarp + of_lane) + i % 4;
         float sum = 0.f;
+        for (int w = 0; w < kWarps; ++w)
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum += share_sum[w * n + e];
+            for (int r = 0; r < L::kRows; ++r) sum += at[(w * (C / 4) * kWarp + r * LANES) * 4];
         return sum;
     };
     if (gridDim.x == 1) {
@@ -567,6 +684,8 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : C > 8 ? 3 : 5) forward_
                [&](uint32_t e) { return count[e]; });
         return;
     }
+    // the totals are cleared by the launch before this one, which may still run
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     for (uint32_t e = threadIdx.x; e < n; e += kThreads) {
         const float sum = block_share(e);
         if (!(sum < INFINITY)) atomicOr(p.ctrl + 2, 1u);
@@ -599,14 +718,14 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
     constexpr bool kJoined = !SIGMOID && !RENORM;
     const uint32_t n = p.num_experts, k = p.top_k;
     const int warp = threadIdx.x / kWarp, wl = threadIdx.x % kWarp, lane = wl % LANES, sub = wl / LANES;
+    constexpr int kPlaces = LCPP_MAX_TOP_K / LANES;  // a lane's entries are j = lane, lane + LANES, ...
     extern __shared__ uint4 dynamic[];
     uint4* tiles = dynamic + warp * 2 * L::kSlots;
     float* pull = reinterpret_cast<float*>(dynamic + kWarps * 2 * L::kSlots);  // [kSpan]
-    // this row's chosen experts and upstream gradients, twice, and their logits: [kRows][k] each
+    // the rows' chosen experts and upstream gradients, twice: [kRows][k] each
     const uint32_t row_k = L::kRows * k;
-    uint32_t* ids = reinterpret_cast<uint32_t*>(pull + L::kSpan) + warp * 5 * row_k + sub * k;
+    uint32_t* ids = reinterpret_cast<uint32_t*>(pull + L::kSpan) + warp * 4 * row_k + sub * k + lane;
     float* ups = reinterpret_cast<float*>(ids + 2 * row_k);
-    float* values = ups + 2 * row_k;
     L::clear(tiles, wl);
     L::clear(tiles + L::kSlots, wl);
     {
@@ -622,106 +741,153 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
     }
     __syncthreads();
 
-    const T* logits = static_cast<const T*>(p.logits);
+    // a row past the last token works on what its tile holds and writes nothing
     const uint32_t tokens = uint32_t(p.tokens), step = gridDim.x * kWarps * L::kRows;
-    const auto fetch = [&](uint32_t t, int stage) {
-        const uint32_t tt = min(t, tokens - 1);
-        L::fetch(tiles + stage * L::kSlots, logits + tt * p.stride, wl, n, p.unit);
-        for (uint32_t j = lane; j < k; j += LANES) {
-            copy_async<4>(ids + stage * row_k + j, p.experts + uint64_t(tt) * k + j);
-            if (p.grad_weights) copy_async<4>(ups + stage * row_k + j, p.grad_weights + uint64_t(tt) * k + j);
-            else ups[stage * row_k + j] = 0.f;
+    uint32_t t = (blockIdx.x * kWarps + warp) * L::kRows + sub;
+    const T* row = static_cast<const T*>(p.logits) + t * p.stride;
+    T* out = static_cast<T*>(p.grad_logits) + t * p.grad_stride;
+    const uint64_t row_step = step * p.stride, out_step = step * p.grad_stride;
+    const auto fetch = [&](uint32_t token, int stage) {
+        L::fetch(tiles + stage * L::kSlots, row, wl, n, p.unit);
+        const uint32_t at = token * k + lane;
+#pragma unroll
+        for (int s = 0; s < kPlaces; ++s) {
+            if (uint32_t(s * LANES) >= k) break;
+            if (uint32_t(s * LANES + lane) < k) {
+                copy_async<4>(ids + stage * row_k + s * LANES, p.experts + at + s * LANES);
+                if (p.grad_weights) copy_async<4>(ups + stage * row_k + s * LANES, p.grad_weights + at + s * LANES);
+            }
         }
     };
-    uint32_t t0 = (blockIdx.x * kWarps + warp) * L::kRows;
-    if (t0 < tokens) fetch(t0 + sub, 0);
+    if (t < tokens) fetch(t, 0);
     copies_commit();
-    for (int stage = 0; t0 < tokens; t0 += step, stage ^= 1) {
-        const uint32_t t = t0 + sub;
+    for (int stage = 0; t - sub < tokens; t += step, stage ^= 1, out += out_step) {
         const bool inside = t < tokens;
         uint4* tile = tiles + stage * L::kSlots;
-        const uint32_t* id = ids + stage * row_k;
-        const float* up = ups + stage * row_k;
-        if (t0 + step < tokens) fetch(t + step, stage ^ 1);
+        row += row_step;
+        if (t + step < tokens) fetch(t + step, stage ^ 1);
         copies_commit();
         copies_wait();
         __syncwarp();
 
-        const bool live = int32_t(id[0]) >= 0;
-        float chosen_top = kNegInf;
-        for (uint32_t j = lane; j < k; j += LANES) {
-            float v = kNegInf;
-            if (id[j] < n) {
-                T* at = L::element(tile, sub, id[j]);
-                v = to_float(*at);
+        // the chosen experts leave the tile
+        uint32_t id[kPlaces];
+        float value[kPlaces], up[kPlaces], chosen_top = kNegInf;
+#pragma unroll
+        for (int s = 0; s < kPlaces; ++s) {
+            id[s] = ~0u;
+            value[s] = kNegInf;
+            up[s] = 0.f;
+            if (uint32_t(s * LANES) >= k) break;
+            if (inside && uint32_t(s * LANES + lane) < k) id[s] = ids[stage * row_k + s * LANES];
+            if (id[s] < n) {
+                T* at = L::element(tile, sub, id[s]);
+                value[s] = to_float(*at);
                 *at = from_float<T>(kNegInf);
+                if (p.grad_weights) up[s] = ups[stage * row_k + s * LANES];
             }
-            values[j] = v;
-            chosen_top = fmaxf(chosen_top, v);
+            chosen_top = fmaxf(chosen_top, value[s]);
         }
-        if (RENORM || !SIGMOID) chosen_top = row_all<LANES>(chosen_top, Max{});
-        __syncwarp();
-        // The expert with most of the row's share, among the chosen: slopes are
-        // taken relative to its own, so that the mean of a row that one expert
-        // dominates is not the difference of two equal numbers.
-        uint32_t lead = 0;
-        for (uint32_t j = 1; j < k; ++j) lead = values[j] > values[lead] ? j : lead;
-        const float up0 = up[lead], c = p.weight_scale;
-        const float pull0 = id[lead] < n ? pull[id[lead]] : 0.f;
-        const float base = kJoined ? fmaf(c, up0, pull0) : pull0;
+        const bool live = int32_t(__shfl_sync(~0u, id[0], sub * LANES)) >= 0;
+        // The expert with most of the row's share, among the chosen: slopes and
+        // upstream gradients are taken relative to its own, so that what is left
+        // of a row that one expert dominates is not the difference of two
+        // nearly equal numbers.
+        const float lane_top = chosen_top;
+        chosen_top = row_all<LANES>(chosen_top, Max{});
+        float pull0 = 0.f, up0 = 0.f;
+#pragma unroll
+        for (int s = 0; s < kPlaces; ++s) {
+            if (uint32_t(s * LANES) >= k) break;
+            if (id[s] < n && value[s] == lane_top) {
+                pull0 = pull[id[s]];
+                up0 = up[s];
+            }
+        }
+        const uint32_t leads = __ballot_sync(~0u, lane_top == chosen_top) >> (sub * LANES) & uint32_t((uint64_t(1) << LANES) - 1);
+        const int lead = sub * LANES + (leads ? __ffs(leads) - 1 : 0);
+        pull0 = __shfl_sync(~0u, pull0, lead);
+        up0 = __shfl_sync(~0u, up0, lead);
+        const float c = p.weight_scale, base = kJoined ? fmaf(c, up0, pull0) : pull0;
 
         float x[C], top = 0.f;
         L::unpack(tile, wl, x);
         if (!SIGMOID) top = fmaxf(row_all<LANES>(lane_max(x), Max{}), chosen_top);
-        float sum = scores<SIGMOID>(x, top, false), weights = 0.f;
-        for (uint32_t j = lane; j < k; j += LANES) {
-            sum += SIGMOID ? sigmoid(values[j]) : exp_of(values[j] - top);
-            if (RENORM) weights += id[j] < n ? weight_score<SIGMOID>(values[j], chosen_top, true) : 0.f;
+        const Reference ref(top);
+        float sum = SIGMOID ? sigmoid_scores(x, 0.f, false) : softmax_scores(x, ref), score[kPlaces];
+#pragma unroll
+        for (int s = 0; s < kPlaces; ++s) {
+            if (uint32_t(s * LANES) >= k) break;
+            score[s] = SIGMOID ? sigmoid(value[s]) : ref.score(value[s]);
+            sum += score[s];
         }
         sum = row_all<LANES>(sum, Add{});
-        if (RENORM) weights = row_all<LANES>(weights, Add{});
         bool deep = false;
         if (SIGMOID) {
             deep = sum < kDeepSigmoid;
             if (__any_sync(~0u, deep)) {
                 L::unpack(tile, wl, x);
-                float most = lane_max(x);
-                for (uint32_t j = lane; j < k; j += LANES) most = fmaxf(most, values[j]);
-                top = row_all<LANES>(most, Max{});
-                sum = scores<SIGMOID>(x, top, deep);
-                for (uint32_t j = lane; j < k; j += LANES) sum += deep ? exp_of(values[j] - top) : sigmoid(values[j]);
+                top = row_all<LANES>(fmaxf(lane_max(x), lane_top), Max{});
+                sum = sigmoid_scores(x, top, deep);
+#pragma unroll
+                for (int s = 0; s < kPlaces; ++s) {
+                    if (uint32_t(s * LANES) >= k) break;
+                    score[s] = deep ? exp_of(value[s] - top) : sigmoid(value[s]);
+                    sum += score[s];
+                }
                 sum = row_all<LANES>(sum, Add{});
             }
         }
         const float inv = __fdividef(1.f, sum);
-        const auto share_of = [&](float v) { return (SIGMOID && !deep ? sigmoid(v) : exp_of(v - top)) * inv; };
-        const auto slope_at = [&](uint32_t j) {
-            const float h = pull[id[j]] - pull0;
-            return kJoined ? fmaf(c, up[j] - up0, h) : h;
-        };
-        float mean = 0.f;
-#pragma unroll
-        for (int v = 0; v < L::kVecs; ++v) {
-            const float* h = pull + L::expert(lane, v * L::kV);
-#pragma unroll
-            for (int i = 0; i < L::kV; ++i) mean = fmaf(x[v * L::kV + i], h[i] - base, mean);
-        }
-        mean *= inv;
-        for (uint32_t j = lane; j < k; j += LANES)
-            if (id[j] < n) mean = fmaf(share_of(values[j]), slope_at(j), mean);
-        mean = row_all<LANES>(mean, Add{});
 
-        T* out = static_cast<T*>(p.grad_logits) + uint64_t(t) * p.grad_stride;
+        // the mean slope; a chosen expert's slope of the loss (and, joined, of its weight)
+        float mean = 0.f, slope[kPlaces];
+#pragma unroll
+        for (int q = 0; q < C; q += 4) {
+            const float4 h = shared_load4(pull + L::expert(lane, q));
+            mean = fmaf(x[q], h.x - base, mean);
+            mean = fmaf(x[q + 1], h.y - base, mean);
+            mean = fmaf(x[q + 2], h.z - base, mean);
+            mean = fmaf(x[q + 3], h.w - base, mean);
+        }
+        float weights = 0.f, dot = 0.f, share[kPlaces];  // of renormalised weights: sum r, sum r (g - g0)
+#pragma unroll
+        for (int s = 0; s < kPlaces; ++s) {
+            if (uint32_t(s * LANES) >= k) break;
+            slope[s] = share[s] = 0.f;
+            up[s] -= up0;
+            if (id[s] < n) {
+                slope[s] = pull[id[s]] - pull0;
+                if (kJoined) slope[s] = fmaf(c, up[s], slope[s]);
+                mean = fmaf(score[s], slope[s], mean);
+                if (RENORM) {
+                    share[s] = weight_score<SIGMOID>(value[s], chosen_top);
+                    weights += share[s];
+                    dot = fmaf(share[s], up[s], dot);
+                }
+            }
+        }
+        mean = row_all<LANES>(mean, Add{}) * inv;
+        if (RENORM) {
+            weights = row_all<LANES>(weights, Add{});
+            dot = row_all<LANES>(dot, Add{});
+        }
+
         const float rest = base + mean;
 #pragma unroll
         for (int v = 0; v < L::kVecs; ++v) {
             const uint32_t e0 = L::expert(lane, v * L::kV);
             float g[L::kV];
 #pragma unroll
-            for (int i = 0; i < L::kV; ++i) {
-                const float s = x[v * L::kV + i];
-                g[i] = s * inv * (pull[e0 + i] - rest);
-                if (SIGMOID && !deep) g[i] *= 1.f - s;
+            for (int q = 0; q < L::kV; q += 4) {
+                const float4 h4 = shared_load4(pull + e0 + q);
+                const float h[4] = {h4.x, h4.y, h4.z, h4.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float s = x[v * L::kV + q + i];
+                    g[q + i] = s * inv * (h[i] - rest);
+                    if (SIGMOID && !deep) g[q + i] = fmaf(-s, g[q + i], g[q + i]);
+                }
             }
             uint4 raw = Vec<T>::pack(g);
             if (!live) raw = uint4{0, 0, 0, 0};
@@ -736,22 +902,19 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
             }
         }
         __syncwarp();
-        for (uint32_t j = lane; j < k; j += LANES) {
-            if (id[j] >= n || !inside) continue;
-            const float v = values[j], g = up[j];
-            const float flat = SIGMOID ? sigmoid(-v) : 1.f;  // 1 - s
-            float d = flat * share_of(v) * (slope_at(j) - mean);
+#pragma unroll
+        for (int s = 0; s < kPlaces; ++s) {
+            if (uint32_t(s * LANES) >= k) break;
+            if (id[s] >= n) continue;
+            const float flat = SIGMOID ? sigmoid(-value[s]) : 1.f;  // 1 - s
+            float d = flat * score[s] * inv * (slope[s] - mean);
             if (RENORM) {
-                // g_j - sum_i r_i g_i as a sum of differences, for the same reason
-                float apart = 0.f;
-                for (uint32_t i = 0; i < k; ++i)
-                    if (id[i] < n)
-                        apart = fmaf(weight_score<SIGMOID>(values[i], chosen_top, true), g - up[i], apart);
-                d += c * flat * __fdividef(weight_score<SIGMOID>(v, chosen_top, true), weights) * __fdividef(apart, weights);
+                const float part = __fdividef(share[s], weights);
+                d = fmaf(c * flat * part, up[s] - __fdividef(dot, weights), d);
             } else if (SIGMOID) {
-                d = fmaf(c * g * flat, sigmoid(v), d);
+                d = fmaf(c * (up[s] + up0) * flat, sigmoid(value[s]), d);
             }
-            out[id[j]] = from_float<T>(d);
+            out[id[s]] = from_float<T>(d);
         }
         __syncwarp();
     }
@@ -760,6 +923,8 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
 // Temp storage: the control words, the share totals, the count totals.
 constexpr size_t kShareOffset = kTempAlign;
 inline size_t cleared_bytes(uint32_t experts) { return kShareOffset + size_t(experts) * 12; }
+
+__global__ void __launch_bounds__(kThreads) clear_kernel(uint32_t* words, uint32_t n);
 
 // Blocks for `tokens` rows: as many as are resident at once, fewer for few rows.
 inline unsigned grid_for(const void* kernel, size_t smem, uint64_t tokens, int rows_per_block)
@@ -772,15 +937,31 @@ template <typename T, int LANES, int C>
 lcpp_status forward_shape(const Params& p, bool sigmoid, cudaStream_t s)
 {
     using L = Tile<T, LANES, C>;
-    const size_t smem = size_t(kWarps) * 2 * L::kSlots * 16 + size_t(p.num_experts) * 8;
+    const size_t fixed = size_t(kWarps) * (2 * L::kSlots * 16 + kWarp * C * 4), smem = fixed + (p.bias ? L::kSpan : 0) * 4 + size_t(p.num_experts) * 4;
     void (*kernel)(Params) =
         sigmoid ? (p.bias ? forward_kernel<T, LANES, C, true, true> : forward_kernel<T, LANES, C, true, false>)
                 : (p.bias ? forward_kernel<T, LANES, C, false, true> : forward_kernel<T, LANES, C, false, false>);
     const void* f = reinterpret_cast<const void*>(kernel);
-    set_max_dynamic_smem(f, size_t(kWarps) * 2 * L::kSlots * 16 + L::kSpan * 8);
+    set_max_dynamic_smem(f, fixed + L::kSpan * 8);
     const unsigned grid = grid_for(f, smem, p.tokens, kWarps * L::kRows);
-    if (grid > 1) LCPP_CUDA_TRY(cudaMemsetAsync(p.ctrl, 0, cleared_bytes(p.num_experts), s));
-    kernel<<<grid, kThreads, smem, s>>>(p);
+    if (grid == 1) {
+        kernel<<<1, kThreads, smem, s>>>(p);
+        return launched();
+    }
+    // The totals are cleared by a small launch of their own, which the kernel
+    // only waits for before it first adds to them.
+    clear_kernel<<<1, kThreads, 0, s>>>(p.ctrl, uint32_t(cleared_bytes(p.num_experts) / 4));
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = s;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
     return launched();
 }
 
@@ -789,12 +970,12 @@ lcpp_status backward_shape(const BackParams& p, bool sigmoid, cudaStream_t s)
 {
     using L = Tile<T, LANES, C>;
     const size_t fixed = size_t(kWarps) * 2 * L::kSlots * 16 + L::kSpan * 4;
-    const size_t smem = fixed + size_t(kWarps) * 5 * L::kRows * p.top_k * 4;
+    const size_t smem = fixed + size_t(kWarps) * 4 * L::kRows * p.top_k * 4;
     void (*kernel)(BackParams) =
         sigmoid ? (p.renormalize ? backward_kernel<T, LANES, C, true, true> : backward_kernel<T, LANES, C, true, false>)
                 : (p.renormalize ? backward_kernel<T, LANES, C, false, true> : backward_kernel<T, LANES, C, false, false>);
     const void* f = reinterpret_cast<const void*>(kernel);
-    set_max_dynamic_smem(f, fixed + size_t(kWarps) * 5 * L::kRows * LCPP_MAX_TOP_K * 4);
+    set_max_dynamic_smem(f, fixed + size_t(kWarps) * 4 * L::kRows * LCPP_MAX_TOP_K * 4);
     kernel<<<grid_for(f, smem, p.tokens, kWarps * L::kRows), kThreads, smem, s>>>(p);
     return launched();
 }

@@ -226,7 +226,10 @@ def check_route_grad(L, logits, kind, k, score, renormalize, chosen, rng, in_pla
                               SCALE, COEF)
     rel, step = ROUND[kind]
     bound = 2e-5 * np.abs(want).max(1, keepdims=True) + rel * np.abs(want) + step
-    assert (np.abs(host64(out) - want) <= bound + 1e-12).all()
+    # a row with an infinite logit has no gradient: NaN on both sides
+    fine = ~np.isnan(want)
+    np.testing.assert_array_equal(np.isnan(host(out.float())), ~fine)
+    assert (np.abs(host64(out) - want) <= bound + 1e-12)[fine].all()
 
 
 SHAPES = [(1, 1, 1), (1, 8, 2), (5, 2, 1), (33, 7, 3), (100, 8, 8), (17, 32, 4), (50, 33, 6), (301, 60, 4),
@@ -278,6 +281,23 @@ def test_route_ties_go_to_the_lower_expert(lcpp, kind):
             check_route(lcpp, cuda(x).to(TYPES[kind]), min(e, 9), ref.SOFTMAX, True, b)
 
 
+@pytest.mark.parametrize("e,k", [(8, 8), (60, 6), (256, 8), (512, 32), (1024, 31)])
+def test_route_near_ties(lcpp, e, k):
+    """32-bit logits in clusters that agree in all but their last bits: of two, of a few, of more than are
+    followed past the last choice, and across it."""
+    rng = np.random.default_rng(e)
+    t = 300
+    x = rng.standard_normal((t, e)).astype(np.float32)
+    for size, rows in ((2, slice(0, 100)), (4, slice(100, 180)), (30, slice(180, 240))):
+        near = np.repeat(x[rows, : -(-e // size)], size, axis=1)[:, :e]
+        bits = near.view(np.int32) ^ rng.integers(0, 4, near.shape).astype(np.int32)
+        x[rows] = np.take_along_axis(bits.view(np.float32), np.argsort(rng.random(near.shape), axis=1), 1)
+    x[240:] = (np.float32(0.1).view(np.int32) + rng.integers(0, 40, (60, e))).astype(np.int32).view(np.float32)
+    bias = (rng.integers(-3, 4, e) * 2.0 ** -24).astype(np.float32)
+    for b in (None, bias):
+        check_route(lcpp, cuda(x), k, ref.SOFTMAX, True, b)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
 @pytest.mark.parametrize("renormalize", [True, False])
@@ -301,6 +321,18 @@ def test_route_masked_experts(lcpp, kind, score, renormalize):
         chosen = check_route(lcpp, logits, 4, score, renormalize, b)
         assert (host(chosen[1])[5] == -1).all()
         check_route_grad(lcpp, logits, kind, 4, score, renormalize, chosen, rng)
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_large_logits(lcpp, renormalize):
+    """Softmax only sees differences: rows far from zero, whose exponents alone would overflow, and rows that
+    span the type (some of the last become infinite)."""
+    rng = np.random.default_rng(21)
+    for size in (300.0, 7e4, 3e6, 5e9, 1e30, 3e38):
+        x = np.sign(rng.standard_normal((30, 1))) * np.float32(size) * (1 + rng.integers(0, 3, (30, 24)) * 2.0 ** -22)
+        x = np.concatenate([x, rng.standard_normal((10, 24)) * size]).astype(np.float32)
+        chosen = check_route(lcpp, cuda(x), 3, ref.SOFTMAX, renormalize)
+        check_route_grad(lcpp, cuda(x), "f32", 3, ref.SOFTMAX, renormalize, chosen, rng)
 
 
 def test_route_nothing_routed(lcpp):
