@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
             return next;
         };
 #pragma unroll
-        for (int s = 0; s <= kPlaces; ++s) {
+        for (int s = 0; s < kPlaces + !kExact; ++s) {
             picked[s] = 0;
             if (uint32_t(s * LANES) >= rounds) break;
             for (uint32_t i = 0, j = s * LANES; i < LANES && j < rounds; ++i, ++j) {
