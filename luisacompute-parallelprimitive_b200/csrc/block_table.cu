@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(kThreads) fused_kernel(const Params p)
 // The three launches for many requests.
 __global__ void __launch_bounds__(kThreads) totals_kernel(const Params p, Sums* tile_sums)
 {
+    let_next_start();
     __shared__ Sums shared[kWarps];
     const Request q = request_at(p, blockIdx.x * kThreads + threadIdx.x);
     Sums of_warp, total;
@@ -324,6 +325,8 @@ __global__ void __launch_bounds__(kThreads) starts_kernel(const Params p, const 
     __shared__ Sums shared[kWarps];
     __shared__ uint32_t used_after;
     if (threadIdx.x == 0) used_after = 0;
+    let_next_start();
+    wait_for_previous();
     Sums mine{0, 0}, of_warp, before, total;
     for (uint32_t i = threadIdx.x; i < blockIdx.x; i += kThreads) mine = mine + tile_sums[i];
     warp_exclusive(mine, of_warp);
@@ -348,6 +351,7 @@ __global__ void __launch_bounds__(kThreads) tokens_kernel(const Params p, const 
     __shared__ uint32_t start[kWindow], free_base[kWindow];
     __shared__ int32_t context[kWindow];
     const uint32_t first = blockIdx.x * p.tokens_per_block, last = min(first + p.tokens_per_block, p.tokens);
+    wait_for_previous();
     const uint32_t end = uint32_t(p.starts[p.requests]);
     const uint32_t lo = block_count_starts(all.start, p.requests, first) - 1;  // the first starts at 0
     const uint32_t window = block_count_starts(all.start + lo, p.requests - lo, last - 1);
@@ -485,13 +489,16 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_block_table_args* a, c
     Sums* sums = reinterpret_cast<Sums*>(t + l.sums);
     const unsigned tiles = unsigned(ceil_div(n, kThreads));
     totals_kernel<<<tiles, kThreads, 0, s>>>(p, sums);
-    starts_kernel<<<tiles, kThreads, 0, s>>>(p, sums, plan);
+    // Each launch starts while the one before it runs and waits for its end on the
+    // device.  The last one waits for the second, which has itself waited.
+    lcpp_status status = launch_early(starts_kernel, tiles, kThreads, 0, s, Params(p), static_cast<const Sums*>(sums), Plan(plan));
+    if (status != LCPP_OK) return status;
     if (p.tokens) {
         auto kernel = many ? tokens_kernel<4> : tokens_kernel<1>;
         const unsigned grid = grid_of(reinterpret_cast<const void*>(kernel), 0);
-        kernel<<<grid, kThreads, 0, s>>>(p, plan);
+        return launch_early(kernel, grid, kThreads, 0, s, Params(p), Plan(plan));
     }
-    return launched();
+    return LCPP_OK;
 }
 
 }  // namespace

@@ -58,6 +58,28 @@ lcpp_status guarded(const char* name, F&& body) noexcept
     }
 }
 
+// Launches `kernel` without waiting for the launch before it on the stream to
+// end: the kernel itself waits (wait_for_previous) before it touches what that
+// one writes.  The launch before must be the same call's.
+template <typename... P>
+lcpp_status launch_early(void (*kernel)(P...), unsigned grid, int block, size_t smem, cudaStream_t s, P... args)
+{
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(block);
+    config.dynamicSmemBytes = smem;
+    config.stream = s;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, args...));
+    return LCPP_OK;
+}
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 inline lcpp_status launched() { return cudaGetLastError() == cudaSuccess ? LCPP_OK : LCPP_ERR_CUDA; }
 
 __device__ __forceinline__ float to_float(float v) { return v; }

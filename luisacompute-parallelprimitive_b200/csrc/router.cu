@@ -10,7 +10,7 @@ namespace router {
 
 __global__ void __launch_bounds__(kThreads) clear_kernel(uint32_t* words, uint32_t n)
 {
-    asm volatile("griddepcontrol.launch_dependents;");
+    let_next_start();
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) words[i] = 0;
 }
 

@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
         return;
     }
     // the totals are cleared by the launch before this one, which may still run
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_previous();
     for (uint32_t e = threadIdx.x; e < n; e += kThreads) {
         const float sum = block_share(e);
         if (!(sum < INFINITY)) atomicOr(p.ctrl + 2, 1u);
@@ -951,18 +951,7 @@ lcpp_status forward_shape(const Params& p, bool sigmoid, cudaStream_t s)
     // The totals are cleared by a small launch of their own, which the kernel
     // only waits for before it first adds to them.
     clear_kernel<<<1, kThreads, 0, s>>>(p.ctrl, uint32_t(cleared_bytes(p.num_experts) / 4));
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid);
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = smem;
-    config.stream = s;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
-    return launched();
+    return launch_early(kernel, grid, kThreads, smem, s, p);
 }
 
 template <typename T, int LANES, int C>

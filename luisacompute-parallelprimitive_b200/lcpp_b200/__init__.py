@@ -895,6 +895,8 @@ def _flat(t, dtype, count, name):
         return None
     if t.dtype != dtype or not t.is_contiguous() or t.numel() < count:
         raise LcppError(ERR_INVALID_ARG, f"{name}: contiguous {dtype} with at least {count} elements")
+    if not t.is_cuda:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a CUDA tensor")
     return t.data_ptr()
 
 
@@ -906,15 +908,25 @@ def _rows(t, rows, columns, code, name):
     stride = t.stride()
     if stride[1] != 1 and shape[1] > 1 and shape[0]:
         raise LcppError(ERR_INVALID_ARG, f"{name}: a row's columns have to be adjacent")
+    if not t.is_cuda:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a CUDA tensor")
     return t.data_ptr(), (stride[0] if shape[0] > 1 else max(stride[0], columns))
+
+
+_raw_stream = None
 
 
 def _queue(stream):
     """Handle of the stream to enqueue on: the one given, else torch's current one."""
+    global _raw_stream
     if stream is not None:
         return stream.cuda_stream
-    cuda = _torch().cuda
-    return cuda.current_stream(cuda.current_device()).cuda_stream
+    torch = _torch()
+    if _raw_stream is None:
+        # the handle without a Stream object around it, where torch offers it
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda device: torch.cuda.current_stream(device).cuda_stream)
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _scratch(temp):
@@ -958,6 +970,8 @@ class DeviceBlockTable:
         if d_block_table.dtype != i32 or d_block_table.dim() != 2 or d_block_table.shape[0] < n or \
                 (d_block_table.stride(1) != 1 and d_block_table.shape[1] > 1 and n):
             raise LcppError(ERR_INVALID_ARG, "d_block_table: int32 [num_requests, width], columns adjacent")
+        if not d_block_table.is_cuda:
+            raise LcppError(ERR_INVALID_ARG, "d_block_table: a CUDA tensor")
         width = d_block_table.shape[1]
         args = BlockTableArgs(
             _flat(d_context_lens, i32, n, "d_context_lens"), _flat(d_new_lens, i32, n, "d_new_lens"),

@@ -180,6 +180,8 @@ def test_python_classes_refuse_tensors(lcpp):
         with pytest.raises(lcpp.LcppError) as err:
             forward(**change)
         assert err.value.status == lcpp.ERR_INVALID_ARG
+    with pytest.raises(lcpp.LcppError, match="CUDA tensor"):
+        forward()
     with pytest.raises(TypeError):
         forward(logits=torch.zeros(t, e, dtype=torch.float64))
     with pytest.raises(lcpp.LcppError):

@@ -166,6 +166,47 @@ def test_extend_longest_sequences(lcpp):
     check_extend(lcpp, context, new, np.zeros((6, 2), np.int32), 2, np.arange(9, dtype=np.int32), 0, 16, 64)
 
 
+@pytest.mark.parametrize("n", [7, 5000])
+def test_extend_step_after_step(lcpp, n):
+    """A captured decode step on another stream, replayed: the lengths and the used counter of one step are the
+    next one's inputs, no page is given twice, and every position of a request keeps its slot."""
+    rng = np.random.default_rng(n)
+    block, width, steps = 4, 40, 20
+    context = rng.integers(0, 60, n).astype(np.int32)
+    held = -(-context // block)
+    pages = rng.permutation(n * width + 3).astype(np.int32)
+    table = np.full((n, width), -1, np.int32)
+    given = 0
+    for r in range(n):
+        table[r, :held[r]] = pages[given:given + held[r]]
+        given += held[r]
+    free = pages[given:]
+    d_table, lens, d_free = cuda(table), [cuda(context), i32(n)], cuda(free)
+    used, starts = [i32(1, fill=0), i32(1)], i32(n + 1)
+    slots = torch.full((n + 5,), -9, dtype=torch.int64, device="cuda")
+    temp = lcpp.alloc_temp(lcpp.DeviceBlockTable.GetTempStorageBytes(n, n + 5))
+    t = lcpp.DeviceBlockTable()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        for i in range(2):
+            t.Extend(temp, lens[i], None, d_table, d_free, used[i], used[1 - i], lens[1 - i], starts, slots, None,
+                     None, n, block)
+    for _ in range(steps // 2):
+        graph.replay()
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(host(lens[0]), context + steps)
+    total = -(-(context + steps) // block)
+    assert int(used[0]) == (total - held).sum()
+    got = host(d_table)
+    filled = got[np.arange(width) < total[:, None]]
+    assert len(np.unique(filled)) == filled.size and set(filled) <= set(pages)
+    position = context + steps - 1
+    expect = got[np.arange(n), position // block].astype(np.int64) * block + position % block
+    np.testing.assert_array_equal(host(slots)[:n], expect)
+    assert (host(slots)[n:] == -1).all()
+
+
 def test_extend_nothing(lcpp):
     empty = np.zeros(0, np.int32)
     check_extend(lcpp, empty, empty, np.zeros((0, 4), np.int32), 4, np.arange(3, dtype=np.int32), 2, 10, 16)
