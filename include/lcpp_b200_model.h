@@ -62,12 +62,13 @@ lcpp_status lcpp_block_table_temp_bytes(uint64_t num_requests, uint64_t max_toke
  * free_blocks ends before its pages.  A refused request takes no page, its
  * row stays as it is, seq_lens_out keeps its context length, and its tokens
  * that lie below max_tokens are marked like the entries past the step's last
- * token: slot -1, position 0, request -1.  Requests after it that need no new page are still served;
- * those that need one are refused too when free_blocks is what ended.  A
- * negative page id in the row gives slot -1.
+ * token: slot -1, position 0, request -1.  Requests after it that need no new
+ * page are still served; those that need one are refused too when free_blocks
+ * is what ended.  A negative page id in the row gives slot -1.
  *
- * free_used_out and seq_lens_out must not overlap the inputs.  Zero requests
- * give num_requests + 1 = 1 start, no pages and marked entries. */
+ * free_used_out and seq_lens_out must not overlap the inputs: a step's outputs
+ * are the next one's inputs through two sets of buffers.  Zero requests give
+ * one start, no pages and marked entries. */
 lcpp_status lcpp_block_table_extend(void* temp, size_t temp_bytes, const lcpp_block_table_args* args,
                                     lcpp_stream_t stream);
 
@@ -97,15 +98,17 @@ lcpp_status lcpp_router_temp_bytes(uint64_t num_tokens, uint32_t num_experts, si
 /* For each token t: the top_k experts with the largest logit + bias (added
  * in 32 bits; equal sums go to the lower expert), in descending order, and
  *   weights[t][j] = weight_scale * s[e_j] (/ sum_i s[e_i] when renormalised).
- * The bias (NULL: none) only takes part in the choice.  An expert whose logit
- * or sum is -inf is never chosen; entries left over hold expert -1, weight 0.
+ * The bias (NULL: none) only takes part in the choice; +inf and NaN in it count
+ * as the largest finite number.  An expert whose logit or sum is -inf is never
+ * chosen; entries left over hold expert -1, weight 0.
  * A token with a negative token_request (NULL: none has), or with no expert
  * to choose, is left out: all its entries are -1 and 0, and it takes no part
  * in the counts or the loss.  With T' tokens that took part (d_num_routed_out)
  * and counts[e] entries that name expert e:
  *   loss = loss_coef * E * sum_e counts[e] / (top_k T') * mean_t s[t][e] / sum_i s[t][i]
- * (0 when T' is 0).  NaN logits order above +inf and make the token's weights
- * and the loss NaN, as does +inf under softmax. */
+ * (0 when T' is 0).  NaN logits order above +inf, and NaN (and +inf under
+ * softmax) go into the token's weights and the loss as the formulas say; a
+ * token that is left out passes nothing on. */
 lcpp_status lcpp_router_forward(void* temp, size_t temp_bytes, const void* d_logits, uint64_t logits_stride,
                                 lcpp_dtype logits_dtype, const float* d_bias, const int32_t* d_token_request,
                                 float* d_weights_out, int32_t* d_experts_out, int32_t* d_counts_out,
@@ -141,8 +144,9 @@ lcpp_status lcpp_dispatch_max_rows(uint64_t num_tokens, uint32_t top_k, uint32_t
  * [num_experts] is the end of the last segment.  d_row_of_out[p] = the pair's
  * row, d_pair_of_out[row] = the row's pair, -1 for rows that pad a segment or
  * lie past the last one.  Pairs whose expert is not in [0, num_experts), or
- * whose row would lie past max_rows, get row -1.  The starts are not cut off at max_rows.
- * num_tokens * top_k and max_rows below 2^31; starts must stay below 2^31. */
+ * whose row would lie past max_rows, get row -1; the starts are not cut off
+ * there.  num_tokens * top_k, max_rows and lcpp_dispatch_max_rows' answer stay
+ * below 2^31. */
 lcpp_status lcpp_dispatch_plan(void* temp, size_t temp_bytes, const int32_t* d_experts, int32_t* d_expert_starts_out,
                                int32_t* d_row_of_out, int32_t* d_pair_of_out, uint64_t num_tokens, uint32_t top_k,
                                uint32_t num_experts, uint32_t row_align, uint64_t max_rows, lcpp_stream_t stream);

@@ -14,6 +14,14 @@
 // its own range of tokens from the sums in shared memory.  Beyond that, the
 // sums take two small launches (totals of 512 requests, then each 512's scan on
 // top of the totals before it) and the third lays out the tokens.
+//
+// What has to move is 8 bytes a request in, and out 16 bytes a token, 8 a
+// request and 4 a new page.  A step of 64 single tokens takes 2.9 us and one of
+// 7001 mixed tokens 3.3 us, a launch and its dependent loads.  4.0 M tokens of
+// 6001 requests in pages of 64 take 25 us (67 MB written at 2.6 TB/s; the copy
+// rate would be 10.5 us): the layout kernel, 20 us of it, is bound by its
+// instructions (283 per 128 tokens, 54 % of the issue slots) and by the page
+// loads it waits for, not by memory, for all it writes stays in L2.
 #include "model.cuh"
 
 using namespace lcpp;
@@ -24,6 +32,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / kWarp;
 constexpr int kItems = 8;                      // requests per thread of the fused kernel, at most
+// One launch up to here: its blocks hold 12 bytes a request in shared memory
+// (48 KB).  A decode step of 8000 requests takes 8.4 us in three launches.
 constexpr uint32_t kFusedRequests = kThreads * kItems;
 constexpr uint32_t kWindow = 1024;             // requests of a block's tokens held in shared memory
 constexpr uint32_t kMost = 0x7fffffffu;        // sums saturate here, past every token and page
@@ -261,7 +271,8 @@ __device__ __forceinline__ void lay_out_run(const Params& p, const Plan& plan, u
 // Lays out tokens [first, last) of the block, whose requests are among
 // [0, window) of the plan, the first of them numbered `base`; `end` is the
 // step's token count.  A thread takes G tokens at a time: where one request has
-// them all they cost one search, one division and, mostly, one page.
+// them all they cost one search, one division and, mostly, one page (G = 4
+// against 1 at 4.0 M tokens: 26 against 28 us).
 template <int G>
 __device__ void lay_out(const Params& p, const Plan& plan, uint32_t base, uint32_t window, uint32_t first,
                         uint32_t last, uint32_t end)
