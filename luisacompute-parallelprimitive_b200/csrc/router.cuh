@@ -223,12 +223,6 @@ __device__ __forceinline__ uint32_t ordered(float f)
     return b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
 }
 
-// ordered() backwards.
-__device__ __forceinline__ float unordered(uint32_t o)
-{
-    return __uint_as_float(o ^ (uint32_t(int32_t(~o) >> 31) | 0x80000000u));
-}
-
 // Pairs of 16-bit logits as order-preserving 16-bit halves and back.
 template <typename T>
 struct Packed;
@@ -308,11 +302,14 @@ __device__ __forceinline__ float lane_max(const float (&x)[C])
 // used as quotients; past 10^6 the factor itself could overflow.
 struct Reference {
     float top, scaled;
-    bool wide;  // of any row of the warp
-    __device__ __forceinline__ explicit Reference(float t) : top(t), scaled(t * -kLog2E), wide(__any_sync(~0u, !(fabsf(t) < 1e6f))) {}
+    bool wide, any_wide;  // this row; any row of the warp
+    __device__ __forceinline__ explicit Reference(float t)
+        : top(t), scaled(t * -kLog2E), wide(!(fabsf(t) < 1e6f)), any_wide(__any_sync(~0u, wide))
+    {
+    }
     __device__ __forceinline__ float score(float x) const
     {
-        return wide ? exp_of(x - top) : exp2_of(fmaf(x, kLog2E, scaled));
+        return any_wide && wide ? exp_of(x - top) : exp2_of(fmaf(x, kLog2E, scaled));
     }
 };
 
@@ -321,9 +318,9 @@ template <int C>
 __device__ __forceinline__ float softmax_scores(float (&x)[C], const Reference& ref)
 {
     float z[2] = {0.f, 0.f};
-    if (ref.wide) {
+    if (ref.any_wide) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) x[i] = exp_of(x[i] - ref.top);
+        for (int i = 0; i < C; ++i) x[i] = ref.score(x[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < C; ++i) x[i] = exp2_of(fmaf(x[i], kLog2E, ref.scaled));

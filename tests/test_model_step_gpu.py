@@ -99,9 +99,9 @@ def test_extend_one_token_each(lcpp, n):
     check_extend(lcpp, context, None, table, 8, free, None, n, 16, optional=False)
 
 
-@pytest.mark.parametrize("n", [3, 700, 4000, 5000])
+@pytest.mark.parametrize("n,block", [(3, 2), (3, 4), (3, 24), (700, 24), (4000, 64), (5000, 24)])
 @pytest.mark.parametrize("offset", [0, 1])
-def test_extend_many_tokens(lcpp, n, offset):
+def test_extend_many_tokens(lcpp, n, block, offset):
     """Enough tokens for four to a thread, in arrays that start on a vector boundary or off it: long prompts,
     single tokens and idle requests side by side."""
     rng = np.random.default_rng(n)
@@ -109,10 +109,10 @@ def test_extend_many_tokens(lcpp, n, offset):
     new[rng.random(n) < 0.2] = 0
     long = rng.choice(n, 3, replace=False)
     new[long] = rng.integers(100_000, 130_000, 3)
-    block, width = 24, 5500
-    table = rng.permutation(n * 3).astype(np.int32).reshape(n, 3)
-    table = np.concatenate([table, np.full((n, width - 3), -1, np.int32)], 1)
-    free = (n * 3 + rng.permutation(20_000)).astype(np.int32)
+    width, held = 130_100 // block + 1, 50 // block + 1
+    table = rng.permutation(n * held).astype(np.int32).reshape(n, held)
+    table = np.concatenate([table, np.full((n, width - held), -1, np.int32)], 1)
+    free = (n * held + rng.permutation(400_000 // block + n)).astype(np.int32)
     tokens = int(new.sum()) + 13
     expect = ref.extend(context, new, table, width, free, 0, tokens, block)
     slots = torch.full((tokens + offset,), -9, dtype=torch.int64, device="cuda")[offset:]
@@ -392,13 +392,15 @@ def test_route_nothing_routed(lcpp):
         assert not host(grad).any()
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("t", [9, 5000])
-def test_route_nan_and_infinity(lcpp, t):
+def test_route_nan_and_infinity(lcpp, t, kind):
     """A NaN or, under softmax, a +inf makes its own token's weights and the loss NaN, and nothing else."""
     rng = np.random.default_rng(2)
     x = rng.standard_normal((t, 16)).astype(np.float32)
-    x[3, 5], x[4, 2] = np.nan, np.inf
-    weights, experts, counts, routed, loss = run_route(lcpp, cuda(x), 2, ref.SOFTMAX, True)
+    x[3, 5], x[4, 2] = -np.nan, np.inf
+    logits = cuda(x).to(TYPES[kind])
+    weights, experts, counts, routed, loss = run_route(lcpp, logits, 2, ref.SOFTMAX, True)
     assert int(host(experts)[3, 0]) == 5 and int(host(experts)[4, 0]) == 2
     bad = np.isnan(host(weights)).any(1)
     assert bad[3] and bad[4] and bad.sum() == 2
@@ -406,11 +408,19 @@ def test_route_nan_and_infinity(lcpp, t):
     # a masked token's NaN reaches nothing
     mask = np.zeros(t, np.int32)
     mask[3:5] = -1
-    check_route(lcpp, torch.nan_to_num(cuda(x), 0.0, 0.0), 2, ref.SOFTMAX, True, None, mask)
-    clean = run_route(lcpp, torch.nan_to_num(cuda(x), 0.0, 0.0), 2, ref.SOFTMAX, True, None, mask)
-    dirty = run_route(lcpp, cuda(x), 2, ref.SOFTMAX, True, None, mask)
+    finite = torch.nan_to_num(logits, 0.0, 0.0)
+    check_route(lcpp, finite, 2, ref.SOFTMAX, True, None, mask)
+    clean = run_route(lcpp, finite, 2, ref.SOFTMAX, True, None, mask)
+    dirty = run_route(lcpp, logits, 2, ref.SOFTMAX, True, None, mask)
     for a, b in zip(clean, dirty):
         assert torch.equal(a, b)
+    grads = []
+    for values in (finite, logits):
+        out = torch.empty_like(values)
+        lcpp.DeviceRouter().Backward(values, *clean[1:4], torch.ones(t, 2, device="cuda"),
+                                     torch.ones(1, device="cuda"), out, t, 16, 2)
+        grads.append(out)
+    assert torch.equal(*grads) and not host(grads[1].float())[3:5].any()
 
 
 @pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
