@@ -99,8 +99,6 @@ struct BackParams {
     uint32_t wide_stores;  // gradient rows start on 16-byte boundaries
 };
 
-constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
-
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* to, const void* from)
 {
@@ -129,7 +127,8 @@ struct Tile {
     static constexpr int kVecs = C / kV;
     static constexpr int kRows = kWarp / LANES;  // rows of a warp
     static constexpr int kSpan = LANES * C;      // experts that fit
-    static constexpr int kIndexBits = log2_of(kSpan);
+    static constexpr int kMaxTopK = kSpan < LCPP_MAX_TOP_K ? kSpan : LCPP_MAX_TOP_K;
+    static constexpr int kPlaces = kMaxTopK / LANES;  // a lane's entries of a row are j = lane, lane + LANES, ...
     static constexpr uint32_t kMask = kSpan - 1;
     static_assert(C % kV == 0 && (kSpan & (kSpan - 1)) == 0, "whole vectors, a power of two of experts");
 
@@ -431,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
     using L = Tile<T, LANES, C>;
     constexpr uint32_t kMask = L::kMask;
     constexpr bool kExact = sizeof(T) == 2 && !BIAS;  // words hold all of a logit
-    constexpr int kPlaces = LCPP_MAX_TOP_K / LANES;   // of a lane's entries
+    constexpr int kPlaces = L::kPlaces;
     constexpr uint32_t kLowest = kExact ? Packed<T>::kLowestChoice : 0x00800000u;
     const uint32_t n = p.num_experts, k = p.top_k;
     const int warp = threadIdx.x / kWarp, wl = threadIdx.x % kWarp, lane = wl % LANES, sub = wl / LANES;
@@ -445,12 +444,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
     float4* sums = all_sums + warp * (C / 4) * kWarp + wl;
     float* bias = reinterpret_cast<float*>(all_sums + kWarps * (C / 4) * kWarp);  // [kSpan]
     uint32_t* count = reinterpret_cast<uint32_t*>(bias + (BIAS ? L::kSpan : 0));   // [n]
-    __shared__ uint32_t chosen_all[kExact ? 1 : kWarps][L::kRows][LCPP_MAX_TOP_K];
-    __shared__ uint64_t lists[kExact ? 1 : kWarps][kExact ? 1 : L::kRows][LCPP_MAX_TOP_K + kMoreRounds];
+    __shared__ uint32_t chosen_all[kExact ? 1 : kWarps][kExact ? 1 : L::kRows][L::kMaxTopK];
+    __shared__ uint64_t lists[kExact ? 1 : kWarps][kExact ? 1 : L::kRows][L::kMaxTopK + kMoreRounds];
     __shared__ double scratch[kThreads];
     __shared__ uint32_t routed_block;
     __shared__ bool is_last;
-    uint32_t* chosen = chosen_all[kExact ? 0 : warp][sub];
+    uint32_t* chosen = chosen_all[kExact ? 0 : warp][kExact ? 0 : sub];
     for (uint32_t e = threadIdx.x; e < n; e += kThreads) count[e] = 0;
     if (BIAS) {
         // finite, so that a logit of -inf stays -inf; NaN counts as the largest too
@@ -724,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
     constexpr bool kJoined = !SIGMOID && !RENORM;
     const uint32_t n = p.num_experts, k = p.top_k;
     const int warp = threadIdx.x / kWarp, wl = threadIdx.x % kWarp, lane = wl % LANES, sub = wl / LANES;
-    constexpr int kPlaces = LCPP_MAX_TOP_K / LANES;  // a lane's entries are j = lane, lane + LANES, ...
+    constexpr int kPlaces = L::kPlaces;
     extern __shared__ uint4 dynamic[];
     uint4* tiles = dynamic + warp * 2 * L::kSlots;
     float* pull = reinterpret_cast<float*>(dynamic + kWarps * 2 * L::kSlots);  // [kSpan]
@@ -975,26 +974,35 @@ lcpp_status backward_shape(const BackParams& p, bool sigmoid, cudaStream_t s)
     return launched();
 }
 
-// The smallest shape that holds the experts.  Lanes times elements: fewer lanes
-// share a round's shuffles among more rows, more elements take more registers.
-// 256 experts as 8 x 32, 16 x 16 and 32 x 8 measured 77, 78 and 104 us (131072
-// bfloat16 rows, before the lane heads).
+// The smallest shape that holds the experts, of those that measured best
+// (bfloat16; lanes x elements): few lanes share a round's shuffles among more
+// rows, many elements take registers.  131072 rows of 256: 8 x 32 45 us, 16 x 16
+// 64, 4 x 64 62; of 64: 4 x 16 20, 8 x 8 23, 8 x 16 29; of 8: 1 x 8 8, 4 x 8 12.
 template <typename T>
 lcpp_status forward_rows(const Params& p, bool sigmoid, cudaStream_t s)
 {
     const uint32_t n = p.num_experts;
+    if (n <= 8) return forward_shape<T, 1, 8>(p, sigmoid, s);
+    if (n <= 16) return forward_shape<T, 2, 8>(p, sigmoid, s);
     if (n <= 32) return forward_shape<T, 4, 8>(p, sigmoid, s);
+    if (n <= 64) return forward_shape<T, 4, 16>(p, sigmoid, s);
     if (n <= 128) return forward_shape<T, 8, 16>(p, sigmoid, s);
     if (n <= 256) return forward_shape<T, 8, 32>(p, sigmoid, s);
     if (n <= 512) return forward_shape<T, 16, 32>(p, sigmoid, s);
     return forward_shape<T, 32, 32>(p, sigmoid, s);
 }
 
+// The same for the gradient.  131072 rows of 256: 8 x 32 42 us, 16 x 16 47, 32 x 8
+// 61; of 64: 8 x 8 18, 4 x 16 17 (but 47 against 29 for 61 experts, whose rows
+// allow no wide access), 8 x 16 23; 65536 of 512: 16 x 32 and 32 x 16 38.
 template <typename T>
 lcpp_status backward_rows(const BackParams& p, bool sigmoid, cudaStream_t s)
 {
     const uint32_t n = p.num_experts;
+    if (n <= 8) return backward_shape<T, 1, 8>(p, sigmoid, s);
+    if (n <= 16) return backward_shape<T, 2, 8>(p, sigmoid, s);
     if (n <= 32) return backward_shape<T, 4, 8>(p, sigmoid, s);
+    if (n <= 64) return backward_shape<T, 8, 8>(p, sigmoid, s);
     if (n <= 128) return backward_shape<T, 8, 16>(p, sigmoid, s);
     if (n <= 256) return backward_shape<T, 8, 32>(p, sigmoid, s);
     if (n <= 512) return backward_shape<T, 16, 32>(p, sigmoid, s);

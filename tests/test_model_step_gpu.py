@@ -273,7 +273,8 @@ def check_route_grad(L, logits, kind, k, score, renormalize, chosen, rng, in_pla
     assert (np.abs(host64(out) - want) <= bound + 1e-12)[fine].all()
 
 
-SHAPES = [(1, 1, 1), (1, 8, 2), (5, 2, 1), (33, 7, 3), (100, 8, 8), (17, 32, 4), (50, 33, 6), (301, 60, 4),
+SHAPES = [(1, 1, 1), (1, 8, 2), (5, 2, 1), (33, 7, 3), (100, 8, 8), (300, 8, 1), (40, 9, 9), (70, 16, 4),
+          (37, 13, 13), (17, 32, 4), (11, 17, 17), (29, 32, 32), (50, 33, 6), (90, 64, 6), (31, 64, 32), (301, 60, 4),
           (64, 128, 8), (257, 129, 32), (77, 160, 6), (1000, 256, 8), (41, 257, 10), (9, 512, 8), (30, 513, 2),
           (21, 1000, 32), (3, 1024, 32)]
 
