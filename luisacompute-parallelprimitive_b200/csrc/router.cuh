@@ -54,7 +54,7 @@ constexpr float kNegInf = -INFINITY;
 constexpr float kDeepSigmoid = 1e-20f;
 constexpr float kDeepLogit = -60.f;  // the same for the largest chosen logit
 constexpr int kHeads = 4;
-constexpr int kMoreRounds = 8;  // words past top_k that a tie is followed for
+constexpr int kMoreRounds = 6;  // words past top_k that a tie is followed for
 
 struct Params {
     const void* logits;
@@ -445,8 +445,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
     float* bias = reinterpret_cast<float*>(all_sums + kWarps * (C / 4) * kWarp);  // [kSpan]
     uint32_t* count = reinterpret_cast<uint32_t*>(bias + (BIAS ? L::kSpan : 0));   // [n]
     __shared__ uint32_t chosen_all[kExact ? 1 : kWarps][kExact ? 1 : L::kRows][L::kMaxTopK];
-    __shared__ uint64_t lists[kExact ? 1 : kWarps][kExact ? 1 : L::kRows][L::kMaxTopK + kMoreRounds];
-    __shared__ double scratch[kThreads];
+    __shared__ uint32_t lists[kExact ? 1 : kWarps][kExact ? 1 : L::kRows][L::kMaxTopK + kMoreRounds];
+    double* scratch = reinterpret_cast<double*>(dynamic);  // [kThreads], after the last row
+    static_assert(kWarps * 2 * L::kSlots * 16 >= kThreads * 8, "the tiles hold it");
     __shared__ uint32_t routed_block;
     __shared__ bool is_last;
     uint32_t* chosen = chosen_all[kExact ? 0 : warp][kExact ? 0 : sub];
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
             if (__any_sync(~0u, unsure && low)) {
                 // Words that tie with the last one are handed out too, then all
                 // are put in the order of their full values.
-                uint64_t* list = lists[warp][sub];
+                uint32_t* list = lists[warp][sub];
                 const auto full = [&](uint32_t w) -> uint64_t {
                     if (w < kLowest) return 0;
                     const uint32_t e = kMask - (w & kMask);
@@ -574,13 +575,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
                 __syncwarp();
 #pragma unroll
                 for (int s = 0; s <= kPlaces; ++s)
-                    if (uint32_t(s * LANES + lane) < rounds) list[s * LANES + lane] = full(picked[s]);
+                    if (uint32_t(s * LANES + lane) < rounds) list[s * LANES + lane] = picked[s];
                 uint32_t m = rounds;
                 for (; m < min(n, k + kMoreRounds) && __any_sync(~0u, tie); ++m) {
                     const uint32_t next = hand_out(true);
                     tie = next >= kLowest && (next & ~kMask) == (best & ~kMask);
                     best = next;
-                    if (lane == 0) list[m] = full(next);
+                    if (lane == 0) list[m] = next;
                 }
                 for (uint32_t j = lane; j < k; j += LANES) chosen[j] = 0;
                 __syncwarp();
@@ -588,10 +589,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
                     choose_exactly<T, LANES, C>(tile, BIAS ? bias : nullptr, wl, n, k, chosen);
                 } else {
                     for (uint32_t j = lane; j < m; j += LANES) {
-                        const uint64_t mine = list[j];
+                        const uint64_t mine = full(list[j]);
                         uint32_t rank = 0;
-                        for (uint32_t i = 0; i < m; ++i) rank += list[i] > mine;
-                        if (mine && rank < k) chosen[rank] = ~kMask | (uint32_t(mine) & kMask);
+                        for (uint32_t i = 0; i < m; ++i) rank += full(list[i]) > mine;
+                        if (mine && rank < k) chosen[rank] = list[j];
                     }
                     __syncwarp();
                 }
