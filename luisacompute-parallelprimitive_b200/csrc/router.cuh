@@ -30,13 +30,12 @@
 // more than kMoreRounds agree is the row chosen again from the full values.
 //
 // What has to move is a row's logits once (and, backward, its gradient) and 8
-// bytes a choice.  131072 rows of 256 bfloat16 logits, top 8: forward 46 us, of
+// bytes a choice.  131072 rows of 256 bfloat16 logits, top 8: forward 45 us, of
 // which the copy rate would take 11.8, gradient 42 us (22.2).  Both are bound by
 // instructions: forward issues 895 per four rows (62 % of the issue slots, the
 // integer pipe at 56 %), about 170 of them the lanes' heads and 180 the rounds;
 // the gradient 788 (58 %, the exponential unit at 43 % with sigmoid scores).
-// Rows of 32-bit logits move twice the bytes for the same work: 65536 x 256,
-// gradient 26 us (84 % of the copy rate).
+// 65536 rows of 256 32-bit logits: forward 37 us (11.1), gradient 26 us (21.6).
 #pragma once
 
 #include "model.cuh"
@@ -487,6 +486,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
         }
         copies_commit();
         copies_wait();
+        if (!kExact) __syncwarp();  // a chosen logit may be another lane's copy
 
         uint32_t word[C], low = 0;
         if constexpr (kExact) {
@@ -816,6 +816,7 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
         up0 = __shfl_sync(~0u, up0, lead);
         const float c = p.weight_scale, base = kJoined ? fmaf(c, up0, pull0) : pull0;
 
+        __syncwarp();
         float x[C], top = 0.f;
         L::unpack(tile, wl, x);
         if (!SIGMOID) top = fmaxf(row_all<LANES>(lane_max(x), Max{}), chosen_top);
