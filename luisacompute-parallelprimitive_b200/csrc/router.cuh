@@ -48,8 +48,8 @@ using namespace lcpp::model;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / kWarp;
 constexpr float kNegInf = -INFINITY;
-// Where a row's sigmoids are all below this, each equals exp(logit) to 32 bits
-// and their sum may underflow: shares are taken as a softmax instead.
+// Where the sum of a row's sigmoids is below this, each equals exp(logit) to 32
+// bits and the sum may underflow: shares are taken as a softmax instead.
 constexpr float kDeepSigmoid = 1e-20f;
 constexpr float kDeepLogit = -60.f;  // the same for the largest chosen logit
 constexpr int kHeads = 4;
@@ -328,7 +328,7 @@ __device__ __forceinline__ float softmax_scores(float (&x)[C], const Reference& 
     return z[0] + z[1];
 }
 
-// The same for sigmoids; where `deep`, exp(x - top).
+// The scores of sigmoids; where `deep`, exp(x - top).
 template <int C>
 __device__ __forceinline__ float sigmoid_scores(float (&x)[C], float top, bool deep)
 {
@@ -530,29 +530,31 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
         const uint32_t lane_bits = L::lane_bits(lane);
         uint32_t picked[kPlaces + 1], best = 0, handed = 0;
         bool unsure = false, tie = false;
-        // the row's largest head; `refill`: a lane may have handed out all it had
-        const auto hand_out = [&](bool refill) {
+        // the row's largest head
+        const auto hand_out = [&] {
             const uint32_t mine = head[0] + lane_bits, next = row_all<LANES>(mine, Max{});
             const bool out = mine == next;
 #pragma unroll
             for (int h = 0; h + 1 < kHeads; ++h) head[h] = out ? head[h + 1] : head[h];
             if (out) head[kHeads - 1] = 0;
             handed += out;
-            if (refill) {
-                const bool empty = head[0] == 0 && handed < C;
-                if (__any_sync(~0u, empty)) {
-                    const uint32_t more = largest_below(word, tail);
-                    if (empty) head[0] = tail = more;
-                }
-            }
             return next;
+        };
+        // a head for lanes that have handed out all they had found
+        const auto refill = [&] {
+            const bool empty = head[0] == 0 && handed < C;
+            if (__any_sync(~0u, empty)) {
+                const uint32_t more = largest_below(word, tail);
+                if (empty) head[0] = tail = more;
+            }
         };
 #pragma unroll
         for (int s = 0; s < kPlaces + !kExact; ++s) {
             picked[s] = 0;
             if (uint32_t(s * LANES) >= rounds) break;
             for (uint32_t i = 0, j = s * LANES; i < LANES && j < rounds; ++i, ++j) {
-                const uint32_t next = hand_out(j + 1 < rounds && j + 1 >= kHeads);
+                if (j >= kHeads) refill();
+                const uint32_t next = hand_out();
                 tie = next >= kLowest && (next & ~kMask) == (best & ~kMask);
                 unsure |= tie;
                 best = next;
@@ -578,7 +580,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
                     if (uint32_t(s * LANES + lane) < rounds) list[s * LANES + lane] = picked[s];
                 uint32_t m = rounds;
                 for (; m < min(n, k + kMoreRounds) && __any_sync(~0u, tie); ++m) {
-                    const uint32_t next = hand_out(true);
+                    refill();
+                    const uint32_t next = hand_out();
                     tie = next >= kLowest && (next & ~kMask) == (best & ~kMask);
                     best = next;
                     if (lane == 0) list[m] = next;

@@ -323,6 +323,15 @@ def test_route_ties_go_to_the_lower_expert(lcpp, kind):
             check_route(lcpp, cuda(x).to(TYPES[kind]), min(e, 9), ref.SOFTMAX, True, b)
 
 
+@pytest.mark.parametrize("e,k", [(39, 23), (213, 16), (256, 8), (256, 1)])
+def test_route_crowded_logits(lcpp, e, k):
+    """Logits far from zero that lie close together, so that many words agree in what they keep of them, also
+    past the last choice and on a lane that has handed out all it had found."""
+    rng = np.random.default_rng(e * k)
+    x = (rng.standard_normal((20_000, e)) * 0.01 + rng.choice([-30.0, 50.0], (20_000, 1))).astype(np.float32)
+    check_route(lcpp, cuda(x), k, ref.SIGMOID, True)
+
+
 @pytest.mark.parametrize("e,k", [(8, 8), (60, 6), (256, 8), (512, 32), (1024, 31)])
 def test_route_near_ties(lcpp, e, k):
     """32-bit logits in clusters that agree in all but their last bits: of two, of a few, of more than are
