@@ -328,6 +328,34 @@ __device__ __forceinline__ float softmax_scores(float (&x)[C], const Reference& 
     return z[0] + z[1];
 }
 
+// For the gradient: x becomes the sigmoid's slope s (1 - s), whose second factor
+// is e s of e = exp(-x), for near 1 a subtraction would leave nothing of it; where
+// `deep`, the score exp(x - top), which is its own slope.  Returns the lane's sum
+// of scores and adds that of s (pull - base) to `mean`.
+constexpr float kLargestPart = 3e38f;  // s is 0 there: keeps infinity times that 0
+template <typename L, int C>
+__device__ __forceinline__ float sigmoid_slopes(float (&x)[C], const float* pull, int lane, float base, float top,
+                                                bool deep, float& mean)
+{
+    float z[2] = {0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < C; q += 4) {
+        const float4 h4 = shared_load4(pull + L::expert(lane, q));
+        const float h[4] = {h4.x, h4.y, h4.z, h4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float part = exp_of(deep ? x[q + i] - top : -x[q + i]);
+            float s;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + part));
+            x[q + i] = deep ? part : fminf(part, kLargestPart) * s * s;
+            if (deep) s = part;
+            z[i % 2] += s;
+            mean = fmaf(s, h[i] - base, mean);
+        }
+    }
+    return z[0] + z[1];
+}
+
 // The scores of sigmoids; where `deep`, exp(x - top).
 template <int C>
 __device__ __forceinline__ float sigmoid_scores(float (&x)[C], float top, bool deep)
@@ -823,8 +851,22 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
         float x[C], top = 0.f;
         L::unpack(tile, wl, x);
         if (!SIGMOID) top = fmaxf(row_all<LANES>(lane_max(x), Max{}), chosen_top);
+        // the scores' sum, and the mean slope before it is divided by that
         const Reference ref(top);
-        float sum = SIGMOID ? sigmoid_scores(x, 0.f, false) : softmax_scores(x, ref), score[kPlaces];
+        float mean = 0.f, score[kPlaces], sum;
+        if constexpr (SIGMOID) {
+            sum = sigmoid_slopes<L>(x, pull, lane, base, 0.f, false, mean);
+        } else {
+            sum = softmax_scores(x, ref);
+#pragma unroll
+            for (int q = 0; q < C; q += 4) {
+                const float4 h = shared_load4(pull + L::expert(lane, q));
+                mean = fmaf(x[q], h.x - base, mean);
+                mean = fmaf(x[q + 1], h.y - base, mean);
+                mean = fmaf(x[q + 2], h.z - base, mean);
+                mean = fmaf(x[q + 3], h.w - base, mean);
+            }
+        }
 #pragma unroll
         for (int s = 0; s < kPlaces; ++s) {
             if (uint32_t(s * LANES) >= k) break;
@@ -833,12 +875,13 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
         }
         sum = row_all<LANES>(sum, Add{});
         bool deep = false;
-        if (SIGMOID) {
+        if constexpr (SIGMOID) {
             deep = sum < kDeepSigmoid;
             if (__any_sync(~0u, deep)) {
                 L::unpack(tile, wl, x);
                 top = row_all<LANES>(fmaxf(lane_max(x), lane_top), Max{});
-                sum = sigmoid_scores(x, top, deep);
+                mean = 0.f;
+                sum = sigmoid_slopes<L>(x, pull, lane, base, top, deep, mean);
 #pragma unroll
                 for (int s = 0; s < kPlaces; ++s) {
                     if (uint32_t(s * LANES) >= k) break;
@@ -850,16 +893,8 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
         }
         const float inv = __fdividef(1.f, sum);
 
-        // the mean slope; a chosen expert's slope of the loss (and, joined, of its weight)
-        float mean = 0.f, slope[kPlaces];
-#pragma unroll
-        for (int q = 0; q < C; q += 4) {
-            const float4 h = shared_load4(pull + L::expert(lane, q));
-            mean = fmaf(x[q], h.x - base, mean);
-            mean = fmaf(x[q + 1], h.y - base, mean);
-            mean = fmaf(x[q + 2], h.z - base, mean);
-            mean = fmaf(x[q + 3], h.w - base, mean);
-        }
+        // a chosen expert's slope of the loss (and, joined, of its weight)
+        float slope[kPlaces];
         float weights = 0.f, dot = 0.f, share[kPlaces];  // of renormalised weights: sum r, sum r (g - g0)
 #pragma unroll
         for (int s = 0; s < kPlaces; ++s) {
@@ -883,7 +918,6 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
             dot = row_all<LANES>(dot, Add{});
         }
 
-        const float rest = base + mean;
 #pragma unroll
         for (int v = 0; v < L::kVecs; ++v) {
             const uint32_t e0 = L::expert(lane, v * L::kV);
@@ -893,11 +927,7 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
                 const float4 h4 = shared_load4(pull + e0 + q);
                 const float h[4] = {h4.x, h4.y, h4.z, h4.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float s = x[v * L::kV + q + i];
-                    g[q + i] = s * inv * (h[i] - rest);
-                    if (SIGMOID && !deep) g[q + i] = fmaf(-s, g[q + i], g[q + i]);
-                }
+                for (int i = 0; i < 4; ++i) g[q + i] = x[v * L::kV + q + i] * inv * (h[i] - (base + mean));
             }
             uint4 raw = Vec<T>::pack(g);
             if (!live) raw = uint4{0, 0, 0, 0};

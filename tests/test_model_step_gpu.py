@@ -332,6 +332,17 @@ def test_route_crowded_logits(lcpp, e, k):
     check_route(lcpp, cuda(x), k, ref.SIGMOID, True)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_saturated_sigmoids(lcpp, kind, renormalize):
+    """Sigmoids so near 1 that 1 - s has to be computed by itself."""
+    rng = np.random.default_rng(17)
+    x = (rng.standard_normal((200, 30)) * 6 + 22).astype(np.float32)
+    logits = cuda(x).to(TYPES[kind])
+    chosen = check_route(lcpp, logits, 3, ref.SIGMOID, renormalize)
+    check_route_grad(lcpp, logits, kind, 3, ref.SIGMOID, renormalize, chosen, rng)
+
+
 @pytest.mark.parametrize("e,k", [(8, 8), (60, 6), (256, 8), (512, 32), (1024, 31)])
 def test_route_near_ties(lcpp, e, k):
     """32-bit logits in clusters that agree in all but their last bits: of two, of a few, of more than are
