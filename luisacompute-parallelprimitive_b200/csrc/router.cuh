@@ -927,7 +927,7 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
                 const float4 h4 = shared_load4(pull + e0 + q);
                 const float h[4] = {h4.x, h4.y, h4.z, h4.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) g[q + i] = x[v * L::kV + q + i] * inv * (h[i] - (base + mean));
+                for (int i = 0; i < 4; ++i) g[q + i] = x[v * L::kV + q + i] * inv * ((h[i] - base) - mean);
             }
             uint4 raw = Vec<T>::pack(g);
             if (!live) raw = uint4{0, 0, 0, 0};

@@ -343,6 +343,18 @@ def test_route_saturated_sigmoids(lcpp, kind, renormalize):
     check_route_grad(lcpp, logits, kind, 3, ref.SIGMOID, renormalize, chosen, rng)
 
 
+@pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
+def test_route_grad_of_equal_counts(lcpp, score):
+    """Two experts with the same count share nearly all of a row: what its gradient is made of comes from the
+    others' small shares, and is far below the slope that the two have in common."""
+    x = np.full((200, 8), -42.0, np.float32)
+    x[:180, :2] = -30.5
+    x[:90, 0] = x[90:180, 1] = x[180:, 2] = -30.0
+    logits = cuda(x)
+    chosen = check_route(lcpp, logits, 1, score, True)
+    check_route_grad(lcpp, logits, "f32", 1, score, True, chosen, np.random.default_rng(3))
+
+
 @pytest.mark.parametrize("e,k", [(8, 8), (60, 6), (256, 8), (512, 32), (1024, 31)])
 def test_route_near_ties(lcpp, e, k):
     """32-bit logits in clusters that agree in all but their last bits: of two, of a few, of more than are
