@@ -900,7 +900,7 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
         for (int s = 0; s < kPlaces; ++s) {
             if (uint32_t(s * LANES) >= k) break;
             slope[s] = share[s] = 0.f;
-            up[s] -= up0;
+            if (kJoined || RENORM) up[s] -= up0;
             if (id[s] < n) {
                 slope[s] = pull[id[s]] - pull0;
                 if (kJoined) slope[s] = fmaf(c, up[s], slope[s]);
@@ -952,7 +952,7 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
                 const float part = __fdividef(share[s], weights);
                 d = fmaf(c * flat * part, up[s] - __fdividef(dot, weights), d);
             } else if (SIGMOID) {
-                d = fmaf(c * (up[s] + up0) * flat, sigmoid(value[s]), d);
+                d = fmaf(c * up[s] * flat, sigmoid(value[s]), d);
             }
             out[id[s]] = from_float<T>(d);
         }

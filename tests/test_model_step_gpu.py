@@ -343,6 +343,20 @@ def test_route_saturated_sigmoids(lcpp, kind, renormalize):
     check_route_grad(lcpp, logits, kind, 3, ref.SIGMOID, renormalize, chosen, rng)
 
 
+def test_route_grad_of_small_upstream(lcpp):
+    """A small upstream gradient beside a large one whose weight is saturated keeps its digits."""
+    x = np.tile(np.array([30.0, 0.0, -3.0, -4.0], np.float32), (40, 1))
+    g = np.tile(np.array([1.0, 1e-6], np.float32), (40, 1))
+    logits = cuda(x)
+    _, experts, counts, routed, _ = check_route(lcpp, logits, 2, ref.SIGMOID, False)
+    want = ref.route_grad(host64(logits), host(experts), host(counts), 40, g.astype(np.float64), 0.0, ref.SIGMOID, False,
+                          SCALE, COEF)
+    out = torch.empty_like(logits)
+    lcpp.DeviceRouter().Backward(logits, experts, counts, routed, cuda(g), None, out, 40, 4, 2, ref.SIGMOID, False, SCALE,
+                                 COEF)
+    assert (np.abs(host64(out) - want) <= 2e-5 * np.abs(want).max(1, keepdims=True)).all()
+
+
 @pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
 def test_route_grad_of_equal_counts(lcpp, score):
     """Two experts with the same count share nearly all of a row: what its gradient is made of comes from the
