@@ -278,11 +278,51 @@ __device__ __forceinline__ float exp2_of(float x)
 }
 __device__ __forceinline__ float exp_of(float x) { return exp2_of(x * kLog2E); }
 
-__device__ __forceinline__ float sigmoid(float x)
+__device__ __forceinline__ float reciprocal(float x)
 {
     float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + exp_of(-x)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+
+__device__ __forceinline__ float sigmoid(float x)
+{
+    return reciprocal(1.f + exp_of(-x));
+}
+
+// Two sums or products in one instruction.
+__device__ __forceinline__ float2 both(float x) { return {x, x}; }
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+template <int C>
+__device__ __forceinline__ float2 pair_of(const float (&x)[C], int i)
+{
+    return {x[i], x[i + 1]};
 }
 
 template <int C>
@@ -315,58 +355,78 @@ struct Reference {
 template <int C>
 __device__ __forceinline__ float softmax_scores(float (&x)[C], const Reference& ref)
 {
-    float z[2] = {0.f, 0.f};
+    float2 z = both(0.f);
     if (ref.any_wide) {
 #pragma unroll
         for (int i = 0; i < C; ++i) x[i] = ref.score(x[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < C; ++i) x[i] = exp2_of(fmaf(x[i], kLog2E, ref.scaled));
+        for (int i = 0; i < C; i += 2) {
+            const float2 at = fma2(pair_of(x, i), both(kLog2E), both(ref.scaled));
+            x[i] = exp2_of(at.x);
+            x[i + 1] = exp2_of(at.y);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < C; ++i) z[i % 2] += x[i];
-    return z[0] + z[1];
+    for (int i = 0; i < C; i += 2) z = add2(z, pair_of(x, i));
+    return z.x + z.y;
+}
+
+// exp(-x) of two logits; where `deep`, exp(x - top).
+template <bool DEEP>
+__device__ __forceinline__ float2 two_parts(float2 x, float top, bool deep)
+{
+    if (DEEP) x = add2(x, both(deep ? -top : 0.f));
+    x = mul2(x, both(DEEP && deep ? kLog2E : -kLog2E));
+    return {exp2_of(x.x), exp2_of(x.y)};
 }
 
 // For the gradient: x becomes the sigmoid's slope s (1 - s), whose second factor
 // is e s of e = exp(-x), for near 1 a subtraction would leave nothing of it; where
 // `deep`, the score exp(x - top), which is its own slope.  Returns the lane's sum
-// of scores and adds that of s (pull - base) to `mean`.
+// of scores, `mean` that of s (pull - base).
 constexpr float kLargestPart = 3e38f;  // s is 0 there: keeps infinity times that 0
-template <typename L, int C>
+template <typename L, bool DEEP, int C>
 __device__ __forceinline__ float sigmoid_slopes(float (&x)[C], const float* pull, int lane, float base, float top,
                                                 bool deep, float& mean)
 {
-    float z[2] = {0.f, 0.f};
+    float2 z = both(0.f), m = both(0.f);
 #pragma unroll
     for (int q = 0; q < C; q += 4) {
-        const float4 h4 = shared_load4(pull + L::expert(lane, q));
-        const float h[4] = {h4.x, h4.y, h4.z, h4.w};
+        const float4 h = shared_load4(pull + L::expert(lane, q));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float part = exp_of(deep ? x[q + i] - top : -x[q + i]);
-            float s;
-            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + part));
-            x[q + i] = deep ? part : fminf(part, kLargestPart) * s * s;
-            if (deep) s = part;
-            z[i % 2] += s;
-            mean = fmaf(s, h[i] - base, mean);
+        for (int i = 0; i < 4; i += 2) {
+            const float2 e = two_parts<DEEP>(pair_of(x, q + i), top, deep), sum = add2(e, both(1.f));
+            float2 s = {reciprocal(sum.x), reciprocal(sum.y)};
+            float2 slope = mul2(mul2({fminf(e.x, kLargestPart), fminf(e.y, kLargestPart)}, s), s);
+            if (DEEP && deep) s = slope = e;
+            x[q + i] = slope.x;
+            x[q + i + 1] = slope.y;
+            z = add2(z, s);
+            m = fma2(s, add2(i ? float2{h.z, h.w} : float2{h.x, h.y}, both(-base)), m);
         }
     }
-    return z[0] + z[1];
+    mean = m.x + m.y;
+    return z.x + z.y;
 }
 
 // The scores of sigmoids; where `deep`, exp(x - top).
-template <int C>
+template <bool DEEP, int C>
 __device__ __forceinline__ float sigmoid_scores(float (&x)[C], float top, bool deep)
 {
-    float z[2] = {0.f, 0.f};
+    float2 z = both(0.f);
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        x[i] = deep ? exp_of(x[i] - top) : sigmoid(x[i]);
-        z[i % 2] += x[i];
+    for (int i = 0; i < C; i += 2) {
+        float2 s = two_parts<DEEP>(pair_of(x, i), top, deep);
+        if (!(DEEP && deep)) {
+            s = add2(s, both(1.f));
+            s = {reciprocal(s.x), reciprocal(s.y)};
+        }
+        x[i] = s.x;
+        x[i + 1] = s.y;
+        z = add2(z, s);
     }
-    return z[0] + z[1];
+    return z.x + z.y;
 }
 
 // What a chosen expert's renormalised weight is made of, `most` being the
@@ -639,25 +699,23 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
         L::unpack(tile, wl, x);
         if (!SIGMOID) top = kExact ? word_value<T>(first) : row_all<LANES>(lane_max(x), Max{});
         const Reference ref(top);
-        float sum = row_all<LANES>(SIGMOID ? sigmoid_scores(x, 0.f, false) : softmax_scores(x, ref), Add{});
+        float sum = row_all<LANES>(SIGMOID ? sigmoid_scores<false>(x, 0.f, false) : softmax_scores(x, ref), Add{});
         if (SIGMOID) {
             const bool deep = sum < kDeepSigmoid;
             if (__any_sync(~0u, deep)) {
                 L::unpack(tile, wl, x);
                 top = row_all<LANES>(lane_max(x), Max{});
-                sum = row_all<LANES>(sigmoid_scores(x, top, deep), Add{});
+                sum = row_all<LANES>(sigmoid_scores<true>(x, top, deep), Add{});
             }
         }
         const float inv = live ? __fdividef(1.f, sum) : 0.f;
         if (live) {
 #pragma unroll
             for (int q = 0; q < C / 4; ++q) {
-                float4 v = sums[q * kWarp];
-                v.x = fmaf(x[4 * q], inv, v.x);
-                v.y = fmaf(x[4 * q + 1], inv, v.y);
-                v.z = fmaf(x[4 * q + 2], inv, v.z);
-                v.w = fmaf(x[4 * q + 3], inv, v.w);
-                sums[q * kWarp] = v;
+                const float4 v = sums[q * kWarp];
+                const float2 low = fma2(pair_of(x, 4 * q), both(inv), {v.x, v.y});
+                const float2 high = fma2(pair_of(x, 4 * q + 2), both(inv), {v.z, v.w});
+                sums[q * kWarp] = {low.x, low.y, high.x, high.y};
             }
         }
 
@@ -855,17 +913,17 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
         const Reference ref(top);
         float mean = 0.f, score[kPlaces], sum;
         if constexpr (SIGMOID) {
-            sum = sigmoid_slopes<L>(x, pull, lane, base, 0.f, false, mean);
+            sum = sigmoid_slopes<L, false>(x, pull, lane, base, 0.f, false, mean);
         } else {
             sum = softmax_scores(x, ref);
+            float2 m = both(0.f);
 #pragma unroll
             for (int q = 0; q < C; q += 4) {
                 const float4 h = shared_load4(pull + L::expert(lane, q));
-                mean = fmaf(x[q], h.x - base, mean);
-                mean = fmaf(x[q + 1], h.y - base, mean);
-                mean = fmaf(x[q + 2], h.z - base, mean);
-                mean = fmaf(x[q + 3], h.w - base, mean);
+                m = fma2(pair_of(x, q), add2({h.x, h.y}, both(-base)), m);
+                m = fma2(pair_of(x, q + 2), add2({h.z, h.w}, both(-base)), m);
             }
+            mean = m.x + m.y;
         }
 #pragma unroll
         for (int s = 0; s < kPlaces; ++s) {
@@ -880,8 +938,7 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
             if (__any_sync(~0u, deep)) {
                 L::unpack(tile, wl, x);
                 top = row_all<LANES>(fmaxf(lane_max(x), lane_top), Max{});
-                mean = 0.f;
-                sum = sigmoid_slopes<L>(x, pull, lane, base, top, deep, mean);
+                sum = sigmoid_slopes<L, true>(x, pull, lane, base, top, deep, mean);
 #pragma unroll
                 for (int s = 0; s < kPlaces; ++s) {
                     if (uint32_t(s * LANES) >= k) break;
@@ -924,10 +981,15 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
             float g[L::kV];
 #pragma unroll
             for (int q = 0; q < L::kV; q += 4) {
-                const float4 h4 = shared_load4(pull + e0 + q);
-                const float h[4] = {h4.x, h4.y, h4.z, h4.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) g[q + i] = x[v * L::kV + q + i] * inv * ((h[i] - base) - mean);
+                const float4 h = shared_load4(pull + e0 + q);
+                const float2 low = add2(add2({h.x, h.y}, both(-base)), both(-mean));
+                const float2 high = add2(add2({h.z, h.w}, both(-base)), both(-mean));
+                const float2 g0 = mul2(mul2(pair_of(x, v * L::kV + q), both(inv)), low);
+                const float2 g1 = mul2(mul2(pair_of(x, v * L::kV + q + 2), both(inv)), high);
+                g[q] = g0.x;
+                g[q + 1] = g0.y;
+                g[q + 2] = g1.x;
+                g[q + 3] = g1.y;
             }
             uint4 raw = Vec<T>::pack(g);
             if (!live) raw = uint4{0, 0, 0, 0};
