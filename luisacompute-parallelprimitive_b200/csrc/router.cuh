@@ -30,11 +30,11 @@
 // more than kMoreRounds agree is the row chosen again from the full values.
 //
 // What has to move is a row's logits once (and, backward, its gradient) and 8
-// bytes a choice.  131072 rows of 256 bfloat16 logits, top 8: forward 45 us, of
+// bytes a choice.  131072 rows of 256 bfloat16 logits, top 8: forward 44 us, of
 // which the copy rate would take 11.8, gradient 42 us (22.2).  Both are bound by
-// instructions: forward issues 895 per four rows (62 % of the issue slots, the
-// integer pipe at 56 %), about 170 of them the lanes' heads and 180 the rounds;
-// the gradient 788 (58 %, the exponential unit at 43 % with sigmoid scores).
+// instructions: forward issues 826 per four rows (59 % of the issue slots, the
+// integer pipe at 57 %), about 170 of them the lanes' heads and 180 the rounds;
+// the gradient 745 (58 %, the exponential unit at 46 % with sigmoid scores).
 // 65536 rows of 256 32-bit logits: forward 37 us (11.1), gradient 26 us (21.6).
 #pragma once
 
@@ -290,7 +290,9 @@ __device__ __forceinline__ float sigmoid(float x)
     return reciprocal(1.f + exp_of(-x));
 }
 
-// Two sums or products in one instruction.
+// Two sums or products in one instruction: forward 895 -> 826 instructions per
+// four rows of 256 (45 -> 44 us), sigmoid gradient 900 -> 745 (43 -> 42 us; 128
+// experts 13.9 -> 12.9 us).
 __device__ __forceinline__ float2 both(float x) { return {x, x}; }
 __device__ __forceinline__ float2 add2(float2 a, float2 b)
 {
@@ -1073,7 +1075,7 @@ lcpp_status backward_shape(const BackParams& p, bool sigmoid, cudaStream_t s)
 
 // The smallest shape that holds the experts, of those that measured best
 // (bfloat16; lanes x elements): few lanes share a round's shuffles among more
-// rows, many elements take registers.  131072 rows of 256: 8 x 32 45 us, 16 x 16
+// rows, many elements take registers.  131072 rows of 256: 8 x 32 44 us, 16 x 16
 // 64, 4 x 64 62; of 64: 4 x 16 20, 8 x 8 23, 8 x 16 29; of 8: 1 x 8 8, 4 x 8 12.
 template <typename T>
 lcpp_status forward_rows(const Params& p, bool sigmoid, cudaStream_t s)
@@ -1090,8 +1092,8 @@ lcpp_status forward_rows(const Params& p, bool sigmoid, cudaStream_t s)
 }
 
 // The same for the gradient.  131072 rows of 256: 8 x 32 42 us, 16 x 16 47, 32 x 8
-// 61; of 64: 8 x 8 18, 4 x 16 17 (but 47 against 29 for 61 experts, whose rows
-// allow no wide access), 8 x 16 23; 65536 of 512: 16 x 32 and 32 x 16 38.
+// 61; of 64: 8 x 8 17, 4 x 16 17 (but 47 against 29 for 61 experts, whose rows
+// allow no wide access), 8 x 16 23; 65536 of 512: 16 x 32 36, 32 x 16 38.
 template <typename T>
 lcpp_status backward_rows(const BackParams& p, bool sigmoid, cudaStream_t s)
 {
