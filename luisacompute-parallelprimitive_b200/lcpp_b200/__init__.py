@@ -972,10 +972,12 @@ class DeviceBlockTable:
             raise LcppError(ERR_INVALID_ARG, "d_block_table: int32 [num_requests, width], columns adjacent")
         if not d_block_table.is_cuda:
             raise LcppError(ERR_INVALID_ARG, "d_block_table: a CUDA tensor")
-        width = d_block_table.shape[1]
+        held, width = d_block_table.shape
+        # as it is, for the library to refuse rows that share memory; one row's stride means nothing
+        stride = d_block_table.stride(0) if held > 1 else max(d_block_table.stride(0), width)
         args = BlockTableArgs(
             _flat(d_context_lens, i32, n, "d_context_lens"), _flat(d_new_lens, i32, n, "d_new_lens"),
-            d_block_table.data_ptr(), max(d_block_table.stride(0), width), width, n, block_size,
+            d_block_table.data_ptr(), stride, width, n, block_size,
             d_free_blocks.numel(), _flat(d_free_blocks, i32, 0, "d_free_blocks"),
             _flat(d_free_used, i32, 1, "d_free_used"), _flat(d_free_used_out, i32, 1, "d_free_used_out"),
             _flat(d_seq_lens_out, i32, n, "d_seq_lens_out"),
