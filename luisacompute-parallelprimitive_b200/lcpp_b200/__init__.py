@@ -972,9 +972,9 @@ class DeviceBlockTable:
             raise LcppError(ERR_INVALID_ARG, "d_block_table: int32 [num_requests, width], columns adjacent")
         if not d_block_table.is_cuda:
             raise LcppError(ERR_INVALID_ARG, "d_block_table: a CUDA tensor")
-        held, width = d_block_table.shape
-        # as it is, for the library to refuse rows that share memory; one row's stride means nothing
-        stride = d_block_table.stride(0) if held > 1 else max(d_block_table.stride(0), width)
+        width = d_block_table.shape[1]
+        # as it is, for the library to refuse rows that share memory; of one request only its row counts
+        stride = d_block_table.stride(0) if n > 1 else max(d_block_table.stride(0), width)
         args = BlockTableArgs(
             _flat(d_context_lens, i32, n, "d_context_lens"), _flat(d_new_lens, i32, n, "d_new_lens"),
             d_block_table.data_ptr(), stride, width, n, block_size,

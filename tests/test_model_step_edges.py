@@ -46,5 +46,6 @@ def test_table_rows_keep_their_stride(lcpp, monkeypatch):
     assert table_stride(lcpp, monkeypatch, torch.zeros(5, 8, dtype=i32)[:, :6], 5) == (8, 6)
     assert table_stride(lcpp, monkeypatch, torch.zeros(1, 8, dtype=i32).expand(5, 8), 5) == (0, 8)
     assert table_stride(lcpp, monkeypatch, torch.zeros(40, dtype=i32).as_strided((5, 8), (3, 1)), 5) == (3, 8)
-    # the stride of a single row means nothing
+    # one request takes one row, whatever follows it
+    assert table_stride(lcpp, monkeypatch, torch.zeros(1, 8, dtype=i32).expand(5, 8), 1) == (8, 8)
     assert table_stride(lcpp, monkeypatch, torch.zeros(8, dtype=i32).as_strided((1, 8), (0, 1)), 1) == (8, 8)
