@@ -66,9 +66,9 @@ lcpp_status lcpp_block_table_temp_bytes(uint64_t num_requests, uint64_t max_toke
  * page are still served; those that need one are refused too when free_blocks
  * is what ended.  A negative page id in the row gives slot -1.
  *
- * free_used_out and seq_lens_out must not overlap the inputs: a step's outputs
- * are the next one's inputs through two sets of buffers.  Zero requests give
- * one start, no pages and marked entries. */
+ * The outputs, temp storage and the table must not overlap one another or the
+ * inputs: a step's outputs are the next one's inputs through two sets of
+ * buffers.  Zero requests give one start, no pages and marked entries. */
 lcpp_status lcpp_block_table_extend(void* temp, size_t temp_bytes, const lcpp_block_table_args* args,
                                     lcpp_stream_t stream);
 

@@ -432,15 +432,22 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_block_table_args* a, c
                            a->free_used_out, a->seq_lens_out,  a->query_starts_out, a->positions_out, a->token_request_out};
     for (const void* w : words)
         if (misaligned(w, 4)) return LCPP_ERR_INVALID_ARG;
-    // blocks read the inputs while one of them writes these
-    const struct { const void* p; uint64_t bytes; } outputs[] = {{a->free_used_out, 4}, {a->seq_lens_out, n * 4}},
-        inputs[] = {{a->context_lens, n * 4}, {a->new_lens, n * 4}, {a->free_used, 4},
-                    {a->free_blocks, uint64_t(a->num_free) * 4}};
-    for (const auto& o : outputs)
-        for (const auto& i : inputs)
-            if (overlap(o.p, o.bytes, i.p, i.bytes)) return LCPP_ERR_INVALID_ARG;
     const Layout l = layout(n);
     if (temp_bytes < l.bytes) return LCPP_ERR_TEMP_TOO_SMALL;
+    const Array arrays[] = {{a->context_lens, n * 4, false},
+                            {a->new_lens, n * 4, false},
+                            {a->free_blocks, uint64_t(a->num_free) * 4, false},
+                            {a->free_used, 4, false},
+                            {a->free_used_out, 4, true},
+                            {a->seq_lens_out, n * 4, true},
+                            {a->query_starts_out, (n + 1) * 4, true},
+                            {a->slots_out, a->max_tokens * 8, true},
+                            {a->positions_out, a->max_tokens * 4, true},
+                            {a->token_request_out, a->max_tokens * 4, true},
+                            {temp, l.bytes, true}};
+    if (clash(arrays)) return LCPP_ERR_INVALID_ARG;
+    for (const Array& o : arrays)  // the table is read and written
+        if (overlap_rows(a->block_table, n, a->table_stride, a->table_width, 4, o.p, o.bytes)) return LCPP_ERR_INVALID_ARG;
 
     Params p{};
     p.context = a->context_lens;

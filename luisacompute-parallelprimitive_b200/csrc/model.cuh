@@ -33,10 +33,42 @@ inline bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_b
     return a && b && a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
 }
 
+// An array that a call reads or writes.
+struct Array {
+    const void* p;
+    uint64_t bytes;
+    bool written;
+};
+
+// Some two of them, one written, share a byte: blocks read an input while
+// another one writes the outputs, and two outputs hold different things.
+template <size_t N>
+bool clash(const Array (&arrays)[N])
+{
+    for (size_t i = 0; i < N; ++i)
+        for (size_t j = 0; j < i; ++j)
+            if ((arrays[i].written || arrays[j].written) &&
+                overlap(arrays[i].p, arrays[i].bytes, arrays[j].p, arrays[j].bytes))
+                return true;
+    return false;
+}
+
 // Bytes from the first to the last element of `rows` strided rows.
 inline uint64_t span_bytes(uint64_t rows, uint64_t stride, uint64_t columns, int element)
 {
     return rows ? ((rows - 1) * stride + columns) * uint64_t(element) : 0;
+}
+
+// An array has a byte in common with the elements of strided rows; it may lie
+// in what is left between them.
+inline bool overlap_rows(const void* base, uint64_t rows, uint64_t stride, uint64_t columns, int element, const void* a,
+                         uint64_t bytes)
+{
+    if (!overlap(base, span_bytes(rows, stride, columns, element), a, bytes)) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(base), y = reinterpret_cast<uintptr_t>(a);
+    if (rows == 1 || y < x) return true;
+    const uint64_t pitch = stride * uint64_t(element), at = (y - x) % pitch;
+    return at < columns * uint64_t(element) || bytes > pitch - at;
 }
 
 // 16-byte loads and stores need every row to start on a 16-byte boundary.

@@ -49,3 +49,36 @@ def test_table_rows_keep_their_stride(lcpp, monkeypatch):
     # one request takes one row, whatever follows it
     assert table_stride(lcpp, monkeypatch, torch.zeros(1, 8, dtype=i32).expand(5, 8), 1) == (8, 8)
     assert table_stride(lcpp, monkeypatch, torch.zeros(8, dtype=i32).as_strided((1, 8), (0, 1)), 1) == (8, 8)
+
+
+def p(i):
+    return 0x1000000 * (i + 1)  # never dereferenced
+
+
+def test_block_table_refuses_every_overlap(lcpp):
+    """Each output, temp storage and the table over each other and over each input, from the front and from
+    behind: another block may still read what one has written."""
+    n, tokens, need = 4, 32, lcpp.DeviceBlockTable.GetTempStorageBytes(4, 32)
+    names = ["context_lens", "new_lens", "block_table", "free_blocks", "free_used", "free_used_out", "seq_lens_out",
+             "query_starts_out", "slots_out", "positions_out", "token_request_out"]
+    sizes = [n * 4, n * 4, n * 8 * 4, 40, 4, 4, n * 4, (n + 1) * 4, tokens * 8, tokens * 4, tokens * 4]
+
+    def extend(temp=p(20), **changes):
+        a = lcpp.BlockTableArgs(p(0), p(1), p(2), 8, 8, n, 16, 10, *(p(i) for i in range(3, 11)), tokens)
+        for name, value in changes.items():
+            setattr(a, name, value)
+        return lcpp.lib().lcpp_block_table_extend(temp, need, a, None)
+
+    place = dict(zip(names, range(11)))
+    for name in ["block_table"] + names[5:]:
+        for other, size in zip(names, sizes):
+            if other == name:
+                continue
+            mine = sizes[place[name]]
+            for at in (p(place[other]) + (size - 1) // 8 * 8, p(place[other]) - (mine - 1) // 8 * 8):
+                assert extend(**{name: at}) == lcpp.ERR_INVALID_ARG, (name, other)
+    for name, size in zip(names, sizes):
+        assert extend(temp=p(place[name])) == lcpp.ERR_INVALID_ARG, name
+    # wider rows: an element, and an array that starts between rows and runs into one
+    for at in (p(2) + 16 * 4, p(2) + 12 * 4):
+        assert extend(table_stride=16, query_starts_out=at) == lcpp.ERR_INVALID_ARG

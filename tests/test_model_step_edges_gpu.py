@@ -1,0 +1,36 @@
+"""Edges of the model-step operators that tests/test_model_step_gpu.py does not reach, against the same 64-bit
+references and with its tolerances (derived at its top)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import model_step_ref as ref
+from test_model_step_gpu import cuda, host, i32
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+def test_extend_outputs_between_rows(lcpp):
+    """Lengths and counters in the spare columns of the table's own rows: no element is shared."""
+    context, new = np.array([30, 0, 17], np.int32), np.array([3, 20, 0], np.int32)
+    buffer = i32(3, 24)
+    buffer[:, :8] = cuda(np.arange(24, dtype=np.int32).reshape(3, 8))
+    flat = buffer.view(-1)
+    d_context, d_new, seq, starts = flat[8:11], flat[12:15], flat[32:35], flat[36:40]
+    used, free = flat[64:65], np.arange(90, 94, dtype=np.int32)
+    d_context.copy_(cuda(context))
+    d_new.copy_(cuda(new))
+    slots = torch.full((30,), -9, dtype=torch.int64, device="cuda")
+    temp = lcpp.alloc_temp(lcpp.DeviceBlockTable.GetTempStorageBytes(3, 30))
+    lcpp.DeviceBlockTable().Extend(temp, d_context, d_new, buffer[:, :8], cuda(free), None, used, seq, starts, slots,
+                                   None, None, 3, 16)
+    table, want, _, _, want_starts, want_seq, want_used = ref.extend(
+        context, new, np.arange(24, dtype=np.int32).reshape(3, 8), 8, free, 0, 30, 16)
+    np.testing.assert_array_equal(host(buffer)[:, :8], table)
+    np.testing.assert_array_equal(host(slots), want)
+    np.testing.assert_array_equal(host(starts), want_starts)
+    np.testing.assert_array_equal(host(seq), want_seq)
+    assert int(used) == want_used
