@@ -108,7 +108,8 @@ lcpp_status lcpp_router_temp_bytes(uint64_t num_tokens, uint32_t num_experts, si
  *   loss = loss_coef * E * sum_e counts[e] / (top_k T') * mean_t s[t][e] / sum_i s[t][i]
  * (0 when T' is 0).  NaN logits order above +inf, and NaN (and +inf under
  * softmax) go into the token's weights and the loss as the formulas say; a
- * token that is left out passes nothing on. */
+ * token that is left out passes nothing on.  The outputs and temp storage must
+ * not overlap one another or the inputs. */
 lcpp_status lcpp_router_forward(void* temp, size_t temp_bytes, const void* d_logits, uint64_t logits_stride,
                                 lcpp_dtype logits_dtype, const float* d_bias, const int32_t* d_token_request,
                                 float* d_weights_out, int32_t* d_experts_out, int32_t* d_counts_out,
@@ -120,7 +121,7 @@ lcpp_status lcpp_router_forward(void* temp, size_t temp_bytes, const void* d_log
  * d_num_routed are forward's outputs; d_grad_weights [num_tokens][top_k] and
  * d_grad_loss [1] may be NULL (zero).  Tokens whose first expert is -1 get
  * zeros.  d_grad_logits_out has the logits' dtype and may be d_logits itself
- * when the strides agree. */
+ * when the strides agree; else it must not overlap the inputs. */
 lcpp_status lcpp_router_backward(const void* d_logits, uint64_t logits_stride, lcpp_dtype logits_dtype,
                                  const int32_t* d_experts, const int32_t* d_counts, const int32_t* d_num_routed,
                                  const float* d_grad_weights, const float* d_grad_loss, void* d_grad_logits_out,

@@ -56,6 +56,13 @@ lcpp_status forward(void* temp, size_t temp_bytes, const void* logits, uint64_t 
         if (misaligned(w, 4)) return LCPP_ERR_INVALID_ARG;
     if (misaligned(logits, size)) return LCPP_ERR_INVALID_ARG;
     if (temp_bytes < temp_size(c->num_experts)) return LCPP_ERR_TEMP_TOO_SMALL;
+    const uint64_t pairs = tokens * c->top_k, n = c->num_experts;
+    const Array arrays[] = {{bias, n * 4, false},     {token_request, tokens * 4, false}, {weights, pairs * 4, true},
+                            {experts, pairs * 4, true}, {counts, n * 4, true},            {num_routed, 4, true},
+                            {loss, 4, true},            {temp, temp_size(uint32_t(n)), true}};
+    if (clash(arrays)) return LCPP_ERR_INVALID_ARG;
+    for (const Array& o : arrays)
+        if (o.written && overlap_rows(logits, tokens, stride, n, size, o.p, o.bytes)) return LCPP_ERR_INVALID_ARG;
 
     unsigned char* t = static_cast<unsigned char*>(temp);
     router::Params p{};
@@ -108,6 +115,12 @@ lcpp_status backward(const void* logits, uint64_t stride, lcpp_dtype dtype, cons
     if (!in_place && overlap(logits, span_bytes(tokens, stride, c->num_experts, size), grad_logits,
                              span_bytes(tokens, grad_stride, c->num_experts, size)))
         return LCPP_ERR_INVALID_ARG;
+    const uint64_t pairs = tokens * c->top_k;
+    const Array inputs[] = {{experts, pairs * 4, false}, {counts, uint64_t(c->num_experts) * 4, false},
+                            {num_routed, 4, false},      {grad_weights, pairs * 4, false},
+                            {grad_loss, 4, false}};
+    for (const Array& i : inputs)
+        if (overlap_rows(grad_logits, tokens, grad_stride, c->num_experts, size, i.p, i.bytes)) return LCPP_ERR_INVALID_ARG;
 
     router::BackParams p{};
     p.logits = logits;

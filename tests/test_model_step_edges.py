@@ -82,3 +82,38 @@ def test_block_table_refuses_every_overlap(lcpp):
     # wider rows: an element, and an array that starts between rows and runs into one
     for at in (p(2) + 16 * 4, p(2) + 12 * 4):
         assert extend(table_stride=16, query_starts_out=at) == lcpp.ERR_INVALID_ARG
+
+
+def overlaps(names, sizes, place, written, size_of):
+    """(name, address) of each written array put over the last and the first bytes of every other one."""
+    for name in written:
+        for other, size in zip(names, sizes):
+            if other != name:
+                yield name, place[other] + (size - 1) // 4 * 4
+                yield name, place[other] - (size_of[name] - 1) // 4 * 4
+
+
+def test_router_refuses_every_overlap(lcpp):
+    t, e, k = 10, 16, 4
+    cfg, lib = lcpp.RouterConfig(e, k, 0, 1, 1.0, 1.0), lcpp.lib()
+    names = ["logits", "bias", "mask", "weights", "experts", "counts", "routed", "loss"]
+    sizes = [t * e * 4, e * 4, t * 4, t * k * 4, t * k * 4, e * 4, 4, 4]
+    place, size_of = {n: p(i) for i, n in enumerate(names)}, dict(zip(names, sizes))
+
+    def forward(temp=p(20), stride=e, **changes):
+        a = {**place, **changes}
+        return lib.lcpp_router_forward(temp, 1 << 16, a["logits"], stride, 2, *(a[n] for n in names[1:]), t, cfg, None)
+
+    for name, at in overlaps(names, sizes, place, names[3:], size_of):
+        assert forward(**{name: at}) == lcpp.ERR_INVALID_ARG, name
+    for name in names:
+        assert forward(temp=place[name]) == lcpp.ERR_INVALID_ARG, name
+    # logits in wider rows: an array that runs from the spare columns into a row
+    assert forward(stride=24, experts=place["logits"] + 20 * 4) == lcpp.ERR_INVALID_ARG
+
+    names = ["experts", "counts", "routed", "grad_weights", "grad_loss", "out"]
+    sizes = [t * k * 4, e * 4, 4, t * k * 4, 4, t * e * 4]
+    place, size_of = {n: p(i) for i, n in enumerate(names)}, dict(zip(names, sizes))
+    for _, at in overlaps(names, sizes, place, ["out"], size_of):
+        assert lib.lcpp_router_backward(p(20), e, 2, *(place[n] for n in names[:-1]), at, e, t, cfg, None) == \
+            lcpp.ERR_INVALID_ARG
