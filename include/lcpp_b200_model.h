@@ -147,7 +147,8 @@ lcpp_status lcpp_dispatch_max_rows(uint64_t num_tokens, uint32_t top_k, uint32_t
  * lie past the last one.  Pairs whose expert is not in [0, num_experts), or
  * whose row would lie past max_rows, get row -1; the starts are not cut off
  * there.  num_tokens * top_k, max_rows and lcpp_dispatch_max_rows' answer stay
- * below 2^31. */
+ * below 2^31.  The outputs of this call and the next three must not overlap one
+ * another, temp storage or the inputs, except where it says so. */
 lcpp_status lcpp_dispatch_plan(void* temp, size_t temp_bytes, const int32_t* d_experts, int32_t* d_expert_starts_out,
                                int32_t* d_row_of_out, int32_t* d_pair_of_out, uint64_t num_tokens, uint32_t top_k,
                                uint32_t num_experts, uint32_t row_align, uint64_t max_rows, lcpp_stream_t stream);
@@ -172,7 +173,8 @@ lcpp_status lcpp_dispatch_combine(const void* d_rows, uint64_t rows_stride, cons
  * weights[t][j] * d_grad_out[t], d_grad_weights_out[t][j] = the dot product of
  * d_grad_out[t] and d_rows[row_of(t, j)] (0 without a row).  Padding rows of
  * d_grad_rows_out get zeros, rows past the last segment are not written.
- * d_grad_rows_out may be d_rows itself when the strides agree. */
+ * d_grad_rows_out may be d_rows itself when the strides agree, and
+ * d_grad_weights_out may be d_weights itself. */
 lcpp_status lcpp_dispatch_combine_backward(const void* d_grad_out, uint64_t grad_out_stride, const void* d_rows,
                                            uint64_t rows_stride, const int32_t* d_row_of, const int32_t* d_pair_of,
                                            const int32_t* d_expert_starts, const float* d_weights,

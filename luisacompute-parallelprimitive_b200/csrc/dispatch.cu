@@ -494,11 +494,13 @@ lcpp_status plan(void* temp, size_t temp_bytes, const int32_t* experts, int32_t*
     const void* words[] = {experts, starts, row_of, pair_of};
     for (const void* w : words)
         if (misaligned(w, 4)) return LCPP_ERR_INVALID_ARG;
-    // the pairs are walked twice
-    if (overlap(experts, pairs * 4, row_of, pairs * 4) || overlap(experts, pairs * 4, pair_of, max_rows * 4) ||
-        overlap(experts, pairs * 4, starts, (uint64_t(num_experts) + 1) * 4))
-        return LCPP_ERR_INVALID_ARG;
     if (temp_bytes < plan_bytes(pairs, num_experts)) return LCPP_ERR_TEMP_TOO_SMALL;
+    const Array arrays[] = {{experts, pairs * 4, false},
+                            {starts, (uint64_t(num_experts) + 1) * 4, true},
+                            {row_of, pairs * 4, true},
+                            {pair_of, max_rows * 4, true},
+                            {temp, plan_bytes(pairs, num_experts), true}};
+    if (clash(arrays)) return LCPP_ERR_INVALID_ARG;
     const uint64_t tiles = std::min(kMaxTiles, tiles_for(pairs));
     PlanParams p{};
     p.experts = experts;
@@ -606,6 +608,10 @@ lcpp_status gather(const void* x, uint64_t x_stride, const int32_t* row_of, cons
         return LCPP_ERR_INVALID_ARG;
     if (overlap(x, span_bytes(tokens, x_stride, hidden, size), rows, span_bytes(max_rows, rows_stride, hidden, size)))
         return LCPP_ERR_INVALID_ARG;
+    const Array inputs[] = {{row_of, tokens * top_k * 4, false}, {pair_of, max_rows * 4, false},
+                            {starts, (uint64_t(num_experts) + 1) * 4, false}};
+    for (const Array& i : inputs)
+        if (overlap_rows(rows, max_rows, rows_stride, hidden, size, i.p, i.bytes)) return LCPP_ERR_INVALID_ARG;
     RowParams p{};
     p.x = static_cast<const unsigned char*>(x);
     p.x_pitch = x_stride * size;
@@ -648,6 +654,8 @@ lcpp_status combine(const void* rows, uint64_t rows_stride, const int32_t* row_o
         return LCPP_ERR_INVALID_ARG;
     if (overlap(out, span_bytes(tokens, out_stride, hidden, size), rows, span_bytes(max_rows, rows_stride, hidden, size)))
         return LCPP_ERR_INVALID_ARG;
+    for (const void* i : {static_cast<const void*>(row_of), static_cast<const void*>(weights)})
+        if (overlap_rows(out, tokens, out_stride, hidden, size, i, tokens * top_k * 4)) return LCPP_ERR_INVALID_ARG;
     RowParams p{};
     p.rows = static_cast<const unsigned char*>(rows);
     p.rows_pitch = rows_stride * size;
@@ -706,6 +714,20 @@ lcpp_status combine_backward(const void* grad_out, uint64_t grad_out_stride, con
         return LCPP_ERR_INVALID_ARG;
     if (overlap(grad_out, span_bytes(tokens, grad_out_stride, hidden, size), grad_rows, grad_rows_span))
         return LCPP_ERR_INVALID_ARG;
+    const uint64_t pairs = tokens * top_k;
+    // a token's threads read a weight before they write its gradient, so the two may share their place
+    const Array arrays[] = {{row_of, pairs * 4, false},
+                            {pair_of, max_rows * 4, false},
+                            {starts, (uint64_t(num_experts) + 1) * 4, false},
+                            {weights == grad_weights ? nullptr : weights, pairs * 4, false},
+                            {grad_weights, pairs * 4, true}};
+    if (clash(arrays)) return LCPP_ERR_INVALID_ARG;
+    for (const Array& a : arrays) {
+        if (overlap_rows(grad_rows, max_rows, grad_rows_stride, hidden, size, a.p, a.bytes) ||
+            (a.written && (overlap_rows(grad_out, tokens, grad_out_stride, hidden, size, a.p, a.bytes) ||
+                           overlap_rows(rows, max_rows, rows_stride, hidden, size, a.p, a.bytes))))
+            return LCPP_ERR_INVALID_ARG;
+    }
     RowParams p{};
     p.x = static_cast<const unsigned char*>(grad_out);
     p.x_pitch = grad_out_stride * size;

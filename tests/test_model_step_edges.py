@@ -117,3 +117,40 @@ def test_router_refuses_every_overlap(lcpp):
     for _, at in overlaps(names, sizes, place, ["out"], size_of):
         assert lib.lcpp_router_backward(p(20), e, 2, *(place[n] for n in names[:-1]), at, e, t, cfg, None) == \
             lcpp.ERR_INVALID_ARG
+
+
+def test_dispatch_refuses_every_overlap(lcpp):
+    t, k, e, rows, h, lib, bad = 10, 4, 16, 60, 64, lcpp.lib(), lcpp.ERR_INVALID_ARG
+    sizes_of = {"experts": t * k * 4, "starts": (e + 1) * 4, "row_of": t * k * 4, "pair_of": rows * 4,
+                "x": t * h * 2, "rows": rows * h * 2, "weights": t * k * 4, "out": t * h * 2, "grad_rows": rows * h * 2,
+                "grad_weights": t * k * 4, "grad_out": t * h * 2}
+    place = {n: p(i) for i, n in enumerate(sizes_of)}
+
+    def check(call, names, written):
+        for name, at in overlaps(names, [sizes_of[n] for n in names], place, written, sizes_of):
+            assert call(**{**place, name: at}) == bad, (name, hex(at))
+
+    def plan(experts, starts, row_of, pair_of, temp=p(20), **_):
+        return lib.lcpp_dispatch_plan(temp, 1 << 16, experts, starts, row_of, pair_of, t, k, e, 1, rows, None)
+
+    names = ["experts", "starts", "row_of", "pair_of"]
+    check(plan, names, names[1:])
+    for name in names:
+        assert plan(**place, temp=place[name]) == bad
+
+    def gather(x, row_of, pair_of, starts, rows, **_):
+        return lib.lcpp_dispatch_gather(x, h, row_of, pair_of, starts, rows, h, t, k, e, 60, h, lcpp.BF16, None)
+
+    check(gather, ["x", "row_of", "pair_of", "starts", "rows"], ["rows"])
+
+    def combine(rows, row_of, weights, out, **_):
+        return lib.lcpp_dispatch_combine(rows, h, row_of, weights, out, h, t, k, 60, h, lcpp.BF16, None)
+
+    check(combine, ["rows", "row_of", "weights", "out"], ["out"])
+
+    def back(grad_out, rows, row_of, pair_of, starts, weights, grad_rows, grad_weights, **_):
+        return lib.lcpp_dispatch_combine_backward(grad_out, h, rows, h, row_of, pair_of, starts, weights, grad_rows, h,
+                                                  grad_weights, t, k, e, 60, h, lcpp.BF16, None)
+
+    check(back, ["grad_out", "rows", "row_of", "pair_of", "starts", "weights", "grad_rows", "grad_weights"],
+          ["grad_rows", "grad_weights"])

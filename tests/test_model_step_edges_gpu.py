@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import model_step_ref as ref
-from test_model_step_gpu import cuda, host, i32
+from test_model_step_gpu import check_plan, cuda, host, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,21 @@ def test_extend_outputs_between_rows(lcpp):
     np.testing.assert_array_equal(host(starts), want_starts)
     np.testing.assert_array_equal(host(seq), want_seq)
     assert int(used) == want_used
+
+
+@pytest.mark.parametrize("h", [24, 640, 4104])
+def test_combine_gradient_over_the_weights(lcpp, h):
+    """The weights' gradient takes the weights' place: the same bits as beside them."""
+    rng = np.random.default_rng(h)
+    t, k, e = 70, 9, 12
+    experts = np.argsort(rng.random((t, e)), axis=1)[:, :k].astype(np.int32)
+    experts[rng.random((t, k)) < 0.1] = -1
+    starts, row_of, pair_of = check_plan(lcpp, experts, e, 4)
+    rows, dy = (cuda(rng.standard_normal((n, h)).astype(np.float32)) for n in (pair_of.numel(), t))
+    weights = cuda(rng.random((t, k)).astype(np.float32))
+    got, apart = torch.zeros_like(rows), torch.zeros_like(rows)
+    grad_weights = torch.empty_like(weights)
+    d = lcpp.DeviceDispatch()
+    d.CombineBackward(dy, rows, row_of, pair_of, starts, weights, apart, grad_weights, t, k, e)
+    d.CombineBackward(dy, rows, row_of, pair_of, starts, weights, got, weights, t, k, e)
+    assert torch.equal(weights, grad_weights) and torch.equal(got, apart)
