@@ -1009,7 +1009,7 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
 #pragma unroll
         for (int s = 0; s < kPlaces; ++s) {
             if (uint32_t(s * LANES) >= k) break;
-            if (id[s] >= n) continue;
+            if (id[s] >= n || !live) continue;  // a token without its first choice has zeros, stored above
             const float flat = SIGMOID ? sigmoid(-value[s]) : 1.f;  // 1 - s
             float d = flat * score[s] * inv * (slope[s] - mean);
             if (RENORM) {

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import model_step_ref as ref
-from test_model_step_gpu import check_plan, cuda, host, i32
+from test_model_step_gpu import COEF, SCALE, check_plan, cuda, host, host64, i32, run_route
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,34 @@ def test_combine_gradient_over_the_weights(lcpp, h):
     d.CombineBackward(dy, rows, row_of, pair_of, starts, weights, apart, grad_weights, t, k, e)
     d.CombineBackward(dy, rows, row_of, pair_of, starts, weights, got, weights, t, k, e)
     assert torch.equal(weights, grad_weights) and torch.equal(got, apart)
+
+
+def route_gradient(L, logits, experts, counts, routed, g, dloss, score, renormalize):
+    """(the kernel's gradient, the formula's)"""
+    t, e = logits.shape
+    k = experts.shape[1]
+    out = torch.full_like(logits, -7.0)
+    L.DeviceRouter().Backward(logits, experts, counts, routed, None if g is None else cuda(g),
+                              None if dloss is None else torch.full((1,), dloss, device="cuda"), out, t, e, k, score,
+                              renormalize, SCALE, COEF)
+    g64 = np.zeros((t, k)) if g is None else g.astype(np.float64)
+    want = ref.route_grad(host64(logits), host(experts), host(counts), int(routed), g64, dloss or 0.0, score,
+                          renormalize, SCALE, COEF)
+    return host64(out), want
+
+
+def test_route_grad_of_rows_cut_short(lcpp):
+    """A caller drops choices by setting them to -1: without its first one a token has no gradient, whatever
+    stands behind it; without a later one it has the remaining ones'."""
+    rng = np.random.default_rng(31)
+    t, e, k = 60, 20, 4
+    for score in (ref.SOFTMAX, ref.SIGMOID):
+        for renormalize in (True, False):
+            logits = cuda(rng.standard_normal((t, e)).astype(np.float32))
+            _, experts, counts, routed, _ = run_route(lcpp, logits, k, score, renormalize)
+            experts[:20, 0] = -1
+            experts[10:40, 2] = -1
+            g = rng.standard_normal((t, k)).astype(np.float32)
+            got, want = route_gradient(lcpp, logits, experts, counts, routed, g, 3.0, score, renormalize)
+            assert not got[:20].any()
+            assert (np.abs(got - want) <= 2e-5 * np.abs(want).max(1, keepdims=True)).all()
