@@ -342,14 +342,14 @@ __device__ __forceinline__ float lane_max(const float (&x)[C])
 // used as quotients; past 10^6 the factor itself could overflow.
 struct Reference {
     float top, scaled;
-    bool wide, any_wide;  // this row; any row of the warp
-    __device__ __forceinline__ explicit Reference(float t)
-        : top(t), scaled(t * -kLog2E), wide(!(fabsf(t) < 1e6f)), any_wide(__any_sync(~0u, wide))
+    bool wide, any_rare;  // this row; it or another rarity in any row of the warp
+    __device__ __forceinline__ explicit Reference(float t, bool rare = false)
+        : top(t), scaled(t * -kLog2E), wide(!(fabsf(t) < 1e6f)), any_rare(__any_sync(~0u, wide || rare))
     {
     }
     __device__ __forceinline__ float score(float x) const
     {
-        return any_wide && wide ? exp_of(x - top) : exp2_of(fmaf(x, kLog2E, scaled));
+        return any_rare && wide ? exp_of(x - top) : exp2_of(fmaf(x, kLog2E, scaled));
     }
 };
 
@@ -358,7 +358,7 @@ template <int C>
 __device__ __forceinline__ float softmax_scores(float (&x)[C], const Reference& ref)
 {
     float2 z = both(0.f);
-    if (ref.any_wide) {
+    if (ref.any_rare) {
 #pragma unroll
         for (int i = 0; i < C; ++i) x[i] = ref.score(x[i]);
     } else {
@@ -802,6 +802,38 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
            [&](uint32_t e) { return __ldcg(p.count_total + e); });
 }
 
+// The first lane of the row that says it leads (its first lane, if none does).
+template <int LANES>
+__device__ __forceinline__ int leading_lane(bool leads, int sub)
+{
+    const uint32_t lanes = __ballot_sync(~0u, leads) >> (sub * LANES) & uint32_t((uint64_t(1) << LANES) - 1);
+    return sub * LANES + (lanes ? __ffs(lanes) - 1 : 0);
+}
+
+// The largest logit left in a row's tile and its slope.  Rarely needed, so it
+// reads the tile again instead of keeping it.
+template <typename T, int LANES, int C>
+__device__ __noinline__ float2 leader_left(const uint4* tile, const float* pull, int wl)
+{
+    using L = Tile<T, LANES, C>;
+    const int lane = wl % LANES, sub = wl / LANES;
+    float top = kNegInf, slope = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < C; ++i) {
+        const float x = to_float(reinterpret_cast<const T*>(tile + i / L::kV * kWarp + wl)[i % L::kV]);
+        if (x > top) {
+            top = x;
+            slope = pull[L::expert(lane, i)];
+        }
+    }
+    const float row_top = row_all<LANES>(top, Max{});
+    return {row_top, __shfl_sync(~0u, slope, leading_lane<LANES>(top == row_top, sub))};
+}
+
+// A sigmoid score is at most 1: in a row whose scores add up to this or more, no
+// expert has more than half of the share.
+constexpr float kLedSum = 2.f;
+
 // The logits' gradient.  The chosen experts of a row are taken out of it first
 // (their logits in the tile become -inf): the dense part of a row then has one
 // formula, and each chosen expert's entry is computed by a lane of its own and
@@ -886,10 +918,11 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
             chosen_top = fmaxf(chosen_top, value[s]);
         }
         const bool live = int32_t(__shfl_sync(~0u, id[0], sub * LANES)) >= 0;
-        // The expert with most of the row's share, among the chosen: slopes and
-        // upstream gradients are taken relative to its own, so that what is left
-        // of a row that one expert dominates is not the difference of two
-        // nearly equal numbers.
+        // The expert with most of the row's share: slopes and upstream gradients
+        // are taken relative to its own, so that what is left of a row that one
+        // expert dominates is not the difference of two nearly equal numbers.
+        // Here the one with most of it among the chosen; where a bias kept a
+        // larger one out, that one's slope takes its place below.
         const float lane_top = chosen_top;
         chosen_top = row_all<LANES>(chosen_top, Max{});
         float pull0 = 0.f, up0 = 0.f;
@@ -901,18 +934,36 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
                 up0 = up[s];
             }
         }
-        const uint32_t leads = __ballot_sync(~0u, lane_top == chosen_top) >> (sub * LANES) & uint32_t((uint64_t(1) << LANES) - 1);
-        const int lead = sub * LANES + (leads ? __ffs(leads) - 1 : 0);
+        const int lead = leading_lane<LANES>(lane_top == chosen_top, sub);
         pull0 = __shfl_sync(~0u, pull0, lead);
         up0 = __shfl_sync(~0u, up0, lead);
-        const float c = p.weight_scale, base = kJoined ? fmaf(c, up0, pull0) : pull0;
+        const float c = p.weight_scale;
 
         __syncwarp();
         float x[C], top = 0.f;
         L::unpack(tile, wl, x);
-        if (!SIGMOID) top = fmaxf(row_all<LANES>(lane_max(x), Max{}), chosen_top);
+        bool outside = false;
+        float lane_left = 0.f, left = 0.f;
+        if (!SIGMOID) {
+            lane_left = lane_max(x);
+            left = row_all<LANES>(lane_left, Max{});
+            outside = left > chosen_top;
+            top = fmaxf(left, chosen_top);
+        }
+        const Reference ref(top, outside);
+        if constexpr (!SIGMOID) {
+            if (ref.any_rare) {
+                float slope = 0.f;
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+                    if (x[i] == left) slope = pull[L::expert(lane, i)];
+                slope = __shfl_sync(~0u, slope, leading_lane<LANES>(lane_left == left, sub));
+                if (outside) pull0 = slope;
+                if (kJoined && outside) up0 = 0.f;  // the leader has no weight
+            }
+        }
+        float base = kJoined ? fmaf(c, up0, pull0) : pull0;
         // the scores' sum, and the mean slope before it is divided by that
-        const Reference ref(top);
         float mean = 0.f, score[kPlaces], sum;
         if constexpr (SIGMOID) {
             sum = sigmoid_slopes<L, false>(x, pull, lane, base, 0.f, false, mean);
@@ -937,7 +988,26 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
         bool deep = false;
         if constexpr (SIGMOID) {
             deep = sum < kDeepSigmoid;
-            if (__any_sync(~0u, deep)) {
+            bool again = deep;
+            if (__any_sync(~0u, sum < kLedSum)) {
+                float chosen = 0.f;
+#pragma unroll
+                for (int s = 0; s < kPlaces; ++s) {
+                    if (uint32_t(s * LANES) >= k) break;
+                    chosen += score[s];
+                }
+                chosen = row_all<LANES>(chosen, Add{});
+                // with half of the share among the chosen, none outside has more
+                const bool led = sum < kLedSum && (2.f * chosen < sum || deep);
+                if (__any_sync(~0u, led)) {
+                    const float2 leader = leader_left<T, LANES, C>(tile, pull, wl);
+                    if (led && leader.x > chosen_top) {
+                        base = pull0 = leader.y;
+                        again = true;
+                    }
+                }
+            }
+            if (__any_sync(~0u, again)) {
                 L::unpack(tile, wl, x);
                 top = row_all<LANES>(fmaxf(lane_max(x), lane_top), Max{});
                 sum = sigmoid_slopes<L, true>(x, pull, lane, base, top, deep, mean);

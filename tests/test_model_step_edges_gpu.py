@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import model_step_ref as ref
-from test_model_step_gpu import COEF, SCALE, check_plan, cuda, host, host64, i32, run_route
+from test_model_step_gpu import COEF, ROUND, SCALE, TYPES, check_plan, cuda, host, host64, i32, run_route
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,50 @@ def test_route_grad_of_rows_cut_short(lcpp):
             got, want = route_gradient(lcpp, logits, experts, counts, routed, g, 3.0, score, renormalize)
             assert not got[:20].any()
             assert (np.abs(got - want) <= 2e-5 * np.abs(want).max(1, keepdims=True)).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_grad_of_unchosen_leader(lcpp, kind, score, renormalize):
+    """A bias keeps the expert with nearly all of a row's share out of the choice: what is left of the slopes
+    once its own is taken off is far below them."""
+    for e, k in ((5, 1), (16, 2), (64, 6), (256, 8), (1000, 4)):
+        rng = np.random.default_rng(e)
+        for shift in (0.0, -8.0, -20.0, -60.0):
+            gap = rng.choice([4.0, 8.0, 12.0, 16.0, 20.0, 30.0], 150)
+            x = rng.standard_normal((150, e))
+            off = e // 3
+            x[:, off] = x.max(1) + gap
+            logits = cuda((x + shift).astype(np.float32)).to(TYPES[kind])
+            bias = np.zeros(e, np.float32)
+            bias[off] = -np.inf
+            _, experts, counts, routed, _ = run_route(lcpp, logits, k, score, renormalize, bias)
+            assert (host(experts) != off).all()
+            g = rng.standard_normal((150, k)).astype(np.float32)
+            for up, dloss in ((g, 3.0), (g, None), (None, 3.0)):
+                got, want = route_gradient(lcpp, logits, experts, counts, routed, up, dloss, score, renormalize)
+                bound = 2e-5 * np.abs(want).max(1, keepdims=True) + ROUND[kind][0] * np.abs(want)
+                assert (np.abs(got - want) <= bound).all(), (e, k, shift, up is None, dloss)
+
+
+@pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_grad_beside_led_rows(lcpp, score, renormalize):
+    """A row has the same bits beside rows that need more care (an unchosen leader, tiny sigmoids) as without them."""
+    rng = np.random.default_rng(23)
+    for e, k in ((8, 2), (64, 6), (256, 8)):
+        x = rng.standard_normal((90, e)).astype(np.float32) - 3
+        mixed = x.copy()
+        mixed[::3, 1] = 12.0
+        mixed[1::9] -= 80.0
+        bias = np.zeros(e, np.float32)
+        bias[1] = -np.inf
+        g = rng.standard_normal((90, k)).astype(np.float32)
+        _, experts, counts, routed, _ = run_route(lcpp, cuda(x), k, score, renormalize, bias)
+        chosen = run_route(lcpp, cuda(mixed), k, score, renormalize, bias)[1]
+        plain, _ = route_gradient(lcpp, cuda(x), experts, counts, routed, g, 3.0, score, renormalize)
+        got, _ = route_gradient(lcpp, cuda(mixed), chosen, counts, routed, g, 3.0, score, renormalize)
+        same = (mixed == x).all(1)
+        assert same.sum() >= 50 and torch.equal(chosen[cuda(same)], experts[cuda(same)])
+        np.testing.assert_array_equal(got[same], plain[same])
