@@ -99,8 +99,8 @@ lcpp_status lcpp_router_temp_bytes(uint64_t num_tokens, uint32_t num_experts, si
  * in 32 bits; equal sums go to the lower expert), in descending order, and
  *   weights[t][j] = weight_scale * s[e_j] (/ sum_i s[e_i] when renormalised).
  * The bias (NULL: none) only takes part in the choice; +inf and NaN in it count
- * as the largest finite number.  An expert whose logit or sum is -inf is never
- * chosen; entries left over hold expert -1, weight 0.
+ * as the largest finite number.  An expert whose logit, bias or sum is -inf is
+ * never chosen; entries left over hold expert -1, weight 0.
  * A token with a negative token_request (NULL: none has), or with no expert
  * to choose, is left out: all its entries are -1 and 0, and it takes no part
  * in the counts or the loss.  With T' tokens that took part (d_num_routed_out)

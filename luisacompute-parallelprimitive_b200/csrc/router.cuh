@@ -456,7 +456,7 @@ __device__ __noinline__ void choose_exactly(const uint4* tile, const float* bias
             if (e >= n) continue;
             const float x = to_float(reinterpret_cast<const T*>(tile + i / L::kV * kWarp + wl)[i % L::kV]);
             const float f = bias ? x + bias[e] : x;
-            if (f == kNegInf) continue;
+            if (f == kNegInf || (bias && bias[e] == kNegInf)) continue;
             const uint64_t word = uint64_t(ordered(f)) << 32 | (0xffffffffu - e);
             if (word < last && word > best) best = word;
         }
@@ -541,14 +541,18 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
     __shared__ bool is_last;
     uint32_t* chosen = chosen_all[kExact ? 0 : warp][kExact ? 0 : sub];
     for (uint32_t e = threadIdx.x; e < n; e += kThreads) count[e] = 0;
+    bool off = false;  // a bias of -inf, which no logit outweighs
     if (BIAS) {
-        // finite, so that a logit of -inf stays -inf; NaN counts as the largest too
-        for (uint32_t e = threadIdx.x; e < L::kSpan; e += kThreads) bias[e] = e < n ? fminf(p.bias[e], 3.402823466e38f) : 0.f;
+        // not +inf, so that a logit of -inf stays -inf; NaN counts as the largest too
+        for (uint32_t e = threadIdx.x; e < L::kSpan; e += kThreads) {
+            bias[e] = e < n ? fminf(p.bias[e], 3.402823466e38f) : 0.f;
+            off |= bias[e] == kNegInf;
+        }
     }
     if (threadIdx.x == 0) routed_block = 0;
     L::clear(tiles, wl);
     L::clear(tiles + L::kSlots, wl);
-    __syncthreads();
+    const bool any_off = __syncthreads_or(off);
 
 #pragma unroll
     for (int q = 0; q < C / 4; ++q) sums[q * kWarp] = float4{0.f, 0.f, 0.f, 0.f};
@@ -605,6 +609,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
                     low |= __float_as_uint(f[i]);
                     word[q + i] = (ordered(f[i]) & ~kMask) | L::register_bits(q + i);
                 }
+            }
+            if (BIAS && any_off) {
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+                    if (bias[L::expert(lane, i)] == kNegInf) word[i] = (kLowest - 1 & ~kMask) | L::register_bits(i);
             }
         }
         // The lane's largest words, then the row's: words below kLowest are

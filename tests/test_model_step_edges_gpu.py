@@ -130,3 +130,26 @@ def test_route_grad_beside_led_rows(lcpp, score, renormalize):
         same = (mixed == x).all(1)
         assert same.sum() >= 50 and torch.equal(chosen[cuda(same)], experts[cuda(same)])
         np.testing.assert_array_equal(got[same], plain[same])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("t", [7, 3000])
+@pytest.mark.parametrize("e", [24, 32, 256])
+def test_route_switched_off_experts_stay_off(lcpp, kind, t, e):
+    """A bias of -inf keeps an expert out of the choice also where its logit is NaN or +inf."""
+    rng = np.random.default_rng(t)
+    x = rng.standard_normal((t, e)).astype(np.float32)
+    off = [4, 9, e - 1]
+    x[:, [4, e - 1]] = np.nan
+    x[::2, 9] = np.inf
+    x[1::3, 9] = np.nan
+    bias = np.zeros(e, np.float32)
+    bias[off] = -np.inf
+    clean = x.copy()
+    clean[:, off] = -np.inf
+    logits = cuda(x).to(TYPES[kind])
+    for k in {1, 4, min(e - 3, 29), min(e, 32)}:
+        _, experts, counts, routed, _ = run_route(lcpp, logits, k, ref.SIGMOID, True, bias)
+        want = ref.choose(host(cuda(clean).to(TYPES[kind]).float()), None, k)
+        np.testing.assert_array_equal(host(experts), want)
+        assert int(routed) == t and not host(counts)[off].any()
