@@ -448,7 +448,7 @@ __device__ __noinline__ void choose_exactly(const uint4* tile, const float* bias
                                             uint32_t* chosen)
 {
     using L = Tile<T, LANES, C>;
-    uint64_t last = ~0ull;
+    uint64_t last = 0;
     for (uint32_t j = 0; j < k; ++j) {
         uint64_t best = 0;
         for (int i = 0; i < C; ++i) {
@@ -458,7 +458,7 @@ __device__ __noinline__ void choose_exactly(const uint4* tile, const float* bias
             const float f = bias ? x + bias[e] : x;
             if (f == kNegInf || (bias && bias[e] == kNegInf)) continue;
             const uint64_t word = uint64_t(ordered(f)) << 32 | (0xffffffffu - e);
-            if (word < last && word > best) best = word;
+            if ((j == 0 || word < last) && word > best) best = word;  // the first may be all ones
         }
         best = row_all<LANES>(best, Max{});
         if (wl % LANES == 0) chosen[j] = best ? ~L::kMask | (uint32_t(best) & L::kMask) : 0u;

@@ -153,3 +153,18 @@ def test_route_switched_off_experts_stay_off(lcpp, kind, t, e):
         want = ref.choose(host(cuda(clean).to(TYPES[kind]).float()), None, k)
         np.testing.assert_array_equal(host(experts), want)
         assert int(routed) == t and not host(counts)[off].any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_rows_of_nan(lcpp, kind, biased):
+    """NaN logits are equal to one another: the lower experts come first, however many there are."""
+    for e, k in ((12, 2), (8, 8), (256, 8), (1000, 32)):
+        x = np.random.default_rng(e).standard_normal((30, e)).astype(np.float32)
+        x[:10] = np.nan
+        x[10:20, : e // 2] = -np.nan
+        x[20:25, 1::2] = np.nan
+        bias = np.random.default_rng(k).standard_normal(e).astype(np.float32) if biased else None
+        logits = cuda(x).to(TYPES[kind])
+        experts = run_route(lcpp, logits, k, ref.SIGMOID, True, bias)[1]
+        np.testing.assert_array_equal(host(experts), ref.choose(host(logits.float()), bias, k))
