@@ -84,10 +84,13 @@ typedef enum lcpp_router_score {
     LCPP_SCORE_SIGMOID = 1  /* s = 1 / (1 + exp(-logit)) */
 } lcpp_router_score;
 
+/* Added to the score: a bias is added to s instead of the logit. */
+#define LCPP_BIAS_ON_SCORE 0x10
+
 typedef struct lcpp_router_config {
     uint32_t num_experts; /* 1 to LCPP_MAX_EXPERTS */
     uint32_t top_k;       /* 1 to min(num_experts, LCPP_MAX_TOP_K) */
-    int32_t score;        /* lcpp_router_score */
+    int32_t score;        /* lcpp_router_score, + LCPP_BIAS_ON_SCORE */
     int32_t renormalize;  /* nonzero: a token's weights are divided by their sum */
     float weight_scale;   /* factor of every weight */
     float loss_coef;      /* factor of the balance loss */
@@ -95,8 +98,10 @@ typedef struct lcpp_router_config {
 
 lcpp_status lcpp_router_temp_bytes(uint64_t num_tokens, uint32_t num_experts, size_t* temp_bytes);
 
-/* For each token t: the top_k experts with the largest logit + bias (added
- * in 32 bits; equal sums go to the lower expert), in descending order, and
+/* For each token t: the top_k experts with the largest logit + bias, or s + bias
+ * with LCPP_BIAS_ON_SCORE (the selection bias of models that balance their
+ * experts without a loss; s is then rounded to 32 bits first), added in 32 bits,
+ * equal sums to the lower expert, in descending order, and
  *   weights[t][j] = weight_scale * s[e_j] (/ sum_i s[e_i] when renormalised).
  * The bias (NULL: none) only takes part in the choice; +inf and NaN in it count
  * as the largest finite number.  An expert whose logit, bias or sum is -inf is

@@ -28,10 +28,12 @@ uint32_t copy_unit(const void* logits, uint64_t stride, uint32_t experts, int si
     return uint32_t(bits & (~bits + 1));
 }
 
+int32_t score_of(const lcpp_router_config* c) { return c->score & ~LCPP_BIAS_ON_SCORE; }
+
 lcpp_status check_config(const lcpp_router_config* c, uint64_t tokens, uint64_t stride)
 {
     if (!c || !c->num_experts || c->num_experts > LCPP_MAX_EXPERTS || !c->top_k || c->top_k > c->num_experts ||
-        c->top_k > LCPP_MAX_TOP_K || (c->score != LCPP_SCORE_SOFTMAX && c->score != LCPP_SCORE_SIGMOID))
+        c->top_k > LCPP_MAX_TOP_K || (score_of(c) != LCPP_SCORE_SOFTMAX && score_of(c) != LCPP_SCORE_SIGMOID))
         return LCPP_ERR_INVALID_ARG;
     // counts are 32-bit, and rows are addressed with 64-bit element offsets
     if (tokens * c->top_k >= uint64_t(1) << 31 || tokens >> 31 || (tokens > 1 && stride < c->num_experts) || stride >> 32)
@@ -81,11 +83,12 @@ lcpp_status forward(void* temp, size_t temp_bytes, const void* logits, uint64_t 
     p.renormalize = c->renormalize != 0;
     p.weight_scale = c->weight_scale;
     p.loss_coef = c->loss_coef;
+    p.bias_on_score = (c->score & LCPP_BIAS_ON_SCORE) != 0;
     p.unit = copy_unit(logits, stride, c->num_experts, size);
     p.ctrl = reinterpret_cast<uint32_t*>(t);
     p.share_total = reinterpret_cast<unsigned long long*>(t + router::kShareOffset);
     p.count_total = reinterpret_cast<uint32_t*>(p.share_total + c->num_experts);
-    const bool sigmoid = c->score == LCPP_SCORE_SIGMOID;
+    const bool sigmoid = score_of(c) == LCPP_SCORE_SIGMOID;
     diag::KernelTimer timer(kTimerRouter, tokens * c->num_experts, s);
     switch (dtype) {
     case LCPP_F32: return router::forward_f32(p, sigmoid, s);
@@ -140,7 +143,7 @@ lcpp_status backward(const void* logits, uint64_t stride, lcpp_dtype dtype, cons
     p.loss_coef = c->loss_coef;
     p.unit = copy_unit(logits, stride, c->num_experts, size);
     p.wide_stores = rows_16b(grad_logits, grad_stride, size);
-    const bool sigmoid = c->score == LCPP_SCORE_SIGMOID;
+    const bool sigmoid = score_of(c) == LCPP_SCORE_SIGMOID;
     diag::KernelTimer timer(kTimerRouter, tokens * c->num_experts, s);
     switch (dtype) {
     case LCPP_F32: return router::backward_f32(p, sigmoid, s);

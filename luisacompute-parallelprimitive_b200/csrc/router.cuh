@@ -71,6 +71,7 @@ struct Params {
     int32_t renormalize;
     float weight_scale;
     float loss_coef;
+    bool bias_on_score;  // else on the logit
     uint32_t unit;  // bytes of a copy: 16, 8, 4, or 2 (plain loads)
     // temp storage, cleared before a launch of several blocks
     uint32_t* ctrl;                  // [0] blocks done, [1] error word, [2] a share was not finite, [3] tokens routed
@@ -439,12 +440,39 @@ __device__ __forceinline__ float weight_score(float x, float most)
     return SIGMOID && !(most < kDeepLogit) ? sigmoid(x) : exp_of(x - most);
 }
 
+// What the choice goes by: logits, logits + bias, or scores + bias.  Scores are
+// computed for it and again for the sums, so that the words' registers are not
+// held beside them (131072 rows of 256 bfloat16, sigmoid: 48, 71 and 86 us).
+enum Choice { kByLogit, kByBiasedLogit, kByBiasedScore };
+
+// The 32-bit value an expert is chosen by.  All that compare two of them go
+// through here and get the same bits: rounded sums and products, no contraction.
+template <bool SIGMOID, Choice BY>
+struct ChoiceKey {
+    const float* bias;
+    Reference ref;  // scores only: the row's, and the inverse of its scores' sum
+    float inv;
+    __device__ __forceinline__ float operator()(float x, float b) const
+    {
+        if (BY == kByLogit) return x;
+        if (BY == kByBiasedLogit) return __fadd_rn(x, b);
+        const float s = SIGMOID ? sigmoid(x) : __fmul_rn(ref.score(x), inv);
+        return x == kNegInf ? kNegInf : __fadd_rn(s, b);
+    }
+    // -inf also for an expert that is switched off
+    __device__ __forceinline__ float of(float x, uint32_t e) const
+    {
+        if (BY == kByLogit) return x;
+        return bias[e] == kNegInf ? kNegInf : (*this)(x, bias[e]);
+    }
+};
+
 // The exact choice of a warp's rows from the full values, one composite word
 // {ordered value, complement of the expert} per element: rare, so it reads the
 // logits again instead of keeping them.  Writes words whose upper part says
 // only whether an expert was chosen.
-template <typename T, int LANES, int C>
-__device__ __noinline__ void choose_exactly(const uint4* tile, const float* bias, int wl, uint32_t n, uint32_t k,
+template <typename T, int LANES, int C, typename Key>
+__device__ __noinline__ void choose_exactly(const uint4* tile, const Key key, int wl, uint32_t n, uint32_t k,
                                             uint32_t* chosen)
 {
     using L = Tile<T, LANES, C>;
@@ -454,9 +482,8 @@ __device__ __noinline__ void choose_exactly(const uint4* tile, const float* bias
         for (int i = 0; i < C; ++i) {
             const uint32_t e = L::expert(wl % LANES, i);
             if (e >= n) continue;
-            const float x = to_float(reinterpret_cast<const T*>(tile + i / L::kV * kWarp + wl)[i % L::kV]);
-            const float f = bias ? x + bias[e] : x;
-            if (f == kNegInf || (bias && bias[e] == kNegInf)) continue;
+            const float f = key.of(to_float(reinterpret_cast<const T*>(tile + i / L::kV * kWarp + wl)[i % L::kV]), e);
+            if (f == kNegInf) continue;
             const uint64_t word = uint64_t(ordered(f)) << 32 | (0xffffffffu - e);
             if ((j == 0 || word < last) && word > best) best = word;  // the first may be all ones
         }
@@ -513,11 +540,12 @@ __device__ void finish(const Params& p, uint32_t routed_tokens, bool broken, dou
     }
 }
 
-template <typename T, int LANES, int C, bool SIGMOID, bool BIAS>
+template <typename T, int LANES, int C, bool SIGMOID, Choice BY>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) forward_kernel(const Params p)
 {
     using L = Tile<T, LANES, C>;
     constexpr uint32_t kMask = L::kMask;
+    constexpr bool BIAS = BY != kByLogit;
     constexpr bool kExact = sizeof(T) == 2 && !BIAS;  // words hold all of a logit
     constexpr int kPlaces = L::kPlaces;
     constexpr uint32_t kLowest = kExact ? Packed<T>::kLowestChoice : 0x00800000u;
@@ -583,6 +611,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
         if (!kExact) __syncwarp();  // a chosen logit may be another lane's copy
 
         uint32_t word[C], low = 0;
+        ChoiceKey<SIGMOID, BY> key{bias, Reference(0.f), 0.f};
         if constexpr (kExact) {
 #pragma unroll
             for (int v = 0; v < L::kVecs; ++v) {
@@ -599,11 +628,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
         } else {
             float x[C];
             L::unpack(tile, wl, x);
+            if constexpr (BY == kByBiasedScore && !SIGMOID) {
+                key.ref = Reference(row_all<LANES>(lane_max(x), Max{}));
+                key.inv = __fdividef(1.f, row_all<LANES>(softmax_scores(x, key.ref), Add{}));
+                L::unpack(tile, wl, x);
+            }
 #pragma unroll
             for (int q = 0; q < C; q += 4) {
                 float4 b{0.f, 0.f, 0.f, 0.f};
                 if (BIAS) b = shared_load4(bias + L::expert(lane, q));
-                const float f[4] = {x[q] + b.x, x[q + 1] + b.y, x[q + 2] + b.z, x[q + 3] + b.w};
+                const float f[4] = {key(x[q], b.x), key(x[q + 1], b.y), key(x[q + 2], b.z), key(x[q + 3], b.w)};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     low |= __float_as_uint(f[i]);
@@ -670,8 +704,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
                 const auto full = [&](uint32_t w) -> uint64_t {
                     if (w < kLowest) return 0;
                     const uint32_t e = kMask - (w & kMask);
-                    const float v = to_float(*L::element(tile, sub, e));
-                    return uint64_t(ordered(BIAS ? v + bias[e] : v)) << 32 | (0xffffffffu - e);
+                    return uint64_t(ordered(key.of(to_float(*L::element(tile, sub, e)), e))) << 32 | (0xffffffffu - e);
                 };
                 __syncwarp();
 #pragma unroll
@@ -688,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
                 for (uint32_t j = lane; j < k; j += LANES) chosen[j] = 0;
                 __syncwarp();
                 if (__any_sync(~0u, tie && m < n)) {
-                    choose_exactly<T, LANES, C>(tile, BIAS ? bias : nullptr, wl, n, k, chosen);
+                    choose_exactly<T, LANES, C>(tile, key, wl, n, k, chosen);
                 } else {
                     for (uint32_t j = lane; j < m; j += LANES) {
                         const uint64_t mine = full(list[j]);
@@ -756,6 +789,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
         float scale = p.weight_scale;
         if (p.renormalize) scale = __fdividef(scale, row_all<LANES>(total, Add{}));
         else if (!SIGMOID) scale = __fdividef(scale, sum);
+        // a NaN among the logits is in every score, also where a bias kept its expert out
+        if (BIAS && !SIGMOID && sum != sum) scale = sum;
         const uint32_t at = t * k + lane;
 #pragma unroll
         for (int s = 0; s < kPlaces; ++s) {
@@ -1121,9 +1156,13 @@ lcpp_status forward_shape(const Params& p, bool sigmoid, cudaStream_t s)
 {
     using L = Tile<T, LANES, C>;
     const size_t fixed = size_t(kWarps) * (2 * L::kSlots * 16 + kWarp * C * 4), smem = fixed + (p.bias ? L::kSpan : 0) * 4 + size_t(p.num_experts) * 4;
-    void (*kernel)(Params) =
-        sigmoid ? (p.bias ? forward_kernel<T, LANES, C, true, true> : forward_kernel<T, LANES, C, true, false>)
-                : (p.bias ? forward_kernel<T, LANES, C, false, true> : forward_kernel<T, LANES, C, false, false>);
+    const auto by = [&](auto is_sigmoid) -> void (*)(Params) {
+        constexpr bool kSigmoid = decltype(is_sigmoid)::value;
+        if (!p.bias) return forward_kernel<T, LANES, C, kSigmoid, kByLogit>;
+        return p.bias_on_score ? forward_kernel<T, LANES, C, kSigmoid, kByBiasedScore>
+                               : forward_kernel<T, LANES, C, kSigmoid, kByBiasedLogit>;
+    };
+    void (*kernel)(Params) = sigmoid ? by(std::true_type{}) : by(std::false_type{});
     const void* f = reinterpret_cast<const void*>(kernel);
     set_max_dynamic_smem(f, fixed + L::kSpan * 8);
     const unsigned grid = grid_for(f, smem, p.tokens, kWarps * L::kRows);

@@ -28,6 +28,7 @@ U8 = 6  # 1-byte (bool) selection flags only
 F16, BF16 = 7, 8  # logits and token rows of the model-step operators only
 # lcpp_router_score
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+BIAS_ON_SCORE = 0x10  # added to either: a bias joins the score instead of the logit
 # lcpp_op
 OP_SUM, OP_MIN, OP_MAX = 0, 1, 2
 # lcpp_testgen_dist
@@ -1001,7 +1002,9 @@ class DeviceRouter:
                 num_tokens, num_experts, top_k, score=SCORE_SOFTMAX, renormalize=True, weight_scale=1.0,
                 loss_coef=1.0, d_bias=None, d_token_request=None, stream=None):
         """lcpp_router_forward: d_logits [num_tokens, num_experts] float32, float16 or bfloat16;
-        weights float32 and experts int32 [num_tokens, top_k], counts int32 [num_experts]."""
+        weights float32 and experts int32 [num_tokens, top_k], counts int32 [num_experts].
+        d_bias [num_experts] float32 joins the logits in the choice, or the scores with
+        score=SCORE_SIGMOID + BIAS_ON_SCORE (or SCORE_SOFTMAX + BIAS_ON_SCORE)."""
         torch = _torch()
         i32, f32, pairs, code = torch.int32, torch.float32, num_tokens * top_k, _row_code(d_logits)
         logits, stride = _rows(d_logits, num_tokens, num_experts, code, "d_logits")

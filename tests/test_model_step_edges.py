@@ -154,3 +154,12 @@ def test_dispatch_refuses_every_overlap(lcpp):
 
     check(back, ["grad_out", "rows", "row_of", "pair_of", "starts", "weights", "grad_rows", "grad_weights"],
           ["grad_rows", "grad_weights"])
+
+
+def test_router_bias_on_scores_is_a_flag(lcpp):
+    """The flag goes with either score, in the gradient's configuration too, and makes no other value valid."""
+    lib = lcpp.lib()
+    for score, status in ((lcpp.BIAS_ON_SCORE, lcpp.OK), (lcpp.BIAS_ON_SCORE + lcpp.SCORE_SIGMOID, lcpp.OK),
+                          (lcpp.BIAS_ON_SCORE + 2, lcpp.ERR_INVALID_ARG), (0x20, lcpp.ERR_INVALID_ARG)):
+        cfg = lcpp.RouterConfig(16, 4, score, 1, 1.0, 1.0)
+        assert lib.lcpp_router_backward(None, 16, 2, None, None, None, None, None, None, 16, 0, cfg, None) == status

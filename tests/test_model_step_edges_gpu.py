@@ -168,3 +168,87 @@ def test_route_rows_of_nan(lcpp, kind, biased):
         logits = cuda(x).to(TYPES[kind])
         experts = run_route(lcpp, logits, k, ref.SIGMOID, True, bias)[1]
         np.testing.assert_array_equal(host(experts), ref.choose(host(logits.float()), bias, k))
+
+
+def route_by_score(L, logits, k, score, renormalize, bias, mask=None):
+    """Forward with the bias on the scores; (experts, 64-bit sums) after weights, counts and loss were checked
+    against those of the experts it chose."""
+    weights, experts, counts, routed, loss = run_route(L, logits, k, score + L.BIAS_ON_SCORE, renormalize, bias, mask)
+    t, e = logits.shape
+    x, chosen = host64(logits), host(experts)
+    log_s, share = ref._scores(x, score)
+    has, live = chosen >= 0, chosen[:, 0] >= 0
+    picked = np.where(has, np.exp(np.take_along_axis(log_s, np.maximum(chosen, 0), 1)), 0.0)
+    if renormalize:
+        picked /= np.where(live[:, None], picked.sum(1, keepdims=True), 1.0)
+    np.testing.assert_allclose(host64(weights), SCALE * picked, rtol=1e-5, atol=1e-9)
+    np.testing.assert_array_equal(host(counts), np.bincount(chosen[has], minlength=e))
+    assert int(routed) == live.sum() == (t if mask is None else (mask >= 0).sum())
+    want = COEF * e * (share[live].sum(0) / live.sum() * host(counts) / (k * live.sum())).sum()
+    assert abs(float(loss) - want) <= 1e-5 * want
+    return chosen, np.where(np.isneginf(x), -np.inf, np.exp(log_s) + bias.astype(np.float64))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_bias_on_scores(lcpp, kind, score, renormalize):
+    """The largest score + bias.  A score is off by at most 4e-7 (1 at most, a quotient of exponentials good to
+    2^-22 each), its sum with a bias below 2 by 2^-23 more: sums that differ by 2e-6 have to be in order."""
+    for t, e, k in ((50, 2, 1), (300, 8, 2), (37, 16, 16), (70, 60, 6), (5000, 64, 6), (400, 160, 6), (900, 256, 8),
+                    (30, 512, 32), (20, 1000, 10)):
+        rng = np.random.default_rng(t + e)
+        x = (rng.standard_normal((t, e)) * 2).astype(np.float32)
+        bias = (rng.standard_normal(e) * (0.1 if score == ref.SIGMOID else 1.0 / e)).astype(np.float32)
+        if e > 16:
+            x[rng.random((t, e)) < 0.1] = -np.inf
+            bias[e // 2] = -np.inf
+        mask = np.where(rng.random(t) < 0.2, -1, 0).astype(np.int32) if t % 20 else None
+        logits = cuda(x).to(TYPES[kind])
+        chosen, sums = route_by_score(lcpp, logits, k, score, renormalize, bias, mask)
+        live = chosen[:, 0] >= 0
+        chosen, sums, rows = chosen[live], sums[live], np.nonzero(live)[0]
+        order = np.argsort(-sums, axis=1, kind="stable")
+        best = np.take_along_axis(sums, order, 1)
+        assert (np.abs(np.take_along_axis(sums, chosen, 1) - best[:, :k]) <= 2e-6).all()
+        assert all(len(set(c)) == k for c in chosen)
+        with np.errstate(invalid="ignore"):
+            gap = -np.diff(best, axis=1, append=-np.inf)
+        clear = (gap[:, :k] > 2e-6) & (np.concatenate([np.full((len(rows), 1), np.inf), gap[:, :k - 1]], 1) > 2e-6)
+        np.testing.assert_array_equal(chosen[clear], order[:, :k][clear])
+        assert clear.mean() > 0.9
+        if e >= 8 and k < e:  # it is another choice than that of logit + bias
+            assert (chosen != ref.choose(host(logits.float()), bias, k)[live]).any(1).mean() > 0.05
+
+
+@pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
+@pytest.mark.parametrize("e,k", [(40, 5), (256, 8), (1000, 32)])
+def test_route_bias_on_equal_scores(lcpp, score, e, k):
+    """Few different logits and biases: equal scores have equal bits, so equal sums go to the lower expert, however
+    many there are; scores that 32 bits do not tell from 1 are equal."""
+    rng = np.random.default_rng(e)
+    x = rng.choice([0.0, 1.0, -4.0], (60, e)).astype(np.float32)
+    x[:10] = 0.5
+    if score == ref.SIGMOID:
+        x[20:30] = rng.choice([40.0, 60.0, 90.0], (10, e))
+    bias = rng.choice([0.0, 0.25, 0.125], e).astype(np.float32)
+    chosen, sums = route_by_score(lcpp, cuda(x), k, score, True, bias)
+    rank = np.lexsort((np.broadcast_to(np.arange(e), sums.shape), -np.round(sums, 5)), axis=1)[:, :k]
+    np.testing.assert_array_equal(chosen, rank)
+
+
+def test_route_bias_on_scores_of_broken_rows(lcpp):
+    """A NaN logit, or +inf under softmax, makes its own row's weights NaN; masked rows pass nothing on; rows of
+    -inf alone are left out; far logits, whose scores are 0 in 32 bits, are told apart by the bias."""
+    x = np.random.default_rng(3).standard_normal((40, 12)).astype(np.float32)
+    x[3, 5], x[4, 2], x[5] = np.nan, np.inf, -np.inf
+    x[6], x[7] = -1e30, -200.0
+    bias = np.linspace(0, 1, 12).astype(np.float32)
+    for score in (ref.SOFTMAX, ref.SIGMOID):
+        weights, experts, counts, routed, _ = run_route(lcpp, cuda(x), 2, score + lcpp.BIAS_ON_SCORE, True, bias)
+        bad = np.isnan(host(weights)).any(1)
+        assert bad[3] and bad.sum() == (2 if score == ref.SOFTMAX else 1)
+        assert host(experts)[3, 0] == (0 if score == ref.SOFTMAX else 5)
+        assert (host(experts)[5] == -1).all() and int(routed) == 39 and host(counts).sum() == 78
+        np.testing.assert_array_equal(host(experts)[6], [11, 10])
+        np.testing.assert_array_equal(host(experts)[7], [11, 10])
