@@ -87,7 +87,7 @@ lcpp_status forward(void* temp, size_t temp_bytes, const void* logits, uint64_t 
     p.unit = copy_unit(logits, stride, c->num_experts, size);
     p.ctrl = reinterpret_cast<uint32_t*>(t);
     p.share_total = reinterpret_cast<unsigned long long*>(t + router::kShareOffset);
-    p.count_total = reinterpret_cast<uint32_t*>(p.share_total + c->num_experts);
+    p.count_total = reinterpret_cast<uint32_t*>(p.share_total + router::kShareScales * c->num_experts);
     const bool sigmoid = score_of(c) == LCPP_SCORE_SIGMOID;
     diag::KernelTimer timer(kTimerRouter, tokens * c->num_experts, s);
     switch (dtype) {

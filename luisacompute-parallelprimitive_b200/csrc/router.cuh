@@ -75,7 +75,7 @@ struct Params {
     uint32_t unit;  // bytes of a copy: 16, 8, 4, or 2 (plain loads)
     // temp storage, cleared before a launch of several blocks
     uint32_t* ctrl;                  // [0] blocks done, [1] error word, [2] a share was not finite, [3] tokens routed
-    unsigned long long* share_total; // [num_experts] sums of shares in units of 2^-32
+    unsigned long long* share_total; // [kShareScales][num_experts] sums of shares
     uint32_t* count_total;           // [num_experts]
 };
 
@@ -510,10 +510,21 @@ __device__ __forceinline__ uint32_t largest_below(const uint32_t (&word)[C], uin
     return __vimax3_u32(a, b, c) + below;
 }
 
-// A block's share of an expert, at most 2^31 tokens, in units of 2^-32: whole
-// numbers add up to the same total in any order, and 2^-32 is far below the
-// rounding of the 32-bit sums that go in.
-constexpr double kShareUnit = 4294967296.0;
+// Blocks' shares of an expert are added up as whole numbers, whose total is the
+// same in any order: in units of 2^-32 those from 2^-8 up (at most 2^31 tokens in
+// all), smaller ones in totals of their own with units of 2^-60, 2^-88, 2^-116 and
+// 2^-144, of which a 32-bit sum is a multiple there (below 2^-121 it is rounded to
+// one) and at most 2^52.
+constexpr int kShareScales = 5;
+__device__ __forceinline__ int share_scale(float share)
+{
+    return (share < 0x1p-8f) + (share < 0x1p-36f) + (share < 0x1p-64f) + (share < 0x1p-92f);
+}
+// 2^(+-(32 + 28 scale)): units in a share of 1, and a unit.
+__device__ __forceinline__ double share_units(int scale, int sign)
+{
+    return __hiloint2double((1023 + sign * (32 + 28 * scale)) << 20, 0);
+}
 
 // Writes the counts and, from sum_e share_e * count_e, the loss.
 template <typename Share, typename Count>
@@ -830,7 +841,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
     for (uint32_t e = threadIdx.x; e < n; e += kThreads) {
         const float sum = block_share(e);
         if (!(sum < INFINITY)) atomicOr(p.ctrl + 2, 1u);
-        else if (sum > 0.f) atomicAdd(p.share_total + e, (unsigned long long)(__double2ull_rn(double(sum) * kShareUnit)));
+        else if (sum > 0.f) {
+            const int scale = share_scale(sum);
+            atomicAdd(p.share_total + scale * n + e, (unsigned long long)(__double2ull_rn(double(sum) * share_units(scale, 1))));
+        }
         if (count[e]) atomicAdd(p.count_total + e, count[e]);
     }
     if (threadIdx.x == 0 && routed_block) atomicAdd(p.ctrl + 3, routed_block);
@@ -842,7 +856,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
     if (!is_last) return;
     __threadfence();
     finish(p, __ldcg(p.ctrl + 3), __ldcg(p.ctrl + 2) != 0, scratch,
-           [&](uint32_t e) { return double(__ldcg(p.share_total + e)) / kShareUnit; },
+           [&](uint32_t e) {
+               double share = 0.0;
+#pragma unroll
+               for (int scale = kShareScales - 1; scale >= 0; --scale)
+                   share += double(__ldcg(p.share_total + scale * n + e)) * share_units(scale, -1);
+               return share;
+           },
            [&](uint32_t e) { return __ldcg(p.count_total + e); });
 }
 
@@ -1140,7 +1160,7 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
 
 // Temp storage: the control words, the share totals, the count totals.
 constexpr size_t kShareOffset = kTempAlign;
-inline size_t cleared_bytes(uint32_t experts) { return kShareOffset + size_t(experts) * 12; }
+inline size_t cleared_bytes(uint32_t experts) { return kShareOffset + size_t(experts) * (kShareScales * 8 + 4); }
 
 __global__ void __launch_bounds__(kThreads) clear_kernel(uint32_t* words, uint32_t n);
 

@@ -252,3 +252,19 @@ def test_route_bias_on_scores_of_broken_rows(lcpp):
         assert (host(experts)[5] == -1).all() and int(routed) == 39 and host(counts).sum() == 78
         np.testing.assert_array_equal(host(experts)[6], [11, 10])
         np.testing.assert_array_equal(host(experts)[7], [11, 10])
+
+
+@pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
+@pytest.mark.parametrize("t", [40, 4000, 60_001])
+@pytest.mark.parametrize("logit", [-12.0, -30.0, -45.0, -60.0, -75.0])
+def test_route_loss_of_small_shares(lcpp, score, t, logit):
+    """A bias sends every token to an expert with next to no share: the loss keeps its digits however many blocks
+    add to it."""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((t, 16)).astype(np.float32)
+    x[:, 3] = logit
+    bias = np.zeros(16, np.float32)
+    bias[3] = 100.0
+    loss = run_route(lcpp, cuda(x), 1, score, True, bias)[4]
+    want = ref.route(x, 1, score, True, SCALE, COEF, bias)[4]
+    assert abs(float(loss) - want) <= 1e-5 * want
