@@ -56,6 +56,11 @@ lcpp_status lcpp_diag_timing_read(lcpp_kernel_time* out, int capacity, int* coun
  * usable.  temp: 256-byte aligned, at least 256 bytes. */
 lcpp_status lcpp_diag_wait_timeout_probe(void* temp, size_t temp_bytes, uint64_t limit_ns, lcpp_stream_t stream);
 
+/* Launch shapes (kernel, device, block size, dynamic shared memory) whose
+ * residency was looked up and is kept.  A call that adds one costs a query;
+ * the number stays small however the sizes of the calls change. */
+lcpp_status lcpp_diag_launch_shapes(uint64_t* count);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -492,7 +492,9 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_block_table_args* a, c
         return unsigned(std::max<uint64_t>(1, ceil_div(p.tokens, p.tokens_per_block)));
     };
     if (n <= kFusedRequests) {
-        const size_t smem = n * 12;
+        // room in a few steps, so that few launch shapes are looked up and kept as n changes
+        const uint64_t room = n <= kThreads ? kThreads : n <= 2 * kThreads ? 2 * kThreads : n <= 4 * kThreads ? 4 * kThreads : kFusedRequests;
+        const size_t smem = room * 12;
         auto kernel = many ? (n <= kThreads ? fused_kernel<1, 4> : n <= 2 * kThreads ? fused_kernel<2, 4> : fused_kernel<kItems, 4>)
                            : (n <= kThreads ? fused_kernel<1, 1> : n <= 2 * kThreads ? fused_kernel<2, 1> : fused_kernel<kItems, 1>);
         if (n > 2 * kThreads)  // up to 48 KB beside the static arrays

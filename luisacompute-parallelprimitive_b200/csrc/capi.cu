@@ -6,6 +6,7 @@
 #include <set>
 #include <utility>
 
+#include "../../include/lcpp_b200_diag.h"
 #include "common.cuh"
 #include "radix_sort.cuh"
 #include "reduce.cuh"
@@ -48,23 +49,26 @@ void set_max_dynamic_smem(const void* kernel, size_t bytes)
     done.insert(key);
 }
 
+namespace {
+std::mutex g_resident_mu;
+std::map<std::pair<std::pair<const void*, int>, std::pair<int, size_t>>, int> g_resident;
+}  // namespace
+
 int resident_blocks(const void* kernel, int block, size_t dynamic_smem)
 {
-    static std::mutex mu;
-    static std::map<std::pair<std::pair<const void*, int>, std::pair<int, size_t>>, int> cache;
     int dev = 0;
     cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lk(mu);
+    std::lock_guard<std::mutex> lk(g_resident_mu);
     const auto key = std::make_pair(std::make_pair(kernel, dev), std::make_pair(block, dynamic_smem));
-    const auto it = cache.find(key);
-    if (it != cache.end()) return it->second;
+    const auto it = g_resident.find(key);
+    if (it != g_resident.end()) return it->second;
     int blocks = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, block, dynamic_smem) != cudaSuccess) {
         cudaGetLastError();
         blocks = 1;
     }
     blocks = blocks < 1 ? 1 : blocks;
-    cache[key] = blocks;
+    g_resident[key] = blocks;
     return blocks;
 }
 
@@ -103,6 +107,14 @@ bool reduce_init(lcpp_dtype dt, lcpp_op op, unsigned char out[8])
 }  // namespace
 
 extern "C" {
+
+lcpp_status lcpp_diag_launch_shapes(uint64_t* count)
+{
+    if (!count) return LCPP_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> lk(lcpp::g_resident_mu);
+    *count = lcpp::g_resident.size();
+    return LCPP_OK;
+}
 
 const char* lcpp_status_string(lcpp_status status)
 {

@@ -196,6 +196,7 @@ def lib() -> ctypes.CDLL:
         "lcpp_dispatch_combine_backward": ([vp, u64, vp, u64, vp, vp, vp, vp, vp, u64, vp, u64, u32, u32, u64, u64,
                                             i, vp], i),
         "lcpp_diag_timing_enable": ([i], i),
+        "lcpp_diag_launch_shapes": ([ctypes.POINTER(u64)], i),
         "lcpp_diag_wait_timeout_probe": ([vp, sz, u64, vp], i),
         "lcpp_diag_timing_read": ([ctypes.POINTER(KernelTime), i, ip], i),
     }

@@ -2,11 +2,13 @@
 references and with its tolerances (derived at its top)."""
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 
 import model_step_ref as ref
-from test_model_step_gpu import COEF, ROUND, SCALE, TYPES, check_plan, cuda, host, host64, i32, run_route
+from test_model_step_gpu import COEF, ROUND, SCALE, TYPES, check_extend, check_plan, cuda, host, host64, i32, run_route
 
 pytestmark = pytest.mark.gpu
 
@@ -52,6 +54,25 @@ def test_combine_gradient_over_the_weights(lcpp, h):
     d.CombineBackward(dy, rows, row_of, pair_of, starts, weights, apart, grad_weights, t, k, e)
     d.CombineBackward(dy, rows, row_of, pair_of, starts, weights, got, weights, t, k, e)
     assert torch.equal(weights, grad_weights) and torch.equal(got, apart)
+
+
+def test_extend_of_changing_request_counts(lcpp):
+    """A server's request count changes from step to step: few launch shapes are looked up and kept for all counts,
+    and each has its results."""
+    def shapes():
+        count = ctypes.c_uint64()
+        lcpp.check(lcpp.lib().lcpp_diag_launch_shapes(ctypes.byref(count)), "launch_shapes")
+        return count.value
+
+    rng = np.random.default_rng(2)
+    before = shapes()
+    for n in [*range(1, 40), *range(41, 4097, 97), 511, 512, 513, 1024, 1025, 2048, 2049, 4096]:
+        context = rng.integers(0, 60, n).astype(np.int32)
+        table = rng.permutation(n * 5).astype(np.int32).reshape(n, 5)
+        free = (n * 5 + rng.permutation(n)).astype(np.int32)
+        check_extend(lcpp, context, None, table, 5, free, None, n + 3, 16, optional=False)
+    assert shapes() - before <= 8
+    assert lcpp.lib().lcpp_diag_launch_shapes(None) == lcpp.ERR_INVALID_ARG
 
 
 def route_gradient(L, logits, experts, counts, routed, g, dloss, score, renormalize):
