@@ -894,9 +894,10 @@ __device__ __noinline__ float2 leader_left(const uint4* tile, const float* pull,
     return {row_top, __shfl_sync(~0u, slope, leading_lane<LANES>(top == row_top, sub))};
 }
 
-// A sigmoid score is at most 1: in a row whose scores add up to this or more, no
-// expert has more than half of the share.
-constexpr float kLedSum = 2.f;
+// With a sigmoid of 0.03 or more among the chosen, of which the others are at most
+// 34 times, a row's slopes lose little by being taken relative to a chosen one's:
+// the largest of the others is looked for below this logit only.
+constexpr float kLedLogit = -3.5f;
 
 // The logits' gradient.  The chosen experts of a row are taken out of it first
 // (their logits in the tile become -inf): the dense part of a row then has one
@@ -1053,22 +1054,12 @@ __global__ void __launch_bounds__(kThreads, C > 16 ? 2 : 3) backward_kernel(cons
         if constexpr (SIGMOID) {
             deep = sum < kDeepSigmoid;
             bool again = deep;
-            if (__any_sync(~0u, sum < kLedSum)) {
-                float chosen = 0.f;
-#pragma unroll
-                for (int s = 0; s < kPlaces; ++s) {
-                    if (uint32_t(s * LANES) >= k) break;
-                    chosen += score[s];
-                }
-                chosen = row_all<LANES>(chosen, Add{});
-                // with half of the share among the chosen, none outside has more
-                const bool led = sum < kLedSum && (2.f * chosen < sum || deep);
-                if (__any_sync(~0u, led)) {
-                    const float2 leader = leader_left<T, LANES, C>(tile, pull, wl);
-                    if (led && leader.x > chosen_top) {
-                        base = pull0 = leader.y;
-                        again = true;
-                    }
+            const bool led = live && chosen_top < kLedLogit;
+            if (__any_sync(~0u, led)) {
+                const float2 leader = leader_left<T, LANES, C>(tile, pull, wl);
+                if (led && leader.x > chosen_top) {
+                    base = pull0 = leader.y;
+                    again = true;
                 }
             }
             if (__any_sync(~0u, again)) {

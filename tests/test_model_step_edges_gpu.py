@@ -133,6 +133,27 @@ def test_route_grad_of_unchosen_leader(lcpp, kind, score, renormalize):
 
 @pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
 @pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("group", [2, 3, 20])
+def test_route_grad_of_unchosen_group(lcpp, score, renormalize, group):
+    """Several experts that a bias keeps out, and that no token counts for, share a row among them: they have one
+    slope, and what is left of it is far below it."""
+    rng = np.random.default_rng(group)
+    for e, k in ((22, 1), (64, 6), (256, 8), (1000, 2)):
+        for low in (-6.0, -9.0, -14.0):
+            x = rng.standard_normal((120, e)) + low
+            x[:, :group] = rng.choice([0.5, 2.0, 6.0, 16.0], (120, group)) + rng.random((120, group))
+            bias = np.zeros(e, np.float32)
+            bias[:group] = -np.inf
+            logits = cuda(x.astype(np.float32))
+            _, experts, counts, routed, _ = run_route(lcpp, logits, k, score, renormalize, bias)
+            g = rng.standard_normal((120, k)).astype(np.float32) * 1e-3
+            for up in (g, None):
+                got, want = route_gradient(lcpp, logits, experts, counts, routed, up, 3.0, score, renormalize)
+                assert (np.abs(got - want) <= 2e-5 * np.abs(want).max(1, keepdims=True)).all(), (e, k, low)
+
+
+@pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
+@pytest.mark.parametrize("renormalize", [True, False])
 def test_route_grad_beside_led_rows(lcpp, score, renormalize):
     """A row has the same bits beside rows that need more care (an unchosen leader, tiny sigmoids) as without them."""
     rng = np.random.default_rng(23)
