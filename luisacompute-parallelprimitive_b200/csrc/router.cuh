@@ -49,9 +49,10 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / kWarp;
 constexpr float kNegInf = -INFINITY;
 // Where the sum of a row's sigmoids is below this, each equals exp(logit) to 32
-// bits and the sum may underflow: shares are taken as a softmax instead.
-constexpr float kDeepSigmoid = 1e-20f;
-constexpr float kDeepLogit = -60.f;  // the same for the largest chosen logit
+// bits (they differ by a factor of 1 + exp(logit)), and smaller ones may underflow
+// beside it: shares are taken as a softmax instead.
+constexpr float kDeepSigmoid = 1e-8f;
+constexpr float kDeepLogit = -18.5f;  // the same for the largest chosen logit
 constexpr int kHeads = 4;
 constexpr int kMoreRounds = 6;  // words past top_k that a tie is followed for
 

@@ -152,6 +152,27 @@ def test_route_grad_of_unchosen_group(lcpp, score, renormalize, group):
                 assert (np.abs(got - want) <= 2e-5 * np.abs(want).max(1, keepdims=True)).all(), (e, k, low)
 
 
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_tiny_sigmoids(lcpp, renormalize):
+    """Sigmoids so small that those next to the largest have no 32-bit value of their own: weights and gradient
+    keep them as parts of the row's."""
+    rng = np.random.default_rng(19)
+    for e, k in ((11, 5), (40, 6), (256, 8)):
+        x = np.empty((160, e), np.float32)
+        x[:] = np.repeat([-20.0, -30.0, -44.7, -45.0, -47.0, -59.0, -61.0, -80.0], 20)[:, None]
+        x[:, 2:] -= rng.uniform(25, 42, (160, e - 2)).astype(np.float32)
+        x[:, 1] -= 30
+        logits = cuda(x)
+        weights, experts, counts, routed, loss = run_route(lcpp, logits, k, ref.SIGMOID, renormalize)
+        want = ref.route(x, k, ref.SIGMOID, renormalize, SCALE, COEF)
+        np.testing.assert_array_equal(host(experts), want[1])
+        np.testing.assert_allclose(host64(weights), want[0], rtol=1e-5, atol=0 if renormalize else 1e-37)
+        assert abs(float(loss) - want[4]) <= 1e-5 * want[4]
+        counts[0] = 0  # no slope of its own for the leading expert's share
+        got, want = route_gradient(lcpp, logits, experts, counts, routed, None, 3.0, ref.SIGMOID, renormalize)
+        assert (np.abs(got - want) <= 2e-5 * np.abs(want).max(1, keepdims=True)).all()
+
+
 @pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_route_grad_beside_led_rows(lcpp, score, renormalize):
