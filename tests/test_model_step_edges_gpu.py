@@ -331,3 +331,36 @@ def test_route_loss_of_small_shares(lcpp, score, t, logit):
     loss = run_route(lcpp, cuda(x), 1, score, True, bias)[4]
     want = ref.route(x, 1, score, True, SCALE, COEF, bias)[4]
     assert abs(float(loss) - want) <= 1e-5 * want
+
+
+# one block of 256 threads up to 1024 pairs and 256 experts, one of 1024 up to 2048 pairs, several beyond
+@pytest.mark.parametrize("pairs", [1023, 1024, 1025, 2047, 2048, 2049, 3073])
+@pytest.mark.parametrize("e", [255, 256, 257, 1024])
+def test_plan_borders(lcpp, pairs, e):
+    rng = np.random.default_rng(pairs * e)
+    experts = rng.integers(-1, e, (pairs, 1)).astype(np.int32)
+    check_plan(lcpp, experts, e, 16)
+    check_plan(lcpp, experts, e, 1, pairs // 2)
+
+
+@pytest.mark.parametrize("kind,t,h,k", [("bf16", 1300, 2048, 8), ("f32", 1300, 1024, 2), ("f16", 2700, 904, 5),
+                                        ("bf16", 400, 8192, 3)])
+def test_combine_gradient_of_long_batches(lcpp, kind, t, h, k):
+    """Enough columns in all for the lanes that take several accesses each."""
+    rng = np.random.default_rng(h)
+    e, dtype, (rel, step) = 24, TYPES[kind], ROUND[kind]
+    experts = np.argsort(rng.random((t, e)), axis=1)[:, :k].astype(np.int32)
+    experts[rng.random((t, k)) < 0.1] = -1
+    starts, row_of, pair_of = check_plan(lcpp, experts, e, 16)
+    end, n = int(starts[-1]), pair_of.numel()
+    rows, dy = (cuda(rng.standard_normal(s).astype(np.float32)).to(dtype) for s in ((n, h), (t, h)))
+    w = rng.random((t, k)).astype(np.float32)
+    grad_rows, grad_weights = torch.full_like(rows, 9), torch.full((t, k), -7.0, device="cuda")
+    lcpp.DeviceDispatch().CombineBackward(dy, rows, row_of, pair_of, starts, cuda(w), grad_rows, grad_weights, t, k, e)
+    want_rows, want_weights = ref.combine_grad(host64(dy), host64(rows), host(row_of), host(pair_of),
+                                               w.astype(np.float64), end)
+    assert (np.abs(host64(grad_rows)[:end] - want_rows) <= (1e-6 + rel) * np.abs(want_rows) + step).all()
+    assert (host64(grad_rows)[end:] == 9).all()
+    _, size = ref.combine_grad(np.abs(host64(dy)), np.abs(host64(rows)), host(row_of), host(pair_of),
+                               w.astype(np.float64), end)
+    assert (np.abs(host64(grad_weights) - want_weights) <= 1e-5 * size + 1e-12).all()

@@ -542,7 +542,7 @@ def choices(rng, t, k, e, missing=0.1):
     return experts
 
 
-# 16384 pairs is the largest plan of one block; 4096 the fewest of a block among several
+# one block up to 2048 pairs, up to one per SM beyond (the borders: tests/test_model_step_edges_gpu.py)
 @pytest.mark.parametrize("t,k,e,align", [(1, 1, 1, 1), (1, 8, 128, 16), (3, 2, 5, 7), (16, 8, 128, 128), (300, 4, 60, 8),
                                          (2048, 8, 256, 128), (2049, 8, 256, 64), (5000, 6, 1000, 1),
                                          (40_000, 2, 16, 128), (3000, 32, 33, 4), (90_001, 8, 257, 16), (500, 1, 1024, 3)])
