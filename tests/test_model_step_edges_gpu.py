@@ -343,8 +343,8 @@ def test_plan_borders(lcpp, pairs, e):
     check_plan(lcpp, experts, e, 1, pairs // 2)
 
 
-@pytest.mark.parametrize("kind,t,h,k", [("bf16", 1300, 2048, 8), ("f32", 1300, 1024, 2), ("f16", 2700, 904, 5),
-                                        ("bf16", 400, 8192, 3)])
+@pytest.mark.parametrize("kind,t,h,k", [("bf16", 1300, 2048, 8), ("f32", 2400, 1024, 2), ("f16", 2700, 904, 5),
+                                        ("bf16", 400, 8192, 3), ("bf16", 500, 2881, 3)])
 def test_combine_gradient_of_long_batches(lcpp, kind, t, h, k):
     """Enough columns in all for the lanes that take several accesses each."""
     rng = np.random.default_rng(h)
