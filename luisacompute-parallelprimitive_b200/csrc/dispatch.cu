@@ -31,9 +31,17 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kFewThreads = 256;
-constexpr uint64_t kFewPairs = 1024;    // these, of at most kFewThreads experts, take a block of kFewThreads
-constexpr uint64_t kSmallPairs = 2048;  // these take one block
-constexpr uint64_t kTilePairs = 1024;   // fewest pairs of a block among several
+// These, of at most kFewThreads experts, take a block of kFewThreads: 256 pairs of
+// 8, 64, 128 and 256 experts 2.5, 3.0, 3.5 and 4.4 us against 3.2, 3.4, 3.7 and 4.3
+// with kPlanThreads, but 512 pairs 3.0, 3.6, 4.0 and 5.0 against 3.2, 3.5, 3.7 and 4.3.
+constexpr uint64_t kFewPairs = 256;
+// These take one block: 2048 pairs of 64, 256 and 1024 experts 5.0, 5.9 and 9.9 us
+// against 6.2, 6.9 and 10.0 in two launches, 4096 pairs 6.5, 7.4 and 11.6 against
+// 6.3, 6.8 and 9.5.
+constexpr uint64_t kSmallPairs = 2048;
+// Fewest pairs of a block among several: 16384 pairs of 256 experts 7.1 us, the
+// same with 256 or 512, 7.9 with 2048.
+constexpr uint64_t kTilePairs = 1024;
 
 struct PlanParams {
     const int32_t* experts;

@@ -333,8 +333,8 @@ def test_route_loss_of_small_shares(lcpp, score, t, logit):
     assert abs(float(loss) - want) <= 1e-5 * want
 
 
-# one block of 256 threads up to 1024 pairs and 256 experts, one of 1024 up to 2048 pairs, several beyond
-@pytest.mark.parametrize("pairs", [1023, 1024, 1025, 2047, 2048, 2049, 3073])
+# one block of 256 threads up to 256 pairs and 256 experts, one of 1024 up to 2048 pairs, several beyond
+@pytest.mark.parametrize("pairs", [255, 256, 257, 1023, 1024, 1025, 2047, 2048, 2049, 3073])
 @pytest.mark.parametrize("e", [255, 256, 257, 1024])
 def test_plan_borders(lcpp, pairs, e):
     rng = np.random.default_rng(pairs * e)
