@@ -345,6 +345,7 @@ __device__ __forceinline__ float lane_max(const float (&x)[C])
 struct Reference {
     float top, scaled;
     bool wide, any_rare;  // this row; it or another rarity in any row of the warp
+    __device__ __forceinline__ Reference() : top(0.f), scaled(0.f), wide(false), any_rare(false) {}
     __device__ __forceinline__ explicit Reference(float t, bool rare = false)
         : top(t), scaled(t * -kLog2E), wide(!(fabsf(t) < 1e6f)), any_rare(__any_sync(~0u, wide || rare))
     {
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && C > 16 ? 2 : 3) fo
         if (!kExact) __syncwarp();  // a chosen logit may be another lane's copy
 
         uint32_t word[C], low = 0;
-        ChoiceKey<SIGMOID, BY> key{bias, Reference(0.f), 0.f};
+        ChoiceKey<SIGMOID, BY> key{bias, Reference(), 0.f};
         if constexpr (kExact) {
 #pragma unroll
             for (int v = 0; v < L::kVecs; ++v) {
