@@ -19,9 +19,10 @@
 // request and 4 a new page.  A step of 64 single tokens takes 2.9 us and one of
 // 7001 mixed tokens 3.3 us, a launch and its dependent loads.  4.0 M tokens of
 // 6001 requests in pages of 64 take 25 us (67 MB written at 2.6 TB/s; the copy
-// rate would be 10.5 us): the layout kernel, 20 us of it, is bound by its
-// instructions (283 per 128 tokens, 54 % of the issue slots) and by the page
-// loads it waits for, not by memory, for all it writes stays in L2.
+// rate would be 10.5 us): the layout kernel, 20 us of it, is bound by the latency
+// of a run's chain (search, page load, stores: 5.2 warps wait for a load per
+// instruction issued, in 54 % of the issue slots), not by memory, for all it writes
+// stays in L2.
 #include "model.cuh"
 
 using namespace lcpp;

@@ -11,9 +11,9 @@
 // launch, and in a second one every block adds up all tiles' counts itself (a
 // few hundred KB from L2) before it ranks its tile.
 //
-// 131072 pairs of 256 experts take 9.4 us in two launches, 128 pairs 4.6 us in
-// one of 256 threads: both are latency (the second launch waits 2.3 us for the
-// tiles' counts and as long for the walks).
+// 131072 pairs of 256 experts take 9.1 us in two launches, 128 pairs of 128
+// experts 3.4 us in one of 256 threads: both are latency (the second launch waits
+// 2.3 us for the tiles' counts and as long for the walks).
 //
 // The row kernels work by token: x (or its gradient) is read once and goes to,
 // or comes from, the token's rows, so nothing but those rows is read or
@@ -21,7 +21,9 @@
 // token, combine the same, combine's gradient 1 + 2k.  Measured with 4096
 // bfloat16 columns, 16384 tokens, 8 of 256 experts, segments of 128: gather
 // 212 us (1.21 GB and 134 MB of zeros in padding rows, 6.3 TB/s), combine 175 us
-// (1.21 GB, 6.9 TB/s), its gradient 373 us (2.28 GB and the padding, 6.5 TB/s).
+// (1.21 GB, 6.9 TB/s: above the copy rate of 6.4, half of which is writes; eight of
+// combine's nine rows are reads, which reach 7.0 alone), its gradient 373 us
+// (2.28 GB and the padding, 6.5 TB/s).
 #include "model.cuh"
 
 using namespace lcpp;

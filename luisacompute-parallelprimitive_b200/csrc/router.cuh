@@ -31,11 +31,13 @@
 //
 // What has to move is a row's logits once (and, backward, its gradient) and 8
 // bytes a choice.  131072 rows of 256 bfloat16 logits, top 8: forward 44 us, of
-// which the copy rate would take 11.8, gradient 42 us (22.2).  Both are bound by
-// instructions: forward issues 826 per four rows (59 % of the issue slots, the
-// integer pipe at 57 %), about 170 of them the lanes' heads and 180 the rounds;
-// the gradient 745 (58 %, the exponential unit at 46 % with sigmoid scores).
-// 65536 rows of 256 32-bit logits: forward 37 us (11.1), gradient 26 us (21.6).
+// which the copy rate would take 11.8, gradient 40 us (22.2; sigmoid scores).
+// Neither memory nor a pipe is what bounds them, but dependent steps and too few
+// warps to fill the time: forward issues 830 instructions per four rows in 59 % of
+// the issue slots (integer pipe 57 %, 24 warps an SM), about 170 of them the lanes'
+// heads and 180 the rounds, each of which waits for shuffles of the one before; the
+// gradient 725 in 58 % (exponential unit 47 %, 16 warps an SM).  65536 rows of 256
+// 32-bit logits: forward 36 us (11.1), gradient 26 us (21.6).
 #pragma once
 
 #include "model.cuh"
@@ -294,7 +296,7 @@ __device__ __forceinline__ float sigmoid(float x)
 
 // Two sums or products in one instruction: forward 895 -> 826 instructions per
 // four rows of 256 (45 -> 44 us), sigmoid gradient 900 -> 745 (43 -> 42 us; 128
-// experts 13.9 -> 12.9 us).
+// experts, softmax 13.9 -> 12.9 us).
 __device__ __forceinline__ float2 both(float x) { return {x, x}; }
 __device__ __forceinline__ float2 add2(float2 a, float2 b)
 {
@@ -443,8 +445,8 @@ __device__ __forceinline__ float weight_score(float x, float most)
 }
 
 // What the choice goes by: logits, logits + bias, or scores + bias.  Scores are
-// computed for it and again for the sums, so that the words' registers are not
-// held beside them (131072 rows of 256 bfloat16, sigmoid: 48, 71 and 86 us).
+// computed for the choice and again for the sums (131072 rows of 256 bfloat16,
+// sigmoid: 48, 72 and 84 us).
 enum Choice { kByLogit, kByBiasedLogit, kByBiasedScore };
 
 // The 32-bit value an expert is chosen by.  All that compare two of them go
@@ -877,7 +879,9 @@ __device__ __forceinline__ int leading_lane(bool leads, int sub)
 }
 
 // The largest logit left in a row's tile and its slope.  Rarely needed, so it
-// reads the tile again instead of keeping it.
+// reads the tile again instead of keeping it; out of line, it also takes the
+// pressure off the sigmoid kernels' registers (131072 rows of 256 bfloat16: 160
+// bytes of spills and 41.4 us before, none and 39.7 now).
 template <typename T, int LANES, int C>
 __device__ __noinline__ float2 leader_left(const uint4* tile, const float* pull, int wl)
 {
@@ -1222,7 +1226,7 @@ lcpp_status forward_rows(const Params& p, bool sigmoid, cudaStream_t s)
     return forward_shape<T, 32, 32>(p, sigmoid, s);
 }
 
-// The same for the gradient.  131072 rows of 256: 8 x 32 42 us, 16 x 16 47, 32 x 8
+// The same for the gradient.  131072 rows of 256: 8 x 32 42 us (40 now), 16 x 16 47, 32 x 8
 // 61; of 64: 8 x 8 17, 4 x 16 17 (but 47 against 29 for 61 experts, whose rows
 // allow no wide access), 8 x 16 23; 65536 of 512: 16 x 32 36, 32 x 16 38.
 template <typename T>
