@@ -64,7 +64,7 @@ inline uint64_t span_bytes(uint64_t rows, uint64_t stride, uint64_t columns, int
 inline bool overlap_rows(const void* base, uint64_t rows, uint64_t stride, uint64_t columns, int element, const void* a,
                          uint64_t bytes)
 {
-    if (!overlap(base, span_bytes(rows, stride, columns, element), a, bytes)) return false;
+    if (!columns || !overlap(base, span_bytes(rows, stride, columns, element), a, bytes)) return false;
     const uintptr_t x = reinterpret_cast<uintptr_t>(base), y = reinterpret_cast<uintptr_t>(a);
     if (rows == 1 || y < x) return true;
     const uint64_t pitch = stride * uint64_t(element), at = (y - x) % pitch;

@@ -38,6 +38,23 @@ def test_extend_outputs_between_rows(lcpp):
     assert int(used) == want_used
 
 
+def test_rows_without_columns_share_nothing(lcpp):
+    """Rows of no elements (through the C entry point: an empty tensor has no address): what lies between their
+    starts is free for other arrays."""
+    t, k, e = 6, 2, 4
+    experts = np.tile(np.array([[0, 3]], np.int32), (t, 1))
+    starts, row_of, pair_of = check_plan(lcpp, experts, e, 2)
+    floats = torch.full((400,), 5.0, device="cuda")
+    weights, grad_weights = floats[1:1 + t * k], floats[201:201 + t * k]
+    rows, grad_rows = floats.data_ptr(), floats[200:].data_ptr()
+    torch.cuda.synchronize()
+    status = lcpp.lib().lcpp_dispatch_combine_backward(
+        rows, 0, rows, 8, row_of.data_ptr(), pair_of.data_ptr(), starts.data_ptr(), weights.data_ptr(), grad_rows, 8,
+        grad_weights.data_ptr(), t, k, e, pair_of.numel(), 0, lcpp.F32, torch.cuda.current_stream().cuda_stream)
+    assert status == lcpp.OK
+    assert not host(grad_weights).any() and (host(floats)[:200] == 5.0).all()
+
+
 @pytest.mark.parametrize("h", [24, 640, 4104])
 def test_combine_gradient_over_the_weights(lcpp, h):
     """The weights' gradient takes the weights' place: the same bits as beside them."""
