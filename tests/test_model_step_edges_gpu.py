@@ -334,6 +334,22 @@ def test_route_bias_on_scores_of_broken_rows(lcpp):
         np.testing.assert_array_equal(host(experts)[7], [11, 10])
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_accuracy(lcpp, kind, score, renormalize):
+    """Ordinary logits: an exponential is good to 2^-22 and half a unit of its argument (below 16: 2^-21), a lane's
+    sum of 32 to 32 half units (2^-19), a quotient to 2^-22: 3.3e-6 in all for a weight, and so for the loss."""
+    rng = np.random.default_rng(29)
+    for t, e, k in ((500, 8, 2), (500, 60, 6), (300, 256, 8), (6000, 160, 6), (100, 1000, 10)):
+        logits = cuda((rng.standard_normal((t, e)) * 1.5).astype(np.float32)).to(TYPES[kind])
+        weights, experts, _, _, loss = run_route(lcpp, logits, k, score, renormalize)
+        want = ref.route(host(logits.float()), k, score, renormalize, SCALE, COEF)
+        np.testing.assert_array_equal(host(experts), want[1])
+        np.testing.assert_allclose(host64(weights), want[0], rtol=3.3e-6, atol=0)
+        assert abs(float(loss) - want[4]) <= 3.3e-6 * want[4]
+
+
 @pytest.mark.parametrize("score", [ref.SOFTMAX, ref.SIGMOID])
 @pytest.mark.parametrize("t", [40, 4000, 60_001])
 @pytest.mark.parametrize("logit", [-12.0, -30.0, -45.0, -60.0, -75.0])
