@@ -29,7 +29,10 @@ typedef enum lcpp_kernel_kind {
     LCPP_KERNEL_SELECT = 8,         /* DeviceSelect / DevicePartition */
     LCPP_KERNEL_BLOCK_TABLE = 9,    /* DeviceBlockTable (lcpp_b200_model.h) */
     LCPP_KERNEL_ROUTER = 10,        /* DeviceRouter */
-    LCPP_KERNEL_DISPATCH = 11       /* DeviceDispatch */
+    LCPP_KERNEL_DISPATCH = 11,      /* DeviceDispatch */
+    LCPP_KERNEL_ROTARY = 12,        /* DeviceRotary */
+    LCPP_KERNEL_PAGED_ATTENTION = 13, /* DevicePagedAttention */
+    LCPP_KERNEL_CACHE_EVICTION = 14 /* DeviceCacheEviction */
 } lcpp_kernel_kind;
 
 typedef struct lcpp_kernel_time {

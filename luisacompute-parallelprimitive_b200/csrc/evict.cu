@@ -1,0 +1,529 @@
+// evict.cu -- DeviceCacheEviction (include/lcpp_b200_model.h): requests cut down
+// to the tokens with the most attention weight.
+//
+// A request's tokens get 32-bit keys that order like (protected, score); the
+// budget-th largest key comes out of four passes over 8 of its bits, each a
+// histogram of the keys that share the bits found so far.  Tokens above it are
+// kept, and of those equal to it the first ones.  A kept token past the first
+// `budget` places fills a place whose token is not kept: numbers within two
+// counts over the tokens pair them off, no other token moves, and moves do not
+// touch one another's slots.
+//
+// A cluster of 1 to 8 blocks works on a request, each on a run of its tokens
+// whose keys stay in shared memory; the blocks read one another's histograms and
+// counts there.  A histogram has a copy for each lane of a warp: scores have few
+// leading bits, and one copy would serialise on them.
+#include <cooperative_groups.h>
+
+#include "cache.cuh"
+
+namespace cg = cooperative_groups;
+using namespace lcpp;
+using namespace lcpp::model;
+
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / kWarp;
+constexpr int kMostCluster = 8;
+constexpr uint32_t kKeys = 40 * 1024;  // keys of a block that stay in shared memory; others are read again
+constexpr uint32_t kProtected = 0xffffffffu, kNaN = 0xfffffffeu;
+
+struct Params {
+    const int32_t* lens;
+    const int32_t* table;
+    uint64_t table_stride;
+    const float* scores;
+    const int32_t* positions;
+    const int32_t* evicted;
+    Divider page;
+    uint32_t longest, num_pages, requests;
+    uint32_t budget, trigger, first, recent, max_moves;
+    int32_t* lens_out;
+    int32_t* evicted_out;
+    int32_t* counts;
+    longlong2* moves;
+};
+
+// What the blocks of a cluster read of one another.
+struct Shared {
+    uint32_t histogram[2][256];
+    uint32_t broken;            // a page id out of range
+    uint32_t holes, fillers;    // of the block's tokens
+};
+
+__device__ __forceinline__ uint32_t key_of(float score)
+{
+    if (score != score) return kNaN;
+    const uint32_t bits = __float_as_uint(score + 0.f);  // + 0: both zeros alike
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+
+__device__ __forceinline__ uint32_t length_of(const int32_t* lens, uint32_t r, uint32_t longest)
+{
+    return min(uint32_t(max(lens[r], 0)), longest);
+}
+
+// Sum over the block, and over the threads before.
+__device__ __forceinline__ uint32_t warps_before(uint32_t of_warp, uint32_t* warps, uint32_t& total)
+{
+    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+    __syncthreads();
+    if (lane == 0) warps[warp] = of_warp;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) before = total;
+        total += warps[w];
+    }
+    return before;
+}
+
+__global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
+{
+    extern __shared__ uint32_t dynamic[];
+    uint32_t* copies = dynamic;  // [256][32]
+    uint32_t* keys = dynamic + 256 * kWarp;
+    __shared__ Shared shared;
+    __shared__ uint32_t warps[kWarps];
+    __shared__ uint32_t found[3];  // digit, keys above it, keys equal to it in the blocks before
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t r = blockIdx.x / blocks;
+    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+    let_next_start();
+
+    const uint32_t n = length_of(p.lens, r, p.longest);
+    const int32_t before = p.evicted ? p.evicted[r] : 0;
+    const auto leave = [&] {  // as it is
+        if (rank == 0 && threadIdx.x == 0) {
+            p.lens_out[r] = int32_t(n);
+            p.counts[r] = 0;
+            if (p.evicted_out) p.evicted_out[r] = before;
+        }
+    };
+    if (n <= p.trigger) {
+        leave();
+        return;
+    }
+    // the block's run of tokens
+    const uint32_t run = (n + blocks - 1) / blocks, lo = min(n, rank * run), count = min(n - lo, run);
+    const int32_t* row = p.table + r * p.table_stride;
+    const int64_t recent = int64_t(n) + before - p.recent;
+    const auto slot_of = [&](uint32_t token, uint32_t& id) {
+        const uint32_t page = p.page.quotient(token);
+        id = uint32_t(row[page]);
+        return uint64_t(id) * p.page.d + (token - page * p.page.d);
+    };
+    const auto look_up = [&](uint32_t i, bool& broken) {
+        uint32_t id;
+        const uint64_t slot = slot_of(lo + i, id);
+        if (id >= p.num_pages) {
+            broken = true;
+            return 0u;
+        }
+        const int64_t position = p.positions ? int64_t(p.positions[slot]) : int64_t(lo + i);
+        return position < p.first || position >= recent ? kProtected : key_of(p.scores[slot]);
+    };
+    const auto key_at = [&](uint32_t i) {
+        bool broken = false;
+        return i < kKeys ? keys[i] : look_up(i, broken);
+    };
+
+    if (threadIdx.x == 0) shared.broken = 0;
+    for (int i = threadIdx.x; i < 256 * kWarp; i += kThreads) copies[i] = 0;
+    __syncthreads();
+    bool broken = false;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        const uint32_t key = look_up(i, broken);
+        if (i < kKeys) keys[i] = key;
+        atomicAdd(&copies[(key >> 24) * kWarp + lane], 1u);
+    }
+    if (broken) shared.broken = 1;
+
+    uint32_t top = 0, need = p.budget;  // bits found; tokens to keep among the keys that share them
+    uint32_t equal_before = 0;          // keys equal to the last one in the blocks before this one
+    for (int pass = 0; pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+        if (pass) {
+            for (int i = threadIdx.x; i < 256 * kWarp; i += kThreads) copies[i] = 0;
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+                const uint32_t key = key_at(i);
+                if ((key ^ top) >> (shift + 8) == 0) atomicAdd(&copies[(key >> shift & 255) * kWarp + lane], 1u);
+            }
+        }
+        __syncthreads();
+        for (int digit = warp; digit < 256; digit += kWarps) {
+            const uint32_t sum = __reduce_add_sync(~0u, copies[digit * kWarp + lane]);
+            if (lane == 0) shared.histogram[pass & 1][digit] = sum;
+        }
+        cluster.sync();  // the other buffer is free again, too
+        if (pass == 0) {
+            uint32_t any = 0;
+            for (uint32_t b = 0; b < blocks; ++b) any |= cluster.map_shared_rank(&shared, b)->broken;
+            if (any) {
+                leave();
+                cluster.sync();
+                return;
+            }
+        }
+        uint32_t mine = 0, equal = 0;  // of digit 255 - thread, in all blocks and in those before
+        if (threadIdx.x < 256) {
+            for (uint32_t b = 0; b < blocks; ++b) {
+                const uint32_t c = cluster.map_shared_rank(&shared, b)->histogram[pass & 1][255 - threadIdx.x];
+                mine += c;
+                if (b < rank) equal += c;
+            }
+        }
+        uint32_t upto = mine;
+#pragma unroll
+        for (int d = 1; d < kWarp; d *= 2) {
+            const uint32_t left = __shfl_up_sync(~0u, upto, d);
+            if (lane >= d) upto += left;
+        }
+        uint32_t all;
+        upto += warps_before(__shfl_sync(~0u, upto, kWarp - 1), warps, all);
+        if (upto >= need && upto - mine < need) {  // one thread: there are more than `need` such keys
+            found[0] = 255 - threadIdx.x;
+            found[1] = upto - mine;
+            found[2] = equal;
+        }
+        __syncthreads();
+        top |= found[0] << shift;
+        need -= found[1];
+        equal_before = found[2];
+        __syncthreads();
+    }
+
+    // Each warp takes a run of the block's tokens, 32 at a time.  Equal keys are
+    // numbered first, then holes and fillers counted, then numbered.
+    const uint32_t part = uint32_t(align_up(ceil_div(count, kWarps), kWarp));
+    const uint32_t from = min(count, warp * part), to = min(count, from + part);
+    uint32_t total;
+    uint32_t equals = 0;
+    for (uint32_t i = from; i < to; i += kWarp) {
+        const bool in = i + lane < to;
+        equals += __popc(__ballot_sync(~0u, in && key_at(i + lane) == top));
+    }
+    const uint32_t equal_base = equal_before + warps_before(equals, warps, total);
+    const auto sort_out = [&](auto take) {  // take(lane's token in the block, hole mask, filler mask)
+        uint32_t number = equal_base;
+        for (uint32_t i = from; i < to; i += kWarp) {
+            const bool in = i + lane < to;
+            const uint32_t key = in ? key_at(i + lane) : 0;
+            const uint32_t same = __ballot_sync(~0u, in && key == top);
+            const bool kept = key > top || (key == top && number + __popc(same & lanemask_lt()) < need);
+            number += __popc(same);
+            const bool front = lo + i + lane < p.budget;
+            take(i + lane, __ballot_sync(~0u, in && front && !kept), __ballot_sync(~0u, in && !front && kept));
+        }
+    };
+    uint32_t holes = 0, fillers = 0;
+    sort_out([&](uint32_t, uint32_t hole, uint32_t filler) {
+        holes += __popc(hole);
+        fillers += __popc(filler);
+    });
+    uint32_t hole = warps_before(holes, warps, total);
+    if (threadIdx.x == 0) shared.holes = total;
+    uint32_t filler = warps_before(fillers, warps, total);
+    if (threadIdx.x == 0) shared.fillers = total;
+    cluster.sync();
+    uint32_t moves = 0;
+    for (uint32_t b = 0; b < blocks; ++b) {
+        const Shared* other = cluster.map_shared_rank(&shared, b);
+        if (b < rank) {
+            hole += other->holes;
+            filler += other->fillers;
+        }
+        moves += other->fillers;
+    }
+    cluster.sync();  // nobody leaves while others read
+    if (moves > p.max_moves) {
+        leave();
+        return;
+    }
+    longlong2* out = p.moves + uint64_t(r) * p.max_moves;
+    sort_out([&](uint32_t i, uint32_t hole_mask, uint32_t filler_mask) {
+        const bool is_hole = hole_mask >> lane & 1, is_filler = filler_mask >> lane & 1;
+        if (is_hole || is_filler) {
+            uint32_t id;
+            const int64_t slot = int64_t(slot_of(lo + i, id));
+            if (is_filler) out[filler + __popc(filler_mask & lanemask_lt())].x = slot;
+            else out[hole + __popc(hole_mask & lanemask_lt())].y = slot;
+        }
+        hole += __popc(hole_mask);
+        filler += __popc(filler_mask);
+    });
+    if (rank == 0 && threadIdx.x == 0) {
+        p.lens_out[r] = int32_t(p.budget);
+        p.counts[r] = int32_t(moves);
+        if (p.evicted_out) p.evicted_out[r] = int32_t(before + int64_t(n) - p.budget);
+    }
+}
+
+// The pages that no token needs any more, back on the free list.
+__global__ void __launch_bounds__(kThreads) release_kernel(const Params p, int32_t* free_blocks, const int32_t* free_used,
+                                                           int32_t* free_used_out, uint32_t num_free)
+{
+    wait_for_previous();
+    const auto pages = [&](uint32_t tokens) { return tokens ? p.page.quotient(tokens - 1) + 1 : 0u; };
+    const auto kept = [&](uint32_t r) { return pages(uint32_t(p.lens_out[r])); };
+    const auto freed = [&](uint32_t r) { return (long long)(pages(length_of(p.lens, r, p.longest)) - kept(r)); };
+    long long begin = -1, end = -1;
+    Place place;
+    const long long total = share_of<kThreads>(
+        p.requests, freed,
+        [&](long long all) {
+            const long long per = (all + gridDim.x - 1) / gridDim.x;
+            begin = blockIdx.x * per;
+            end = min(all, begin + per);
+            return begin < all ? begin : -1;
+        },
+        place);
+    const long long used = min((long long)max(*free_used, 0), (long long)num_free);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *free_used_out = int32_t(max(used - total, 0ll));
+    if (begin >= total) return;
+    uint32_t r = place.item;
+    long long first = place.first;
+    for (long long i = begin + threadIdx.x; i < end; i += kThreads) {
+        while (i >= first + freed(r)) first += freed(r++);
+        const long long at = used - total + i;
+        if (at >= 0) free_blocks[at] = p.table[r * p.table_stride + kept(r) + uint32_t(i - first)];
+    }
+}
+
+struct Moves {
+    unsigned char* k;
+    unsigned char* v;
+    uint64_t page, token, head;  // strides in bytes
+    Divider vectors;             // accesses of a head
+    uint32_t heads, block_size;
+    uint64_t num_slots;
+    const longlong2* moves;
+    const int32_t* counts;
+    uint32_t max_moves, requests;
+    float* scores;
+    int32_t* positions;
+};
+
+// A warp takes a move: all heads' keys and values of a token, V at a time, four
+// of them (or a head's last ones) under way in each lane.
+constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / kWarp, kMoveAhead = 4;
+template <typename V>
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const Moves p)
+{
+    const auto moves_of = [&](uint32_t r) { return (long long)min(uint32_t(max(p.counts[r], 0)), p.max_moves); };
+    long long begin = -1, end = -1;
+    Place place;
+    const long long total = share_of<kMoveThreads>(
+        p.requests, moves_of,
+        [&](long long all) {
+            const long long per = (all + gridDim.x - 1) / gridDim.x;
+            begin = blockIdx.x * per;
+            end = min(all, begin + per);
+            return begin < all ? begin : -1;
+        },
+        place);
+    if (begin >= total) return;
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    const uint32_t each = p.heads * p.vectors.d;
+    uint32_t r = place.item;
+    long long first = place.first;
+    for (long long i = begin + warp; i < end; i += kMoveWarps) {
+        while (i >= first + moves_of(r)) first += moves_of(r++);
+        const longlong2 move = p.moves[uint64_t(r) * p.max_moves + uint64_t(i - first)];
+        const uint64_t from = uint64_t(move.x), to = uint64_t(move.y);
+        if (from >= p.num_slots || to >= p.num_slots) continue;
+        const uint64_t from_page = from / p.block_size, to_page = to / p.block_size;
+        const uint64_t from_at = from_page * p.page + (from - from_page * p.block_size) * p.token;
+        const uint64_t to_at = to_page * p.page + (to - to_page * p.block_size) * p.token;
+        for (uint32_t at = lane; at < each; at += kWarp * kMoveAhead) {
+            V k[kMoveAhead], v[kMoveAhead];
+            uint64_t offset[kMoveAhead];
+#pragma unroll
+            for (int u = 0; u < kMoveAhead; ++u) {
+                const uint32_t x = at + u * kWarp;
+                if (x >= each) continue;
+                const uint32_t head = p.vectors.quotient(x);
+                offset[u] = head * p.head + (x - head * p.vectors.d) * sizeof(V);
+                k[u] = *reinterpret_cast<const V*>(p.k + from_at + offset[u]);
+                v[u] = *reinterpret_cast<const V*>(p.v + from_at + offset[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kMoveAhead; ++u) {
+                if (at + u * kWarp >= each) continue;
+                *reinterpret_cast<V*>(p.k + to_at + offset[u]) = k[u];
+                *reinterpret_cast<V*>(p.v + to_at + offset[u]) = v[u];
+            }
+        }
+        if (lane == 0) {
+            if (p.scores) p.scores[to] = p.scores[from];
+            if (p.positions) p.positions[to] = p.positions[from];
+        }
+    }
+}
+
+lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
+{
+    if (!a || !a->block_size || !a->budget || a->budget >= uint32_t(1) << 31 || a->trigger < a->budget ||
+        uint64_t(a->keep_first) + a->keep_recent > a->budget || a->num_requests > LCPP_MAX_REQUESTS ||
+        a->table_stride < a->table_width || a->table_stride > kMostStride ||
+        uint64_t(a->num_pages) * a->block_size >= kMostSlots)
+        return LCPP_ERR_INVALID_ARG;
+    const uint64_t n = a->num_requests, slots = uint64_t(a->num_pages) * a->block_size;
+    const bool release = a->free_blocks || a->free_used || a->free_used_out;
+    if (release && (!a->free_used || !a->free_used_out || (a->num_free && !a->free_blocks))) return LCPP_ERR_INVALID_ARG;
+    if (n && (!a->seq_lens || !a->seq_lens_out || !a->move_counts_out || (a->max_moves && !a->moves_out) ||
+              (a->table_width && !a->block_table) || (slots && !a->slot_scores)))
+        return LCPP_ERR_INVALID_ARG;
+    const void* words[] = {a->seq_lens,        a->block_table,  a->slot_scores,     a->slot_positions, a->evicted,
+                           a->seq_lens_out,    a->evicted_out,  a->move_counts_out, a->free_blocks,    a->free_used,
+                           a->free_used_out};
+    for (const void* w : words)
+        if (misaligned(w, 4)) return LCPP_ERR_INVALID_ARG;
+    if (misaligned(a->moves_out, 16)) return LCPP_ERR_INVALID_ARG;
+    const bool in_place = a->evicted == a->evicted_out;
+    const Array arrays[] = {{a->seq_lens, n * 4, false},
+                            {a->slot_scores, slots * 4, false},
+                            {a->slot_positions, a->slot_positions ? slots * 4 : 0, false},
+                            {in_place ? nullptr : a->evicted, n * 4, false},
+                            {a->seq_lens_out, n * 4, true},
+                            {a->evicted_out, n * 4, true},
+                            {a->move_counts_out, n * 4, true},
+                            {a->moves_out, n * a->max_moves * 16, true},
+                            {a->free_blocks, uint64_t(a->num_free) * 4, true},
+                            {a->free_used, 4, false},
+                            {a->free_used_out, 4, true}};
+    if (clash(arrays)) return LCPP_ERR_INVALID_ARG;
+    for (const Array& o : arrays)
+        if (o.written && overlap_rows(a->block_table, n, a->table_stride, a->table_width, 4, o.p, o.bytes))
+            return LCPP_ERR_INVALID_ARG;
+
+    Params p{};
+    p.lens = a->seq_lens;
+    p.table = a->block_table;
+    p.table_stride = a->table_stride;
+    p.scores = a->slot_scores;
+    p.positions = a->slot_positions;
+    p.evicted = a->evicted;
+    p.page = Divider(a->block_size);
+    p.longest = uint32_t(std::min<uint64_t>(uint64_t(a->table_width) * a->block_size, 0x7fffffffu));
+    p.num_pages = a->num_pages;
+    p.requests = a->num_requests;
+    p.budget = a->budget;
+    p.trigger = a->trigger;
+    p.first = a->keep_first;
+    p.recent = a->keep_recent;
+    p.max_moves = a->max_moves;
+    p.lens_out = a->seq_lens_out;
+    p.evicted_out = a->evicted_out;
+    p.counts = a->move_counts_out;
+    p.moves = reinterpret_cast<longlong2*>(a->moves_out);
+
+    diag::KernelTimer timer(kTimerEviction, n, s);
+    if (n) {
+        // Blocks of 2048 tokens and more, as long as the requests leave SMs for them.
+        uint32_t cluster = 1;
+        while (cluster < kMostCluster && p.longest / cluster > 4096 && n * cluster * 2 <= uint64_t(device_sm_count()) * 2)
+            cluster *= 2;
+        const uint32_t run = uint32_t(ceil_div(p.longest, cluster));
+        // room in a few steps, so that few launch shapes are set up
+        uint32_t room = 4096;
+        while (room < kKeys && room < run) room *= 2;
+        const size_t smem = (256 * kWarp + std::min(room, kKeys)) * 4;
+        set_max_dynamic_smem(reinterpret_cast<const void*>(plan_kernel), (256 * kWarp + kKeys) * 4);
+        cudaLaunchAttribute shape{};
+        shape.id = cudaLaunchAttributeClusterDimension;
+        shape.val.clusterDim.x = cluster;
+        shape.val.clusterDim.y = shape.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(unsigned(n * cluster));
+        config.blockDim = dim3(kThreads);
+        config.dynamicSmemBytes = smem;
+        config.stream = s;
+        config.attrs = &shape;
+        config.numAttrs = 1;
+        LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, plan_kernel, p));
+    }
+    if (!release) return LCPP_OK;
+    if (n == 0) {
+        release_kernel<<<1, kThreads, 0, s>>>(p, a->free_blocks, a->free_used, a->free_used_out, a->num_free);
+        return launched();
+    }
+    return launch_early(release_kernel, unsigned(std::min<uint64_t>(n, device_sm_count())), kThreads, 0, s, Params(p),
+                        static_cast<int32_t*>(a->free_blocks), static_cast<const int32_t*>(a->free_used),
+                        static_cast<int32_t*>(a->free_used_out), uint32_t(a->num_free));
+}
+
+lcpp_status move(const lcpp_kv_cache* c, const int64_t* moves, uint32_t max_moves, const int32_t* counts,
+                 uint32_t num_requests, float* scores, int32_t* positions, cudaStream_t s)
+{
+    if (!c || !sane_cache(*c) || num_requests > LCPP_MAX_REQUESTS) return LCPP_ERR_INVALID_ARG;
+    const int e = row_dtype_bytes(c->dtype);
+    if (!e) return LCPP_ERR_UNSUPPORTED_DTYPE;
+    const uint64_t n = num_requests, slots = uint64_t(c->num_pages) * c->block_size;
+    if (!n || !max_moves || !slots) return LCPP_OK;
+    if (!moves || !counts || !c->k || !c->v || misaligned(moves, 16) || misaligned(counts, 4) || misaligned(c->k, e) ||
+        misaligned(c->v, e) || misaligned(scores, 4) || misaligned(positions, 4) || !writable_cache(*c))
+        return LCPP_ERR_INVALID_ARG;
+    const Strided k = pages_of(*c, c->k), v = pages_of(*c, c->v);
+    const Array arrays[] = {{moves, n * max_moves * 16, false},
+                            {counts, n * 4, false},
+                            {scores, slots * 4, true},
+                            {positions, slots * 4, true}};
+    if (clash(arrays)) return LCPP_ERR_INVALID_ARG;
+    for (const Array& x : arrays)
+        if (overlap(k.p, k.bytes(), x.p, x.bytes) || overlap(v.p, v.bytes(), x.p, x.bytes)) return LCPP_ERR_INVALID_ARG;
+    if (uint64_t(c->num_kv_heads) * c->head_dim >= uint64_t(1) << 31) return LCPP_ERR_INVALID_ARG;
+
+    const bool wide = c->head_dim * e % 16 == 0 && rows_aligned(c->k, {c->page_stride, c->token_stride, c->head_stride}, e, 16) &&
+                      !misaligned(c->v, 16);
+    const uint32_t access = wide ? 16 : e;
+    Moves p{};
+    p.k = static_cast<unsigned char*>(c->k);
+    p.v = static_cast<unsigned char*>(c->v);
+    p.page = c->page_stride * e;
+    p.token = c->token_stride * e;
+    p.head = c->head_stride * e;
+    p.vectors = Divider(c->head_dim * e / access);
+    p.heads = c->num_kv_heads;
+    p.block_size = c->block_size;
+    p.num_slots = slots;
+    p.moves = reinterpret_cast<const longlong2*>(moves);
+    p.counts = counts;
+    p.max_moves = max_moves;
+    p.requests = num_requests;
+    p.scores = scores;
+    p.positions = positions;
+    const auto launch = [&](auto kernel) {
+        const uint64_t most = uint64_t(device_sm_count()) * resident_blocks(reinterpret_cast<const void*>(kernel), kMoveThreads, 0);
+        const unsigned blocks = unsigned(std::min<uint64_t>(most, ceil_div(n * max_moves, kMoveWarps)));
+        kernel<<<blocks, kMoveThreads, 0, s>>>(p);
+        return launched();
+    };
+    diag::KernelTimer timer(kTimerEviction, n, s);
+    return wide ? launch(move_kernel<uint4>) : e == 4 ? launch(move_kernel<uint32_t>) : launch(move_kernel<unsigned short>);
+}
+
+}  // namespace
+
+extern "C" {
+
+lcpp_status lcpp_cache_evict_plan(const lcpp_cache_evict_args* args, lcpp_stream_t stream)
+{
+    return guarded("lcpp_cache_evict_plan", [&] { return plan(args, reinterpret_cast<cudaStream_t>(stream)); });
+}
+
+lcpp_status lcpp_cache_evict_move(const lcpp_kv_cache* cache, const int64_t* moves, uint32_t max_moves,
+                                  const int32_t* move_counts, uint32_t num_requests, float* slot_scores,
+                                  int32_t* slot_positions, lcpp_stream_t stream)
+{
+    return guarded("lcpp_cache_evict_move", [&] {
+        return move(cache, moves, max_moves, move_counts, num_requests, slot_scores, slot_positions,
+                    reinterpret_cast<cudaStream_t>(stream));
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,899 @@
+// paged_attention.cuh -- DevicePagedAttention (include/lcpp_b200_model.h): one
+// new query of each request over the pages of its keys and values.
+//
+// With x_t = scale q . k_t (base 2 from here on), one pass over the tokens keeps
+// a reference m, the sum l of 2^(x_t - m) and the vector o of 2^(x_t - m) v_t;
+// parts of the tokens join as o = sum_i 2^(m_i - M) o_i, l alike, out = o / l.
+// m follows the maximum only when a logit passes it by 2^8: between, a tile costs
+// a vote instead of reductions and rescaling, and no term leaves its range.
+//
+// Work.  A unit is a request's tokens under one kv head, with up to 8 to 32
+// query heads on it, cut into tiles of 16 tokens.  All tiles of the call are
+// numbered and every block takes an equal run of them, so a few long requests
+// fill the GPU as well as many short ones.  The lengths are on the device: each
+// block sums them itself.  A unit that a run covers whole is written out by its
+// block, the parts of the others by join_kernel, which starts early and waits.
+//
+// A warp works on its own: it takes every fourth tile of the run, copies the
+// tile's rows (16 keys, 16 values) into a ring of its own with cp.async, some
+// tiles ahead and across the borders of units, and needs the block's other warps
+// only where a unit ends.  The page ids of the next tile are read one tile before
+// they are needed.
+#pragma once
+
+#include "cache.cuh"
+
+namespace lcpp {
+namespace model {
+namespace attention {
+
+constexpr int kTile = 16;              // tokens of a tile
+constexpr uint32_t kMostBlocks = 640;  // the partial results' room
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Params {
+    const void* q;
+    void* out;
+    const void* k;
+    const void* v;
+    uint64_t q_request, q_head, out_request, out_head;
+    uint64_t page_stride, token_stride, head_stride;
+    const int32_t* table;
+    uint64_t table_stride;
+    const int32_t* lens;
+    Divider page;         // by the page size
+    uint32_t longest;     // tokens that a row of the table holds
+    uint32_t num_pages;
+    uint32_t requests, heads, kv_heads, group;
+    uint32_t chunks;      // units that a kv head's queries are divided into
+    uint32_t per_unit;    // query heads of a unit, at most
+    uint32_t dim;
+    uint32_t window;
+    float scale;          // with log2 e, or with 1 / softcap
+    float softcap;        // with log2 e; 0: none
+    float* lse;
+    float* part;          // [block][2][heads of a unit][columns] and, behind them, [block][2][heads of a unit][2]
+    int32_t* meta;        // [block][4]
+    float* logits;        // [tile][per_unit][16] in base 2, or NULL
+    long long logit_tiles;
+    float* lse2;          // [request][head] in base 2 for the scores
+    long long* first;     // [request] number of its first tile, for the scores
+    const float* scores;
+    float* scores_out;
+    float decay;
+};
+
+// A request's tokens: [first, end) in tiles of 16.
+struct Tokens {
+    uint32_t first, end;
+    __device__ __forceinline__ uint32_t tiles() const { return (end - first + kTile - 1) / kTile; }
+};
+__device__ __forceinline__ Tokens tokens_of(const Params& p, uint32_t r)
+{
+    const uint32_t n = min(uint32_t(max(p.lens[r], 0)), p.longest);
+    return Tokens{p.window && n > p.window ? n - p.window : 0u, n};
+}
+
+// The block's run of tiles, and the walk over the parts of units in it.
+struct Walk {
+    uint32_t r, unit, tiles, t, t_end;
+    Tokens tokens;
+    long long left;  // tiles of the run behind this part
+
+    __device__ __forceinline__ void part()
+    {
+        const long long room = left;
+        t_end = uint32_t(min((long long)tiles, t + room));
+        left = room - (t_end - t);
+    }
+    // To the part after this one; false: the run has ended.
+    __device__ __forceinline__ bool next(const Params& p)
+    {
+        if (left == 0) return false;
+        t = 0;
+        if (++unit == p.kv_heads * p.chunks) {
+            unit = 0;
+            do {
+                tokens = tokens_of(p, ++r);  // the run has tiles left, so there is such a request
+                tiles = tokens.tiles();
+            } while (tiles == 0);
+        }
+        part();
+        return true;
+    }
+};
+
+__device__ __forceinline__ uint32_t smem_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void copy_16b(uint32_t to, const void* from, bool valid)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float logit(const Params& p, float dot)
+{
+    const float x = dot * p.scale;
+    return p.softcap > 0.f ? p.softcap * tanhf(x) : x;
+}
+// Factor of what was summed under reference `from` when it becomes `to`.
+__device__ __forceinline__ float rebase(float from, float to) { return from == -INFINITY ? 0.f : exp2_fast(from - to); }
+
+// ---------------------------------------------------------------------------
+// A warp's tile in 16 bits: tensor cores, tokens as rows and heads as columns
+// of the first product, the head's columns as rows of the second one.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void load_matrices_transposed(uint32_t (&r)[4], uint32_t at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x)
+{
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <typename T>
+__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void multiply<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void multiply<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Swizzle of a row's 16-byte chunks: 8 rows of one chunk, or 8 chunks of one row,
+// lie in different banks.
+__device__ __forceinline__ int swizzled(int row, int chunk) { return chunk ^ (row & 7); }
+
+template <typename T, int D, int H>
+struct Tile;
+
+// H is a multiple of 8: H / 8 tiles of 8 heads.
+template <typename T, int D, int H>
+struct Tile16 {
+    static constexpr int kN = H / 8;
+    static constexpr int kQueryBytes = D * H * 2;
+    static constexpr int kWarpBytes = 0;
+    // float16's range: terms are kept at up to 2^8 of the reference, whose own is
+    // set 2^7 up, so that they end at 2^15 and small ones keep their digits.
+    static constexpr float kShift = std::is_same<T, __half>::value ? 7.f : 0.f;
+
+    float o[D / 16][kN][4];  // column lane / 4 (+ 8), heads lane % 4 * 2 (+ 1)
+    float m[kN][2], l[kN][2];
+
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[i][n][c] = 0.f;
+        }
+    }
+
+    // Queries as the first product's second operand: lane's two words for each
+    // 16 columns and 8 heads, [16 columns][8 heads][lane].
+    static __device__ void load_queries(const Params& p, void* smem, const T* q, uint32_t heads)
+    {
+        uint32_t* to = static_cast<uint32_t*>(smem);
+        for (int i = threadIdx.x; i < D * H / 2; i += blockDim.x) {
+            const int word = i & 1, lane = (i >> 1) & 31, n = (i >> 6) % kN, step = (i >> 6) / kN;
+            const uint32_t head = n * 8 + lane / 4, column = step * 16 + word * 8 + lane % 4 * 2;
+            T pair[2] = {from_float<T>(0.f), from_float<T>(0.f)};
+            if (head < heads) {
+                if (column < p.dim) pair[0] = q[head * p.q_head + column];
+                if (column + 1 < p.dim) pair[1] = q[head * p.q_head + column + 1];
+            }
+            to[i] = uint32_t(*reinterpret_cast<const uint16_t*>(&pair[0])) |
+                    uint32_t(*reinterpret_cast<const uint16_t*>(&pair[1])) << 16;
+        }
+    }
+
+    __device__ __forceinline__ void add(const Params& p, const unsigned char* keys, const unsigned char* values,
+                                        const void* queries, void*, uint32_t valid, float* logits, uint32_t heads)
+    {
+        const int lane = threadIdx.x % kWarp;
+        float s[kN][4];
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[n][c] = 0.f;
+        const uint2* q = static_cast<const uint2*>(queries) + lane;
+        const int key_row = lane % 16;
+        const uint32_t key_at = smem_address(keys) + key_row * (D * 2);
+#pragma unroll
+        for (int step = 0; step < D / 16; ++step) {
+            uint32_t a[4];
+            load_matrices(a, key_at + swizzled(key_row, step * 2 + lane / 16) * 16);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+                const uint2 b = q[(step * kN + n) * kWarp];
+                multiply<T>(s[n], a, b.x, b.y);
+            }
+        }
+        const bool valid0 = valid >> (lane / 4) & 1, valid1 = valid >> (lane / 4 + 8) & 1;
+        bool past = false;
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                s[n][c] = (c < 2 ? valid0 : valid1) ? logit(p, s[n][c]) : -INFINITY;
+                past |= s[n][c] > m[n][c & 1] + (8.f + kShift);
+                if (logits) {
+                    const uint32_t head = n * 8 + lane % 4 * 2 + (c & 1);
+                    if (head < heads) logits[head * kTile + lane / 4 + (c < 2 ? 0 : 8)] = s[n][c];
+                }
+            }
+        }
+        if (__any_sync(~0u, past)) {
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float top = fmaxf(s[n][h], s[n][h + 2]);
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                    const float to = fmaxf(m[n][h], top - kShift), factor = rebase(m[n][h], to);
+                    m[n][h] = to;
+                    l[n][h] *= factor;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        o[i][n][h] *= factor;
+                        o[i][n][h + 2] *= factor;
+                    }
+                }
+        }
+        // Each term as two 16-bit numbers, high part and rest: 16 digits of bfloat16
+        // and 22 of float16, against 8 and 11 that one would leave.  The products with
+        // the rest cost tensor-core time that the copies leave free.
+        uint32_t high[kN][2], rest[kN][2];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            float e[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float reference = m[n][c & 1] == -INFINITY ? 0.f : m[n][c & 1];
+                e[c] = exp2_fast(s[n][c] - reference);
+                l[n][c & 1] += e[c];
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                T hi[2], lo[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    hi[h] = from_float<T>(e[w * 2 + h]);
+                    lo[h] = from_float<T>(e[w * 2 + h] - to_float(hi[h]));
+                }
+                high[n][w] = transposed(*reinterpret_cast<const uint16_t*>(&hi[0]) |
+                                        uint32_t(*reinterpret_cast<const uint16_t*>(&hi[1])) << 16);
+                rest[n][w] = transposed(*reinterpret_cast<const uint16_t*>(&lo[0]) |
+                                        uint32_t(*reinterpret_cast<const uint16_t*>(&lo[1])) << 16);
+            }
+        }
+        const int value_row = lane % 8 + lane / 16 * 8;
+        const uint32_t value_at = smem_address(values) + value_row * (D * 2);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            uint32_t a[4];
+            load_matrices_transposed(a, value_at + swizzled(value_row, i * 2 + lane / 8 % 2) * 16);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+                multiply<T>(o[i][n], a, high[n][0], high[n][1]);
+                multiply<T>(o[i][n], a, rest[n][0], rest[n][1]);
+            }
+        }
+    }
+
+    // The warp's references and sums, [head].
+    __device__ __forceinline__ void put_sums(float* m_out, float* l_out)
+    {
+        const int lane = threadIdx.x % kWarp;
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) l[n][h] += __shfl_xor_sync(~0u, l[n][h], d);
+                if (lane < 4) {
+                    m_out[n * 8 + lane * 2 + h] = m[n][h];
+                    l_out[n * 8 + lane * 2 + h] = l[n][h];
+                }
+            }
+    }
+    // Puts or adds the warp's vectors times factor[head] to sum[head][D + 4].
+    __device__ __forceinline__ void put(float* sum, const float* factor, bool first)
+    {
+        const int lane = threadIdx.x % kWarp;
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int head = n * 8 + lane % 4 * 2 + h;
+                const float f = factor[head];
+                float* to = sum + head * (D + 4) + lane / 4;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float x = o[i][n][h + c * 2] * f;
+                        float* at = to + i * 16 + c * 8;
+                        *at = first ? x : *at + x;
+                    }
+            }
+    }
+};
+
+template <int D, int H>
+struct Tile<__nv_bfloat16, D, H> : Tile16<__nv_bfloat16, D, H> {};
+template <int D, int H>
+struct Tile<__half, D, H> : Tile16<__half, D, H> {};
+
+// ---------------------------------------------------------------------------
+// A warp's tile in 32 bits: multiply-adds.  A lane takes a token and half of the
+// columns for the logits, then 4 columns (or 8, or 4 of every second token) of
+// all tokens for the vectors; the terms pass through shared memory.
+// ---------------------------------------------------------------------------
+template <int D, int H>
+struct Tile<float, D, H> {
+    static constexpr int kQueryBytes = D * H * 4;
+    static constexpr int kWarpBytes = kTile * H * 4;
+    static constexpr int kChunks = D / 4;
+    static constexpr int kLanes = kChunks < kWarp ? kChunks : kWarp;  // lanes of a row
+    static constexpr int kPer = kChunks / kLanes;                    // chunks of a lane
+    static constexpr int kTokenStep = kWarp / kLanes;
+    static constexpr float kShift = 0.f;
+    static_assert(kChunks % kLanes == 0 && kWarp % kLanes == 0, "");
+
+    float4 o[H][kPer];
+    float m[H], l[H];
+
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            m[h] = -INFINITY;
+            l[h] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) o[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+
+    static __device__ void load_queries(const Params& p, void* smem, const float* q, uint32_t heads)
+    {
+        float* to = static_cast<float*>(smem);
+        for (int i = threadIdx.x; i < D * H; i += blockDim.x) {
+            const uint32_t head = i / D, column = i % D;
+            to[i] = head < heads && column < p.dim ? q[head * p.q_head + column] : 0.f;
+        }
+    }
+
+    __device__ __forceinline__ void add(const Params& p, const unsigned char* keys, const unsigned char* values,
+                                        const void* queries, void* own, uint32_t valid, float* logits, uint32_t heads)
+    {
+        const int lane = threadIdx.x % kWarp, token = lane % 16, part = lane / 16;
+        const float4* k = reinterpret_cast<const float4*>(keys) + token * kChunks;
+        const float4* q = static_cast<const float4*>(queries);
+        float s[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) s[h] = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < kChunks / 2; ++i) {
+            const int chunk = part * (kChunks / 2) + i;
+            const float4 a = k[swizzled(token, chunk)];
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const float4 b = q[h * kChunks + chunk];
+                s[h] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s[h]))));
+            }
+        }
+        bool past = false;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            s[h] += __shfl_xor_sync(~0u, s[h], 16);
+            s[h] = valid >> token & 1 ? logit(p, s[h]) : -INFINITY;
+            past |= s[h] > m[h] + 8.f;
+            if (logits && part == 0 && h < int(heads)) logits[h * kTile + token] = s[h];
+        }
+        if (__any_sync(~0u, past)) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                float top = s[h];
+#pragma unroll
+                for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                const float to = fmaxf(m[h], top), factor = rebase(m[h], to);
+                m[h] = to;
+                l[h] *= factor;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    o[h][i].x *= factor, o[h][i].y *= factor, o[h][i].z *= factor, o[h][i].w *= factor;
+                }
+            }
+        }
+        float* term = static_cast<float*>(own);
+        __syncwarp();  // the tile before has been read
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const float e = exp2_fast(s[h] - (m[h] == -INFINITY ? 0.f : m[h]));
+            if (part == 0) {
+                l[h] += e;
+                term[token * H + h] = e;
+            }
+        }
+        __syncwarp();
+        const int column = lane % kLanes;
+        const float4* v = reinterpret_cast<const float4*>(values);
+#pragma unroll 4
+        for (int t = lane / kLanes; t < kTile; t += kTokenStep) {
+            float e[H];
+#pragma unroll
+            for (int h = 0; h < H; ++h) e[h] = term[t * H + h];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const float4 x = v[t * kChunks + swizzled(t, column + i * kLanes)];
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    o[h][i].x = fmaf(e[h], x.x, o[h][i].x);
+                    o[h][i].y = fmaf(e[h], x.y, o[h][i].y);
+                    o[h][i].z = fmaf(e[h], x.z, o[h][i].z);
+                    o[h][i].w = fmaf(e[h], x.w, o[h][i].w);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void put_sums(float* m_out, float* l_out)
+    {
+        const int lane = threadIdx.x % kWarp;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) l[h] += __shfl_xor_sync(~0u, l[h], d);
+            if (lane == 0) {
+                m_out[h] = m[h];
+                l_out[h] = l[h];
+            }
+        }
+    }
+    __device__ __forceinline__ void put(float* sum, const float* factor, bool first)
+    {
+        const int lane = threadIdx.x % kWarp;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                float4 x = o[h][i];
+#pragma unroll
+                for (int d = kLanes; d < kWarp; d *= 2) {  // the lanes of the other tokens
+                    x.x += __shfl_xor_sync(~0u, x.x, d);
+                    x.y += __shfl_xor_sync(~0u, x.y, d);
+                    x.z += __shfl_xor_sync(~0u, x.z, d);
+                    x.w += __shfl_xor_sync(~0u, x.w, d);
+                }
+                if (lane < kLanes) {
+                    const float f = factor[h];
+                    float4* at = reinterpret_cast<float4*>(sum + h * (D + 4) + (lane + i * kLanes) * 4);
+                    float4 y = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
+                    y.x += x.x * f, y.y += x.y * f, y.z += x.z * f, y.w += x.w * f;
+                    *at = y;
+                }
+            }
+    }
+};
+
+// Shared memory of a block.
+template <typename T, int D, int H, int STAGES, int WARPS>
+struct Room {
+    using Work = Tile<T, D, H>;
+    static constexpr int kRowBytes = D * int(sizeof(T));
+    static constexpr int kStageBytes = 2 * kTile * kRowBytes;  // keys, then values
+    static constexpr int kRing = STAGES * kStageBytes;         // of a warp
+    static constexpr int kQueries = WARPS * kRing;
+    static constexpr int kOwn = kQueries + Work::kQueryBytes;
+    static constexpr int kSum = kOwn + WARPS * Work::kWarpBytes;
+    static constexpr int kStats = kSum + H * (D + 4) * 4;      // m, l, factor [warp][head], then of the unit [head]
+    static constexpr int kMasks = kStats + (3 * WARPS + 2) * H * 4;
+    static constexpr int kBytes = kMasks + WARPS * STAGES * 4;
+};
+
+// kWide: 16-byte copies; else element by element, for rows that start anywhere.
+template <typename T, int D, int H, int STAGES, int WARPS, bool kWide>
+__global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
+{
+    using Work = Tile<T, D, H>;
+    using R = Room<T, D, H, STAGES, WARPS>;
+    constexpr int kWarps = WARPS, kThreads = kWarps * kWarp;
+    constexpr int kRowBytes = R::kRowBytes, kChunks = kRowBytes / 16;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    let_next_start();
+
+    unsigned char* ring = smem + warp * R::kRing;
+    if (p.dim < D)  // columns past the head's are zeros throughout
+        for (int i = lane; i < R::kRing / 16; i += kWarp) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
+
+    const uint32_t units = p.kv_heads * p.chunks;
+    const auto weight = [&](uint32_t r) { return (long long)(tokens_of(p, r).tiles()) * units; };
+    long long begin = -1, end = -1, per = 1;
+    Place place;
+    const long long total = share_of<kThreads>(
+        p.requests, weight,
+        [&](long long all) {
+            // not less than a tile for each warp
+            per = max((all + gridDim.x - 1) / gridDim.x, (long long)kWarps);
+            begin = blockIdx.x * per;
+            end = min(all, begin + per);
+            return begin < all ? begin : -1;
+        },
+        place);
+
+    // requests without tokens
+    for (uint32_t r = blockIdx.x; r < p.requests; r += gridDim.x) {
+        if (tokens_of(p, r).tiles()) continue;
+        for (uint32_t i = threadIdx.x; i < p.heads * p.dim; i += kThreads) {
+            const uint32_t h = i / p.dim;
+            static_cast<T*>(p.out)[r * p.out_request + h * p.out_head + (i - h * p.dim)] = from_float<T>(0.f);
+        }
+        for (uint32_t h = threadIdx.x; h < p.heads; h += kThreads) {
+            if (p.lse) p.lse[uint64_t(r) * p.heads + h] = -INFINITY;
+            if (p.lse2) p.lse2[uint64_t(r) * p.heads + h] = -INFINITY;
+        }
+    }
+    int32_t* meta = p.meta + blockIdx.x * 4;
+    if (begin >= total) {
+        if (threadIdx.x == 0) meta[2] = 0;
+        return;
+    }
+
+    Walk now;
+    now.r = place.item;
+    now.tokens = tokens_of(p, now.r);
+    now.tiles = now.tokens.tiles();
+    now.unit = uint32_t((begin - place.first) / now.tiles);
+    now.t = uint32_t((begin - place.first) - (long long)now.unit * now.tiles);
+    now.left = end - begin;
+    now.part();
+
+    uint32_t* masks = reinterpret_cast<uint32_t*>(smem + R::kMasks) + warp * STAGES;
+    // the warp's next tile to copy, and whether there is one
+    Walk ahead = now;
+    uint32_t ahead_t = ahead.t + warp;
+    bool more = true;
+    const auto settle = [&] {
+        while (ahead_t >= ahead.t_end) {
+            if (!ahead.next(p)) {
+                more = false;
+                return;
+            }
+            ahead_t = warp;
+        }
+    };
+    settle();
+    // lane's row of the tile: its page and place in it, read ahead
+    int32_t id = -1;
+    uint32_t in_page = 0;
+    const auto look_up = [&] {
+        id = -1;
+        if (!more) return;
+        const uint32_t token = ahead.tokens.first + ahead_t * kTile + lane % 16;
+        if (token < ahead.tokens.end) {
+            const uint32_t page = p.page.quotient(token);
+            in_page = token - page * p.page.d;
+            id = p.table[ahead.r * p.table_stride + page];
+        }
+    };
+    look_up();
+    int stage_in = 0;
+    const auto copy_next = [&] {
+        if (more) {
+            unsigned char* to = ring + stage_in * R::kStageBytes;
+            const bool valid = uint32_t(id) < p.num_pages;
+            const uint32_t mask = __ballot_sync(~0u, valid) & 0xffffu;
+            if (lane == 0) masks[stage_in] = mask;
+            const uint64_t row_offset = valid ? uint64_t(uint32_t(id)) * p.page_stride + in_page * p.token_stride +
+                                                    uint64_t(ahead.unit / p.chunks) * p.head_stride
+                                              : 0;
+            const T* k = static_cast<const T*>(p.k);
+            const T* v = static_cast<const T*>(p.v);
+            if (kWide) {
+                const uint32_t address = smem_address(to);
+#pragma unroll
+                for (int i = 0; i < kTile * kChunks / kWarp; ++i) {
+                    const int at = i * kWarp + lane, row = at / kChunks, chunk = at % kChunks;
+                    const uint64_t offset = __shfl_sync(~0u, row_offset, row) + chunk * (16 / sizeof(T));
+                    if (chunk * (16 / sizeof(T)) < p.dim) {
+                        const uint32_t into = address + row * kRowBytes + swizzled(row, chunk) * 16;
+                        copy_16b(into, k + offset, mask >> row & 1);
+                        copy_16b(into + kTile * kRowBytes, v + offset, mask >> row & 1);
+                    }
+                }
+            } else {
+                __syncwarp();  // the stage's last use is over
+                constexpr int kIn = 16 / int(sizeof(T));
+                for (int row = 0; row < kTile; ++row) {
+                    const uint64_t offset = __shfl_sync(~0u, row_offset, row);
+                    const bool live = mask >> row & 1;
+                    for (uint32_t c = lane; c < p.dim; c += kWarp) {
+                        T* into = reinterpret_cast<T*>(to + row * kRowBytes + swizzled(row, c / kIn) * 16) + c % kIn;
+                        into[0] = live ? k[offset + c] : from_float<T>(0.f);
+                        into[kTile * kRowBytes / int(sizeof(T))] = live ? v[offset + c] : from_float<T>(0.f);
+                    }
+                }
+            }
+            ahead_t += kWarps;
+            settle();
+            look_up();
+        }
+        commit_copies();
+        stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+    };
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) copy_next();
+
+    float* sum = reinterpret_cast<float*>(smem + R::kSum);
+    float* m_all = reinterpret_cast<float*>(smem + R::kStats);
+    float* l_all = m_all + kWarps * H;
+    float* factor = l_all + kWarps * H;
+    float* unit_m = factor + kWarps * H;
+    float* unit_l = unit_m + H;
+    int stage = 0;
+    int32_t starts = 0;  // blocks behind this one that go on with the run's last unit
+    uint32_t start_request = 0, start_unit = 0;
+    long long first_tile = begin;  // number of the part's first tile
+    Work work;
+    do {
+        const uint32_t kv_head = now.unit / p.chunks, chunk = now.unit - kv_head * p.chunks;
+        const uint32_t head0 = chunk * p.per_unit, heads = min(p.per_unit, p.group - head0);
+        const uint32_t head = kv_head * p.group + head0;
+        Work::load_queries(p, smem + R::kQueries,
+                           static_cast<const T*>(p.q) + now.r * p.q_request + head * p.q_head, heads);
+        work.clear();
+        __syncthreads();
+        for (uint32_t t = now.t + warp; t < now.t_end; t += kWarps) {
+            wait_copies<STAGES - 2>();
+            __syncwarp();
+            copy_next();
+            const unsigned char* keys = ring + stage * R::kStageBytes;
+            const long long number = first_tile + (t - now.t);
+            float* logits = p.logits && number < p.logit_tiles ? p.logits + number * p.per_unit * kTile : nullptr;
+            work.add(p, keys, keys + kTile * kRowBytes, smem + R::kQueries,
+                     smem + R::kOwn + warp * Work::kWarpBytes, masks[stage], logits, heads);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+        }
+
+        // the warps' parts, in the order of the warps
+        work.put_sums(m_all + warp * H, l_all + warp * H);
+        __syncthreads();
+        if (threadIdx.x < H) {
+            float top = -INFINITY, all = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_all[w * H + threadIdx.x]);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                // a warp whose logits were all NaN has no reference, but a sum
+                const float from = m_all[w * H + threadIdx.x], part = l_all[w * H + threadIdx.x];
+                const float f = from == -INFINITY ? (part == 0.f ? 0.f : part) : exp2_fast(from - top);
+                factor[w * H + threadIdx.x] = f;
+                all += f * part;
+            }
+            unit_m[threadIdx.x] = top;
+            unit_l[threadIdx.x] = all;
+        }
+        __syncthreads();
+        const int busy = int(min(uint32_t(kWarps), now.t_end - now.t));
+        for (int w = 0; w < busy; ++w) {
+            if (warp == w) work.put(sum, factor + w * H, w == 0);
+            __syncthreads();
+        }
+        if (now.t == 0 && now.t_end == now.tiles) {
+            T* out = static_cast<T*>(p.out) + now.r * p.out_request + head * p.out_head;
+            for (uint32_t i = threadIdx.x; i < heads * D; i += kThreads) {
+                const uint32_t h = i / D, c = i % D;
+                const float all = unit_l[h];
+                if (c < p.dim) out[h * p.out_head + c] = from_float<T>(all == 0.f ? 0.f : sum[h * (D + 4) + c] / all);
+            }
+            if (threadIdx.x < heads) {
+                const float base2 = unit_m[threadIdx.x] + log2f(unit_l[threadIdx.x]);
+                const uint64_t at = uint64_t(now.r) * p.heads + head + threadIdx.x;
+                const float value = unit_l[threadIdx.x] == 0.f ? -INFINITY : base2;
+                if (p.lse) p.lse[at] = value * kLn2;
+                if (p.lse2) p.lse2[at] = value;
+            }
+        } else {
+            const uint32_t slot = blockIdx.x * 2 + (now.t ? 0 : 1);
+            float* part = p.part + uint64_t(slot) * H * D;
+            for (uint32_t i = threadIdx.x; i < heads * D; i += kThreads) part[i] = sum[i / D * (D + 4) + i % D];
+            float2* stats = reinterpret_cast<float2*>(p.part + uint64_t(gridDim.x) * 2 * H * D) + uint64_t(slot) * H;
+            if (threadIdx.x < heads) stats[threadIdx.x] = make_float2(unit_m[threadIdx.x], unit_l[threadIdx.x]);
+            if (now.t == 0) {
+                starts = int32_t((first_tile + now.tiles - 1) / per - blockIdx.x);
+                start_request = now.r;
+                start_unit = now.unit;
+            }
+        }
+        if (p.first && now.unit == 0 && now.t == 0 && threadIdx.x == 0) p.first[now.r] = first_tile;
+        first_tile += now.t_end - now.t;
+        __syncthreads();
+    } while (now.next(p));
+    wait_copies<0>();
+    if (threadIdx.x == 0) {
+        meta[0] = int32_t(start_request);
+        meta[1] = int32_t(start_unit);
+        meta[2] = starts;
+    }
+}
+
+// Block (b, h): head h of the unit that block b's run ends in and others go on
+// with.  Its parts are b's last and the first of the next `count` blocks; the
+// warps take every eighth and join in order.
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * kWarp;
+template <typename T, int D, int H>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
+{
+    __shared__ float sums[kJoinWarps][D];
+    __shared__ float top_of[kJoinWarps], all_of[kJoinWarps];
+    let_next_start();
+    wait_for_previous();
+    const int32_t* meta = p.meta + blockIdx.x * 4;
+    const int32_t count = meta[2];
+    if (count <= 0) return;
+    const uint32_t r = uint32_t(meta[0]), unit = uint32_t(meta[1]);
+    const uint32_t kv_head = unit / p.chunks, chunk = unit - kv_head * p.chunks;
+    const uint32_t head0 = chunk * p.per_unit, heads = min(p.per_unit, p.group - head0);
+    const uint32_t h = blockIdx.y;
+    if (h >= heads) return;
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    const float2* stats = reinterpret_cast<const float2*>(p.part + uint64_t(gridDim.x) * 2 * H * D);
+    const auto slot_of = [&](int32_t i) { return uint64_t(blockIdx.x + i) * 2 + (i ? 0 : 1); };
+
+    // each thread takes parts for the common reference
+    float top = -INFINITY;
+    for (int32_t i = threadIdx.x; i <= count; i += kJoinThreads) top = fmaxf(top, stats[slot_of(i) * H + h].x);
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    if (lane == 0) top_of[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, top_of[w]);
+
+    constexpr int kPer = (D + kWarp - 1) / kWarp;
+    float o[kPer], all = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] = 0.f;
+#pragma unroll 4
+    for (int32_t i = warp; i <= count; i += kJoinWarps) {
+        const uint64_t slot = slot_of(i);
+        const float2 s = stats[slot * H + h];
+        const float f = s.x == -INFINITY ? (s.y == 0.f ? 0.f : s.y) : exp2_fast(s.x - top);
+        all += f * s.y;
+        const float* part = p.part + (slot * H + h) * D;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) o[c] += f * part[c * kWarp + lane];
+    }
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) sums[warp][c * kWarp + lane] = o[c];
+    if (lane == 0) all_of[warp] = all;
+    __syncthreads();
+    all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) all += all_of[w];
+    const uint32_t head = kv_head * p.group + head0 + h;
+    T* out = static_cast<T*>(p.out) + r * p.out_request + head * p.out_head;
+    for (uint32_t c = threadIdx.x; c < p.dim; c += kJoinThreads) {
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) x += sums[w][c];
+        out[c] = from_float<T>(all == 0.f ? 0.f : x / all);
+    }
+    if (threadIdx.x == 0) {
+        const float value = all == 0.f ? -INFINITY : top + log2f(all);
+        const uint64_t at = uint64_t(r) * p.heads + head;
+        if (p.lse) p.lse[at] = value * kLn2;
+        if (p.lse2) p.lse2[at] = value;
+    }
+}
+
+template <typename T, int D, int H, int STAGES, int WARPS>
+lcpp_status launch(const Params& base, bool wide, size_t part_bytes_at_most, cudaStream_t s)
+{
+    Params p = base;
+    using R = Room<T, D, H, STAGES, WARPS>;
+    constexpr int kThreads = WARPS * kWarp;
+    static_assert(R::kBytes <= 227 * 1024, "");
+    auto kernel = wide ? decode_kernel<T, D, H, STAGES, WARPS, true> : decode_kernel<T, D, H, STAGES, WARPS, false>;
+    set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), R::kBytes);
+    const unsigned blocks = std::min<unsigned>(
+        kMostBlocks, unsigned(device_sm_count()) * resident_blocks(reinterpret_cast<const void*>(kernel), kThreads, R::kBytes));
+    if (uint64_t(blocks) * 2 * H * (D + 2) * 4 > part_bytes_at_most) return LCPP_ERR_INTERNAL;
+    kernel<<<blocks, kThreads, R::kBytes, s>>>(p);
+    const lcpp_status status = launched();
+    if (status != LCPP_OK) return status;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(blocks, std::min<uint32_t>(p.per_unit, H));
+    config.blockDim = dim3(kJoinThreads);
+    config.stream = s;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H>, p));
+    return LCPP_OK;
+}
+
+// Heads of a unit and padded columns for a group of `group` query heads and
+// heads of `dim` columns; the temp query and the launch go by the same choice.
+struct Choice {
+    uint32_t columns, heads, chunks, per_unit;
+};
+inline Choice choose(uint32_t group, uint32_t dim, bool f32)
+{
+    Choice c{};
+    c.columns = dim <= 64 ? 64 : dim <= 128 ? 128 : (f32 || dim > 192) ? 256 : 192;
+    // what a warp's accumulators hold: 128 registers of them
+    const uint32_t most = f32 ? (c.columns == 256 ? 4 : 8) : (c.columns <= 128 ? 32 : 16);
+    c.chunks = (group + most - 1) / most;
+    c.per_unit = (group + c.chunks - 1) / c.chunks;
+    c.chunks = (group + c.per_unit - 1) / c.per_unit;
+    c.heads = f32 ? 1 : 8;
+    while (c.heads < c.per_unit) c.heads *= 2;
+    return c;
+}
+
+lcpp_status run_f32(const Params& p, const Choice& c, bool wide, size_t part_bytes, cudaStream_t s);
+lcpp_status run_f16(const Params& p, const Choice& c, bool wide, size_t part_bytes, cudaStream_t s);
+lcpp_status run_bf16(const Params& p, const Choice& c, bool wide, size_t part_bytes, cudaStream_t s);
+
+template <typename T>
+lcpp_status run_16bit(const Params& p, const Choice& c, bool wide, size_t part_bytes, cudaStream_t s)
+{
+    switch (c.columns) {
+    case 64:
+        return c.heads == 8    ? launch<T, 64, 8, 3, 4>(p, wide, part_bytes, s)
+               : c.heads == 16 ? launch<T, 64, 16, 3, 4>(p, wide, part_bytes, s)
+                               : launch<T, 64, 32, 3, 4>(p, wide, part_bytes, s);
+    case 128:
+        return c.heads == 8    ? launch<T, 128, 8, 3, 4>(p, wide, part_bytes, s)
+               : c.heads == 16 ? launch<T, 128, 16, 3, 4>(p, wide, part_bytes, s)
+                               : launch<T, 128, 32, 3, 4>(p, wide, part_bytes, s);
+    case 192:
+        return c.heads == 8 ? launch<T, 192, 8, 3, 4>(p, wide, part_bytes, s) : launch<T, 192, 16, 3, 4>(p, wide, part_bytes, s);
+    default:
+        return c.heads == 8 ? launch<T, 256, 8, 3, 4>(p, wide, part_bytes, s) : launch<T, 256, 16, 3, 4>(p, wide, part_bytes, s);
+    }
+}
+
+}  // namespace attention
+}  // namespace model
+}  // namespace lcpp

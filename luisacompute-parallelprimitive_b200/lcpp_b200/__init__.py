@@ -29,6 +29,9 @@ F16, BF16 = 7, 8  # logits and token rows of the model-step operators only
 # lcpp_router_score
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 BIAS_ON_SCORE = 0x10  # added to either: a bias joins the score instead of the logit
+# lcpp_rotary_layout, lcpp_rotary_scaling
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BY_ROTATIONS = 0, 1, 2, 3
 # lcpp_op
 OP_SUM, OP_MIN, OP_MAX = 0, 1, 2
 # lcpp_testgen_dist
@@ -43,6 +46,7 @@ KERNEL_ARG_REDUCE = 6
 KERNEL_BY_KEY = 7
 KERNEL_SELECT = 8
 KERNEL_BLOCK_TABLE, KERNEL_ROUTER, KERNEL_DISPATCH = 9, 10, 11
+KERNEL_ROTARY, KERNEL_PAGED_ATTENTION, KERNEL_CACHE_EVICTION = 12, 13, 14
 
 _lib = None
 
@@ -76,6 +80,61 @@ class RouterConfig(ctypes.Structure):
                 ("renormalize", ctypes.c_int32), ("weight_scale", ctypes.c_float), ("loss_coef", ctypes.c_float)]
 
 
+class HeadRows(ctypes.Structure):
+    """lcpp_head_rows (include/lcpp_b200_model.h)."""
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("in_token_stride", ctypes.c_uint64),
+                ("in_head_stride", ctypes.c_uint64), ("out_token_stride", ctypes.c_uint64),
+                ("out_head_stride", ctypes.c_uint64), ("num_heads", ctypes.c_uint32)]
+
+
+class KVCache(ctypes.Structure):
+    """lcpp_kv_cache (include/lcpp_b200_model.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_uint64),
+                ("token_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64), ("num_pages", ctypes.c_uint32),
+                ("block_size", ctypes.c_uint32), ("num_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("dtype", ctypes.c_int)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """lcpp_rotary_args (include/lcpp_b200_model.h)."""
+    _fields_ = [("q", HeadRows), ("k", HeadRows), ("positions", ctypes.c_void_p), ("token_request", ctypes.c_void_p),
+                ("position_offset", ctypes.c_void_p), ("frequencies", ctypes.c_void_p),
+                ("num_tokens", ctypes.c_uint64), ("num_requests", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("rotary_dim", ctypes.c_uint32), ("layout", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("dtype", ctypes.c_int)]
+
+
+class CacheAppendArgs(ctypes.Structure):
+    """lcpp_cache_append_args (include/lcpp_b200_model.h)."""
+    _fields_ = [("cache", KVCache), ("v", ctypes.c_void_p), ("v_token_stride", ctypes.c_uint64),
+                ("v_head_stride", ctypes.c_uint64), ("slots", ctypes.c_void_p), ("slot_positions", ctypes.c_void_p),
+                ("slot_scores", ctypes.c_void_p)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """lcpp_paged_attention_args (include/lcpp_b200_model.h)."""
+    _fields_ = [("cache", KVCache), ("q", ctypes.c_void_p), ("q_request_stride", ctypes.c_uint64),
+                ("q_head_stride", ctypes.c_uint64), ("out", ctypes.c_void_p), ("out_request_stride", ctypes.c_uint64),
+                ("out_head_stride", ctypes.c_uint64), ("block_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_uint64), ("table_width", ctypes.c_uint32),
+                ("num_requests", ctypes.c_uint32), ("seq_lens", ctypes.c_void_p), ("num_heads", ctypes.c_uint32),
+                ("window", ctypes.c_uint32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+                ("lse_out", ctypes.c_void_p), ("slot_scores", ctypes.c_void_p), ("slot_scores_out", ctypes.c_void_p),
+                ("score_decay", ctypes.c_float)]
+
+
+class CacheEvictArgs(ctypes.Structure):
+    """lcpp_cache_evict_args (include/lcpp_b200_model.h)."""
+    _fields_ = [("seq_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_uint64),
+                ("table_width", ctypes.c_uint32), ("num_requests", ctypes.c_uint32), ("num_pages", ctypes.c_uint32),
+                ("block_size", ctypes.c_uint32), ("slot_scores", ctypes.c_void_p),
+                ("slot_positions", ctypes.c_void_p), ("evicted", ctypes.c_void_p), ("budget", ctypes.c_uint32),
+                ("trigger", ctypes.c_uint32), ("keep_first", ctypes.c_uint32), ("keep_recent", ctypes.c_uint32),
+                ("max_moves", ctypes.c_uint32), ("seq_lens_out", ctypes.c_void_p), ("evicted_out", ctypes.c_void_p),
+                ("move_counts_out", ctypes.c_void_p), ("moves_out", ctypes.c_void_p), ("free_blocks", ctypes.c_void_p),
+                ("free_used", ctypes.c_void_p), ("free_used_out", ctypes.c_void_p), ("num_free", ctypes.c_uint32)]
+
+
 class LcppError(RuntimeError):
     def __init__(self, status: int, what: str):
         self.status = status
@@ -97,7 +156,7 @@ def lib() -> ctypes.CDLL:
     szp = ctypes.POINTER(ctypes.c_size_t)
     ip = ctypes.POINTER(ctypes.c_int)
     vpa = ctypes.c_void_p * 2
-    u32, cfg = ctypes.c_uint32, ctypes.POINTER(RouterConfig)
+    u32, cfg, f64 = ctypes.c_uint32, ctypes.POINTER(RouterConfig), ctypes.c_double
     sigs = {
         "lcpp_status_string": ([i], ctypes.c_char_p),
         "lcpp_version": ([], i),
@@ -195,6 +254,14 @@ def lib() -> ctypes.CDLL:
         "lcpp_dispatch_combine": ([vp, u64, vp, vp, vp, u64, u64, u32, u64, u64, i, vp], i),
         "lcpp_dispatch_combine_backward": ([vp, u64, vp, u64, vp, vp, vp, vp, vp, u64, vp, u64, u32, u32, u64, u64,
                                             i, vp], i),
+        "lcpp_rotary_frequencies": ([vp, u32, f64, i, f64, f64, f64, f64], i),
+        "lcpp_rotary_forward": ([ctypes.POINTER(RotaryArgs), vp], i),
+        "lcpp_rotary_backward": ([ctypes.POINTER(RotaryArgs), vp], i),
+        "lcpp_rotary_append": ([ctypes.POINTER(RotaryArgs), ctypes.POINTER(CacheAppendArgs), vp], i),
+        "lcpp_paged_attention_temp_bytes": ([u32, u32, u32, u32, u64, szp], i),
+        "lcpp_paged_attention_decode": ([vp, sz, ctypes.POINTER(PagedAttentionArgs), vp], i),
+        "lcpp_cache_evict_plan": ([ctypes.POINTER(CacheEvictArgs), vp], i),
+        "lcpp_cache_evict_move": ([ctypes.POINTER(KVCache), vp, u32, vp, u32, vp, vp, vp], i),
         "lcpp_diag_timing_enable": ([i], i),
         "lcpp_diag_launch_shapes": ([ctypes.POINTER(u64)], i),
         "lcpp_diag_wait_timeout_probe": ([vp, sz, u64, vp], i),
@@ -931,6 +998,50 @@ def _queue(stream):
     return _raw_stream(torch.cuda.current_device())
 
 
+def _here(t, name):
+    """Refuses a tensor of another device than the current one: its memory is not the kernels' to use."""
+    if t.get_device() != _torch().cuda.current_device():
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a tensor of the current device")
+
+
+def _heads(t, tokens, heads, dim, code, name):
+    """(pointer, token stride, head stride) of a [tokens, heads, dim] tensor whose columns are adjacent."""
+    shape = t.shape
+    if _row_code(t) != code or len(shape) != 3 or shape[0] < tokens or shape[1] != heads or shape[2] != dim:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: one dtype, at least {tokens} x {heads} x {dim}")
+    a, b, c = t.stride()
+    if c != 1 and dim > 1 and shape[0]:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a head's columns have to be adjacent")
+    if not t.is_cuda:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a CUDA tensor")
+    return t.data_ptr(), a, b
+
+
+def _kv_cache(k, v):
+    """The lcpp_kv_cache of two [pages, block_size, heads, dim] tensors of equal strides."""
+    shape, stride, code = k.shape, k.stride(), _row_code(k)
+    if len(shape) != 4 or v.shape != shape or v.stride() != stride or _row_code(v) != code:
+        raise LcppError(ERR_INVALID_ARG, "keys and values: [pages, block_size, heads, dim] of one dtype, shape and layout")
+    if stride[3] != 1 and shape[3] > 1:
+        raise LcppError(ERR_INVALID_ARG, "keys and values: a head's columns have to be adjacent")
+    if not k.is_cuda or not v.is_cuda:
+        raise LcppError(ERR_INVALID_ARG, "keys and values: CUDA tensors")
+    _here(k, "keys")
+    return KVCache(k.data_ptr(), v.data_ptr(), stride[0], stride[1], stride[2], shape[0], shape[1], shape[2], shape[3],
+                   code)
+
+
+def _table(t, rows):
+    """(pointer, row stride, width) of an int32 block table of at least `rows` rows."""
+    if t.dtype != _torch().int32 or t.dim() != 2 or t.shape[0] < rows or \
+            (t.stride(1) != 1 and t.shape[1] > 1 and rows):
+        raise LcppError(ERR_INVALID_ARG, "d_block_table: int32 [num_requests, width], columns adjacent")
+    if not t.is_cuda:
+        raise LcppError(ERR_INVALID_ARG, "d_block_table: a CUDA tensor")
+    width = t.shape[1]
+    return t.data_ptr(), (t.stride(0) if rows > 1 else max(t.stride(0), width)), width
+
+
 def _scratch(temp):
     """(pointer, bytes) of temp storage."""
     return (None, 0) if temp is None else (temp.data_ptr(), temp.numel() * temp.element_size())
@@ -1100,3 +1211,159 @@ class DeviceDispatch:
             _flat(d_weights, f32, pairs, "d_weights"), out, out_stride,
             _flat(d_grad_weights_out, f32, pairs, "d_grad_weights_out"), num_tokens, top_k, num_experts, max_rows,
             hidden, code, _queue(stream)), "CombineBackward")
+
+
+class DeviceRotary:
+    """Rotary positions of queries and keys, with the gradient and the write of keys and values into a paged cache."""
+
+    @staticmethod
+    def Frequencies(rotary_dim: int, base: float = 10000.0, scaling: int = ROTARY_PLAIN, factor: float = 1.0,
+                    original_context: float = 0.0, low: float = 1.0, high: float = 4.0, device=None):
+        """lcpp_rotary_frequencies as a CUDA tensor: float64 [rotary_dim / 2], radians per position."""
+        torch = _torch()
+        out = (ctypes.c_double * max(1, rotary_dim // 2))()
+        check(lib().lcpp_rotary_frequencies(out, rotary_dim, base, scaling, factor, original_context, low, high),
+              "Frequencies")
+        return torch.tensor(list(out)[:rotary_dim // 2], dtype=torch.float64, device=device or "cuda")
+
+    @staticmethod
+    def _args(q, k, q_out, k_out, positions, frequencies, tokens, layout, scale, token_request, position_offset):
+        torch = _torch()
+        some = q if q is not None else k
+        if some is None:
+            raise LcppError(ERR_INVALID_ARG, "d_q or d_k: a tensor")
+        if some.dim() != 3:
+            raise LcppError(ERR_INVALID_ARG, "d_q, d_k: [tokens, heads, dim]")
+        code, dim = _row_code(some), some.shape[2]
+        rows = []
+        for x, out, name in ((q, q_out, "d_q"), (k, k_out, "d_k")):
+            if x is None:
+                rows.append(HeadRows())
+                continue
+            heads = x.shape[1] if x.dim() == 3 else 0
+            at, a, b = _heads(x, tokens, heads, dim, code, name)
+            to, c, d = (None, 0, 0) if out is None else _heads(out, tokens, heads, dim, code, name + "_out")
+            rows.append(HeadRows(at, to, a, b, c, d, heads))
+        _here(some, "d_q, d_k")
+        requests = 0 if token_request is None else (1 << 31) - 1 if position_offset is None else position_offset.numel()
+        return RotaryArgs(
+            rows[0], rows[1], _flat(positions, torch.int32, tokens, "d_positions"),
+            _flat(token_request, torch.int32, tokens, "d_token_request"),
+            _flat(position_offset, torch.int32, 0, "d_position_offset"),
+            _flat(frequencies, torch.float64, 0, "d_frequencies"), tokens, requests, dim, 2 * frequencies.numel(),
+            layout, scale, code)
+
+    def Forward(self, d_q, d_k, d_q_out, d_k_out, d_positions, d_frequencies, num_tokens, layout=ROTARY_HALF, scale=1.0,
+                d_token_request=None, d_position_offset=None, stream=None):
+        """Turns q and k (either may be None) by their positions (lcpp_rotary_forward): [tokens, heads, dim] tensors
+        with any strides of tokens and heads, in place where the output is the input; positions int32; as many
+        columns as twice the frequencies (float64) are turned.  Tokens whose request (int32) is negative are left
+        out; a request's offset (int32) is added to its tokens' positions."""
+        args = self._args(d_q, d_k, d_q_out, d_k_out, d_positions, d_frequencies, num_tokens, layout, scale,
+                          d_token_request, d_position_offset)
+        check(lib().lcpp_rotary_forward(args, _queue(stream)), "Forward")
+
+    def Backward(self, d_grad_q, d_grad_k, d_grad_q_out, d_grad_k_out, d_positions, d_frequencies, num_tokens,
+                 layout=ROTARY_HALF, scale=1.0, d_token_request=None, d_position_offset=None, stream=None):
+        """Gradients of Forward's inputs from those of its outputs (lcpp_rotary_backward)."""
+        args = self._args(d_grad_q, d_grad_k, d_grad_q_out, d_grad_k_out, d_positions, d_frequencies, num_tokens,
+                          layout, scale, d_token_request, d_position_offset)
+        check(lib().lcpp_rotary_backward(args, _queue(stream)), "Backward")
+
+    def Append(self, d_q, d_k, d_v, d_q_out, d_k_cache, d_v_cache, d_slots, d_positions, d_frequencies, num_tokens,
+               layout=ROTARY_HALF, scale=1.0, d_token_request=None, d_position_offset=None, d_slot_positions=None,
+               d_slot_scores=None, stream=None):
+        """Forward for q (None: no queries), with keys and values going to their slots of the cache
+        (lcpp_rotary_append): caches [pages, block_size, heads, dim] with any strides, slots int64 as
+        DeviceBlockTable.Extend gives them.  d_slot_positions (int32, one per slot) gets the tokens' positions,
+        d_slot_scores (float32) zeros."""
+        torch = _torch()
+        args = self._args(d_q, d_k, d_q_out, None, d_positions, d_frequencies, num_tokens, layout, scale,
+                          d_token_request, d_position_offset)
+        cache = _kv_cache(d_k_cache, d_v_cache)
+        slots = cache.num_pages * cache.block_size
+        v, v_token, v_head = _heads(d_v, num_tokens, cache.num_kv_heads, cache.head_dim, cache.dtype, "d_v")
+        append = CacheAppendArgs(cache, v, v_token, v_head, _flat(d_slots, torch.int64, num_tokens, "d_slots"),
+                                 _flat(d_slot_positions, torch.int32, slots, "d_slot_positions"),
+                                 _flat(d_slot_scores, torch.float32, slots, "d_slot_scores"))
+        check(lib().lcpp_rotary_append(args, append, _queue(stream)), "Append")
+
+
+class DevicePagedAttention:
+    """Attention of one new token of each request over a paged cache."""
+
+    @staticmethod
+    def GetTempStorageBytes(num_requests: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                            score_slots: int = 0) -> int:
+        """score_slots: pages * block_size when scores are wanted."""
+        out = ctypes.c_size_t()
+        check(lib().lcpp_paged_attention_temp_bytes(num_requests, num_heads, num_kv_heads, head_dim, score_slots,
+                                                    ctypes.byref(out)), "GetTempStorageBytes")
+        return out.value
+
+    def Decode(self, temp, d_q, d_k_cache, d_v_cache, d_block_table, d_seq_lens, d_out, num_requests, scale=None,
+               window=0, softcap=0.0, d_lse_out=None, d_scores=None, d_scores_out=None, score_decay=1.0, stream=None):
+        """lcpp_paged_attention_decode: q and out [requests, heads, dim], caches [pages, block_size, kv_heads, dim]
+        with any strides, block table and lengths int32 as DeviceBlockTable.Extend leaves them.  scale None:
+        dim ** -0.5.  d_lse_out float32 [requests, heads]; scores float32, one per slot: the outputs are
+        score_decay * d_scores (None: zeros) plus each token's attention weight, summed over the heads."""
+        torch = _torch()
+        cache = _kv_cache(d_k_cache, d_v_cache)
+        heads, dim, n, f32 = d_q.shape[1] if d_q.dim() == 3 else 0, cache.head_dim, num_requests, torch.float32
+        slots = cache.num_pages * cache.block_size
+        q, q_request, q_head = _heads(d_q, n, heads, dim, cache.dtype, "d_q")
+        out, out_request, out_head = _heads(d_out, n, heads, dim, cache.dtype, "d_out")
+        table, table_stride, width = _table(d_block_table, n)
+        args = PagedAttentionArgs(
+            cache, q, q_request, q_head, out, out_request, out_head, table, table_stride, width, n,
+            _flat(d_seq_lens, torch.int32, n, "d_seq_lens"), heads, window, dim ** -0.5 if scale is None else scale,
+            softcap, _flat(d_lse_out, f32, n * heads, "d_lse_out"), _flat(d_scores, f32, slots, "d_scores"),
+            _flat(d_scores_out, f32, slots, "d_scores_out"), score_decay)
+        check(lib().lcpp_paged_attention_decode(*_scratch(temp), args, _queue(stream)), "Decode")
+
+
+class DeviceCacheEviction:
+    """Requests of a paged cache cut down to their heaviest tokens."""
+
+    def Plan(self, d_seq_lens, d_block_table, d_scores, d_seq_lens_out, d_move_counts_out, d_moves_out, num_requests,
+             block_size, budget, trigger=None, keep_first=0, keep_recent=0, d_positions=None, d_evicted=None,
+             d_evicted_out=None, d_free_blocks=None, d_free_used=None, d_free_used_out=None, stream=None):
+        """Chooses the tokens that stay (lcpp_cache_evict_plan): requests longer than trigger (None: budget) keep
+        budget tokens, by d_scores (float32, one per slot).  d_moves_out int64 [requests, max_moves, 2]; the lengths
+        and counts int32.  With the free list that DeviceBlockTable.Extend takes pages from, pages that are not
+        needed any more go back to it."""
+        torch = _torch()
+        i32, n = torch.int32, num_requests
+        table, table_stride, width = _table(d_block_table, n)
+        if d_moves_out.dim() != 3 or d_moves_out.shape[2] != 2 or d_moves_out.shape[0] < n:
+            raise LcppError(ERR_INVALID_ARG, "d_moves_out: int64 [num_requests, max_moves, 2]")
+        if block_size < 1:
+            raise LcppError(ERR_INVALID_ARG, "block_size: at least 1")
+        pages = d_scores.numel() // block_size
+        args = CacheEvictArgs(
+            _flat(d_seq_lens, i32, n, "d_seq_lens"), table, table_stride, width, n, pages, block_size,
+            _flat(d_scores, torch.float32, 0, "d_scores"),
+            _flat(d_positions, i32, pages * block_size, "d_positions"), _flat(d_evicted, i32, n, "d_evicted"), budget,
+            budget if trigger is None else trigger, keep_first, keep_recent, d_moves_out.shape[1],
+            _flat(d_seq_lens_out, i32, n, "d_seq_lens_out"), _flat(d_evicted_out, i32, n, "d_evicted_out"),
+            _flat(d_move_counts_out, i32, n, "d_move_counts_out"),
+            _flat(d_moves_out, torch.int64, 2 * n * d_moves_out.shape[1], "d_moves_out"),
+            _flat(d_free_blocks, i32, 0, "d_free_blocks"), _flat(d_free_used, i32, 1, "d_free_used"),
+            _flat(d_free_used_out, i32, 1, "d_free_used_out"), 0 if d_free_blocks is None else d_free_blocks.numel())
+        _here(d_scores, "d_scores")
+        check(lib().lcpp_cache_evict_plan(args, _queue(stream)), "Plan")
+
+    def Move(self, d_moves, d_move_counts, d_k_cache, d_v_cache, num_requests, d_scores=None, d_positions=None,
+             stream=None):
+        """Moves a layer's keys and values as a plan says (lcpp_cache_evict_move), and where given the scores and
+        positions, which belong in one call only."""
+        torch = _torch()
+        cache = _kv_cache(d_k_cache, d_v_cache)
+        slots = cache.num_pages * cache.block_size
+        if d_moves.dim() != 3 or d_moves.shape[2] != 2 or d_moves.shape[0] < num_requests:
+            raise LcppError(ERR_INVALID_ARG, "d_moves: int64 [num_requests, max_moves, 2]")
+        check(lib().lcpp_cache_evict_move(
+            cache, _flat(d_moves, torch.int64, 2 * num_requests * d_moves.shape[1], "d_moves"), d_moves.shape[1],
+            _flat(d_move_counts, torch.int32, num_requests, "d_move_counts"), num_requests,
+            _flat(d_scores, torch.float32, slots, "d_scores"), _flat(d_positions, torch.int32, slots, "d_positions"),
+            _queue(stream)), "Move")
