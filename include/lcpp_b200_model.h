@@ -244,7 +244,8 @@ typedef struct lcpp_cache_evict_args {
     int32_t* seq_lens_out;       /* [num_requests] */
     int32_t* evicted_out;        /* [num_requests], or NULL; may be evicted itself */
     int32_t* move_counts_out;    /* [num_requests] */
-    int64_t* moves_out;          /* [num_requests][max_moves][2] slots, from and to */
+    int64_t* moves_out;          /* [num_requests][moves_stride][2] slots, from and to */
+    uint64_t moves_stride;       /* pairs from request to request, >= max_moves */
     int32_t* free_blocks;        /* [num_free] the list that lcpp_block_table_extend takes pages from, or NULL */
     const int32_t* free_used;    /* [1] its entries that are taken */
     int32_t* free_used_out;      /* [1] the same after the pages came back; not free_used itself */
@@ -273,12 +274,12 @@ typedef struct lcpp_cache_evict_args {
 lcpp_status lcpp_cache_evict_plan(const lcpp_cache_evict_args* args, lcpp_stream_t stream);
 
 /* Copies keys and values, and where given scores and positions, of the first
- * move_counts[r] entries of moves[r] [max_moves][2] from slot to slot.  The slots
+ * min(move_counts[r], max_moves) pairs of moves[r] from slot to slot.  The slots
  * of one call have to differ, as a plan's do; moves from or to a slot outside
  * the cache are left out. */
-lcpp_status lcpp_cache_evict_move(const lcpp_kv_cache* cache, const int64_t* moves, uint32_t max_moves,
-                                  const int32_t* move_counts, uint32_t num_requests, float* slot_scores,
-                                  int32_t* slot_positions, lcpp_stream_t stream);
+lcpp_status lcpp_cache_evict_move(const lcpp_kv_cache* cache, const int64_t* moves, uint64_t moves_stride,
+                                  uint32_t max_moves, const int32_t* move_counts, uint32_t num_requests,
+                                  float* slot_scores, int32_t* slot_positions, lcpp_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * DeviceRouter: experts of each token, their weights, counts and balance loss

@@ -42,6 +42,7 @@ struct Params {
     int32_t* evicted_out;
     int32_t* counts;
     longlong2* moves;
+    uint64_t moves_stride;
 };
 
 // What the blocks of a cluster read of one another.
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         leave();
         return;
     }
-    longlong2* out = p.moves + uint64_t(r) * p.max_moves;
+    longlong2* out = p.moves + r * p.moves_stride;
     sort_out([&](uint32_t i, uint32_t hole_mask, uint32_t filler_mask) {
         const bool is_hole = hole_mask >> lane & 1, is_filler = filler_mask >> lane & 1;
         if (is_hole || is_filler) {
@@ -302,6 +303,7 @@ struct Moves {
     uint32_t heads, block_size;
     uint64_t num_slots;
     const longlong2* moves;
+    uint64_t moves_stride;
     const int32_t* counts;
     uint32_t max_moves, requests;
     float* scores;
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Moves p)
     long long first = place.first;
     for (long long i = begin + warp; i < end; i += kMoveWarps) {
         while (i >= first + moves_of(r)) first += moves_of(r++);
-        const longlong2 move = p.moves[uint64_t(r) * p.max_moves + uint64_t(i - first)];
+        const longlong2 move = p.moves[r * p.moves_stride + uint64_t(i - first)];
         const uint64_t from = uint64_t(move.x), to = uint64_t(move.y);
         if (from >= p.num_slots || to >= p.num_slots) continue;
         const uint64_t from_page = from / p.block_size, to_page = to / p.block_size;
@@ -369,8 +371,8 @@ lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
 {
     if (!a || !a->block_size || !a->budget || a->budget >= uint32_t(1) << 31 || a->trigger < a->budget ||
         uint64_t(a->keep_first) + a->keep_recent > a->budget || a->num_requests > LCPP_MAX_REQUESTS ||
-        a->table_stride < a->table_width || a->table_stride > kMostStride ||
-        uint64_t(a->num_pages) * a->block_size >= kMostSlots)
+        a->table_stride < a->table_width || a->table_stride > kMostStride || a->moves_stride < a->max_moves ||
+        a->moves_stride > kMostStride / 16 || uint64_t(a->num_pages) * a->block_size >= kMostSlots)
         return LCPP_ERR_INVALID_ARG;
     const uint64_t n = a->num_requests, slots = uint64_t(a->num_pages) * a->block_size;
     const bool release = a->free_blocks || a->free_used || a->free_used_out;
@@ -392,7 +394,7 @@ lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
                             {a->seq_lens_out, n * 4, true},
                             {a->evicted_out, n * 4, true},
                             {a->move_counts_out, n * 4, true},
-                            {a->moves_out, n * a->max_moves * 16, true},
+                            {a->moves_out, span_bytes(n, a->moves_stride, a->max_moves, 16), true},
                             {a->free_blocks, uint64_t(a->num_free) * 4, true},
                             {a->free_used, 4, false},
                             {a->free_used_out, 4, true}};
@@ -421,6 +423,7 @@ lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
     p.evicted_out = a->evicted_out;
     p.counts = a->move_counts_out;
     p.moves = reinterpret_cast<longlong2*>(a->moves_out);
+    p.moves_stride = a->moves_stride;
 
     diag::KernelTimer timer(kTimerEviction, n, s);
     if (n) {
@@ -457,10 +460,12 @@ lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
                         static_cast<int32_t*>(a->free_used_out), uint32_t(a->num_free));
 }
 
-lcpp_status move(const lcpp_kv_cache* c, const int64_t* moves, uint32_t max_moves, const int32_t* counts,
-                 uint32_t num_requests, float* scores, int32_t* positions, cudaStream_t s)
+lcpp_status move(const lcpp_kv_cache* c, const int64_t* moves, uint64_t moves_stride, uint32_t max_moves,
+                 const int32_t* counts, uint32_t num_requests, float* scores, int32_t* positions, cudaStream_t s)
 {
-    if (!c || !sane_cache(*c) || num_requests > LCPP_MAX_REQUESTS) return LCPP_ERR_INVALID_ARG;
+    if (!c || !sane_cache(*c) || num_requests > LCPP_MAX_REQUESTS || moves_stride < max_moves ||
+        moves_stride > kMostStride / 16)
+        return LCPP_ERR_INVALID_ARG;
     const int e = row_dtype_bytes(c->dtype);
     if (!e) return LCPP_ERR_UNSUPPORTED_DTYPE;
     const uint64_t n = num_requests, slots = uint64_t(c->num_pages) * c->block_size;
@@ -469,7 +474,7 @@ lcpp_status move(const lcpp_kv_cache* c, const int64_t* moves, uint32_t max_move
         misaligned(c->v, e) || misaligned(scores, 4) || misaligned(positions, 4) || !writable_cache(*c))
         return LCPP_ERR_INVALID_ARG;
     const Strided k = pages_of(*c, c->k), v = pages_of(*c, c->v);
-    const Array arrays[] = {{moves, n * max_moves * 16, false},
+    const Array arrays[] = {{moves, span_bytes(n, moves_stride, max_moves, 16), false},
                             {counts, n * 4, false},
                             {scores, slots * 4, true},
                             {positions, slots * 4, true}};
@@ -492,6 +497,7 @@ lcpp_status move(const lcpp_kv_cache* c, const int64_t* moves, uint32_t max_move
     p.block_size = c->block_size;
     p.num_slots = slots;
     p.moves = reinterpret_cast<const longlong2*>(moves);
+    p.moves_stride = moves_stride;
     p.counts = counts;
     p.max_moves = max_moves;
     p.requests = num_requests;
@@ -516,12 +522,12 @@ lcpp_status lcpp_cache_evict_plan(const lcpp_cache_evict_args* args, lcpp_stream
     return guarded("lcpp_cache_evict_plan", [&] { return plan(args, reinterpret_cast<cudaStream_t>(stream)); });
 }
 
-lcpp_status lcpp_cache_evict_move(const lcpp_kv_cache* cache, const int64_t* moves, uint32_t max_moves,
-                                  const int32_t* move_counts, uint32_t num_requests, float* slot_scores,
-                                  int32_t* slot_positions, lcpp_stream_t stream)
+lcpp_status lcpp_cache_evict_move(const lcpp_kv_cache* cache, const int64_t* moves, uint64_t moves_stride,
+                                  uint32_t max_moves, const int32_t* move_counts, uint32_t num_requests,
+                                  float* slot_scores, int32_t* slot_positions, lcpp_stream_t stream)
 {
     return guarded("lcpp_cache_evict_move", [&] {
-        return move(cache, moves, max_moves, move_counts, num_requests, slot_scores, slot_positions,
+        return move(cache, moves, moves_stride, max_moves, move_counts, num_requests, slot_scores, slot_positions,
                     reinterpret_cast<cudaStream_t>(stream));
     });
 }

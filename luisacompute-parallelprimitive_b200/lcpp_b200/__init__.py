@@ -131,8 +131,8 @@ class CacheEvictArgs(ctypes.Structure):
                 ("slot_positions", ctypes.c_void_p), ("evicted", ctypes.c_void_p), ("budget", ctypes.c_uint32),
                 ("trigger", ctypes.c_uint32), ("keep_first", ctypes.c_uint32), ("keep_recent", ctypes.c_uint32),
                 ("max_moves", ctypes.c_uint32), ("seq_lens_out", ctypes.c_void_p), ("evicted_out", ctypes.c_void_p),
-                ("move_counts_out", ctypes.c_void_p), ("moves_out", ctypes.c_void_p), ("free_blocks", ctypes.c_void_p),
-                ("free_used", ctypes.c_void_p), ("free_used_out", ctypes.c_void_p), ("num_free", ctypes.c_uint32)]
+                ("move_counts_out", ctypes.c_void_p), ("moves_out", ctypes.c_void_p), ("moves_stride", ctypes.c_uint64),
+                ("free_blocks", ctypes.c_void_p), ("free_used", ctypes.c_void_p), ("free_used_out", ctypes.c_void_p), ("num_free", ctypes.c_uint32)]
 
 
 class LcppError(RuntimeError):
@@ -261,7 +261,7 @@ def lib() -> ctypes.CDLL:
         "lcpp_paged_attention_temp_bytes": ([u32, u32, u32, u32, u64, szp], i),
         "lcpp_paged_attention_decode": ([vp, sz, ctypes.POINTER(PagedAttentionArgs), vp], i),
         "lcpp_cache_evict_plan": ([ctypes.POINTER(CacheEvictArgs), vp], i),
-        "lcpp_cache_evict_move": ([ctypes.POINTER(KVCache), vp, u32, vp, u32, vp, vp, vp], i),
+        "lcpp_cache_evict_move": ([ctypes.POINTER(KVCache), vp, u64, u32, vp, u32, vp, vp, vp], i),
         "lcpp_diag_timing_enable": ([i], i),
         "lcpp_diag_launch_shapes": ([ctypes.POINTER(u64)], i),
         "lcpp_diag_wait_timeout_probe": ([vp, sz, u64, vp], i),
@@ -1042,6 +1042,17 @@ def _table(t, rows):
     return t.data_ptr(), (t.stride(0) if rows > 1 else max(t.stride(0), width)), width
 
 
+def _moves(t, requests, name):
+    """(pointer, pairs from request to request, pairs of a request) of an int64 [requests, moves, 2] tensor."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype != _torch().int64 or len(shape) != 3 or shape[2] != 2 or shape[0] < requests or stride[2] != 1 or \
+            (stride[1] != 2 and shape[1] > 1) or (stride[0] % 2 and shape[0] > 1):
+        raise LcppError(ERR_INVALID_ARG, f"{name}: int64 [num_requests, max_moves, 2], pairs adjacent")
+    if not t.is_cuda:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a CUDA tensor")
+    return t.data_ptr(), (stride[0] // 2 if shape[0] > 1 else shape[1]), shape[1]
+
+
 def _scratch(temp):
     """(pointer, bytes) of temp storage."""
     return (None, 0) if temp is None else (temp.data_ptr(), temp.numel() * temp.element_size())
@@ -1335,8 +1346,7 @@ class DeviceCacheEviction:
         torch = _torch()
         i32, n = torch.int32, num_requests
         table, table_stride, width = _table(d_block_table, n)
-        if d_moves_out.dim() != 3 or d_moves_out.shape[2] != 2 or d_moves_out.shape[0] < n:
-            raise LcppError(ERR_INVALID_ARG, "d_moves_out: int64 [num_requests, max_moves, 2]")
+        moves, moves_stride, max_moves = _moves(d_moves_out, n, "d_moves_out")
         if block_size < 1:
             raise LcppError(ERR_INVALID_ARG, "block_size: at least 1")
         pages = d_scores.numel() // block_size
@@ -1344,10 +1354,10 @@ class DeviceCacheEviction:
             _flat(d_seq_lens, i32, n, "d_seq_lens"), table, table_stride, width, n, pages, block_size,
             _flat(d_scores, torch.float32, 0, "d_scores"),
             _flat(d_positions, i32, pages * block_size, "d_positions"), _flat(d_evicted, i32, n, "d_evicted"), budget,
-            budget if trigger is None else trigger, keep_first, keep_recent, d_moves_out.shape[1],
+            budget if trigger is None else trigger, keep_first, keep_recent, max_moves,
             _flat(d_seq_lens_out, i32, n, "d_seq_lens_out"), _flat(d_evicted_out, i32, n, "d_evicted_out"),
             _flat(d_move_counts_out, i32, n, "d_move_counts_out"),
-            _flat(d_moves_out, torch.int64, 2 * n * d_moves_out.shape[1], "d_moves_out"),
+            moves, moves_stride,
             _flat(d_free_blocks, i32, 0, "d_free_blocks"), _flat(d_free_used, i32, 1, "d_free_used"),
             _flat(d_free_used_out, i32, 1, "d_free_used_out"), 0 if d_free_blocks is None else d_free_blocks.numel())
         _here(d_scores, "d_scores")
@@ -1360,10 +1370,8 @@ class DeviceCacheEviction:
         torch = _torch()
         cache = _kv_cache(d_k_cache, d_v_cache)
         slots = cache.num_pages * cache.block_size
-        if d_moves.dim() != 3 or d_moves.shape[2] != 2 or d_moves.shape[0] < num_requests:
-            raise LcppError(ERR_INVALID_ARG, "d_moves: int64 [num_requests, max_moves, 2]")
+        moves, moves_stride, max_moves = _moves(d_moves, num_requests, "d_moves")
         check(lib().lcpp_cache_evict_move(
-            cache, _flat(d_moves, torch.int64, 2 * num_requests * d_moves.shape[1], "d_moves"), d_moves.shape[1],
-            _flat(d_move_counts, torch.int32, num_requests, "d_move_counts"), num_requests,
+            cache, moves, moves_stride, max_moves, _flat(d_move_counts, torch.int32, num_requests, "d_move_counts"), num_requests,
             _flat(d_scores, torch.float32, slots, "d_scores"), _flat(d_positions, torch.int32, slots, "d_positions"),
             _queue(stream)), "Move")
