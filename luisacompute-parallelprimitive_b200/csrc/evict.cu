@@ -23,8 +23,9 @@ using namespace lcpp::model;
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / kWarp;
+constexpr int kThreads = 1024, kWarps = kThreads / kWarp;
 constexpr int kMostCluster = 8;
+constexpr int kAhead = 4;              // tokens whose loads a thread has under way
 constexpr uint32_t kKeys = 40 * 1024;  // keys of a block that stay in shared memory; others are read again
 constexpr uint32_t kProtected = 0xffffffffu, kNaN = 0xfffffffeu;
 
@@ -117,29 +118,54 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         id = uint32_t(row[page]);
         return uint64_t(id) * p.page.d + (token - page * p.page.d);
     };
-    const auto look_up = [&](uint32_t i, bool& broken) {
-        uint32_t id;
-        const uint64_t slot = slot_of(lo + i, id);
-        if (id >= p.num_pages) {
-            broken = true;
-            return 0u;
+    // keys of tokens i, i + kThreads, ..., whose loads are under way together
+    const auto look_up = [&](uint32_t i, uint32_t (&key)[kAhead], bool& broken) {
+        uint64_t slot[kAhead];
+        float score[kAhead];
+        int32_t position[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            uint32_t id = 0;
+            slot[u] = i + u * kThreads < count ? slot_of(lo + i + u * kThreads, id) : ~0ull;
+            if (id >= p.num_pages) {
+                broken = true;
+                slot[u] = ~0ull;
+            }
         }
-        const int64_t position = p.positions ? int64_t(p.positions[slot]) : int64_t(lo + i);
-        return position < p.first || position >= recent ? kProtected : key_of(p.scores[slot]);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const bool in = slot[u] != ~0ull;
+            score[u] = in ? p.scores[slot[u]] : 0.f;
+            position[u] = in && p.positions ? p.positions[slot[u]] : int32_t(lo + i + u * kThreads);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t at = position[u];
+            key[u] = at < p.first || at >= recent ? kProtected : key_of(score[u]);
+        }
     };
     const auto key_at = [&](uint32_t i) {
-        bool broken = false;
-        return i < kKeys ? keys[i] : look_up(i, broken);
+        if (i < kKeys) return keys[i];
+        uint32_t id;
+        const uint64_t slot = slot_of(lo + i, id);  // looked up before: in range
+        const int64_t at = p.positions ? int64_t(p.positions[slot]) : int64_t(lo + i);
+        return at < p.first || at >= recent ? kProtected : key_of(p.scores[slot]);
     };
 
     if (threadIdx.x == 0) shared.broken = 0;
     for (int i = threadIdx.x; i < 256 * kWarp; i += kThreads) copies[i] = 0;
     __syncthreads();
     bool broken = false;
-    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
-        const uint32_t key = look_up(i, broken);
-        if (i < kKeys) keys[i] = key;
-        atomicAdd(&copies[(key >> 24) * kWarp + lane], 1u);
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads * kAhead) {
+        uint32_t key[kAhead];
+        look_up(i, key, broken);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t at = i + u * kThreads;
+            if (at >= count) continue;
+            if (at < kKeys) keys[at] = key[u];
+            atomicAdd(&copies[(key[u] >> 24) * kWarp + lane], 1u);
+        }
     }
     if (broken) shared.broken = 1;
 
@@ -148,8 +174,6 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
     for (int pass = 0; pass < 4; ++pass) {
         const int shift = 24 - 8 * pass;
         if (pass) {
-            for (int i = threadIdx.x; i < 256 * kWarp; i += kThreads) copies[i] = 0;
-            __syncthreads();
             for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
                 const uint32_t key = key_at(i);
                 if ((key ^ top) >> (shift + 8) == 0) atomicAdd(&copies[(key >> shift & 255) * kWarp + lane], 1u);
@@ -158,6 +182,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         __syncthreads();
         for (int digit = warp; digit < 256; digit += kWarps) {
             const uint32_t sum = __reduce_add_sync(~0u, copies[digit * kWarp + lane]);
+            copies[digit * kWarp + lane] = 0;  // for the next pass
             if (lane == 0) shared.histogram[pass & 1][digit] = sum;
         }
         cluster.sync();  // the other buffer is free again, too
@@ -427,9 +452,9 @@ lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
 
     diag::KernelTimer timer(kTimerEviction, n, s);
     if (n) {
-        // Blocks of 2048 tokens and more, as long as the requests leave SMs for them.
+        // blocks of 1024 tokens and more, as long as the requests leave SMs for them
         uint32_t cluster = 1;
-        while (cluster < kMostCluster && p.longest / cluster > 4096 && n * cluster * 2 <= uint64_t(device_sm_count()) * 2)
+        while (cluster < kMostCluster && p.longest / cluster > 2048 && n * cluster * 2 <= uint64_t(device_sm_count()))
             cluster *= 2;
         const uint32_t run = uint32_t(ceil_div(p.longest, cluster));
         // room in a few steps, so that few launch shapes are set up

@@ -14,64 +14,87 @@ using namespace lcpp::model::attention;
 
 namespace {
 
-constexpr int kScoreThreads = 256;
+constexpr int kScoreThreads = 256, kScoreWarps = kScoreThreads / kWarp;
 
+// A warp takes 16 tokens: a lane four of them under every eighth head.
 __global__ void __launch_bounds__(kScoreThreads) scores_kernel(const Params p)
 {
-    const auto all_tokens = [&](uint32_t r) { return min(uint32_t(max(p.lens[r], 0)), p.longest); };
+    const auto weight = [&](uint32_t r) {  // tiles before the window, then those of the logits
+        const Tokens t = tokens_of(p, r);
+        return (long long)((t.first + kTile - 1) / kTile + t.tiles());
+    };
     long long begin = -1, end = -1;
     Place place;
     const long long total = share_of<kScoreThreads>(
-        p.requests, [&](uint32_t r) { return (long long)((all_tokens(r) + kScoreThreads - 1) / kScoreThreads); },
+        p.requests, weight,
         [&](long long all) {
-            const long long per = (all + gridDim.x - 1) / gridDim.x;
+            const long long per = run_of(all, gridDim.x, kScoreWarps);
             begin = blockIdx.x * per;
             end = min(all, begin + per);
             return begin < all ? begin : -1;
         },
         place);
-    if (begin >= total) return;
+    if (begin >= total) {
+        if (blockIdx.x == 0) wait_for_previous();  // this launch ends after the ones before
+        return;
+    }
     wait_for_previous();
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp, quad = lane % 4, part = lane / 4;
     const uint32_t units = p.kv_heads * p.chunks;
     uint32_t r = place.item;
     long long first = place.first;
-    for (long long at = begin; at < end; ++at) {
-        uint32_t n = all_tokens(r);
-        while (at >= first + (n + kScoreThreads - 1) / kScoreThreads) {
-            first += (n + kScoreThreads - 1) / kScoreThreads;
-            n = all_tokens(++r);
-        }
-        const uint32_t token = uint32_t(at - first) * kScoreThreads + threadIdx.x;
+    for (long long at = begin + warp; at < end; at += kScoreWarps) {
+        while (at >= first + weight(r)) first += weight(r++);
         const Tokens seen = tokens_of(p, r);
-        const uint32_t tiles = seen.tiles();
+        const uint32_t before = (seen.first + kTile - 1) / kTile, tiles = seen.tiles();
         const long long number = p.first[r];
-        if (token >= n || number + (long long)tiles * units > p.logit_tiles) continue;
-        const uint32_t page = p.page.quotient(token), id = uint32_t(p.table[r * p.table_stride + page]);
-        if (id >= p.num_pages) continue;
-        float mass = 0.f;
-        if (token >= seen.first) {
-            const uint32_t t = (token - seen.first) / kTile, row = (token - seen.first) % kTile;
+        if (number + (long long)tiles * units > p.logit_tiles) continue;
+        uint32_t token = uint32_t(at - first) * kTile, stop = seen.first;
+        float mass[4] = {0.f, 0.f, 0.f, 0.f};
+        if (at - first >= before) {
+            const uint32_t t = uint32_t(at - first) - before;
+            token = seen.first + t * kTile;
+            stop = seen.end;
             const float* lse = p.lse2 + uint64_t(r) * p.heads;
-            const float* x = p.logits + (number + t) * p.per_unit * kTile + row;
-            for (uint32_t head = 0, u = 0; u < units; ++u, x += (long long)tiles * p.per_unit * kTile) {
-                const uint32_t heads = min(p.per_unit, p.group - u % p.chunks * p.per_unit);
+            const float4* x = reinterpret_cast<const float4*>(p.logits) + (number + t) * p.per_unit * (kTile / 4) + quad;
+            const long long pitch = (long long)tiles * p.per_unit * (kTile / 4);
 #pragma unroll 8
-                for (uint32_t h = 0; h < heads; ++h) {
-                    const float of = __ldg(lse + head + h);
-                    mass += of == -INFINITY ? 0.f : exp2_fast(x[h * kTile] - of);
+            for (uint32_t u = 0; u < units; ++u) {
+                // the first heads of kv head u / chunks' group come in chunks of per_unit, the last one shorter
+                const uint32_t kv_head = u / p.chunks, head0 = (u - kv_head * p.chunks) * p.per_unit;
+                const uint32_t heads = min(p.per_unit, p.group - head0);
+                for (uint32_t h = part; h < heads; h += kWarp / 4) {
+                    const float of = lse[kv_head * p.group + head0 + h];
+                    const float4 logits = x[u * pitch + h * (kTile / 4)];
+                    if (of == -INFINITY) continue;
+                    mass[0] += exp2_fast(logits.x - of);
+                    mass[1] += exp2_fast(logits.y - of);
+                    mass[2] += exp2_fast(logits.z - of);
+                    mass[3] += exp2_fast(logits.w - of);
                 }
-                head += heads;
             }
         }
-        const uint64_t slot = uint64_t(id) * p.page.d + (token - page * p.page.d);
-        p.scores_out[slot] = (p.scores ? p.decay * p.scores[slot] : 0.f) + mass;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 4; d < kWarp; d *= 2) mass[i] += __shfl_xor_sync(~0u, mass[i], d);
+        // lane 4 i + quad writes token 4 quad + i
+        const float own = part == 0 ? mass[0] : part == 1 ? mass[1] : part == 2 ? mass[2] : mass[3];
+        token += quad * 4 + part;
+        if (part < 4 && token < stop) {
+            const uint32_t page = p.page.quotient(token), id = uint32_t(p.table[r * p.table_stride + page]);
+            if (id < p.num_pages) {
+                const uint64_t slot = uint64_t(id) * p.page.d + (token - page * p.page.d);
+                p.scores_out[slot] = (p.scores ? p.decay * p.scores[slot] : 0.f) + own;
+            }
+        }
     }
 }
 
 constexpr uint32_t kMostHeads = 1u << 16;
 
 struct Layout {
-    size_t meta, part, lse2, first, logits, part_bytes, bytes;
+    size_t part, lse2, first, logits, part_bytes, bytes;
     uint64_t tiles;
 };
 
@@ -83,7 +106,6 @@ Layout layout(uint64_t requests, uint32_t heads, uint32_t kv_heads, const Choice
         l.bytes += align_up(bytes, kTempAlign);
         return at;
     };
-    l.meta = take(kMostBlocks * 16);
     l.part_bytes = size_t(kMostBlocks) * 2 * c.heads * (c.columns + 2) * 4;
     l.part = take(l.part_bytes);
     if (!score_slots) return l;
@@ -176,7 +198,6 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_paged_attention_args* 
     p.scale = a->softcap > 0.f ? a->scale / a->softcap : a->scale * kLog2e;
     p.softcap = a->softcap * kLog2e;
     p.lse = a->lse_out;
-    p.meta = reinterpret_cast<int32_t*>(t + l.meta);
     p.part = reinterpret_cast<float*>(t + l.part);
     if (score_slots) {
         p.lse2 = reinterpret_cast<float*>(t + l.lse2);

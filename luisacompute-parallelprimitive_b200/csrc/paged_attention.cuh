@@ -15,10 +15,10 @@
 // block, the parts of the others by join_kernel, which starts early and waits.
 //
 // A warp works on its own: it takes every fourth tile of the run, copies the
-// tile's rows (16 keys, 16 values) into a ring of its own with cp.async, some
-// tiles ahead and across the borders of units, and needs the block's other warps
-// only where a unit ends.  The page ids of the next tile are read one tile before
-// they are needed.
+// tile's 16 keys, then its 16 values, into slots of a ring of its own with
+// cp.async, some slots ahead and across the borders of units, and needs the
+// block's other warps only where a unit ends.  The page ids of the next tile are
+// read one tile before they are needed.
 #pragma once
 
 #include "cache.cuh"
@@ -53,7 +53,6 @@ struct Params {
     float softcap;        // with log2 e; 0: none
     float* lse;
     float* part;          // [block][2][heads of a unit][columns] and, behind them, [block][2][heads of a unit][2]
-    int32_t* meta;        // [block][4]
     float* logits;        // [tile][per_unit][16] in base 2, or NULL
     long long logit_tiles;
     float* lse2;          // [request][head] in base 2 for the scores
@@ -72,6 +71,12 @@ __device__ __forceinline__ Tokens tokens_of(const Params& p, uint32_t r)
 {
     const uint32_t n = min(uint32_t(max(p.lens[r], 0)), p.longest);
     return Tokens{p.window && n > p.window ? n - p.window : 0u, n};
+}
+
+// Tiles of a block's run: equal ones, of not less than a tile for each warp.
+__device__ __forceinline__ long long run_of(long long all, uint32_t blocks, int warps)
+{
+    return max((all + blocks - 1) / blocks, (long long)warps);
 }
 
 // The block's run of tiles, and the walk over the parts of units in it.
@@ -127,6 +132,19 @@ __device__ __forceinline__ float logit(const Params& p, float dot)
 }
 // Factor of what was summed under reference `from` when it becomes `to`.
 __device__ __forceinline__ float rebase(float from, float to) { return from == -INFINITY ? 0.f : exp2_fast(from - to); }
+
+// The same for a part that is joined; one whose logits were all NaN has no
+// reference, but a sum that says so.
+__device__ __forceinline__ float share(float from, float sum, float to)
+{
+    return from == -INFINITY ? (sum == 0.f ? 0.f : sum) : exp2_fast(from - to);
+}
+__device__ __forceinline__ void put_lse(const Params& p, uint64_t at, float reference, float sum)
+{
+    const float value = sum == 0.f ? -INFINITY : reference + log2f(sum);
+    if (p.lse) p.lse[at] = value * kLn2;
+    if (p.lse2) p.lse2[at] = value;
+}
 
 // ---------------------------------------------------------------------------
 // A warp's tile in 16 bits: tensor cores, tokens as rows and heads as columns
@@ -220,39 +238,52 @@ struct Tile16 {
         }
     }
 
-    __device__ __forceinline__ void add(const Params& p, const unsigned char* keys, const unsigned char* values,
-                                        const void* queries, void*, uint32_t valid, float* logits, uint32_t heads)
+    // The tile's logits from its keys, and its terms: the second product's second
+    // operand, as two 16-bit numbers each, high part and rest: 16 digits of bfloat16
+    // and 22 of float16, against 8 and 11 that one would leave.  The products with
+    // the rest cost tensor-core time that the copies leave free.
+    uint32_t high[kN][2], rest[kN][2];
+
+    __device__ __forceinline__ void keys(const Params& p, const unsigned char* rows, const void* queries, void*,
+                                         uint32_t valid, float* logits, uint32_t heads)
     {
+        // the sum over the columns in several chains: a product waits for the one before it in its chain
+        constexpr int kChains = kN == 1 ? 4 : 2;
         const int lane = threadIdx.x % kWarp;
-        float s[kN][4];
+        float c[kChains][kN][4];
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
+        for (int i = 0; i < kChains; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[n][c] = 0.f;
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[i][n][j] = 0.f;
         const uint2* q = static_cast<const uint2*>(queries) + lane;
-        const int key_row = lane % 16;
-        const uint32_t key_at = smem_address(keys) + key_row * (D * 2);
+        const int row = lane % 16;
+        const uint32_t at = smem_address(rows) + row * (D * 2);
 #pragma unroll
         for (int step = 0; step < D / 16; ++step) {
             uint32_t a[4];
-            load_matrices(a, key_at + swizzled(key_row, step * 2 + lane / 16) * 16);
+            load_matrices(a, at + swizzled(row, step * 2 + lane / 16) * 16);
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
                 const uint2 b = q[(step * kN + n) * kWarp];
-                multiply<T>(s[n], a, b.x, b.y);
+                multiply<T>(c[step % kChains][n], a, b.x, b.y);
             }
         }
         const bool valid0 = valid >> (lane / 4) & 1, valid1 = valid >> (lane / 4 + 8) & 1;
         bool past = false;
+        float s[kN][4];
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                s[n][c] = (c < 2 ? valid0 : valid1) ? logit(p, s[n][c]) : -INFINITY;
-                past |= s[n][c] > m[n][c & 1] + (8.f + kShift);
+            for (int j = 0; j < 4; ++j) {
+                float dot = c[0][n][j] + c[1][n][j];
+                if (kChains == 4) dot += c[kChains - 2][n][j] + c[kChains - 1][n][j];
+                s[n][j] = (j < 2 ? valid0 : valid1) ? logit(p, dot) : -INFINITY;
+                past |= s[n][j] > m[n][j & 1] + (8.f + kShift);
                 if (logits) {
-                    const uint32_t head = n * 8 + lane % 4 * 2 + (c & 1);
-                    if (head < heads) logits[head * kTile + lane / 4 + (c < 2 ? 0 : 8)] = s[n][c];
+                    const uint32_t head = n * 8 + lane % 4 * 2 + (j & 1);
+                    if (head < heads) logits[head * kTile + lane / 4 + (j < 2 ? 0 : 8)] = s[n][j];
                 }
             }
         }
@@ -274,18 +305,14 @@ struct Tile16 {
                     }
                 }
         }
-        // Each term as two 16-bit numbers, high part and rest: 16 digits of bfloat16
-        // and 22 of float16, against 8 and 11 that one would leave.  The products with
-        // the rest cost tensor-core time that the copies leave free.
-        uint32_t high[kN][2], rest[kN][2];
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
             float e[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float reference = m[n][c & 1] == -INFINITY ? 0.f : m[n][c & 1];
-                e[c] = exp2_fast(s[n][c] - reference);
-                l[n][c & 1] += e[c];
+            for (int j = 0; j < 4; ++j) {
+                const float reference = m[n][j & 1] == -INFINITY ? 0.f : m[n][j & 1];
+                e[j] = exp2_fast(s[n][j] - reference);
+                l[n][j & 1] += e[j];
             }
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
@@ -301,12 +328,16 @@ struct Tile16 {
                                         uint32_t(*reinterpret_cast<const uint16_t*>(&lo[1])) << 16);
             }
         }
-        const int value_row = lane % 8 + lane / 16 * 8;
-        const uint32_t value_at = smem_address(values) + value_row * (D * 2);
+    }
+
+    __device__ __forceinline__ void values(const unsigned char* rows, const void*)
+    {
+        const int lane = threadIdx.x % kWarp, row = lane % 8 + lane / 16 * 8;
+        const uint32_t at = smem_address(rows) + row * (D * 2);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             uint32_t a[4];
-            load_matrices_transposed(a, value_at + swizzled(value_row, i * 2 + lane / 8 % 2) * 16);
+            load_matrices_transposed(a, at + swizzled(row, i * 2 + lane / 8 % 2) * 16);
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
                 multiply<T>(o[i][n], a, high[n][0], high[n][1]);
@@ -398,18 +429,19 @@ struct Tile<float, D, H> {
         }
     }
 
-    __device__ __forceinline__ void add(const Params& p, const unsigned char* keys, const unsigned char* values,
-                                        const void* queries, void* own, uint32_t valid, float* logits, uint32_t heads)
+    __device__ __forceinline__ void keys(const Params& p, const unsigned char* rows, const void* queries, void* own,
+                                         uint32_t valid, float* logits, uint32_t heads)
     {
         const int lane = threadIdx.x % kWarp, token = lane % 16, part = lane / 16;
-        const float4* k = reinterpret_cast<const float4*>(keys) + token * kChunks;
+        const float4* k = reinterpret_cast<const float4*>(rows) + token * kChunks;
         const float4* q = static_cast<const float4*>(queries);
         float s[H];
 #pragma unroll
         for (int h = 0; h < H; ++h) s[h] = 0.f;
+        const int half = int(p.dim + 7) / 8;  // the chunks that hold columns, in two halves
 #pragma unroll 4
-        for (int i = 0; i < kChunks / 2; ++i) {
-            const int chunk = part * (kChunks / 2) + i;
+        for (int i = 0; i < half; ++i) {
+            const int chunk = part * half + i;
             const float4 a = k[swizzled(token, chunk)];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
@@ -451,8 +483,13 @@ struct Tile<float, D, H> {
             }
         }
         __syncwarp();
-        const int column = lane % kLanes;
-        const float4* v = reinterpret_cast<const float4*>(values);
+    }
+
+    __device__ __forceinline__ void values(const unsigned char* rows, const void* own)
+    {
+        const int lane = threadIdx.x % kWarp, column = lane % kLanes;
+        const float* term = static_cast<const float*>(own);
+        const float4* v = reinterpret_cast<const float4*>(rows);
 #pragma unroll 4
         for (int t = lane / kLanes; t < kTile; t += kTokenStep) {
             float e[H];
@@ -512,26 +549,27 @@ struct Tile<float, D, H> {
 };
 
 // Shared memory of a block.
-template <typename T, int D, int H, int STAGES, int WARPS>
+template <typename T, int D, int H, int SLOTS, int WARPS>
 struct Room {
     using Work = Tile<T, D, H>;
     static constexpr int kRowBytes = D * int(sizeof(T));
-    static constexpr int kStageBytes = 2 * kTile * kRowBytes;  // keys, then values
-    static constexpr int kRing = STAGES * kStageBytes;         // of a warp
+    static constexpr int kSlotBytes = kTile * kRowBytes;  // a tile's keys, or its values
+    static constexpr int kRing = SLOTS * kSlotBytes;      // of a warp
+    static constexpr int kMasks = SLOTS / 2 + 2;          // tiles between the copies and the products
     static constexpr int kQueries = WARPS * kRing;
     static constexpr int kOwn = kQueries + Work::kQueryBytes;
     static constexpr int kSum = kOwn + WARPS * Work::kWarpBytes;
     static constexpr int kStats = kSum + H * (D + 4) * 4;      // m, l, factor [warp][head], then of the unit [head]
-    static constexpr int kMasks = kStats + (3 * WARPS + 2) * H * 4;
-    static constexpr int kBytes = kMasks + WARPS * STAGES * 4;
+    static constexpr int kValid = kStats + (3 * WARPS + 2) * H * 4;
+    static constexpr int kBytes = kValid + WARPS * kMasks * 4;
 };
 
 // kWide: 16-byte copies; else element by element, for rows that start anywhere.
-template <typename T, int D, int H, int STAGES, int WARPS, bool kWide>
+template <typename T, int D, int H, int SLOTS, int WARPS, bool kWide>
 __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
 {
     using Work = Tile<T, D, H>;
-    using R = Room<T, D, H, STAGES, WARPS>;
+    using R = Room<T, D, H, SLOTS, WARPS>;
     constexpr int kWarps = WARPS, kThreads = kWarps * kWarp;
     constexpr int kRowBytes = R::kRowBytes, kChunks = kRowBytes / 16;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -544,13 +582,12 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
 
     const uint32_t units = p.kv_heads * p.chunks;
     const auto weight = [&](uint32_t r) { return (long long)(tokens_of(p, r).tiles()) * units; };
-    long long begin = -1, end = -1, per = 1;
+    long long begin = -1, end = -1;
     Place place;
     const long long total = share_of<kThreads>(
         p.requests, weight,
         [&](long long all) {
-            // not less than a tile for each warp
-            per = max((all + gridDim.x - 1) / gridDim.x, (long long)kWarps);
+            const long long per = run_of(all, gridDim.x, kWarps);
             begin = blockIdx.x * per;
             end = min(all, begin + per);
             return begin < all ? begin : -1;
@@ -569,11 +606,7 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
             if (p.lse2) p.lse2[uint64_t(r) * p.heads + h] = -INFINITY;
         }
     }
-    int32_t* meta = p.meta + blockIdx.x * 4;
-    if (begin >= total) {
-        if (threadIdx.x == 0) meta[2] = 0;
-        return;
-    }
+    if (begin >= total) return;
 
     Walk now;
     now.r = place.item;
@@ -584,7 +617,7 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
     now.left = end - begin;
     now.part();
 
-    uint32_t* masks = reinterpret_cast<uint32_t*>(smem + R::kMasks) + warp * STAGES;
+    uint32_t* masks = reinterpret_cast<uint32_t*>(smem + R::kValid) + warp * R::kMasks;
     // the warp's next tile to copy, and whether there is one
     Walk ahead = now;
     uint32_t ahead_t = ahead.t + warp;
@@ -613,53 +646,60 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
         }
     };
     look_up();
-    int stage_in = 0;
-    const auto copy_next = [&] {
-        if (more) {
-            unsigned char* to = ring + stage_in * R::kStageBytes;
-            const bool valid = uint32_t(id) < p.num_pages;
-            const uint32_t mask = __ballot_sync(~0u, valid) & 0xffffu;
-            if (lane == 0) masks[stage_in] = mask;
-            const uint64_t row_offset = valid ? uint64_t(uint32_t(id)) * p.page_stride + in_page * p.token_stride +
-                                                    uint64_t(ahead.unit / p.chunks) * p.head_stride
-                                              : 0;
-            const T* k = static_cast<const T*>(p.k);
-            const T* v = static_cast<const T*>(p.v);
-            if (kWide) {
-                const uint32_t address = smem_address(to);
+    int slot_in = 0, mask_in = 0;
+    uint64_t row_offset = 0;
+    uint32_t mask = 0;
+    // A tile's keys, and at the next call its values.
+    bool values_next = false;
+    const auto copy_rows = [&](const T* from) {
+        unsigned char* to = ring + slot_in * R::kSlotBytes;
+        if (kWide) {
+            const uint32_t address = smem_address(to);
 #pragma unroll
-                for (int i = 0; i < kTile * kChunks / kWarp; ++i) {
-                    const int at = i * kWarp + lane, row = at / kChunks, chunk = at % kChunks;
-                    const uint64_t offset = __shfl_sync(~0u, row_offset, row) + chunk * (16 / sizeof(T));
-                    if (chunk * (16 / sizeof(T)) < p.dim) {
-                        const uint32_t into = address + row * kRowBytes + swizzled(row, chunk) * 16;
-                        copy_16b(into, k + offset, mask >> row & 1);
-                        copy_16b(into + kTile * kRowBytes, v + offset, mask >> row & 1);
-                    }
-                }
-            } else {
-                __syncwarp();  // the stage's last use is over
-                constexpr int kIn = 16 / int(sizeof(T));
-                for (int row = 0; row < kTile; ++row) {
-                    const uint64_t offset = __shfl_sync(~0u, row_offset, row);
-                    const bool live = mask >> row & 1;
-                    for (uint32_t c = lane; c < p.dim; c += kWarp) {
-                        T* into = reinterpret_cast<T*>(to + row * kRowBytes + swizzled(row, c / kIn) * 16) + c % kIn;
-                        into[0] = live ? k[offset + c] : from_float<T>(0.f);
-                        into[kTile * kRowBytes / int(sizeof(T))] = live ? v[offset + c] : from_float<T>(0.f);
-                    }
+            for (int i = 0; i < kTile * kChunks / kWarp; ++i) {
+                const int at = i * kWarp + lane, row = at / kChunks, chunk = at % kChunks;
+                const uint64_t offset = __shfl_sync(~0u, row_offset, row) + chunk * (16 / sizeof(T));
+                if (chunk * (16 / sizeof(T)) < p.dim)
+                    copy_16b(address + row * kRowBytes + swizzled(row, chunk) * 16, from + offset, mask >> row & 1);
+            }
+        } else {
+            __syncwarp();  // the slot's last use is over
+            constexpr int kIn = 16 / int(sizeof(T));
+            for (int row = 0; row < kTile; ++row) {
+                const uint64_t offset = __shfl_sync(~0u, row_offset, row);
+                const bool live = mask >> row & 1;
+                for (uint32_t c = lane; c < p.dim; c += kWarp) {
+                    T* into = reinterpret_cast<T*>(to + row * kRowBytes + swizzled(row, c / kIn) * 16) + c % kIn;
+                    *into = live ? from[offset + c] : from_float<T>(0.f);
                 }
             }
-            ahead_t += kWarps;
-            settle();
-            look_up();
+        }
+    };
+    const auto copy_next = [&] {
+        if (more) {
+            if (!values_next) {
+                const bool valid = uint32_t(id) < p.num_pages;
+                mask = __ballot_sync(~0u, valid) & 0xffffu;
+                if (lane == 0) masks[mask_in] = mask;
+                mask_in = mask_in + 1 == R::kMasks ? 0 : mask_in + 1;
+                row_offset = valid ? uint64_t(uint32_t(id)) * p.page_stride + in_page * p.token_stride +
+                                         uint64_t(ahead.unit / p.chunks) * p.head_stride
+                                   : 0;
+                copy_rows(static_cast<const T*>(p.k));
+            } else {
+                copy_rows(static_cast<const T*>(p.v));
+                ahead_t += kWarps;
+                settle();
+                look_up();
+            }
+            values_next = !values_next;
         }
         commit_copies();
-        stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+        slot_in = slot_in + 1 == SLOTS ? 0 : slot_in + 1;
     };
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) copy_next();
+    for (int i = 0; i < SLOTS - 1; ++i) copy_next();
 
     float* sum = reinterpret_cast<float*>(smem + R::kSum);
     float* m_all = reinterpret_cast<float*>(smem + R::kStats);
@@ -667,11 +707,18 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
     float* factor = l_all + kWarps * H;
     float* unit_m = factor + kWarps * H;
     float* unit_l = unit_m + H;
-    int stage = 0;
-    int32_t starts = 0;  // blocks behind this one that go on with the run's last unit
-    uint32_t start_request = 0, start_unit = 0;
+    int slot = 0, mask_out = 0;
     long long first_tile = begin;  // number of the part's first tile
     Work work;
+    // The oldest slot, once its copies have come; the newest is filled meanwhile.
+    const auto next_slot = [&] {
+        wait_copies<SLOTS - 2>();
+        __syncwarp();
+        copy_next();
+        const unsigned char* rows = ring + slot * R::kSlotBytes;
+        slot = slot + 1 == SLOTS ? 0 : slot + 1;
+        return rows;
+    };
     do {
         const uint32_t kv_head = now.unit / p.chunks, chunk = now.unit - kv_head * p.chunks;
         const uint32_t head0 = chunk * p.per_unit, heads = min(p.per_unit, p.group - head0);
@@ -681,15 +728,13 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
         work.clear();
         __syncthreads();
         for (uint32_t t = now.t + warp; t < now.t_end; t += kWarps) {
-            wait_copies<STAGES - 2>();
-            __syncwarp();
-            copy_next();
-            const unsigned char* keys = ring + stage * R::kStageBytes;
             const long long number = first_tile + (t - now.t);
             float* logits = p.logits && number < p.logit_tiles ? p.logits + number * p.per_unit * kTile : nullptr;
-            work.add(p, keys, keys + kTile * kRowBytes, smem + R::kQueries,
-                     smem + R::kOwn + warp * Work::kWarpBytes, masks[stage], logits, heads);
-            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            void* own = smem + R::kOwn + warp * Work::kWarpBytes;
+            const unsigned char* keys = next_slot();
+            work.keys(p, keys, smem + R::kQueries, own, masks[mask_out], logits, heads);
+            mask_out = mask_out + 1 == R::kMasks ? 0 : mask_out + 1;
+            work.values(next_slot(), own);
         }
 
         // the warps' parts, in the order of the warps
@@ -701,11 +746,9 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
             for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_all[w * H + threadIdx.x]);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                // a warp whose logits were all NaN has no reference, but a sum
-                const float from = m_all[w * H + threadIdx.x], part = l_all[w * H + threadIdx.x];
-                const float f = from == -INFINITY ? (part == 0.f ? 0.f : part) : exp2_fast(from - top);
+                const float f = share(m_all[w * H + threadIdx.x], l_all[w * H + threadIdx.x], top);
                 factor[w * H + threadIdx.x] = f;
-                all += f * part;
+                all += f * l_all[w * H + threadIdx.x];
             }
             unit_m[threadIdx.x] = top;
             unit_l[threadIdx.x] = all;
@@ -723,115 +766,135 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
                 const float all = unit_l[h];
                 if (c < p.dim) out[h * p.out_head + c] = from_float<T>(all == 0.f ? 0.f : sum[h * (D + 4) + c] / all);
             }
-            if (threadIdx.x < heads) {
-                const float base2 = unit_m[threadIdx.x] + log2f(unit_l[threadIdx.x]);
-                const uint64_t at = uint64_t(now.r) * p.heads + head + threadIdx.x;
-                const float value = unit_l[threadIdx.x] == 0.f ? -INFINITY : base2;
-                if (p.lse) p.lse[at] = value * kLn2;
-                if (p.lse2) p.lse2[at] = value;
-            }
+            if (threadIdx.x < heads)
+                put_lse(p, uint64_t(now.r) * p.heads + head + threadIdx.x, unit_m[threadIdx.x], unit_l[threadIdx.x]);
         } else {
-            const uint32_t slot = blockIdx.x * 2 + (now.t ? 0 : 1);
-            float* part = p.part + uint64_t(slot) * H * D;
+            const uint32_t place_of = blockIdx.x * 2 + (now.t ? 0 : 1);
+            float* part = p.part + uint64_t(place_of) * H * D;
             for (uint32_t i = threadIdx.x; i < heads * D; i += kThreads) part[i] = sum[i / D * (D + 4) + i % D];
-            float2* stats = reinterpret_cast<float2*>(p.part + uint64_t(gridDim.x) * 2 * H * D) + uint64_t(slot) * H;
+            float2* stats = reinterpret_cast<float2*>(p.part + uint64_t(gridDim.x) * 2 * H * D) + uint64_t(place_of) * H;
             if (threadIdx.x < heads) stats[threadIdx.x] = make_float2(unit_m[threadIdx.x], unit_l[threadIdx.x]);
-            if (now.t == 0) {
-                starts = int32_t((first_tile + now.tiles - 1) / per - blockIdx.x);
-                start_request = now.r;
-                start_unit = now.unit;
-            }
         }
         if (p.first && now.unit == 0 && now.t == 0 && threadIdx.x == 0) p.first[now.r] = first_tile;
         first_tile += now.t_end - now.t;
         __syncthreads();
     } while (now.next(p));
     wait_copies<0>();
-    if (threadIdx.x == 0) {
-        meta[0] = int32_t(start_request);
-        meta[1] = int32_t(start_unit);
-        meta[2] = starts;
-    }
 }
 
 // Block (b, h): head h of the unit that block b's run ends in and others go on
 // with.  Its parts are b's last and the first of the next `count` blocks; the
-// warps take every eighth and join in order.
+// warps take every eighth and join in order.  Where the unit lies is worked out
+// from the lengths while the decode kernel still runs.
 constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * kWarp;
 template <typename T, int D, int H>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, int decode_warps)
 {
     __shared__ float sums[kJoinWarps][D];
-    __shared__ float top_of[kJoinWarps], all_of[kJoinWarps];
+    __shared__ float2 stats_of[kJoinWarps];
     let_next_start();
-    wait_for_previous();
-    const int32_t* meta = p.meta + blockIdx.x * 4;
-    const int32_t count = meta[2];
-    if (count <= 0) return;
-    const uint32_t r = uint32_t(meta[0]), unit = uint32_t(meta[1]);
-    const uint32_t kv_head = unit / p.chunks, chunk = unit - kv_head * p.chunks;
-    const uint32_t head0 = chunk * p.per_unit, heads = min(p.per_unit, p.group - head0);
+    const uint32_t units = p.kv_heads * p.chunks;
+    long long per = 1, begin = 0, end = 0;
+    Place place;
+    const long long total = share_of<kJoinThreads>(
+        p.requests, [&](uint32_t r) { return (long long)(tokens_of(p, r).tiles()) * units; },
+        [&](long long all) {
+            per = run_of(all, gridDim.x, decode_warps);
+            begin = blockIdx.x * per;
+            end = min(all, begin + per);
+            return begin < all ? end - 1 : -1;
+        },
+        place);
+    uint32_t r = 0, unit = 0, head0 = 0, heads = 0;
+    int32_t count = 0;
     const uint32_t h = blockIdx.y;
-    if (h >= heads) return;
+    if (begin < total) {
+        r = place.item;
+        const uint32_t tiles = tokens_of(p, r).tiles();
+        unit = uint32_t((end - 1 - place.first) / tiles);
+        const long long unit_begin = place.first + (long long)unit * tiles, unit_end = unit_begin + tiles;
+        if (unit_begin >= begin && unit_end > end) count = int32_t((unit_end - 1) / per - blockIdx.x);
+        head0 = unit % p.chunks * p.per_unit;
+        heads = min(p.per_unit, p.group - head0);
+    }
+    if (count == 0 || h >= heads) {
+        // this launch ends after the one before, for whatever comes after it
+        if (blockIdx.x == 0 && h == 0) wait_for_previous();
+        return;
+    }
+    const uint32_t kv_head = unit / p.chunks;
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     const float2* stats = reinterpret_cast<const float2*>(p.part + uint64_t(gridDim.x) * 2 * H * D);
-    const auto slot_of = [&](int32_t i) { return uint64_t(blockIdx.x + i) * 2 + (i ? 0 : 1); };
+    wait_for_previous();
 
-    // each thread takes parts for the common reference
-    float top = -INFINITY;
-    for (int32_t i = threadIdx.x; i <= count; i += kJoinThreads) top = fmaxf(top, stats[slot_of(i) * H + h].x);
+    constexpr int kPer = D / kWarp, kAhead = 4;
+    float o[kPer], top = -INFINITY, all = 0.f;
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    if (lane == 0) top_of[warp] = top;
-    __syncthreads();
+    for (int c = 0; c < kPer; ++c) o[c] = 0.f;
+    for (int32_t i = warp; i <= count; i += kJoinWarps * kAhead) {
+        float2 s[kAhead];
+        float x[kAhead][kPer];
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, top_of[w]);
-
-    constexpr int kPer = (D + kWarp - 1) / kWarp;
-    float o[kPer], all = 0.f;
+        for (int u = 0; u < kAhead; ++u) {
+            const int32_t at = i + u * kJoinWarps;
+            s[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-#pragma unroll 4
-    for (int32_t i = warp; i <= count; i += kJoinWarps) {
-        const uint64_t slot = slot_of(i);
-        const float2 s = stats[slot * H + h];
-        const float f = s.x == -INFINITY ? (s.y == 0.f ? 0.f : s.y) : exp2_fast(s.x - top);
-        all += f * s.y;
-        const float* part = p.part + (slot * H + h) * D;
+            for (int c = 0; c < kPer; ++c) x[u][c] = 0.f;
+            if (at > count) continue;
+            const uint64_t slot = uint64_t(blockIdx.x + at) * 2 + (at ? 0 : 1);
+            s[u] = stats[slot * H + h];
+            const float* part = p.part + (slot * H + h) * D + lane;
 #pragma unroll
-        for (int c = 0; c < kPer; ++c) o[c] += f * part[c * kWarp + lane];
+            for (int c = 0; c < kPer; ++c) x[u][c] = part[c * kWarp];
+        }
+        float to = top;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) to = fmaxf(to, s[u].x);
+        const float keep = share(top, all, to);
+        all *= keep;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) o[c] *= keep;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const float f = share(s[u].x, s[u].y, to);
+            all += f * s[u].y;
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) o[c] += f * x[u][c];
+        }
+        top = to;
     }
 #pragma unroll
     for (int c = 0; c < kPer; ++c) sums[warp][c * kWarp + lane] = o[c];
-    if (lane == 0) all_of[warp] = all;
+    if (lane == 0) stats_of[warp] = make_float2(top, all);
     __syncthreads();
-    all = 0.f;
+    float factor[kJoinWarps];
+    top = -INFINITY, all = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) all += all_of[w];
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, stats_of[w].x);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        factor[w] = share(stats_of[w].x, stats_of[w].y, top);
+        all += factor[w] * stats_of[w].y;
+    }
     const uint32_t head = kv_head * p.group + head0 + h;
     T* out = static_cast<T*>(p.out) + r * p.out_request + head * p.out_head;
     for (uint32_t c = threadIdx.x; c < p.dim; c += kJoinThreads) {
         float x = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) x += sums[w][c];
+        for (int w = 0; w < kJoinWarps; ++w) x += factor[w] * sums[w][c];
         out[c] = from_float<T>(all == 0.f ? 0.f : x / all);
     }
-    if (threadIdx.x == 0) {
-        const float value = all == 0.f ? -INFINITY : top + log2f(all);
-        const uint64_t at = uint64_t(r) * p.heads + head;
-        if (p.lse) p.lse[at] = value * kLn2;
-        if (p.lse2) p.lse2[at] = value;
-    }
+    if (threadIdx.x == 0) put_lse(p, uint64_t(r) * p.heads + head, top, all);
 }
 
-template <typename T, int D, int H, int STAGES, int WARPS>
+template <typename T, int D, int H, int SLOTS, int WARPS>
 lcpp_status launch(const Params& base, bool wide, size_t part_bytes_at_most, cudaStream_t s)
 {
     Params p = base;
-    using R = Room<T, D, H, STAGES, WARPS>;
+    using R = Room<T, D, H, SLOTS, WARPS>;
     constexpr int kThreads = WARPS * kWarp;
     static_assert(R::kBytes <= 227 * 1024, "");
-    auto kernel = wide ? decode_kernel<T, D, H, STAGES, WARPS, true> : decode_kernel<T, D, H, STAGES, WARPS, false>;
+    auto kernel = wide ? decode_kernel<T, D, H, SLOTS, WARPS, true> : decode_kernel<T, D, H, SLOTS, WARPS, false>;
     set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), R::kBytes);
     const unsigned blocks = std::min<unsigned>(
         kMostBlocks, unsigned(device_sm_count()) * resident_blocks(reinterpret_cast<const void*>(kernel), kThreads, R::kBytes));
@@ -848,7 +911,7 @@ lcpp_status launch(const Params& base, bool wide, size_t part_bytes_at_most, cud
     config.stream = s;
     config.attrs = &early;
     config.numAttrs = 1;
-    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H>, p));
+    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H>, p, WARPS));
     return LCPP_OK;
 }
 
@@ -880,15 +943,15 @@ lcpp_status run_16bit(const Params& p, const Choice& c, bool wide, size_t part_b
 {
     switch (c.columns) {
     case 64:
-        return c.heads == 8    ? launch<T, 64, 8, 3, 4>(p, wide, part_bytes, s)
-               : c.heads == 16 ? launch<T, 64, 16, 3, 4>(p, wide, part_bytes, s)
-                               : launch<T, 64, 32, 3, 4>(p, wide, part_bytes, s);
+        return c.heads == 8    ? launch<T, 64, 8, 6, 4>(p, wide, part_bytes, s)
+               : c.heads == 16 ? launch<T, 64, 16, 6, 4>(p, wide, part_bytes, s)
+                               : launch<T, 64, 32, 6, 4>(p, wide, part_bytes, s);
     case 128:
-        return c.heads == 8    ? launch<T, 128, 8, 3, 4>(p, wide, part_bytes, s)
-               : c.heads == 16 ? launch<T, 128, 16, 3, 4>(p, wide, part_bytes, s)
-                               : launch<T, 128, 32, 3, 4>(p, wide, part_bytes, s);
+        return c.heads == 8    ? launch<T, 128, 8, 6, 4>(p, wide, part_bytes, s)
+               : c.heads == 16 ? launch<T, 128, 16, 6, 4>(p, wide, part_bytes, s)
+                               : launch<T, 128, 32, 6, 4>(p, wide, part_bytes, s);
     case 192:
-        return c.heads == 8 ? launch<T, 192, 8, 3, 4>(p, wide, part_bytes, s) : launch<T, 192, 16, 3, 4>(p, wide, part_bytes, s);
+        return c.heads == 8 ? launch<T, 192, 8, 4, 4>(p, wide, part_bytes, s) : launch<T, 192, 16, 4, 4>(p, wide, part_bytes, s);
     default:
         return c.heads == 8 ? launch<T, 256, 8, 3, 4>(p, wide, part_bytes, s) : launch<T, 256, 16, 3, 4>(p, wide, part_bytes, s);
     }
