@@ -1,18 +1,18 @@
 // evict.cu -- DeviceCacheEviction (include/lcpp_b200_model.h): requests cut down
 // to the tokens with the most attention weight.
 //
-// A request's tokens get 32-bit keys that order like (protected, score); the
-// budget-th largest key comes out of four passes over 8 of its bits, each a
-// histogram of the keys that share the bits found so far.  Tokens above it are
-// kept, and of those equal to it the first ones.  A kept token past the first
-// `budget` places fills a place whose token is not kept: numbers within two
-// counts over the tokens pair them off, no other token moves, and moves do not
-// touch one another's slots.
+// A request's tokens get 32-bit keys that order like (protected, score).  The
+// budget-th largest comes out of up to three passes over 11, 11 and 10 of their
+// bits, each a histogram of the keys that share the bits found so far; they end
+// when all keys that share them are kept.  Tokens above it are kept, and of those
+// equal to it the first ones.  A kept token past the first `budget` places fills a
+// place whose token is not kept: numbers within two counts over the tokens pair
+// them off, no other token moves, and moves do not touch one another's slots.
 //
 // A cluster of 1 to 8 blocks works on a request, each on a run of its tokens
 // whose keys stay in shared memory; the blocks read one another's histograms and
-// counts there.  A histogram has a copy for each lane of a warp: scores have few
-// leading bits, and one copy would serialise on them.
+// counts there.  A histogram has four copies, for every fourth lane one: equal
+// scores would serialise on a single one.
 #include <cooperative_groups.h>
 
 #include "cache.cuh"
@@ -47,8 +47,9 @@ struct Params {
 };
 
 // What the blocks of a cluster read of one another.
-struct Shared {
-    uint32_t histogram[2][256];
+constexpr int kBins = 2048, kCopies = 4;
+struct alignas(16) Shared {
+    uint32_t histogram[2][kBins];  // from the largest digit down
     uint32_t broken;            // a page id out of range
     uint32_t holes, fillers;    // of the block's tokens
 };
@@ -65,31 +66,32 @@ __device__ __forceinline__ uint32_t length_of(const int32_t* lens, uint32_t r, u
     return min(uint32_t(max(lens[r], 0)), longest);
 }
 
-// Sum over the block, and over the threads before.
+// Sum over the block's warps, and over the warps before.
 __device__ __forceinline__ uint32_t warps_before(uint32_t of_warp, uint32_t* warps, uint32_t& total)
 {
+    static_assert(kWarps == kWarp, "a lane for each warp");
     const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
     __syncthreads();
     if (lane == 0) warps[warp] = of_warp;
     __syncthreads();
-    uint32_t before = 0;
-    total = 0;
+    uint32_t upto = warps[lane];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w == warp) before = total;
-        total += warps[w];
+    for (int d = 1; d < kWarp; d *= 2) {
+        const uint32_t left = __shfl_up_sync(~0u, upto, d);
+        if (lane >= d) upto += left;
     }
-    return before;
+    total = __shfl_sync(~0u, upto, kWarp - 1);
+    return __shfl_sync(~0u, upto, warp) - of_warp;
 }
 
 __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
 {
     extern __shared__ uint32_t dynamic[];
-    uint32_t* copies = dynamic;  // [256][32]
-    uint32_t* keys = dynamic + 256 * kWarp;
+    uint32_t* copies = dynamic;  // [kBins][kCopies], from the largest digit down
+    uint32_t* keys = dynamic + kBins * kCopies;
     __shared__ Shared shared;
     __shared__ uint32_t warps[kWarps];
-    __shared__ uint32_t found[3];  // digit, keys above it, keys equal to it in the blocks before
+    __shared__ uint32_t found[4];  // digit, keys above it, keys of it in the blocks before and in all
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t r = blockIdx.x / blocks;
@@ -118,32 +120,6 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         id = uint32_t(row[page]);
         return uint64_t(id) * p.page.d + (token - page * p.page.d);
     };
-    // keys of tokens i, i + kThreads, ..., whose loads are under way together
-    const auto look_up = [&](uint32_t i, uint32_t (&key)[kAhead], bool& broken) {
-        uint64_t slot[kAhead];
-        float score[kAhead];
-        int32_t position[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            uint32_t id = 0;
-            slot[u] = i + u * kThreads < count ? slot_of(lo + i + u * kThreads, id) : ~0ull;
-            if (id >= p.num_pages) {
-                broken = true;
-                slot[u] = ~0ull;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const bool in = slot[u] != ~0ull;
-            score[u] = in ? p.scores[slot[u]] : 0.f;
-            position[u] = in && p.positions ? p.positions[slot[u]] : int32_t(lo + i + u * kThreads);
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int64_t at = position[u];
-            key[u] = at < p.first || at >= recent ? kProtected : key_of(score[u]);
-        }
-    };
     const auto key_at = [&](uint32_t i) {
         if (i < kKeys) return keys[i];
         uint32_t id;
@@ -153,74 +129,122 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
     };
 
     if (threadIdx.x == 0) shared.broken = 0;
-    for (int i = threadIdx.x; i < 256 * kWarp; i += kThreads) copies[i] = 0;
+    for (int i = threadIdx.x; i < kBins * kCopies; i += kThreads) copies[i] = 0;
     __syncthreads();
     bool broken = false;
+    // kAhead tokens at a time, whose loads are under way together; the page ids of
+    // the next ones come meanwhile
+    uint32_t id[kAhead];
+    const auto look_up = [&](uint32_t i) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t at = i + u * kThreads;
+            id[u] = at < count ? uint32_t(row[p.page.quotient(lo + at)]) : 0;
+        }
+    };
+    look_up(threadIdx.x);
     for (uint32_t i = threadIdx.x; i < count; i += kThreads * kAhead) {
-        uint32_t key[kAhead];
-        look_up(i, key, broken);
+        float score[kAhead];
+        int32_t position[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t at = i + u * kThreads, token = lo + at;
+            const bool in = at < count && id[u] < p.num_pages;
+            broken |= at < count && !in;
+            const uint64_t slot = uint64_t(id[u]) * p.page.d + (token - p.page.quotient(token) * p.page.d);
+            score[u] = in ? p.scores[slot] : 0.f;
+            position[u] = in && p.positions ? p.positions[slot] : int32_t(token);
+        }
+        look_up(i + kThreads * kAhead);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const uint32_t at = i + u * kThreads;
             if (at >= count) continue;
-            if (at < kKeys) keys[at] = key[u];
-            atomicAdd(&copies[(key[u] >> 24) * kWarp + lane], 1u);
+            const int64_t place = position[u];
+            const uint32_t key = place < p.first || place >= recent ? kProtected : key_of(score[u]);
+            if (at < kKeys) keys[at] = key;
+            atomicAdd(&copies[(kBins - 1 - (key >> 21)) * kCopies + lane % kCopies], 1u);
         }
     }
     if (broken) shared.broken = 1;
 
     uint32_t top = 0, need = p.budget;  // bits found; tokens to keep among the keys that share them
     uint32_t equal_before = 0;          // keys equal to the last one in the blocks before this one
-    for (int pass = 0; pass < 4; ++pass) {
-        const int shift = 24 - 8 * pass;
+    const auto meet = [&] {
+        if (blocks > 1) cluster.sync();
+        else __syncthreads();
+    };
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
         if (pass) {
             for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
                 const uint32_t key = key_at(i);
-                if ((key ^ top) >> (shift + 8) == 0) atomicAdd(&copies[(key >> shift & 255) * kWarp + lane], 1u);
+                if ((key ^ top) >> (shift + bits) == 0) {
+                    const uint32_t digit = key >> shift & ((1u << bits) - 1);
+                    atomicAdd(&copies[(kBins - 1 - digit) * kCopies + lane % kCopies], 1u);
+                }
             }
         }
         __syncthreads();
-        for (int digit = warp; digit < 256; digit += kWarps) {
-            const uint32_t sum = __reduce_add_sync(~0u, copies[digit * kWarp + lane]);
-            copies[digit * kWarp + lane] = 0;  // for the next pass
-            if (lane == 0) shared.histogram[pass & 1][digit] = sum;
+        // a thread's two bins
+        static_assert(kBins == 2 * kThreads && kCopies == 4, "");
+        uint4* bin = reinterpret_cast<uint4*>(copies) + threadIdx.x * 2;
+        const uint4 x = bin[0], y = bin[1];
+        bin[0] = bin[1] = make_uint4(0, 0, 0, 0);  // for the next pass
+        uint2 mine = make_uint2(x.x + x.y + x.z + x.w, y.x + y.y + y.z + y.w), earlier = make_uint2(0, 0);
+        if (blocks > 1) {
+            reinterpret_cast<uint2*>(shared.histogram[pass & 1])[threadIdx.x] = mine;
+            cluster.sync();  // the other buffer is free again, too
+            uint2 of[kMostCluster];
+#pragma unroll
+            for (uint32_t b = 0; b < kMostCluster; ++b)
+                of[b] = b < blocks ? reinterpret_cast<const uint2*>(
+                                         cluster.map_shared_rank(&shared, b)->histogram[pass & 1])[threadIdx.x]
+                                   : make_uint2(0, 0);
+            mine = make_uint2(0, 0);
+#pragma unroll
+            for (uint32_t b = 0; b < kMostCluster; ++b) {
+                mine.x += of[b].x, mine.y += of[b].y;
+                if (b < rank) earlier.x += of[b].x, earlier.y += of[b].y;
+            }
         }
-        cluster.sync();  // the other buffer is free again, too
         if (pass == 0) {
             uint32_t any = 0;
             for (uint32_t b = 0; b < blocks; ++b) any |= cluster.map_shared_rank(&shared, b)->broken;
             if (any) {
                 leave();
-                cluster.sync();
+                meet();  // nobody leaves while others read
                 return;
             }
         }
-        uint32_t mine = 0, equal = 0;  // of digit 255 - thread, in all blocks and in those before
-        if (threadIdx.x < 256) {
-            for (uint32_t b = 0; b < blocks; ++b) {
-                const uint32_t c = cluster.map_shared_rank(&shared, b)->histogram[pass & 1][255 - threadIdx.x];
-                mine += c;
-                if (b < rank) equal += c;
-            }
-        }
-        uint32_t upto = mine;
+        uint32_t upto = mine.x + mine.y;
 #pragma unroll
         for (int d = 1; d < kWarp; d *= 2) {
             const uint32_t left = __shfl_up_sync(~0u, upto, d);
             if (lane >= d) upto += left;
         }
         uint32_t all;
-        upto += warps_before(__shfl_sync(~0u, upto, kWarp - 1), warps, all);
-        if (upto >= need && upto - mine < need) {  // one thread: there are more than `need` such keys
-            found[0] = 255 - threadIdx.x;
-            found[1] = upto - mine;
-            found[2] = equal;
+        const uint32_t before_warp = warps_before(__shfl_sync(~0u, upto, kWarp - 1), warps, all);
+        const uint32_t above = before_warp + upto - mine.x - mine.y;
+        // one thread finds the bin: there are at least `need` such keys
+        if (above < need && above + mine.x + mine.y >= need) {
+            const bool second = above + mine.x < need;
+            found[0] = kBins - 1 - 2 * threadIdx.x - second;
+            found[1] = above + (second ? mine.x : 0);
+            found[2] = second ? earlier.y : earlier.x;
+            found[3] = second ? mine.y : mine.x;
         }
         __syncthreads();
         top |= found[0] << shift;
         need -= found[1];
         equal_before = found[2];
+        const bool all_kept = found[3] == need;
         __syncthreads();
+        if (all_kept) {  // so the keys above top - 1 are; top is not 0, for some key is not kept
+            top -= 1;
+            need = 0;
+            break;
+        }
     }
 
     // Each warp takes a run of the block's tokens, 32 at a time.  Equal keys are
@@ -255,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
     if (threadIdx.x == 0) shared.holes = total;
     uint32_t filler = warps_before(fillers, warps, total);
     if (threadIdx.x == 0) shared.fillers = total;
-    cluster.sync();
+    meet();
     uint32_t moves = 0;
     for (uint32_t b = 0; b < blocks; ++b) {
         const Shared* other = cluster.map_shared_rank(&shared, b);
@@ -265,7 +289,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         }
         moves += other->fillers;
     }
-    cluster.sync();  // nobody leaves while others read
+    meet();  // nobody leaves while others read
     if (moves > p.max_moves) {
         leave();
         return;
@@ -452,16 +476,16 @@ lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
 
     diag::KernelTimer timer(kTimerEviction, n, s);
     if (n) {
-        // blocks of 1024 tokens and more, as long as the requests leave SMs for them
+        // blocks of 2048 tokens and more, as long as the requests leave SMs for them
         uint32_t cluster = 1;
-        while (cluster < kMostCluster && p.longest / cluster > 2048 && n * cluster * 2 <= uint64_t(device_sm_count()))
+        while (cluster < kMostCluster && p.longest / cluster > 4096 && n * cluster * 2 <= uint64_t(device_sm_count()))
             cluster *= 2;
         const uint32_t run = uint32_t(ceil_div(p.longest, cluster));
         // room in a few steps, so that few launch shapes are set up
         uint32_t room = 4096;
         while (room < kKeys && room < run) room *= 2;
-        const size_t smem = (256 * kWarp + std::min(room, kKeys)) * 4;
-        set_max_dynamic_smem(reinterpret_cast<const void*>(plan_kernel), (256 * kWarp + kKeys) * 4);
+        const size_t smem = (kBins * kCopies + std::min(room, kKeys)) * 4;
+        set_max_dynamic_smem(reinterpret_cast<const void*>(plan_kernel), (kBins * kCopies + kKeys) * 4);
         cudaLaunchAttribute shape{};
         shape.id = cudaLaunchAttributeClusterDimension;
         shape.val.clusterDim.x = cluster;

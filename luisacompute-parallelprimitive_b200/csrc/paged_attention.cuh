@@ -557,9 +557,10 @@ struct Room {
     static constexpr int kRing = SLOTS * kSlotBytes;      // of a warp
     static constexpr int kMasks = SLOTS / 2 + 2;          // tiles between the copies and the products
     static constexpr int kQueries = WARPS * kRing;
-    static constexpr int kOwn = kQueries + Work::kQueryBytes;
-    static constexpr int kSum = kOwn + WARPS * Work::kWarpBytes;
-    static constexpr int kStats = kSum + H * (D + 4) * 4;      // m, l, factor [warp][head], then of the unit [head]
+    static constexpr int kSum = kQueries;  // when the queries are not needed any more
+    static constexpr int kSumBytes = H * (D + 4) * 4;
+    static constexpr int kOwn = kQueries + (Work::kQueryBytes > kSumBytes ? Work::kQueryBytes : kSumBytes);
+    static constexpr int kStats = kOwn + WARPS * Work::kWarpBytes;  // m, l, factor [warp][head], then of the unit [head]
     static constexpr int kValid = kStats + (3 * WARPS + 2) * H * 4;
     static constexpr int kBytes = kValid + WARPS * kMasks * 4;
 };
@@ -782,66 +783,77 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
     wait_copies<0>();
 }
 
-// Block (b, h): head h of the unit that block b's run ends in and others go on
-// with.  Its parts are b's last and the first of the next `count` blocks; the
-// warps take every eighth and join in order.  Where the unit lies is worked out
-// from the lengths while the decode kernel still runs.
+// Head h = blockIdx.y of a unit whose tiles lie in several blocks' runs: the last
+// part of the first of them and the first parts of the next `count`; the warps take
+// every eighth and join in order.  Which unit is worked out from the lengths while
+// the decode kernel still runs: where the call has fewer units than the decode
+// kernel has blocks it is unit blockIdx.x, else the one that block blockIdx.x's run
+// ends in (blocks for all units of 2 x 2, or all runs: 2 x 131072 tokens 85 or 91 us).
 constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * kWarp;
 template <typename T, int D, int H>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, int decode_warps)
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, uint32_t decode_blocks, int decode_warps, bool by_unit)
 {
     __shared__ float sums[kJoinWarps][D];
     __shared__ float2 stats_of[kJoinWarps];
     let_next_start();
-    const uint32_t units = p.kv_heads * p.chunks;
-    long long per = 1, begin = 0, end = 0;
-    Place place;
-    const long long total = share_of<kJoinThreads>(
-        p.requests, [&](uint32_t r) { return (long long)(tokens_of(p, r).tiles()) * units; },
-        [&](long long all) {
-            per = run_of(all, gridDim.x, decode_warps);
-            begin = blockIdx.x * per;
-            end = min(all, begin + per);
-            return begin < all ? end - 1 : -1;
-        },
-        place);
-    uint32_t r = 0, unit = 0, head0 = 0, heads = 0;
-    int32_t count = 0;
-    const uint32_t h = blockIdx.y;
-    if (begin < total) {
-        r = place.item;
+    const uint32_t units = p.kv_heads * p.chunks, h = blockIdx.y;
+    const auto weight = [&](uint32_t i) { return (long long)(tokens_of(p, i).tiles()) * units; };
+    uint32_t r = 0, unit = 0, block = 0, count = 0;
+    if (by_unit) {
+        r = blockIdx.x / units;
+        unit = blockIdx.x - r * units;
+        long long total;
+        const long long before = sum_before<kJoinThreads>(p.requests, r, weight, total);
         const uint32_t tiles = tokens_of(p, r).tiles();
-        unit = uint32_t((end - 1 - place.first) / tiles);
-        const long long unit_begin = place.first + (long long)unit * tiles, unit_end = unit_begin + tiles;
-        if (unit_begin >= begin && unit_end > end) count = int32_t((unit_end - 1) / per - blockIdx.x);
-        head0 = unit % p.chunks * p.per_unit;
-        heads = min(p.per_unit, p.group - head0);
+        const long long per = run_of(total, decode_blocks, decode_warps), first = before + (long long)unit * tiles;
+        block = uint32_t(first / per);
+        if (tiles) count = uint32_t((first + tiles - 1) / per) - block;
+    } else {
+        long long per = 1, begin = 0, end = 0;
+        Place place;
+        block = blockIdx.x;
+        const long long total = share_of<kJoinThreads>(
+            p.requests, weight,
+            [&](long long all) {
+                per = run_of(all, decode_blocks, decode_warps);
+                begin = block * per;
+                end = min(all, begin + per);
+                return begin < all ? end - 1 : -1;
+            },
+            place);
+        if (begin < total) {
+            r = place.item;
+            const uint32_t tiles = tokens_of(p, r).tiles();
+            unit = uint32_t((end - 1 - place.first) / tiles);
+            const long long unit_begin = place.first + (long long)unit * tiles, unit_end = unit_begin + tiles;
+            if (unit_begin >= begin && unit_end > end) count = uint32_t((unit_end - 1) / per - block);
+        }
     }
-    if (count == 0 || h >= heads) {
+    const uint32_t kv_head = unit / p.chunks, head0 = unit % p.chunks * p.per_unit;
+    if (count == 0 || h >= min(p.per_unit, p.group - head0)) {
         // this launch ends after the one before, for whatever comes after it
         if (blockIdx.x == 0 && h == 0) wait_for_previous();
         return;
     }
-    const uint32_t kv_head = unit / p.chunks;
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-    const float2* stats = reinterpret_cast<const float2*>(p.part + uint64_t(gridDim.x) * 2 * H * D);
+    const float2* stats = reinterpret_cast<const float2*>(p.part + uint64_t(decode_blocks) * 2 * H * D);
     wait_for_previous();
 
     constexpr int kPer = D / kWarp, kAhead = 4;
     float o[kPer], top = -INFINITY, all = 0.f;
 #pragma unroll
     for (int c = 0; c < kPer; ++c) o[c] = 0.f;
-    for (int32_t i = warp; i <= count; i += kJoinWarps * kAhead) {
+    for (uint32_t i = warp; i <= count; i += kJoinWarps * kAhead) {
         float2 s[kAhead];
         float x[kAhead][kPer];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int32_t at = i + u * kJoinWarps;
+            const uint32_t at = i + u * kJoinWarps;
             s[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int c = 0; c < kPer; ++c) x[u][c] = 0.f;
             if (at > count) continue;
-            const uint64_t slot = uint64_t(blockIdx.x + at) * 2 + (at ? 0 : 1);
+            const uint64_t slot = uint64_t(block + at) * 2 + (at ? 0 : 1);
             s[u] = stats[slot * H + h];
             const float* part = p.part + (slot * H + h) * D + lane;
 #pragma unroll
@@ -906,12 +918,14 @@ lcpp_status launch(const Params& base, bool wide, size_t part_bytes_at_most, cud
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(blocks, std::min<uint32_t>(p.per_unit, H));
+    const uint64_t units = uint64_t(p.requests) * p.kv_heads * p.chunks;
+    const bool by_unit = units < blocks;
+    config.gridDim = dim3(by_unit ? unsigned(units) : blocks, std::min<uint32_t>(p.per_unit, H));
     config.blockDim = dim3(kJoinThreads);
     config.stream = s;
     config.attrs = &early;
     config.numAttrs = 1;
-    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H>, p, WARPS));
+    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H>, p, uint32_t(blocks), WARPS, by_unit));
     return LCPP_OK;
 }
 

@@ -4,11 +4,13 @@
 // A pair (a, b) at angle t = position * f becomes scale * (a cos t - b sin t,
 // b cos t + a sin t); the gradient is the same with -t.  The angle is taken in
 // 64 bits as a number of turns, whose fraction alone goes to sincospi in 32: a
-// position of 10^6 leaves a 32-bit angle 4 bits of fraction.  A block takes a
-// few tokens, computes their cosines and sines once into shared memory (half a
-// head's columns each, next to nothing beside the heads that use them), and its
-// threads turn vectors of pairs; a thread's first loads are on their way while
-// it works on the angles.
+// position of 10^6 leaves a 32-bit angle 4 bits of fraction.
+//
+// A team of 1 to 8 warps takes a token: each warp puts the token's cosines and
+// sines into shared memory of its own (half a head's columns each, next to
+// nothing beside the heads that use them) while its lanes' first vectors of pairs
+// are on their way, and turns its share of the vectors.  No warp waits for
+// another.
 //
 // Bound by memory: every element is read once and written once.
 #include "cache.cuh"
@@ -18,17 +20,19 @@ using namespace lcpp::model;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kAhead = 2;                 // vectors that a thread loads before the angles are ready
-constexpr int kMaxTokens = 16;            // tokens of a block
-constexpr uint32_t kItemsPerBlock = kThreads * kAhead;
+constexpr int kThreads = 256, kWarps = kThreads / kWarp;
+constexpr int kAhead = 2;  // vectors (of pairs) that a lane has under way
 
 struct Section {
     const void* in;
     void* out;
     uint64_t in_token, in_head, out_token, out_head;
-    uint32_t items;  // vectors of all heads of a token
-    uint32_t copied; // 0: the columns past rotary_dim are in place already
+    // From a lane's vector to its next one, 32 * team on, in elements; and what
+    // is added where that lies in the next head.
+    int64_t in_step, in_wrap, out_step, out_wrap;
+    uint32_t vectors;             // of a token
+    uint32_t step, per_head;      // a lane's step past whole heads, and a head's vectors
+    uint32_t copied;              // 0: the columns past rotary_dim are in place already
 };
 
 struct Params {
@@ -45,203 +49,203 @@ struct Params {
     uint32_t block_size;
     uint32_t tokens, requests;
     uint32_t half;       // rotary_dim / 2
-    uint32_t turned;     // vectors (of pairs) of a head that are turned
-    uint32_t per_head;   // and those with the ones that are copied
-    uint32_t plain;      // vectors of a head of v
-    uint32_t items;      // vectors of a token
-    uint32_t per_block;  // tokens of a block
+    uint32_t turned;     // vectors (of pairs) of a head that are turned, the first ones
+    uint32_t team;       // warps that share a token, a power of two
     float scale, sign;
 };
 
-template <int BYTES>
-struct Raw;
-template <>
-struct Raw<16> { using type = uint4; };
-template <>
-struct Raw<8> { using type = uint2; };
-template <>
-struct Raw<4> { using type = uint32_t; };
-template <>
-struct Raw<2> { using type = unsigned short; };
-
-// N adjacent elements.
+// N adjacent elements, as the 32-bit words of one access (two bytes in the low half of one).
 template <typename T, int N>
-struct alignas(N * sizeof(T)) Pack {
-    T e[N];
+struct Pack {
+    static constexpr int kBytes = N * int(sizeof(T)), kWords = kBytes < 4 ? 1 : kBytes / 4;
+    uint32_t w[kWords];
 };
 template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load(const T* p)
+__device__ __forceinline__ void load(Pack<T, N>& v, const T* p)
 {
-    using R = typename Raw<N * int(sizeof(T))>::type;
-    union {
-        R raw;
-        Pack<T, N> pack;
-    } u;
-    u.raw = *reinterpret_cast<const R*>(p);
-    return u.pack;
+    if constexpr (Pack<T, N>::kBytes == 16) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        v.w[0] = x.x, v.w[1] = x.y, v.w[2] = x.z, v.w[3] = x.w;
+    } else if constexpr (Pack<T, N>::kBytes == 8) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        v.w[0] = x.x, v.w[1] = x.y;
+    } else if constexpr (Pack<T, N>::kBytes == 4) {
+        v.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+        v.w[0] = *reinterpret_cast<const unsigned short*>(p);
+    }
 }
 template <typename T, int N>
 __device__ __forceinline__ void store(T* p, const Pack<T, N>& v)
 {
-    using R = typename Raw<N * int(sizeof(T))>::type;
-    union {
-        R raw;
-        Pack<T, N> pack;
-    } u;
-    u.pack = v;
-    *reinterpret_cast<R*>(p) = u.raw;
+    if constexpr (Pack<T, N>::kBytes == 16) *reinterpret_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    else if constexpr (Pack<T, N>::kBytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(v.w[0], v.w[1]);
+    else if constexpr (Pack<T, N>::kBytes == 4) *reinterpret_cast<uint32_t*>(p) = v.w[0];
+    else *reinterpret_cast<unsigned short*>(p) = static_cast<unsigned short>(v.w[0]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void floats_of(const Pack<T, N>& v, float (&out)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (sizeof(T) == 4) out[i] = __uint_as_float(v.w[i]);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+            out[i] = __uint_as_float(i % 2 ? v.w[i / 2] & 0xffff0000u : v.w[i / 2] << 16);
+        else out[i] = __half2float(__ushort_as_half(static_cast<unsigned short>(i % 2 ? v.w[i / 2] >> 16 : v.w[i / 2])));
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void pack(Pack<T, N>& v, const float (&in)[N])
+{
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v.w[i] = __float_as_uint(in[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float high = N > 1 ? in[(i + 1) % N] : 0.f;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value)
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.w[i / 2]) : "f"(high), "f"(in[i]));
+            else
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v.w[i / 2]) : "f"(high), "f"(in[i]));
+        }
+    }
 }
 
 // One order of roundings, so that a pair's bits do not depend on the vector it is part of.
-template <typename T>
-__device__ __forceinline__ void turn_pair(float2 cs, float x, float y, T& a, T& b)
+__device__ __forceinline__ void turn_pair(float2 cs, float& a, float& b)
 {
-    a = from_float<T>(fmaf(x, cs.x, -__fmul_rn(y, cs.y)));
-    b = from_float<T>(fmaf(y, cs.x, __fmul_rn(x, cs.y)));
+    const float x = a, y = b;
+    a = fmaf(x, cs.x, -__fmul_rn(y, cs.y));
+    b = fmaf(y, cs.x, __fmul_rn(x, cs.y));
 }
 
-// One vector's work: where it comes from and goes to, and its first angle.
-// kHalf: N pairs (i, i + half), two vectors apart; else N / 2 adjacent pairs, or
-// for N = 1 one pair as two elements.
-template <typename T>
-struct Item {
-    const T* in;
-    T* out;
-    int angle;  // in the block's table; below 0: copied
-    bool live;
-};
-
 template <typename T, int N, bool kHalf, bool kAppend>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const Params p)
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const Params p)
 {
-    extern __shared__ float2 turn[];  // [per_block][half] cosine and sine with the scale
-    __shared__ int64_t place_of[kMaxTokens];  // elements from the cache's start; below 0: the token is left out
-    constexpr int kElements = kHalf ? N : (N == 1 ? 2 : N);
-    const uint32_t first = blockIdx.x * p.per_block, tokens = min(p.per_block, p.tokens - first);
+    // kHalf: vectors of N pairs (i, i + half) in two places; else of N / 2 adjacent
+    // pairs, or for N = 1 of one pair as two elements
+    constexpr bool kTwo = kHalf || N == 1;  // a pair's second half is loaded by itself
+    constexpr int kPairs = kHalf ? N : N == 1 ? 1 : N / 2;
+    extern __shared__ __align__(16) float2 tables[];  // [warp][half] cosine and sine with the scale
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    float2* turn = tables + warp * ((p.half + 1) / 2 * 2);
+    const uint32_t worker = blockIdx.x * kWarps + warp, part = worker & (p.team - 1);
+    const uint32_t teams = gridDim.x * kWarps / p.team;
+    const uint32_t start = part * kWarp + lane;  // the lane's first vector
+    using P = Pack<T, N>;
 
-    if (threadIdx.x < tokens) {
-        const uint32_t t = first + threadIdx.x;
-        int64_t slot = 0;
+    for (uint32_t t = worker / p.team; t < p.tokens; t += teams) {
+        int64_t position = p.positions[t], place = 0;
+        bool live = true;
         if (kAppend) {
-            slot = p.slots[t];
-            if (uint64_t(slot) >= p.num_slots) slot = -1;
+            const int64_t slot = p.slots[t];
+            live = uint64_t(slot) < p.num_slots;
+            if (live) {
+                const uint64_t page = uint64_t(slot) / p.block_size;
+                place = int64_t(page * p.page_stride + (uint64_t(slot) - page * p.block_size) * p.s[1].out_token);
+            }
         }
-        int64_t position = p.positions[t];
         if (p.token_request) {
             const int32_t r = p.token_request[t];
-            if (uint32_t(r) >= p.requests) slot = -1;
+            if (uint32_t(r) >= p.requests) live = false;
             else if (p.position_offset) position += p.position_offset[r];
         }
-        int64_t place = slot;
-        if (kAppend && slot >= 0) {
-            const uint64_t page = uint64_t(slot) / p.block_size;
-            place = int64_t(page * p.page_stride + (uint64_t(slot) - page * p.block_size) * p.s[1].out_token);
-        }
-        place_of[threadIdx.x] = place;
-        if (kAppend && slot >= 0) {
+        if (!live) continue;
+        if (kAppend && part == 0 && lane == 0) {
+            const int64_t slot = p.slots[t];
             if (p.slot_positions) p.slot_positions[slot] = int32_t(position);
             if (p.slot_scores) p.slot_scores[slot] = 0.f;
         }
-    }
-    __syncthreads();
-
-    const auto item_at = [&](uint32_t i) {
-        Item<T> item{nullptr, nullptr, -1, false};
-        if (i >= tokens * p.items) return item;
-        const uint32_t t = i / p.items;
-        uint32_t rest = i - t * p.items;
-        const int64_t place = place_of[t];
-        if (place < 0) return item;
-        int s = 0;
-        if (rest >= p.s[0].items) {
-            rest -= p.s[0].items;
-            s = 1;
-            if (kAppend && rest >= p.s[1].items) {
-                rest -= p.s[1].items;
-                s = 2;
+        // The first vectors of q, or of k, are loaded before the angles are worked out.
+        bool ready = false;
+        const auto section = [&](const Section& c, uint64_t to, bool turns) {
+            const uint32_t head = start / c.per_head;
+            uint32_t j = start - head * c.per_head;
+            const T* in = static_cast<const T*>(c.in) + t * c.in_token + head * c.in_head + j * N;
+            T* out = static_cast<T*>(c.out) + to + head * c.out_head + j * N;
+            for (uint32_t v = start; v - lane < c.vectors; ) {  // the warp's lanes together
+                P a[kAhead], b[kAhead];
+                T* at[kAhead];
+                int angle[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    at[u] = nullptr;
+                    angle[u] = -1;
+                    const bool turned = turns && j < p.turned;
+                    if (v < c.vectors && (turned || c.copied)) {
+                        // from a vector's number to its column: past the turned ones for those that are copied
+                        const int64_t more = !turns ? 0 : kHalf ? (turned ? 0 : p.half) : N > 1 ? 0 : turned ? j : p.half;
+                        at[u] = out + more;
+                        load(a[u], in + more);
+                        if (turned) {
+                            angle[u] = int(j);
+                            if (kTwo) load(b[u], in + more + (kHalf ? p.half : 1));
+                        }
+                    }
+                    v += p.team * kWarp;
+                    in += c.in_step;
+                    out += c.out_step;
+                    j += c.step;
+                    if (j >= c.per_head) {
+                        j -= c.per_head;
+                        in += c.in_wrap;
+                        out += c.out_wrap;
+                    }
+                }
+                if (!ready) {
+                    for (uint32_t i = lane; i < p.half; i += kWarp) {
+                        // turns = position * f / 2 pi, whose whole part is dropped before 32 bits
+                        const double of = double(position) * (p.frequencies[i] * 0.15915494309189533577);
+                        float sine, cosine;
+                        sincospif(2.f * float(of - rint(of)), &sine, &cosine);
+                        // two pairs of a vector together, those of the lanes' vectors side by side
+                        const uint32_t to = kPairs == 1 ? i : (i % kPairs / 2 * p.turned + i / kPairs) * 2 + i % 2;
+                        turn[to] = make_float2(p.scale * cosine, p.sign * sine);
+                    }
+                    __syncwarp();
+                    ready = true;
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    if (!at[u]) continue;
+                    if (angle[u] < 0) {
+                        store(at[u], a[u]);
+                        continue;
+                    }
+                    float x[N], y[N];
+                    floats_of(a[u], x);
+                    if constexpr (kTwo) floats_of(b[u], y);
+                    if constexpr (kPairs == 1) {
+                        const float2 cs = turn[angle[u]];
+                        if constexpr (kTwo) turn_pair(cs, x[0], y[0]);
+                        else turn_pair(cs, x[0], x[1 % N]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kPairs; i += 2) {
+                            const float4 cs = *reinterpret_cast<const float4*>(turn + (i / 2 * p.turned + angle[u]) * 2);
+                            if constexpr (kTwo) {
+                                turn_pair(make_float2(cs.x, cs.y), x[i], y[i]);
+                                turn_pair(make_float2(cs.z, cs.w), x[i + 1], y[i + 1]);
+                            } else {
+                                turn_pair(make_float2(cs.x, cs.y), x[i * 2], x[i * 2 + 1]);
+                                turn_pair(make_float2(cs.z, cs.w), x[i * 2 + 2], x[i * 2 + 3]);
+                            }
+                        }
+                    }
+                    if constexpr (kTwo) {
+                        pack(b[u], y);
+                        store(at[u] + (kHalf ? p.half : 1), b[u]);
+                    }
+                    pack(a[u], x);
+                    store(at[u], a[u]);
+                }
             }
-        }
-        const Section& c = p.s[s];
-        const uint32_t wide = kAppend && s == 2 ? p.plain : p.per_head;
-        const uint32_t head = rest / wide;
-        uint32_t j = rest - head * wide;
-        uint32_t column;
-        if ((!kAppend || s < 2) && j < p.turned) {
-            item.angle = int(t * p.half + (kHalf ? j * N : j * (kElements / 2)));
-            column = kHalf ? j * N : j * kElements;
-        } else {
-            if (!c.copied) return item;
-            column = kAppend && s == 2 ? j * N : 2 * p.half + (j - p.turned) * N;
-        }
-        item.live = true;
-        item.in = static_cast<const T*>(c.in) + uint64_t(first + t) * c.in_token + head * c.in_head + column;
-        const uint64_t to = kAppend && s > 0 ? uint64_t(place) : uint64_t(first + t) * c.out_token;
-        item.out = static_cast<T*>(c.out) + to + head * c.out_head + column;
-        return item;
-    };
-    using P = Pack<T, N>;
-    const auto fetch = [&](const Item<T>& item, P& a, P& b) {
-        if (!item.live) return;
-        a = load<T, N>(item.in);
-        if (item.angle >= 0) {
-            if (kHalf) b = load<T, N>(item.in + p.half);
-            else if (N == 1) b = load<T, N>(item.in + 1);
-        }
-    };
-    const auto finish = [&](const Item<T>& item, P a, P b) {
-        if (!item.live) return;
-        if (item.angle < 0) {
-            store<T, N>(item.out, a);
-            return;
-        }
-        if (kHalf || N == 1) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float2 cs = turn[item.angle + i];
-                const float x = to_float(a.e[i]), y = to_float(b.e[i]);
-                turn_pair(cs, x, y, a.e[i], b.e[i]);
-            }
-            store<T, N>(item.out, a);
-            store<T, N>(item.out + (kHalf ? p.half : 1), b);
-        } else {
-#pragma unroll
-            for (int i = 0; i + 1 < N; i += 2) {
-                const float2 cs = turn[item.angle + i / 2];
-                const float x = to_float(a.e[i]), y = to_float(a.e[i + 1]);
-                turn_pair(cs, x, y, a.e[i], a.e[i + 1]);
-            }
-            store<T, N>(item.out, a);
-        }
-    };
-
-    Item<T> item[kAhead];
-    P a[kAhead], b[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-        item[i] = item_at(threadIdx.x + i * kThreads);
-        fetch(item[i], a[i], b[i]);
-    }
-    for (uint32_t i = threadIdx.x; i < tokens * p.half; i += kThreads) {
-        const uint32_t t = i / p.half;
-        int64_t position = p.positions[first + t];
-        if (p.position_offset) {
-            const int32_t r = p.token_request[first + t];
-            if (uint32_t(r) < p.requests) position += p.position_offset[r];
-        }
-        // turns = position * f / 2 pi, whose whole part is dropped before 32 bits
-        const double turns = double(position) * (p.frequencies[i - t * p.half] * 0.15915494309189533577);
-        float sine, cosine;
-        sincospif(2.f * float(turns - rint(turns)), &sine, &cosine);
-        turn[i] = make_float2(p.scale * cosine, p.sign * sine);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) finish(item[i], a[i], b[i]);
-    for (uint32_t i = threadIdx.x + kItemsPerBlock; i < tokens * p.items; i += kThreads) {
-        const Item<T> more = item_at(i);
-        P x, y;
-        fetch(more, x, y);
-        finish(more, x, y);
+        };
+        section(p.s[0], t * p.s[0].out_token, true);
+        section(p.s[1], kAppend ? uint64_t(place) : t * p.s[1].out_token, true);
+        if (kAppend) section(p.s[2], uint64_t(place), false);
+        __syncwarp();  // the table is free
     }
 }
 
@@ -258,10 +262,13 @@ Strided flat(const void* p, uint64_t n, int e) { return Strided(p, e, n, {}); }
 template <typename T, int N, bool kHalf>
 lcpp_status launch(const Params& p, bool append, cudaStream_t s)
 {
-    const unsigned grid = unsigned(ceil_div(p.tokens, p.per_block));
-    const size_t smem = size_t(p.per_block) * p.half * sizeof(float2);
-    if (append) rotary_kernel<T, N, kHalf, true><<<grid, kThreads, smem, s>>>(p);
-    else rotary_kernel<T, N, kHalf, false><<<grid, kThreads, smem, s>>>(p);
+    auto kernel = append ? rotary_kernel<T, N, kHalf, true> : rotary_kernel<T, N, kHalf, false>;
+    const size_t smem = size_t(kWarps) * align_up(p.half, 2) * sizeof(float2);
+    // as for the longest tables, so that few launch shapes are looked up and kept
+    const size_t room = size_t(kWarps) * (LCPP_MAX_HEAD_DIM / 2) * sizeof(float2);
+    const uint64_t most = uint64_t(device_sm_count()) * resident_blocks(reinterpret_cast<const void*>(kernel), kThreads, room);
+    const unsigned grid = unsigned(std::min<uint64_t>(most, ceil_div(uint64_t(p.tokens) * p.team, kWarps)));
+    kernel<<<grid, kThreads, smem, s>>>(p);
     return launched();
 }
 
@@ -269,18 +276,28 @@ template <typename T, int N>
 lcpp_status launch(Params& p, const lcpp_rotary_args& a, bool append, cudaStream_t s)
 {
     const bool half = a.layout == LCPP_ROTARY_HALF;
-    const uint32_t in_vector = half ? N : (N == 1 ? 2 : N);
-    p.turned = (half ? p.half : 2 * p.half) / in_vector;
-    p.per_head = p.turned + (a.head_dim - a.rotary_dim) / N;
-    p.plain = a.head_dim / N;
-    p.s[0].items = a.q.num_heads * p.per_head;
-    p.s[1].items = a.k.num_heads * p.per_head;
-    p.s[2].items = append ? a.k.num_heads * p.plain : 0;
-    p.items = p.s[0].items + p.s[1].items + p.s[2].items;
-    // as many tokens as the loads ahead cover, when there are tokens for every SM
-    const uint32_t fit = std::max<uint32_t>(1, kItemsPerBlock / std::max<uint32_t>(1, p.items));
-    const uint32_t spread = uint32_t(ceil_div(p.tokens, uint64_t(device_sm_count()) * 4));
-    p.per_block = std::min<uint32_t>({fit, std::max<uint32_t>(spread, 1), uint32_t(kMaxTokens)});
+    p.turned = (half ? p.half : 2 * p.half) / (half ? N : (N == 1 ? 2 : N));
+    const uint32_t heads[3] = {a.q.num_heads, a.k.num_heads, append ? a.k.num_heads : 0};
+    // a head's vectors: of pairs, then of columns
+    const uint32_t per_head = p.turned + (a.head_dim - a.rotary_dim) / N;
+    for (int i = 0; i < 3; ++i) {
+        p.s[i].per_head = i < 2 ? per_head : a.head_dim / N;
+        p.s[i].vectors = heads[i] * p.s[i].per_head;
+    }
+    // warps to a token until every SM has some rounds of 32, but no more than have work for each lane
+    p.team = 1;
+    while (p.team < kWarps && p.team * p.tokens < uint64_t(device_sm_count()) * 128 &&
+           p.s[0].vectors + p.s[1].vectors > p.team * kWarp)
+        p.team *= 2;
+    for (Section& c : p.s) {
+        const uint32_t step = p.team * kWarp;
+        c.step = step % c.per_head;
+        const int64_t over = step / c.per_head;
+        c.in_step = over * int64_t(c.in_head) + int64_t(c.step) * N;
+        c.out_step = over * int64_t(c.out_head) + int64_t(c.step) * N;
+        c.in_wrap = int64_t(c.in_head) - int64_t(c.per_head) * N;
+        c.out_wrap = int64_t(c.out_head) - int64_t(c.per_head) * N;
+    }
     return half ? launch<T, N, true>(p, append, s) : launch<T, N, false>(p, append, s);
 }
 
@@ -364,8 +381,13 @@ lcpp_status run(const lcpp_rotary_args* a, const lcpp_cache_append_args* c, floa
         p.num_slots = slots;
         p.page_stride = c->cache.page_stride;
         p.block_size = c->cache.block_size;
-        p.s[2] = Section{c->v, c->cache.v, c->v_token_stride, c->v_head_stride, c->cache.token_stride,
-                         c->cache.head_stride, 0, 1};
+        p.s[2].in = c->v;
+        p.s[2].out = c->cache.v;
+        p.s[2].in_token = c->v_token_stride;
+        p.s[2].in_head = c->v_head_stride;
+        p.s[2].out_token = c->cache.token_stride;
+        p.s[2].out_head = c->cache.head_stride;
+        p.s[2].copied = 1;
     }
     for (size_t i = 0; i < out.size(); ++i) {
         for (const Strided& x : in)
@@ -377,14 +399,13 @@ lcpp_status run(const lcpp_rotary_args* a, const lcpp_cache_append_args* c, floa
     for (int i = 0; i < 2; ++i) {
         const lcpp_head_rows& r = *rows[i];
         const bool cached = c && i == 1;
-        p.s[i] = Section{r.in,
-                         cached ? c->cache.k : r.out,
-                         r.in_token_stride,
-                         r.in_head_stride,
-                         cached ? c->cache.token_stride : r.out_token_stride,
-                         cached ? c->cache.head_stride : r.out_head_stride,
-                         0,
-                         uint32_t(cached || r.in != r.out)};
+        p.s[i].in = r.in;
+        p.s[i].out = cached ? c->cache.k : r.out;
+        p.s[i].in_token = r.in_token_stride;
+        p.s[i].in_head = r.in_head_stride;
+        p.s[i].out_token = cached ? c->cache.token_stride : r.out_token_stride;
+        p.s[i].out_head = cached ? c->cache.head_stride : r.out_head_stride;
+        p.s[i].copied = cached || r.in != r.out;
     }
     p.positions = a->positions;
     p.token_request = a->token_request;
