@@ -21,7 +21,6 @@ using namespace lcpp::model;
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / kWarp;
-constexpr int kAhead = 2;  // vectors (of pairs) that a lane has under way
 
 struct Section {
     const void* in;
@@ -127,6 +126,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const Params p)
     // pairs, or for N = 1 of one pair as two elements
     constexpr bool kTwo = kHalf || N == 1;  // a pair's second half is loaded by itself
     constexpr int kPairs = kHalf ? N : N == 1 ? 1 : N / 2;
+    constexpr int kAhead = 2;    // vectors that a lane has under way
     extern __shared__ __align__(16) float2 tables[];  // [warp][half] cosine and sine with the scale
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     float2* turn = tables + warp * ((p.half + 1) / 2 * 2);
@@ -284,9 +284,9 @@ lcpp_status launch(Params& p, const lcpp_rotary_args& a, bool append, cudaStream
         p.s[i].per_head = i < 2 ? per_head : a.head_dim / N;
         p.s[i].vectors = heads[i] * p.s[i].per_head;
     }
-    // warps to a token until every SM has some rounds of 32, but no more than have work for each lane
+    // warps to a token until every SM has 32, but no more than have work for each lane
     p.team = 1;
-    while (p.team < kWarps && p.team * p.tokens < uint64_t(device_sm_count()) * 128 &&
+    while (p.team < kWarps && p.team * p.tokens < uint64_t(device_sm_count()) * 32 &&
            p.s[0].vectors + p.s[1].vectors > p.team * kWarp)
         p.team *= 2;
     for (Section& c : p.s) {
