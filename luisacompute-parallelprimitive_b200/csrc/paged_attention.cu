@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(kScoreThreads) scores_kernel(const Params p)
 {
     const auto weight = [&](uint32_t r) {  // tiles before the window, then those of the logits
         const Tokens t = tokens_of(p, r);
-        return (long long)((t.first + kTile - 1) / kTile + t.tiles());
+        return (long long)(t.base() / kTile + t.tiles());
     };
     long long begin = -1, end = -1;
     Place place;
@@ -46,15 +46,14 @@ __global__ void __launch_bounds__(kScoreThreads) scores_kernel(const Params p)
     for (long long at = begin + warp; at < end; at += kScoreWarps) {
         while (at >= first + weight(r)) first += weight(r++);
         const Tokens seen = tokens_of(p, r);
-        const uint32_t before = (seen.first + kTile - 1) / kTile, tiles = seen.tiles();
+        const uint32_t before = seen.base() / kTile, tiles = seen.tiles();
         const long long number = p.first[r];
         if (number + (long long)tiles * units > p.logit_tiles) continue;
-        uint32_t token = uint32_t(at - first) * kTile, stop = seen.first;
+        uint32_t token = uint32_t(at - first) * kTile;
         float mass[4] = {0.f, 0.f, 0.f, 0.f};
         if (at - first >= before) {
             const uint32_t t = uint32_t(at - first) - before;
-            token = seen.first + t * kTile;
-            stop = seen.end;
+            token = seen.base() + t * kTile;
             const float* lse = p.lse2 + uint64_t(r) * p.heads;
             const float4* x = reinterpret_cast<const float4*>(p.logits) + (number + t) * p.per_unit * (kTile / 4) + quad;
             const long long pitch = (long long)tiles * p.per_unit * (kTile / 4);
@@ -81,7 +80,7 @@ __global__ void __launch_bounds__(kScoreThreads) scores_kernel(const Params p)
         // lane 4 i + quad writes token 4 quad + i
         const float own = part == 0 ? mass[0] : part == 1 ? mass[1] : part == 2 ? mass[2] : mass[3];
         token += quad * 4 + part;
-        if (part < 4 && token < stop) {
+        if (part < 4 && token < seen.end) {
             const uint32_t page = p.page.quotient(token), id = uint32_t(p.table[r * p.table_stride + page]);
             if (id < p.num_pages) {
                 const uint64_t slot = uint64_t(id) * p.page.d + (token - page * p.page.d);
@@ -111,8 +110,8 @@ Layout layout(uint64_t requests, uint32_t heads, uint32_t kv_heads, const Choice
     if (!score_slots) return l;
     l.lse2 = take(requests * heads * 4);
     l.first = take(requests * 8);
-    // every request's tokens in tiles of 16, no slot twice
-    l.tiles = (score_slots + (kTile - 1) * requests) / kTile * kv_heads * c.chunks;
+    // every request's tokens in tiles of 16, a partial one at either end, no slot twice
+    l.tiles = (score_slots + 2 * (kTile - 1) * requests) / kTile * kv_heads * c.chunks;
     l.logits = take(l.tiles * c.per_unit * kTile * 4);
     return l;
 }
@@ -186,6 +185,8 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_paged_attention_args* 
     p.lens = a->seq_lens;
     p.page = Divider(cache.block_size);
     p.longest = uint32_t(std::min<uint64_t>(uint64_t(a->table_width) * cache.block_size, 0x7fffffffu));
+    p.page_tiles = cache.block_size % kTile == 0;
+    p.wide_q = rows_aligned(a->q, {a->q_request_stride, a->q_head_stride}, e, 16) && cache.head_dim * e % 16 == 0;
     p.num_pages = cache.num_pages;
     p.requests = a->num_requests;
     p.heads = a->num_heads;

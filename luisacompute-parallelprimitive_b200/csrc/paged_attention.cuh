@@ -42,6 +42,8 @@ struct Params {
     uint64_t table_stride;
     const int32_t* lens;
     Divider page;         // by the page size
+    bool page_tiles;      // a tile lies in one page
+    bool wide_q;          // queries start on 16-byte boundaries
     uint32_t longest;     // tokens that a row of the table holds
     uint32_t num_pages;
     uint32_t requests, heads, kv_heads, group;
@@ -62,10 +64,12 @@ struct Params {
     float decay;
 };
 
-// A request's tokens: [first, end) in tiles of 16.
+// A request's tokens that are looked at, [first, end), in tiles that start at
+// multiples of 16.
 struct Tokens {
     uint32_t first, end;
-    __device__ __forceinline__ uint32_t tiles() const { return (end - first + kTile - 1) / kTile; }
+    __device__ __forceinline__ uint32_t base() const { return first / kTile * kTile; }
+    __device__ __forceinline__ uint32_t tiles() const { return (end - base() + kTile - 1) / kTile; }
 };
 __device__ __forceinline__ Tokens tokens_of(const Params& p, uint32_t r)
 {
@@ -198,7 +202,6 @@ struct Tile;
 template <typename T, int D, int H>
 struct Tile16 {
     static constexpr int kN = H / 8;
-    static constexpr int kQueryBytes = D * H * 2;
     static constexpr int kWarpBytes = 0;
     // float16's range: terms are kept at up to 2^8 of the reference, whose own is
     // set 2^7 up, so that they end at 2^15 and small ones keep their digits.
@@ -217,24 +220,6 @@ struct Tile16 {
             for (int i = 0; i < D / 16; ++i)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[i][n][c] = 0.f;
-        }
-    }
-
-    // Queries as the first product's second operand: lane's two words for each
-    // 16 columns and 8 heads, [16 columns][8 heads][lane].
-    static __device__ void load_queries(const Params& p, void* smem, const T* q, uint32_t heads)
-    {
-        uint32_t* to = static_cast<uint32_t*>(smem);
-        for (int i = threadIdx.x; i < D * H / 2; i += blockDim.x) {
-            const int word = i & 1, lane = (i >> 1) & 31, n = (i >> 6) % kN, step = (i >> 6) / kN;
-            const uint32_t head = n * 8 + lane / 4, column = step * 16 + word * 8 + lane % 4 * 2;
-            T pair[2] = {from_float<T>(0.f), from_float<T>(0.f)};
-            if (head < heads) {
-                if (column < p.dim) pair[0] = q[head * p.q_head + column];
-                if (column + 1 < p.dim) pair[1] = q[head * p.q_head + column + 1];
-            }
-            to[i] = uint32_t(*reinterpret_cast<const uint16_t*>(&pair[0])) |
-                    uint32_t(*reinterpret_cast<const uint16_t*>(&pair[1])) << 16;
         }
     }
 
@@ -257,17 +242,19 @@ struct Tile16 {
             for (int n = 0; n < kN; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) c[i][n][j] = 0.f;
-        const uint2* q = static_cast<const uint2*>(queries) + lane;
-        const int row = lane % 16;
-        const uint32_t at = smem_address(rows) + row * (D * 2);
+        const int row = lane % 16, head = lane % 8;
+        const uint32_t at = smem_address(rows) + row * (D * 2), q = smem_address(queries) + head * (D * 2);
 #pragma unroll
-        for (int step = 0; step < D / 16; ++step) {
-            uint32_t a[4];
-            load_matrices(a, at + swizzled(row, step * 2 + lane / 16) * 16);
+        for (int step = 0; step < D / 16; step += 2) {
+            uint32_t a[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) load_matrices(a[i], at + swizzled(row, (step + i) * 2 + lane / 16) * 16);
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
-                const uint2 b = q[(step * kN + n) * kWarp];
-                multiply<T>(c[step % kChains][n], a, b.x, b.y);
+                uint32_t b[4];  // the heads' next 32 columns
+                load_matrices(b, q + n * 8 * (D * 2) + swizzled(head, step * 2 + lane / 8) * 16);
+                multiply<T>(c[step % kChains][n], a[0], b[0], b[1]);
+                multiply<T>(c[(step + 1) % kChains][n], a[1], b[2], b[3]);
             }
         }
         const bool valid0 = valid >> (lane / 4) & 1, valid1 = valid >> (lane / 4 + 8) & 1;
@@ -362,26 +349,47 @@ struct Tile16 {
                 }
             }
     }
-    // Puts or adds the warp's vectors times factor[head] to sum[head][D + 4].
-    __device__ __forceinline__ void put(float* sum, const float* factor, bool first)
+    // The vectors relative to the largest of the warps' references, [warp][head].
+    template <int WARPS>
+    __device__ __forceinline__ void rescale(const float* m_all)
     {
         const int lane = threadIdx.x % kWarp;
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int head = n * 8 + lane % 4 * 2 + h;
-                const float f = factor[head];
-                float* to = sum + head * (D + 4) + lane / 4;
+                float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
+                for (int w = 0; w < WARPS; ++w) top = fmaxf(top, m_all[w * H + n * 8 + lane % 4 * 2 + h]);
+                const float f = share(m[n][h], l[n][h], top);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    o[i][n][h] *= f;
+                    o[i][n][h + 2] *= f;
+                }
+            }
+    }
+    // Puts or adds the piece-th quarter of the warp's vectors to sum[head][D + 4].
+    static constexpr int kPieces = 4;
+    __device__ __forceinline__ void put(float* sum, int piece, bool first)
+    {
+        const int lane = threadIdx.x % kWarp;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            if (i / (D / 64) != piece) continue;
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int head = n * 8 + lane % 4 * 2 + h;
+                    float* to = sum + head * (D + 4) + lane / 4 + i * 16;
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const float x = o[i][n][h + c * 2] * f;
-                        float* at = to + i * 16 + c * 8;
-                        *at = first ? x : *at + x;
+                        const float x = o[i][n][h + c * 2];
+                        to[c * 8] = first ? x : to[c * 8] + x;
                     }
-            }
+                }
+        }
     }
 };
 
@@ -397,7 +405,6 @@ struct Tile<__half, D, H> : Tile16<__half, D, H> {};
 // ---------------------------------------------------------------------------
 template <int D, int H>
 struct Tile<float, D, H> {
-    static constexpr int kQueryBytes = D * H * 4;
     static constexpr int kWarpBytes = kTile * H * 4;
     static constexpr int kChunks = D / 4;
     static constexpr int kLanes = kChunks < kWarp ? kChunks : kWarp;  // lanes of a row
@@ -420,15 +427,6 @@ struct Tile<float, D, H> {
         }
     }
 
-    static __device__ void load_queries(const Params& p, void* smem, const float* q, uint32_t heads)
-    {
-        float* to = static_cast<float*>(smem);
-        for (int i = threadIdx.x; i < D * H; i += blockDim.x) {
-            const uint32_t head = i / D, column = i % D;
-            to[i] = head < heads && column < p.dim ? q[head * p.q_head + column] : 0.f;
-        }
-    }
-
     __device__ __forceinline__ void keys(const Params& p, const unsigned char* rows, const void* queries, void* own,
                                          uint32_t valid, float* logits, uint32_t heads)
     {
@@ -445,7 +443,7 @@ struct Tile<float, D, H> {
             const float4 a = k[swizzled(token, chunk)];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                const float4 b = q[h * kChunks + chunk];
+                const float4 b = q[h * kChunks + swizzled(h, chunk)];
                 s[h] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s[h]))));
             }
         }
@@ -522,13 +520,28 @@ struct Tile<float, D, H> {
             }
         }
     }
-    __device__ __forceinline__ void put(float* sum, const float* factor, bool first)
+    template <int WARPS>
+    __device__ __forceinline__ void rescale(const float* m_all)
+    {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, m_all[w * H + h]);
+            const float f = share(m[h], l[h], top);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) o[h][i].x *= f, o[h][i].y *= f, o[h][i].z *= f, o[h][i].w *= f;
+        }
+    }
+    static constexpr int kPieces = H < 4 ? 1 : 4;
+    __device__ __forceinline__ void put(float* sum, int piece, bool first)
     {
         const int lane = threadIdx.x % kWarp;
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
+                if (kPieces > 1 && h / (H / kPieces > 0 ? H / kPieces : 1) != piece) continue;
                 float4 x = o[h][i];
 #pragma unroll
                 for (int d = kLanes; d < kWarp; d *= 2) {  // the lanes of the other tokens
@@ -538,10 +551,9 @@ struct Tile<float, D, H> {
                     x.w += __shfl_xor_sync(~0u, x.w, d);
                 }
                 if (lane < kLanes) {
-                    const float f = factor[h];
                     float4* at = reinterpret_cast<float4*>(sum + h * (D + 4) + (lane + i * kLanes) * 4);
                     float4 y = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
-                    y.x += x.x * f, y.y += x.y * f, y.z += x.z * f, y.w += x.w * f;
+                    y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
                     *at = y;
                 }
             }
@@ -557,17 +569,34 @@ struct Room {
     static constexpr int kRing = SLOTS * kSlotBytes;      // of a warp
     static constexpr int kMasks = SLOTS / 2 + 2;          // tiles between the copies and the products
     static constexpr int kQueries = WARPS * kRing;
-    static constexpr int kSum = kQueries;  // when the queries are not needed any more
-    static constexpr int kSumBytes = H * (D + 4) * 4;
-    static constexpr int kOwn = kQueries + (Work::kQueryBytes > kSumBytes ? Work::kQueryBytes : kSumBytes);
-    static constexpr int kStats = kOwn + WARPS * Work::kWarpBytes;  // m, l, factor [warp][head], then of the unit [head]
-    static constexpr int kValid = kStats + (3 * WARPS + 2) * H * 4;
+    static constexpr int kQueryBytes = H * kRowBytes;
+    static constexpr int kSum = kQueries + kQueryBytes;
+    static constexpr int kOwn = kSum + H * (D + 4) * 4;
+    static constexpr int kStats = kOwn + WARPS * Work::kWarpBytes;  // m, l [warp][head], then of the unit [head]
+    static constexpr int kValid = kStats + (2 * WARPS + 2) * H * 4;
     static constexpr int kBytes = kValid + WARPS * kMasks * 4;
 };
 
+// Zeros for the requests without tokens, divided among the blocks.
+template <typename T>
+__device__ __forceinline__ void clear_empty(const Params& p)
+{
+    for (uint32_t r = blockIdx.x; r < p.requests; r += gridDim.x) {
+        if (tokens_of(p, r).tiles()) continue;
+        for (uint32_t i = threadIdx.x; i < p.heads * p.dim; i += blockDim.x) {
+            const uint32_t h = i / p.dim;
+            static_cast<T*>(p.out)[r * p.out_request + h * p.out_head + (i - h * p.dim)] = from_float<T>(0.f);
+        }
+        for (uint32_t h = threadIdx.x; h < p.heads; h += blockDim.x) {
+            if (p.lse) p.lse[uint64_t(r) * p.heads + h] = -INFINITY;
+            if (p.lse2) p.lse2[uint64_t(r) * p.heads + h] = -INFINITY;
+        }
+    }
+}
+
 // kWide: 16-byte copies; else element by element, for rows that start anywhere.
-template <typename T, int D, int H, int SLOTS, int WARPS, bool kWide>
-__global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
+template <typename T, int D, int H, int SLOTS, int WARPS, int BLOCKS, bool kWide>
+__global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Params p)
 {
     using Work = Tile<T, D, H>;
     using R = Room<T, D, H, SLOTS, WARPS>;
@@ -595,19 +624,10 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
         },
         place);
 
-    // requests without tokens
-    for (uint32_t r = blockIdx.x; r < p.requests; r += gridDim.x) {
-        if (tokens_of(p, r).tiles()) continue;
-        for (uint32_t i = threadIdx.x; i < p.heads * p.dim; i += kThreads) {
-            const uint32_t h = i / p.dim;
-            static_cast<T*>(p.out)[r * p.out_request + h * p.out_head + (i - h * p.dim)] = from_float<T>(0.f);
-        }
-        for (uint32_t h = threadIdx.x; h < p.heads; h += kThreads) {
-            if (p.lse) p.lse[uint64_t(r) * p.heads + h] = -INFINITY;
-            if (p.lse2) p.lse2[uint64_t(r) * p.heads + h] = -INFINITY;
-        }
+    if (begin >= total) {
+        clear_empty<T>(p);
+        return;
     }
-    if (begin >= total) return;
 
     Walk now;
     now.r = place.item;
@@ -633,13 +653,14 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
         }
     };
     settle();
-    // lane's row of the tile: its page and place in it, read ahead
+    // lane's row of the tile (or the row that all have in common): its page and
+    // place in it, read ahead
     int32_t id = -1;
     uint32_t in_page = 0;
     const auto look_up = [&] {
         id = -1;
         if (!more) return;
-        const uint32_t token = ahead.tokens.first + ahead_t * kTile + lane % 16;
+        const uint32_t token = ahead.tokens.base() + ahead_t * kTile + (p.page_tiles ? 0 : lane % 16);
         if (token < ahead.tokens.end) {
             const uint32_t page = p.page.quotient(token);
             in_page = token - page * p.page.d;
@@ -650,24 +671,39 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
     int slot_in = 0, mask_in = 0;
     uint64_t row_offset = 0;
     uint32_t mask = 0;
-    // A tile's keys, and at the next call its values.
     bool values_next = false;
     const auto copy_rows = [&](const T* from) {
         unsigned char* to = ring + slot_in * R::kSlotBytes;
         if (kWide) {
             const uint32_t address = smem_address(to);
+            constexpr int kIn = 16 / int(sizeof(T)), kCopies = kTile * kChunks / kWarp;
+            if (p.page_tiles && kWarp % kChunks == 0) {
+                // a lane's rows are so many apart
+                constexpr int kApart = kWarp % kChunks == 0 ? kWarp / kChunks : 1;
+                const int row0 = lane / kChunks, chunk = lane % kChunks;
+                const T* at = from + row_offset + row0 * p.token_stride + chunk * kIn;
+                if (chunk * kIn < p.dim) {
 #pragma unroll
-            for (int i = 0; i < kTile * kChunks / kWarp; ++i) {
-                const int at = i * kWarp + lane, row = at / kChunks, chunk = at % kChunks;
-                const uint64_t offset = __shfl_sync(~0u, row_offset, row) + chunk * (16 / sizeof(T));
-                if (chunk * (16 / sizeof(T)) < p.dim)
-                    copy_16b(address + row * kRowBytes + swizzled(row, chunk) * 16, from + offset, mask >> row & 1);
+                    for (int i = 0; i < kCopies; ++i) {
+                        const int row = row0 + i * kApart;
+                        copy_16b(address + row * kRowBytes + swizzled(row, chunk) * 16, at, mask >> row & 1);
+                        at += kApart * p.token_stride;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kCopies; ++i) {
+                    const int at = i * kWarp + lane, row = at / kChunks, chunk = at % kChunks;
+                    const uint64_t offset = p.page_tiles ? row_offset + row * p.token_stride : __shfl_sync(~0u, row_offset, row);
+                    if (chunk * kIn < p.dim)
+                        copy_16b(address + row * kRowBytes + swizzled(row, chunk) * 16, from + offset + chunk * kIn, mask >> row & 1);
+                }
             }
         } else {
             __syncwarp();  // the slot's last use is over
             constexpr int kIn = 16 / int(sizeof(T));
             for (int row = 0; row < kTile; ++row) {
-                const uint64_t offset = __shfl_sync(~0u, row_offset, row);
+                const uint64_t offset = p.page_tiles ? row_offset + row * p.token_stride : __shfl_sync(~0u, row_offset, row);
                 const bool live = mask >> row & 1;
                 for (uint32_t c = lane; c < p.dim; c += kWarp) {
                     T* into = reinterpret_cast<T*>(to + row * kRowBytes + swizzled(row, c / kIn) * 16) + c % kIn;
@@ -676,11 +712,16 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
             }
         }
     };
+    // A tile's keys, and at the next call its values.
     const auto copy_next = [&] {
         if (more) {
             if (!values_next) {
                 const bool valid = uint32_t(id) < p.num_pages;
-                mask = __ballot_sync(~0u, valid) & 0xffffu;
+                // rows of the window, and of pages that there are
+                const uint32_t token = ahead.tokens.base() + ahead_t * kTile;
+                const uint32_t skip = ahead.tokens.first > token ? ahead.tokens.first - token : 0;
+                mask = (0xffffu << skip) & (0xffffu >> (kTile - min(ahead.tokens.end - token, uint32_t(kTile))));
+                mask &= __ballot_sync(~0u, valid);
                 if (lane == 0) masks[mask_in] = mask;
                 mask_in = mask_in + 1 == R::kMasks ? 0 : mask_in + 1;
                 row_offset = valid ? uint64_t(uint32_t(id)) * p.page_stride + in_page * p.token_stride +
@@ -702,15 +743,56 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
 #pragma unroll
     for (int i = 0; i < SLOTS - 1; ++i) copy_next();
 
+    clear_empty<T>(p);
+
     float* sum = reinterpret_cast<float*>(smem + R::kSum);
     float* m_all = reinterpret_cast<float*>(smem + R::kStats);
     float* l_all = m_all + kWarps * H;
-    float* factor = l_all + kWarps * H;
-    float* unit_m = factor + kWarps * H;
+    float* unit_m = l_all + kWarps * H;
     float* unit_l = unit_m + H;
     int slot = 0, mask_out = 0;
     long long first_tile = begin;  // number of the part's first tile
     Work work;
+    // A part's queries, [head] rows swizzled like the keys': on their way in
+    // registers, then in shared memory.
+    constexpr int kQueryLoads = (R::kQueryBytes / 16 + kThreads - 1) / kThreads;
+    uint4 queries[kQueryLoads];
+    const auto load_queries = [&](const Walk& w) {
+        const uint32_t kv_head = w.unit / p.chunks, head0 = (w.unit - kv_head * p.chunks) * p.per_unit;
+        const uint32_t heads = min(p.per_unit, p.group - head0);
+        const T* q = static_cast<const T*>(p.q) + w.r * p.q_request + (kv_head * p.group + head0) * p.q_head;
+        constexpr int kIn = 16 / int(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < kQueryLoads; ++i) {
+            const uint32_t at = i * kThreads + threadIdx.x, head = at / kChunks, column = at % kChunks * kIn;
+            queries[i] = make_uint4(0, 0, 0, 0);
+            if (head >= heads || column >= p.dim) continue;
+            const T* from = q + head * p.q_head + column;
+            if (p.wide_q) {
+                queries[i] = *reinterpret_cast<const uint4*>(from);
+            } else {
+                uint32_t words[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < kIn; ++c) {
+                    if (column + c >= p.dim) continue;
+                    if constexpr (sizeof(T) == 4) words[c] = __float_as_uint(from[c]);
+                    else words[c / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(from)[c]) << (c % 2 * 16);
+                }
+                queries[i] = make_uint4(words[0], words[1], words[2], words[3]);
+            }
+        }
+    };
+    const auto keep_queries = [&] {
+#pragma unroll
+        for (int i = 0; i < kQueryLoads; ++i) {
+            const int at = i * kThreads + threadIdx.x, head = at / kChunks, chunk = at % kChunks;
+            if (at < R::kQueryBytes / 16)
+                *reinterpret_cast<uint4*>(smem + R::kQueries + head * kRowBytes + swizzled(head, chunk) * 16) = queries[i];
+        }
+    };
+    load_queries(now);
+    keep_queries();
+    __syncthreads();
     // The oldest slot, once its copies have come; the newest is filled meanwhile.
     const auto next_slot = [&] {
         wait_copies<SLOTS - 2>();
@@ -720,14 +802,11 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
         return rows;
     };
-    do {
+    while (true) {
         const uint32_t kv_head = now.unit / p.chunks, chunk = now.unit - kv_head * p.chunks;
         const uint32_t head0 = chunk * p.per_unit, heads = min(p.per_unit, p.group - head0);
         const uint32_t head = kv_head * p.group + head0;
-        Work::load_queries(p, smem + R::kQueries,
-                           static_cast<const T*>(p.q) + now.r * p.q_request + head * p.q_head, heads);
         work.clear();
-        __syncthreads();
         for (uint32_t t = now.t + warp; t < now.t_end; t += kWarps) {
             const long long number = first_tile + (t - now.t);
             float* logits = p.logits && number < p.logit_tiles ? p.logits + number * p.per_unit * kTile : nullptr;
@@ -738,26 +817,38 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
             work.values(next_slot(), own);
         }
 
-        // the warps' parts, in the order of the warps
+        // The warps' parts add up in shared memory, each warp a piece of its vectors at
+        // a time, every piece in an order of its own that never changes.  The next
+        // part's queries are on their way meanwhile.
+        Walk then = now;
+        const bool again = then.next(p);
+        if (again) load_queries(then);
         work.put_sums(m_all + warp * H, l_all + warp * H);
         __syncthreads();
+        if (again) keep_queries();
+        work.template rescale<kWarps>(m_all);
         if (threadIdx.x < H) {
             float top = -INFINITY, all = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_all[w * H + threadIdx.x]);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float f = share(m_all[w * H + threadIdx.x], l_all[w * H + threadIdx.x], top);
-                factor[w * H + threadIdx.x] = f;
-                all += f * l_all[w * H + threadIdx.x];
+                const float l = l_all[w * H + threadIdx.x];
+                all += share(m_all[w * H + threadIdx.x], l, top) * l;
             }
             unit_m[threadIdx.x] = top;
             unit_l[threadIdx.x] = all;
         }
-        __syncthreads();
-        const int busy = int(min(uint32_t(kWarps), now.t_end - now.t));
-        for (int w = 0; w < busy; ++w) {
-            if (warp == w) work.put(sum, factor + w * H, w == 0);
+#pragma unroll
+        for (int round = 0; round < kWarps; ++round) {
+            if (Work::kPieces == 1) {
+                if (warp == round) work.put(sum, 0, round == 0);
+            } else {
+                static_assert(Work::kPieces == 1 || Work::kPieces % kWarps == 0, "");
+                constexpr int kEach = Work::kPieces / kWarps > 0 ? Work::kPieces / kWarps : 1;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) work.put(sum, (warp + round) % kWarps * kEach + i, round == 0);
+            }
             __syncthreads();
         }
         if (now.t == 0 && now.t_end == now.tiles) {
@@ -777,33 +868,42 @@ __global__ void __launch_bounds__(WARPS * kWarp) decode_kernel(const Params p)
             if (threadIdx.x < heads) stats[threadIdx.x] = make_float2(unit_m[threadIdx.x], unit_l[threadIdx.x]);
         }
         if (p.first && now.unit == 0 && now.t == 0 && threadIdx.x == 0) p.first[now.r] = first_tile;
+        if (!again) break;
+        // the next part writes what this one reads behind a barrier of its own
         first_tile += now.t_end - now.t;
-        __syncthreads();
-    } while (now.next(p));
+        now = then;
+    }
     wait_copies<0>();
 }
 
-// Head h = blockIdx.y of a unit whose tiles lie in several blocks' runs: the last
-// part of the first of them and the first parts of the next `count`; the warps take
-// every eighth and join in order.  Which unit is worked out from the lengths while
-// the decode kernel still runs: where the call has fewer units than the decode
-// kernel has blocks it is unit blockIdx.x, else the one that block blockIdx.x's run
-// ends in (blocks for all units of 2 x 2, or all runs: 2 x 131072 tokens 85 or 91 us).
-constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * kWarp;
-template <typename T, int D, int H>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, uint32_t decode_blocks, int decode_warps, bool by_unit)
+// A unit whose tiles lie in several blocks' runs: the last part of the first of
+// them and the first parts of the next `count` join, in order; every warp takes a
+// head and each so-many-th part of it.  Which unit is worked out from the lengths
+// while the decode kernel still runs.  Where the call has fewer units than the
+// decode kernel has blocks (and a unit many parts), block (u, h) takes head h of
+// unit u; else (and mostly two) block b all heads of the one that b's run ends in.
+template <int H, bool kByUnit>
+struct Join {
+    static constexpr int kWarps = kByUnit ? 8 : 16, kThreads = kWarps * kWarp;
+    static constexpr int kHeads = kByUnit ? 1 : H < kWarps ? H : kWarps;  // at once
+    static constexpr int kGroups = kWarps / kHeads;
+};
+template <typename T, int D, int H, bool kByUnit>
+__global__ void __launch_bounds__(Join<H, kByUnit>::kThreads) join_kernel(const Params p, uint32_t decode_blocks, int decode_warps)
 {
-    __shared__ float sums[kJoinWarps][D];
-    __shared__ float2 stats_of[kJoinWarps];
+    using J = Join<H, kByUnit>;
+    constexpr int kThreads = J::kThreads, kGroups = J::kGroups;
+    __shared__ float sums[J::kHeads][kGroups > 1 ? D : 1];
+    __shared__ float2 stats_of[J::kHeads][kGroups];
     let_next_start();
-    const uint32_t units = p.kv_heads * p.chunks, h = blockIdx.y;
+    const uint32_t units = p.kv_heads * p.chunks;
     const auto weight = [&](uint32_t i) { return (long long)(tokens_of(p, i).tiles()) * units; };
     uint32_t r = 0, unit = 0, block = 0, count = 0;
-    if (by_unit) {
+    if (kByUnit) {
         r = blockIdx.x / units;
         unit = blockIdx.x - r * units;
         long long total;
-        const long long before = sum_before<kJoinThreads>(p.requests, r, weight, total);
+        const long long before = sum_before<kThreads>(p.requests, r, weight, total);
         const uint32_t tiles = tokens_of(p, r).tiles();
         const long long per = run_of(total, decode_blocks, decode_warps), first = before + (long long)unit * tiles;
         block = uint32_t(first / per);
@@ -812,7 +912,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, uint
         long long per = 1, begin = 0, end = 0;
         Place place;
         block = blockIdx.x;
-        const long long total = share_of<kJoinThreads>(
+        const long long total = share_of<kThreads>(
             p.requests, weight,
             [&](long long all) {
                 per = run_of(all, decode_blocks, decode_warps);
@@ -830,83 +930,104 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, uint
         }
     }
     const uint32_t kv_head = unit / p.chunks, head0 = unit % p.chunks * p.per_unit;
-    if (count == 0 || h >= min(p.per_unit, p.group - head0)) {
+    const uint32_t heads = min(p.per_unit, p.group - head0);
+    if (count == 0 || blockIdx.y >= heads) {
         // this launch ends after the one before, for whatever comes after it
-        if (blockIdx.x == 0 && h == 0) wait_for_previous();
+        if (blockIdx.x == 0 && blockIdx.y == 0) wait_for_previous();
         return;
     }
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    const int place_in = warp % J::kHeads, group = warp / J::kHeads;
     const float2* stats = reinterpret_cast<const float2*>(p.part + uint64_t(decode_blocks) * 2 * H * D);
     wait_for_previous();
 
-    constexpr int kPer = D / kWarp, kAhead = 4;
-    float o[kPer], top = -INFINITY, all = 0.f;
+    for (uint32_t h0 = kByUnit ? blockIdx.y : 0; h0 < heads; h0 += kByUnit ? heads : J::kHeads) {
+        const uint32_t h = h0 + place_in;
+        const bool live = h < heads;
+        constexpr int kPer = D / kWarp, kAhead = 4;
+        float o[kPer], top = -INFINITY, all = 0.f;
 #pragma unroll
-    for (int c = 0; c < kPer; ++c) o[c] = 0.f;
-    for (uint32_t i = warp; i <= count; i += kJoinWarps * kAhead) {
-        float2 s[kAhead];
-        float x[kAhead][kPer];
+        for (int c = 0; c < kPer; ++c) o[c] = 0.f;
+        for (uint32_t i = live ? group : count + 1; i <= count; i += kGroups * kAhead) {
+            float2 s[kAhead];
+            float x[kAhead][kPer];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const uint32_t at = i + u * kJoinWarps;
-            s[u] = make_float2(-INFINITY, 0.f);
+            for (int u = 0; u < kAhead; ++u) {
+                const uint32_t at = i + u * kGroups;
+                s[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-            for (int c = 0; c < kPer; ++c) x[u][c] = 0.f;
-            if (at > count) continue;
-            const uint64_t slot = uint64_t(block + at) * 2 + (at ? 0 : 1);
-            s[u] = stats[slot * H + h];
-            const float* part = p.part + (slot * H + h) * D + lane;
+                for (int c = 0; c < kPer; ++c) x[u][c] = 0.f;
+                if (at > count) continue;
+                const uint64_t slot = uint64_t(block + at) * 2 + (at ? 0 : 1);
+                s[u] = stats[slot * H + h];
+                const float* part = p.part + (slot * H + h) * D + lane;
 #pragma unroll
-            for (int c = 0; c < kPer; ++c) x[u][c] = part[c * kWarp];
+                for (int c = 0; c < kPer; ++c) x[u][c] = part[c * kWarp];
+            }
+            float to = top;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) to = fmaxf(to, s[u].x);
+            const float keep = share(top, all, to);
+            all *= keep;
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) o[c] *= keep;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const float f = share(s[u].x, s[u].y, to);
+                all += f * s[u].y;
+#pragma unroll
+                for (int c = 0; c < kPer; ++c) o[c] += f * x[u][c];
+            }
+            top = to;
         }
-        float to = top;
+        if (kGroups > 1) {
+            if (lane == 0) stats_of[place_in][group] = make_float2(top, all);
+            __syncthreads();
+            const float own = all;
+            float to = -INFINITY;
+            all = 0.f;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) to = fmaxf(to, s[u].x);
-        const float keep = share(top, all, to);
-        all *= keep;
+            for (int g = 0; g < kGroups; ++g) to = fmaxf(to, stats_of[place_in][g].x);
 #pragma unroll
-        for (int c = 0; c < kPer; ++c) o[c] *= keep;
+            for (int g = 0; g < kGroups; ++g) {
+                const float2 of = stats_of[place_in][g];
+                all += share(of.x, of.y, to) * of.y;
+            }
+            const float factor = share(top, own, to);
+            top = to;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const float f = share(s[u].x, s[u].y, to);
-            all += f * s[u].y;
+            for (int g = 0; g < kGroups; ++g) {
+                if (group == g) {
 #pragma unroll
-            for (int c = 0; c < kPer; ++c) o[c] += f * x[u][c];
+                    for (int c = 0; c < kPer; ++c) {
+                        float& sum = sums[place_in][c * kWarp + lane];
+                        o[c] = factor * o[c] + (g ? sum : 0.f);
+                        sum = o[c];
+                    }
+                }
+                __syncthreads();
+            }
         }
-        top = to;
+        if (live && group == kGroups - 1) {
+            const uint32_t head = kv_head * p.group + head0 + h;
+            T* out = static_cast<T*>(p.out) + r * p.out_request + head * p.out_head;
+#pragma unroll
+            for (int c = 0; c < kPer; ++c)
+                if (c * kWarp + lane < p.dim) out[c * kWarp + lane] = from_float<T>(all == 0.f ? 0.f : o[c] / all);
+            if (lane == 0) put_lse(p, uint64_t(r) * p.heads + head, top, all);
+        }
     }
-#pragma unroll
-    for (int c = 0; c < kPer; ++c) sums[warp][c * kWarp + lane] = o[c];
-    if (lane == 0) stats_of[warp] = make_float2(top, all);
-    __syncthreads();
-    float factor[kJoinWarps];
-    top = -INFINITY, all = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, stats_of[w].x);
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-        factor[w] = share(stats_of[w].x, stats_of[w].y, top);
-        all += factor[w] * stats_of[w].y;
-    }
-    const uint32_t head = kv_head * p.group + head0 + h;
-    T* out = static_cast<T*>(p.out) + r * p.out_request + head * p.out_head;
-    for (uint32_t c = threadIdx.x; c < p.dim; c += kJoinThreads) {
-        float x = 0.f;
-#pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) x += factor[w] * sums[w][c];
-        out[c] = from_float<T>(all == 0.f ? 0.f : x / all);
-    }
-    if (threadIdx.x == 0) put_lse(p, uint64_t(r) * p.heads + head, top, all);
 }
 
-template <typename T, int D, int H, int SLOTS, int WARPS>
+// SLOTS of the warps' rings, WARPS of a block, BLOCKS on an SM.
+template <typename T, int D, int H, int SLOTS, int WARPS, int BLOCKS>
 lcpp_status launch(const Params& base, bool wide, size_t part_bytes_at_most, cudaStream_t s)
 {
     Params p = base;
     using R = Room<T, D, H, SLOTS, WARPS>;
     constexpr int kThreads = WARPS * kWarp;
-    static_assert(R::kBytes <= 227 * 1024, "");
-    auto kernel = wide ? decode_kernel<T, D, H, SLOTS, WARPS, true> : decode_kernel<T, D, H, SLOTS, WARPS, false>;
+    static_assert(BLOCKS * (R::kBytes + 1024) <= 228 * 1024, "shared memory of an SM");
+    auto kernel = wide ? decode_kernel<T, D, H, SLOTS, WARPS, BLOCKS, true> : decode_kernel<T, D, H, SLOTS, WARPS, BLOCKS, false>;
     set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), R::kBytes);
     const unsigned blocks = std::min<unsigned>(
         kMostBlocks, unsigned(device_sm_count()) * resident_blocks(reinterpret_cast<const void*>(kernel), kThreads, R::kBytes));
@@ -918,14 +1039,19 @@ lcpp_status launch(const Params& base, bool wide, size_t part_bytes_at_most, cud
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
-    const uint64_t units = uint64_t(p.requests) * p.kv_heads * p.chunks;
-    const bool by_unit = units < blocks;
-    config.gridDim = dim3(by_unit ? unsigned(units) : blocks, std::min<uint32_t>(p.per_unit, H));
-    config.blockDim = dim3(kJoinThreads);
     config.stream = s;
     config.attrs = &early;
     config.numAttrs = 1;
-    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H>, p, uint32_t(blocks), WARPS, by_unit));
+    const uint64_t units = uint64_t(p.requests) * p.kv_heads * p.chunks;
+    if (units < blocks) {
+        config.gridDim = dim3(unsigned(units), std::min<uint32_t>(p.per_unit, H));
+        config.blockDim = dim3(Join<H, true>::kThreads);
+        LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H, true>, p, uint32_t(blocks), WARPS));
+    } else {
+        config.gridDim = dim3(blocks);
+        config.blockDim = dim3(Join<H, false>::kThreads);
+        LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H, false>, p, uint32_t(blocks), WARPS));
+    }
     return LCPP_OK;
 }
 
@@ -957,17 +1083,17 @@ lcpp_status run_16bit(const Params& p, const Choice& c, bool wide, size_t part_b
 {
     switch (c.columns) {
     case 64:
-        return c.heads == 8    ? launch<T, 64, 8, 6, 4>(p, wide, part_bytes, s)
-               : c.heads == 16 ? launch<T, 64, 16, 6, 4>(p, wide, part_bytes, s)
-                               : launch<T, 64, 32, 6, 4>(p, wide, part_bytes, s);
+        return c.heads == 8    ? launch<T, 64, 8, 4, 4, 4>(p, wide, part_bytes, s)
+               : c.heads == 16 ? launch<T, 64, 16, 4, 4, 4>(p, wide, part_bytes, s)
+                               : launch<T, 64, 32, 4, 4, 2>(p, wide, part_bytes, s);
     case 128:
-        return c.heads == 8    ? launch<T, 128, 8, 6, 4>(p, wide, part_bytes, s)
-               : c.heads == 16 ? launch<T, 128, 16, 6, 4>(p, wide, part_bytes, s)
-                               : launch<T, 128, 32, 6, 4>(p, wide, part_bytes, s);
+        return c.heads == 8    ? launch<T, 128, 8, 3, 4, 4>(p, wide, part_bytes, s)
+               : c.heads == 16 ? launch<T, 128, 16, 3, 4, 3>(p, wide, part_bytes, s)
+                               : launch<T, 128, 32, 4, 4, 2>(p, wide, part_bytes, s);
     case 192:
-        return c.heads == 8 ? launch<T, 192, 8, 4, 4>(p, wide, part_bytes, s) : launch<T, 192, 16, 4, 4>(p, wide, part_bytes, s);
+        return c.heads == 8 ? launch<T, 192, 8, 3, 4, 2>(p, wide, part_bytes, s) : launch<T, 192, 16, 3, 4, 2>(p, wide, part_bytes, s);
     default:
-        return c.heads == 8 ? launch<T, 256, 8, 3, 4>(p, wide, part_bytes, s) : launch<T, 256, 16, 3, 4>(p, wide, part_bytes, s);
+        return c.heads == 8 ? launch<T, 256, 8, 3, 4, 2>(p, wide, part_bytes, s) : launch<T, 256, 16, 2, 4, 2>(p, wide, part_bytes, s);
     }
 }
 
