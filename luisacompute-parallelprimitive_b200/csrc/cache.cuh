@@ -131,36 +131,6 @@ struct Place {
     uint32_t valid;
 };
 
-// Sums of weight(i) of the items before `item`, and of all.
-template <int THREADS, typename Weight>
-__device__ __forceinline__ long long sum_before(uint32_t n, uint32_t item, Weight weight, long long& total)
-{
-    __shared__ long long warps[THREADS / kWarp][2];
-    long long mine = 0, before = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-        const long long w = weight(i);
-        mine += w;
-        if (i < item) before += w;
-    }
-#pragma unroll
-    for (int d = 1; d < kWarp; d *= 2) {
-        mine += __shfl_xor_sync(~0u, mine, d);
-        before += __shfl_xor_sync(~0u, before, d);
-    }
-    if (threadIdx.x % kWarp == 0) {
-        warps[threadIdx.x / kWarp][0] = mine;
-        warps[threadIdx.x / kWarp][1] = before;
-    }
-    __syncthreads();
-    total = before = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / kWarp; ++w) {
-        total += warps[w][0];
-        before += warps[w][1];
-    }
-    return before;
-}
-
 // Equal shares of ragged work: items 0..n-1 have weight(i) units each; returns
 // the sum of all units, and in `place` the item of unit number begin(sum).
 // Every block that asks sums the weights itself (they come from L2): a thread

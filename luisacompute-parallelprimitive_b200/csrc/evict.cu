@@ -66,22 +66,36 @@ __device__ __forceinline__ uint32_t length_of(const int32_t* lens, uint32_t r, u
     return min(uint32_t(max(lens[r], 0)), longest);
 }
 
-// Sum over the block's warps, and over the warps before.
-__device__ __forceinline__ uint32_t warps_before(uint32_t of_warp, uint32_t* warps, uint32_t& total)
+// Exclusive sum over the lanes of a warp, and the sum of all.
+__device__ __forceinline__ uint32_t lanes_before(uint32_t mine, uint32_t& total)
 {
-    static_assert(kWarps == kWarp, "a lane for each warp");
-    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-    __syncthreads();
-    if (lane == 0) warps[warp] = of_warp;
-    __syncthreads();
-    uint32_t upto = warps[lane];
+    const int lane = threadIdx.x % kWarp;
+    uint32_t upto = mine;
 #pragma unroll
     for (int d = 1; d < kWarp; d *= 2) {
         const uint32_t left = __shfl_up_sync(~0u, upto, d);
         if (lane >= d) upto += left;
     }
     total = __shfl_sync(~0u, upto, kWarp - 1);
-    return __shfl_sync(~0u, upto, warp) - of_warp;
+    return upto - mine;
+}
+// Sum over the warps before, and over all; nobody may be reading `warps` any more.
+__device__ __forceinline__ uint32_t warps_before(uint32_t of_warp, uint32_t* warps, uint32_t& total)
+{
+    static_assert(kWarps == kWarp, "a lane for each warp");
+    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+    if (lane == 0) warps[warp] = of_warp;
+    __syncthreads();
+    return __shfl_sync(~0u, lanes_before(warps[lane], total), warp);
+}
+
+// The key of one token, read again: for those that have no room in shared memory.
+__device__ __noinline__ uint32_t key_again(const Params& p, const int32_t* row, uint32_t token, int64_t recent)
+{
+    const uint32_t page = p.page.quotient(token), id = uint32_t(row[page]);  // looked up before: in range
+    const uint64_t slot = uint64_t(id) * p.page.d + (token - page * p.page.d);
+    const int64_t at = p.positions ? int64_t(p.positions[slot]) : int64_t(token);
+    return at < p.first || at >= recent ? kProtected : key_of(p.scores[slot]);
 }
 
 __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
@@ -90,7 +104,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
     uint32_t* copies = dynamic;  // [kBins][kCopies], from the largest digit down
     uint32_t* keys = dynamic + kBins * kCopies;
     __shared__ Shared shared;
-    __shared__ uint32_t warps[kWarps];
+    __shared__ uint32_t warps[3][kWarps];
     __shared__ uint32_t found[4];  // digit, keys above it, keys of it in the blocks before and in all
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -120,15 +134,15 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         id = uint32_t(row[page]);
         return uint64_t(id) * p.page.d + (token - page * p.page.d);
     };
-    const auto key_at = [&](uint32_t i) {
-        if (i < kKeys) return keys[i];
-        uint32_t id;
-        const uint64_t slot = slot_of(lo + i, id);  // looked up before: in range
-        const int64_t at = p.positions ? int64_t(p.positions[slot]) : int64_t(lo + i);
-        return at < p.first || at >= recent ? kProtected : key_of(p.scores[slot]);
+    // four tokens' keys; 0, which no token has, past the last one
+    const auto keys_at = [&](uint32_t i) {
+        if (i + 3 < kKeys) return *reinterpret_cast<const uint4*>(keys + i);
+        const auto one = [&](uint32_t at) { return at >= count ? 0u : at < kKeys ? keys[at] : key_again(p, row, lo + at, recent); };
+        return make_uint4(one(i), one(i + 1), one(i + 2), one(i + 3));
     };
 
     if (threadIdx.x == 0) shared.broken = 0;
+    if (threadIdx.x < 3 && count + threadIdx.x < kKeys) keys[count + threadIdx.x] = 0;
     for (int i = threadIdx.x; i < kBins * kCopies; i += kThreads) copies[i] = 0;
     __syncthreads();
     bool broken = false;
@@ -177,10 +191,13 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
         if (pass) {
-            for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
-                const uint32_t key = key_at(i);
-                if ((key ^ top) >> (shift + bits) == 0) {
-                    const uint32_t digit = key >> shift & ((1u << bits) - 1);
+            for (uint32_t i = threadIdx.x * 4; i < count; i += kThreads * 4) {
+                const uint4 k = keys_at(i);
+                const uint32_t key[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (key[u] == 0 || (key[u] ^ top) >> (shift + bits)) continue;
+                    const uint32_t digit = key[u] >> shift & ((1u << bits) - 1);
                     atomicAdd(&copies[(kBins - 1 - digit) * kCopies + lane % kCopies], 1u);
                 }
             }
@@ -217,15 +234,9 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
                 return;
             }
         }
-        uint32_t upto = mine.x + mine.y;
-#pragma unroll
-        for (int d = 1; d < kWarp; d *= 2) {
-            const uint32_t left = __shfl_up_sync(~0u, upto, d);
-            if (lane >= d) upto += left;
-        }
-        uint32_t all;
-        const uint32_t before_warp = warps_before(__shfl_sync(~0u, upto, kWarp - 1), warps, all);
-        const uint32_t above = before_warp + upto - mine.x - mine.y;
+        uint32_t of_warp, all;
+        uint32_t above = lanes_before(mine.x + mine.y, of_warp);
+        above += warps_before(of_warp, warps[0], all);
         // one thread finds the bin: there are at least `need` such keys
         if (above < need && above + mine.x + mine.y >= need) {
             const bool second = above + mine.x < need;
@@ -238,36 +249,50 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         top |= found[0] << shift;
         need -= found[1];
         equal_before = found[2];
-        const bool all_kept = found[3] == need;
-        __syncthreads();
-        if (all_kept) {  // so the keys above top - 1 are; top is not 0, for some key is not kept
+        if (found[3] == need) {  // so the keys above top - 1 are; top is not 0, for some key is not kept
             top -= 1;
             need = 0;
             break;
         }
     }
 
-    // Each warp takes a run of the block's tokens, 32 at a time.  Equal keys are
-    // numbered first, then holes and fillers counted, then numbered.
-    const uint32_t part = uint32_t(align_up(ceil_div(count, kWarps), kWarp));
+    // Each warp takes a run of the block's tokens, 128 at a time and a lane four.
+    // Equal keys are numbered first (where not all or none of them are kept), then
+    // holes and fillers counted, then numbered.
+    const uint32_t part = uint32_t(align_up(ceil_div(count, kWarps), 4 * kWarp));
     const uint32_t from = min(count, warp * part), to = min(count, from + part);
-    uint32_t total;
-    uint32_t equals = 0;
-    for (uint32_t i = from; i < to; i += kWarp) {
-        const bool in = i + lane < to;
-        equals += __popc(__ballot_sync(~0u, in && key_at(i + lane) == top));
+    uint32_t total, equal_base = 0;
+    if (need) {
+        uint32_t equals = 0;
+        for (uint32_t i = from + lane * 4; i < to; i += 4 * kWarp) {
+            const uint4 k = keys_at(i);
+            equals += (k.x == top) + (k.y == top) + (k.z == top) + (k.w == top);
+        }
+        equal_base = equal_before + warps_before(__reduce_add_sync(~0u, equals), warps[1], total);
     }
-    const uint32_t equal_base = equal_before + warps_before(equals, warps, total);
-    const auto sort_out = [&](auto take) {  // take(lane's token in the block, hole mask, filler mask)
+    const auto sort_out = [&](auto take) {  // take(lane's first token in the block, masks of its holes and fillers)
         uint32_t number = equal_base;
-        for (uint32_t i = from; i < to; i += kWarp) {
-            const bool in = i + lane < to;
-            const uint32_t key = in ? key_at(i + lane) : 0;
-            const uint32_t same = __ballot_sync(~0u, in && key == top);
-            const bool kept = key > top || (key == top && number + __popc(same & lanemask_lt()) < need);
-            number += __popc(same);
-            const bool front = lo + i + lane < p.budget;
-            take(i + lane, __ballot_sync(~0u, in && front && !kept), __ballot_sync(~0u, in && !front && kept));
+        for (uint32_t i0 = from; i0 < to; i0 += 4 * kWarp) {
+            const uint32_t i = i0 + lane * 4;
+            const uint4 k = i < to ? keys_at(i) : make_uint4(0, 0, 0, 0);
+            const uint32_t key[4] = {k.x, k.y, k.z, k.w};
+            uint32_t same = 0, before_me = 0;
+            if (need) {
+                uint32_t in_warp;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) same += key[u] == top;
+                before_me = number + lanes_before(same, in_warp);
+                number += in_warp;
+            }
+            uint32_t hole = 0, filler = 0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool kept = key[u] > top || (key[u] == top && before_me++ < need);
+                const bool front = lo + i + u < p.budget;
+                hole |= uint32_t(key[u] && front && !kept) << u;
+                filler |= uint32_t(!front && kept) << u;
+            }
+            take(i, hole, filler);
         }
     };
     uint32_t holes = 0, fillers = 0;
@@ -275,9 +300,16 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         holes += __popc(hole);
         fillers += __popc(filler);
     });
-    uint32_t hole = warps_before(holes, warps, total);
+    holes = __reduce_add_sync(~0u, holes);
+    fillers = __reduce_add_sync(~0u, fillers);
+    if (lane == 0) {
+        warps[0][warp] = holes;
+        warps[2][warp] = fillers;
+    }
+    __syncthreads();
+    uint32_t hole = __shfl_sync(~0u, lanes_before(warps[0][lane], total), warp);
     if (threadIdx.x == 0) shared.holes = total;
-    uint32_t filler = warps_before(fillers, warps, total);
+    uint32_t filler = __shfl_sync(~0u, lanes_before(warps[2][lane], total), warp);
     if (threadIdx.x == 0) shared.fillers = total;
     meet();
     uint32_t moves = 0;
@@ -296,15 +328,20 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
     }
     longlong2* out = p.moves + r * p.moves_stride;
     sort_out([&](uint32_t i, uint32_t hole_mask, uint32_t filler_mask) {
-        const bool is_hole = hole_mask >> lane & 1, is_filler = filler_mask >> lane & 1;
-        if (is_hole || is_filler) {
+        uint32_t in_warp;
+        if (!__any_sync(~0u, hole_mask | filler_mask)) return;
+        uint32_t to_hole = hole + lanes_before(__popc(hole_mask), in_warp);
+        hole += in_warp;
+        uint32_t to_filler = filler + lanes_before(__popc(filler_mask), in_warp);
+        filler += in_warp;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (!((hole_mask | filler_mask) >> u & 1)) continue;
             uint32_t id;
-            const int64_t slot = int64_t(slot_of(lo + i, id));
-            if (is_filler) out[filler + __popc(filler_mask & lanemask_lt())].x = slot;
-            else out[hole + __popc(hole_mask & lanemask_lt())].y = slot;
+            const int64_t slot = int64_t(slot_of(lo + i + u, id));
+            if (filler_mask >> u & 1) out[to_filler++].x = slot;
+            else out[to_hole++].y = slot;
         }
-        hole += __popc(hole_mask);
-        filler += __popc(filler_mask);
     });
     if (rank == 0 && threadIdx.x == 0) {
         p.lens_out[r] = int32_t(p.budget);
@@ -314,7 +351,8 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
 }
 
 // The pages that no token needs any more, back on the free list.
-__global__ void __launch_bounds__(kThreads) release_kernel(const Params p, int32_t* free_blocks, const int32_t* free_used,
+constexpr int kReleaseThreads = 256;
+__global__ void __launch_bounds__(kReleaseThreads) release_kernel(const Params p, int32_t* free_blocks, const int32_t* free_used,
                                                            int32_t* free_used_out, uint32_t num_free)
 {
     wait_for_previous();
@@ -323,7 +361,7 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const Params p, int32
     const auto freed = [&](uint32_t r) { return (long long)(pages(length_of(p.lens, r, p.longest)) - kept(r)); };
     long long begin = -1, end = -1;
     Place place;
-    const long long total = share_of<kThreads>(
+    const long long total = share_of<kReleaseThreads>(
         p.requests, freed,
         [&](long long all) {
             const long long per = (all + gridDim.x - 1) / gridDim.x;
@@ -337,7 +375,7 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const Params p, int32
     if (begin >= total) return;
     uint32_t r = place.item;
     long long first = place.first;
-    for (long long i = begin + threadIdx.x; i < end; i += kThreads) {
+    for (long long i = begin + threadIdx.x; i < end; i += kReleaseThreads) {
         while (i >= first + freed(r)) first += freed(r++);
         const long long at = used - total + i;
         if (at >= 0) free_blocks[at] = p.table[r * p.table_stride + kept(r) + uint32_t(i - first)];
@@ -501,10 +539,10 @@ lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
     }
     if (!release) return LCPP_OK;
     if (n == 0) {
-        release_kernel<<<1, kThreads, 0, s>>>(p, a->free_blocks, a->free_used, a->free_used_out, a->num_free);
+        release_kernel<<<1, kReleaseThreads, 0, s>>>(p, a->free_blocks, a->free_used, a->free_used_out, a->num_free);
         return launched();
     }
-    return launch_early(release_kernel, unsigned(std::min<uint64_t>(n, device_sm_count())), kThreads, 0, s, Params(p),
+    return launch_early(release_kernel, unsigned(std::min<uint64_t>(n, device_sm_count())), kReleaseThreads, 0, s, Params(p),
                         static_cast<int32_t*>(a->free_blocks), static_cast<const int32_t*>(a->free_used),
                         static_cast<int32_t*>(a->free_used_out), uint32_t(a->num_free));
 }

@@ -57,20 +57,18 @@ __global__ void __launch_bounds__(kScoreThreads) scores_kernel(const Params p)
             const float* lse = p.lse2 + uint64_t(r) * p.heads;
             const float4* x = reinterpret_cast<const float4*>(p.logits) + (number + t) * p.per_unit * (kTile / 4) + quad;
             const long long pitch = (long long)tiles * p.per_unit * (kTile / 4);
-#pragma unroll 8
-            for (uint32_t u = 0; u < units; ++u) {
-                // the first heads of kv head u / chunks' group come in chunks of per_unit, the last one shorter
-                const uint32_t kv_head = u / p.chunks, head0 = (u - kv_head * p.chunks) * p.per_unit;
-                const uint32_t heads = min(p.per_unit, p.group - head0);
-                for (uint32_t h = part; h < heads; h += kWarp / 4) {
-                    const float of = lse[kv_head * p.group + head0 + h];
-                    const float4 logits = x[u * pitch + h * (kTile / 4)];
-                    if (of == -INFINITY) continue;
-                    mass[0] += exp2_fast(logits.x - of);
-                    mass[1] += exp2_fast(logits.y - of);
-                    mass[2] += exp2_fast(logits.z - of);
-                    mass[3] += exp2_fast(logits.w - of);
-                }
+#pragma unroll 4
+            for (uint32_t head = part; head < p.heads; head += kWarp / 4) {
+                // the head's unit, and its place in it
+                const uint32_t kv_head = p.by_group.quotient(head), in_group = head - kv_head * p.group;
+                const uint32_t chunk = p.by_unit.quotient(in_group), h = in_group - chunk * p.per_unit;
+                const float of = lse[head];
+                const float4 logits = x[(kv_head * p.chunks + chunk) * pitch + h * (kTile / 4)];
+                if (of == -INFINITY) continue;
+                mass[0] += exp2_fast(logits.x - of);
+                mass[1] += exp2_fast(logits.y - of);
+                mass[2] += exp2_fast(logits.z - of);
+                mass[3] += exp2_fast(logits.w - of);
             }
         }
 #pragma unroll
@@ -93,7 +91,7 @@ __global__ void __launch_bounds__(kScoreThreads) scores_kernel(const Params p)
 constexpr uint32_t kMostHeads = 1u << 16;
 
 struct Layout {
-    size_t part, lse2, first, logits, part_bytes, bytes;
+    size_t part, split, lse2, first, logits, part_bytes, bytes;
     uint64_t tiles;
 };
 
@@ -107,6 +105,7 @@ Layout layout(uint64_t requests, uint32_t heads, uint32_t kv_heads, const Choice
     };
     l.part_bytes = size_t(kMostBlocks) * 2 * c.heads * (c.columns + 2) * 4;
     l.part = take(l.part_bytes);
+    l.split = take(kMostBlocks * 16);
     if (!score_slots) return l;
     l.lse2 = take(requests * heads * 4);
     l.first = take(requests * 8);
@@ -187,6 +186,7 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_paged_attention_args* 
     p.longest = uint32_t(std::min<uint64_t>(uint64_t(a->table_width) * cache.block_size, 0x7fffffffu));
     p.page_tiles = cache.block_size % kTile == 0;
     p.wide_q = rows_aligned(a->q, {a->q_request_stride, a->q_head_stride}, e, 16) && cache.head_dim * e % 16 == 0;
+    p.wide_out = rows_aligned(a->out, {a->out_request_stride, a->out_head_stride}, e, 4 * e) && cache.head_dim % 4 == 0;
     p.num_pages = cache.num_pages;
     p.requests = a->num_requests;
     p.heads = a->num_heads;
@@ -200,7 +200,10 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_paged_attention_args* 
     p.softcap = a->softcap * kLog2e;
     p.lse = a->lse_out;
     p.part = reinterpret_cast<float*>(t + l.part);
+    p.split = reinterpret_cast<int32_t*>(t + l.split);
     if (score_slots) {
+        p.by_group = Divider(p.group);
+        p.by_unit = Divider(p.per_unit);
         p.lse2 = reinterpret_cast<float*>(t + l.lse2);
         p.first = reinterpret_cast<long long*>(t + l.first);
         p.logits = reinterpret_cast<float*>(t + l.logits);

@@ -28,7 +28,7 @@ namespace model {
 namespace attention {
 
 constexpr int kTile = 16;              // tokens of a tile
-constexpr uint32_t kMostBlocks = 640;  // the partial results' room
+constexpr uint32_t kMostBlocks = 800;  // the partial results' room
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -44,6 +44,7 @@ struct Params {
     Divider page;         // by the page size
     bool page_tiles;      // a tile lies in one page
     bool wide_q;          // queries start on 16-byte boundaries
+    bool wide_out;        // rows of the output on boundaries of four elements
     uint32_t longest;     // tokens that a row of the table holds
     uint32_t num_pages;
     uint32_t requests, heads, kv_heads, group;
@@ -55,6 +56,8 @@ struct Params {
     float softcap;        // with log2 e; 0: none
     float* lse;
     float* part;          // [block][2][heads of a unit][columns] and, behind them, [block][2][heads of a unit][2]
+    int32_t* split;       // [block][4]: request, unit, first block and further blocks of the unit that its run ends in
+    Divider by_group, by_unit;  // by `group` and `per_unit`, for the scores
     float* logits;        // [tile][per_unit][16] in base 2, or NULL
     long long logit_tiles;
     float* lse2;          // [request][head] in base 2 for the scores
@@ -71,11 +74,12 @@ struct Tokens {
     __device__ __forceinline__ uint32_t base() const { return first / kTile * kTile; }
     __device__ __forceinline__ uint32_t tiles() const { return (end - base() + kTile - 1) / kTile; }
 };
-__device__ __forceinline__ Tokens tokens_of(const Params& p, uint32_t r)
+__device__ __forceinline__ Tokens tokens_of_length(const Params& p, int32_t length)
 {
-    const uint32_t n = min(uint32_t(max(p.lens[r], 0)), p.longest);
+    const uint32_t n = min(uint32_t(max(length, 0)), p.longest);
     return Tokens{p.window && n > p.window ? n - p.window : 0u, n};
 }
+__device__ __forceinline__ Tokens tokens_of(const Params& p, uint32_t r) { return tokens_of_length(p, p.lens[r]); }
 
 // Tiles of a block's run: equal ones, of not less than a tile for each warp.
 __device__ __forceinline__ long long run_of(long long all, uint32_t blocks, int warps)
@@ -87,7 +91,8 @@ __device__ __forceinline__ long long run_of(long long all, uint32_t blocks, int 
 struct Walk {
     uint32_t r, unit, tiles, t, t_end;
     Tokens tokens;
-    long long left;  // tiles of the run behind this part
+    int32_t next_length;  // of request r + 1, read ahead
+    long long left;       // tiles of the run behind this part
 
     __device__ __forceinline__ void part()
     {
@@ -95,6 +100,7 @@ struct Walk {
         t_end = uint32_t(min((long long)tiles, t + room));
         left = room - (t_end - t);
     }
+    __device__ __forceinline__ void read_ahead(const Params& p) { next_length = r + 1 < p.requests ? p.lens[r + 1] : 0; }
     // To the part after this one; false: the run has ended.
     __device__ __forceinline__ bool next(const Params& p)
     {
@@ -102,9 +108,11 @@ struct Walk {
         t = 0;
         if (++unit == p.kv_heads * p.chunks) {
             unit = 0;
-            do {
-                tokens = tokens_of(p, ++r);  // the run has tiles left, so there is such a request
+            do {  // the run has tiles left, so there is such a request
+                tokens = tokens_of_length(p, next_length);
                 tiles = tokens.tiles();
+                ++r;
+                read_ahead(p);
             } while (tiles == 0);
         }
         part();
@@ -116,6 +124,10 @@ __device__ __forceinline__ uint32_t smem_address(const void* p) { return uint32_
 __device__ __forceinline__ void copy_16b(uint32_t to, const void* from, bool valid)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_4b(uint32_t to, const void* from)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -369,26 +381,20 @@ struct Tile16 {
                 }
             }
     }
-    // Puts or adds the piece-th quarter of the warp's vectors to sum[head][D + 4].
-    static constexpr int kPieces = 4;
-    __device__ __forceinline__ void put(float* sum, int piece, bool first)
+    // Puts the vectors of the pass-th kPass heads to to[head][D], 8 columns swapped
+    // with 8 so that the lanes' heads lie in different banks.
+    static constexpr int kPass = 8;
+    static __device__ __forceinline__ int place(int head, int column) { return head * D + (column ^ (head / 2 % 4 * 8)); }
+    __device__ __forceinline__ void put(float* to, int pass)
     {
         const int lane = threadIdx.x % kWarp;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            if (i / (D / 64) != piece) continue;
+        for (int n = 0; n < kN; ++n) {
+            if (n != pass) continue;
 #pragma unroll
-            for (int n = 0; n < kN; ++n)
+            for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int head = n * 8 + lane % 4 * 2 + h;
-                    float* to = sum + head * (D + 4) + lane / 4 + i * 16;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const float x = o[i][n][h + c * 2];
-                        to[c * 8] = first ? x : to[c * 8] + x;
-                    }
-                }
+                for (int j = 0; j < 4; ++j) to[place(lane % 4 * 2 + j % 2, i * 16 + j / 2 * 8 + lane / 4)] = o[i][n][j];
         }
     }
 };
@@ -533,15 +539,15 @@ struct Tile<float, D, H> {
             for (int i = 0; i < kPer; ++i) o[h][i].x *= f, o[h][i].y *= f, o[h][i].z *= f, o[h][i].w *= f;
         }
     }
-    static constexpr int kPieces = H < 4 ? 1 : 4;
-    __device__ __forceinline__ void put(float* sum, int piece, bool first)
+    static constexpr int kPass = H;
+    static __device__ __forceinline__ int place(int head, int column) { return head * D + column; }
+    __device__ __forceinline__ void put(float* to, int)
     {
         const int lane = threadIdx.x % kWarp;
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                if (kPieces > 1 && h / (H / kPieces > 0 ? H / kPieces : 1) != piece) continue;
                 float4 x = o[h][i];
 #pragma unroll
                 for (int d = kLanes; d < kWarp; d *= 2) {  // the lanes of the other tokens
@@ -550,14 +556,16 @@ struct Tile<float, D, H> {
                     x.z += __shfl_xor_sync(~0u, x.z, d);
                     x.w += __shfl_xor_sync(~0u, x.w, d);
                 }
-                if (lane < kLanes) {
-                    float4* at = reinterpret_cast<float4*>(sum + h * (D + 4) + (lane + i * kLanes) * 4);
-                    float4 y = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
-                    y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
-                    *at = y;
-                }
+                if (lane < kLanes) *reinterpret_cast<float4*>(to + place(h, (lane + i * kLanes) * 4)) = x;
             }
     }
+};
+
+// A tile that a warp will copy: what its rows' places are worked out from.
+struct alignas(16) Note {
+    uint64_t head;   // the kv head's offset
+    uint32_t token;  // the first one
+    uint32_t mask;   // rows of the request and its window
 };
 
 // Shared memory of a block.
@@ -568,13 +576,18 @@ struct Room {
     static constexpr int kSlotBytes = kTile * kRowBytes;  // a tile's keys, or its values
     static constexpr int kRing = SLOTS * kSlotBytes;      // of a warp
     static constexpr int kMasks = SLOTS / 2 + 2;          // tiles between the copies and the products
-    static constexpr int kQueries = WARPS * kRing;
+    static constexpr int kNotes = 4;                      // tiles whose page ids come ahead of the copies
+    static constexpr int kNoteBytes = 16 + kTile * 4;
+    static constexpr int kQueries = WARPS * kRing;        // this part's, the next one's
     static constexpr int kQueryBytes = H * kRowBytes;
-    static constexpr int kSum = kQueries + kQueryBytes;
-    static constexpr int kOwn = kSum + H * (D + 4) * 4;
+    static constexpr int kAhead = kQueries + 2 * kQueryBytes;
+    static constexpr int kOwn = kAhead + WARPS * kNotes * kNoteBytes;
     static constexpr int kStats = kOwn + WARPS * Work::kWarpBytes;  // m, l [warp][head], then of the unit [head]
     static constexpr int kValid = kStats + (2 * WARPS + 2) * H * 4;
-    static constexpr int kBytes = kValid + WARPS * kMasks * 4;
+    static constexpr int kFree = kValid + WARPS * kMasks * 4;
+    static constexpr int kBytes = kFree + WARPS * 4;
+    static_assert(Work::kPass * D * 4 <= kSlotBytes, "a warp's vectors fit its free slot");
+    static_assert(SLOTS <= 2 * kNotes, "page ids have come when they are needed");
 };
 
 // Zeros for the requests without tokens, divided among the blocks.
@@ -594,6 +607,29 @@ __device__ __forceinline__ void clear_empty(const Params& p)
     }
 }
 
+// Four adjacent elements, as far as the row goes.
+template <typename T>
+__device__ __forceinline__ void store_4(T* to, float4 x, bool wide, uint32_t columns)
+{
+    if (wide) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(to) = x;
+        } else {
+            const T e[4] = {from_float<T>(x.x), from_float<T>(x.y), from_float<T>(x.z), from_float<T>(x.w)};
+            const auto word = [&](int i) {
+                return uint32_t(*reinterpret_cast<const uint16_t*>(&e[i])) |
+                       uint32_t(*reinterpret_cast<const uint16_t*>(&e[i + 1])) << 16;
+            };
+            *reinterpret_cast<uint2*>(to) = make_uint2(word(0), word(2));
+        }
+    } else {
+        to[0] = from_float<T>(x.x);
+        if (columns > 1) to[1] = from_float<T>(x.y);
+        if (columns > 2) to[2] = from_float<T>(x.z);
+        if (columns > 3) to[3] = from_float<T>(x.w);
+    }
+}
+
 // kWide: 16-byte copies; else element by element, for rows that start anywhere.
 template <typename T, int D, int H, int SLOTS, int WARPS, int BLOCKS, bool kWide>
 __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Params p)
@@ -601,7 +637,8 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
     using Work = Tile<T, D, H>;
     using R = Room<T, D, H, SLOTS, WARPS>;
     constexpr int kWarps = WARPS, kThreads = kWarps * kWarp;
-    constexpr int kRowBytes = R::kRowBytes, kChunks = kRowBytes / 16;
+    constexpr int kRowBytes = R::kRowBytes, kChunks = kRowBytes / 16, kIn = 16 / int(sizeof(T));
+    static_assert((kWarps & (kWarps - 1)) == 0, "");
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     let_next_start();
@@ -611,11 +648,10 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
         for (int i = lane; i < R::kRing / 16; i += kWarp) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
 
     const uint32_t units = p.kv_heads * p.chunks;
-    const auto weight = [&](uint32_t r) { return (long long)(tokens_of(p, r).tiles()) * units; };
     long long begin = -1, end = -1;
     Place place;
     const long long total = share_of<kThreads>(
-        p.requests, weight,
+        p.requests, [&](uint32_t r) { return (long long)(tokens_of(p, r).tiles()) * units; },
         [&](long long all) {
             const long long per = run_of(all, gridDim.x, kWarps);
             begin = blockIdx.x * per;
@@ -623,8 +659,9 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
             return begin < all ? begin : -1;
         },
         place);
-
+    int4* split = reinterpret_cast<int4*>(p.split) + blockIdx.x;
     if (begin >= total) {
+        if (threadIdx.x == 0) *split = make_int4(0, 0, 0, 0);
         clear_empty<T>(p);
         return;
     }
@@ -632,51 +669,83 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
     Walk now;
     now.r = place.item;
     now.tokens = tokens_of(p, now.r);
+    now.read_ahead(p);
     now.tiles = now.tokens.tiles();
     now.unit = uint32_t((begin - place.first) / now.tiles);
     now.t = uint32_t((begin - place.first) - (long long)now.unit * now.tiles);
     now.left = end - begin;
     now.part();
 
-    uint32_t* masks = reinterpret_cast<uint32_t*>(smem + R::kValid) + warp * R::kMasks;
-    // the warp's next tile to copy, and whether there is one
+    // A part's queries, [head] rows swizzled like the keys'.
+    const auto load_queries = [&](const Walk& w, int buffer) {
+        const uint32_t kv_head = w.unit / p.chunks, head0 = (w.unit - kv_head * p.chunks) * p.per_unit;
+        const uint32_t heads = min(p.per_unit, p.group - head0);
+        const T* q = static_cast<const T*>(p.q) + w.r * p.q_request + (kv_head * p.group + head0) * p.q_head;
+        unsigned char* to = smem + R::kQueries + buffer * R::kQueryBytes;
+        for (int at = threadIdx.x; at < H * kChunks; at += kThreads) {
+            const uint32_t head = at / kChunks, chunk = at % kChunks, column = chunk * kIn;
+            unsigned char* into = to + head * kRowBytes + swizzled(head, chunk) * 16;
+            const bool live = head < heads && column < p.dim;
+            const T* from = live ? q + head * p.q_head + column : q;
+            if (p.wide_q) {
+                copy_16b(smem_address(into), from, live);
+            } else {
+                for (int c = 0; c < kIn; ++c)
+                    reinterpret_cast<T*>(into)[c] = live && column + c < p.dim ? from[c] : from_float<T>(0.f);
+            }
+        }
+    };
+
+    // Three walks over the run: its tiles go to the warps in turn, also across its
+    // parts.  `ahead` notes a warp's tiles and sends for their page ids, kNotes tiles
+    // before the copies of their rows, for a load waits a microsecond and more behind
+    // the copies of the whole GPU.
     Walk ahead = now;
     uint32_t ahead_t = ahead.t + warp;
     bool more = true;
     const auto settle = [&] {
         while (ahead_t >= ahead.t_end) {
+            const uint32_t turn = ahead_t - ahead.t_end;  // tiles of the next part before the warp's
             if (!ahead.next(p)) {
                 more = false;
                 return;
             }
-            ahead_t = warp;
+            ahead_t = turn;
         }
+    };
+    unsigned char* notes = smem + R::kAhead + warp * R::kNotes * R::kNoteBytes;
+    int note_in = 0, note_out = 0, noted = 0;
+    const auto note_next = [&] {
+        if (!more) return;
+        unsigned char* at = notes + note_in * R::kNoteBytes;
+        const uint32_t token = ahead.tokens.base() + ahead_t * kTile, row = p.page_tiles ? 0 : lane;
+        if (row < kTile && token + row < ahead.tokens.end && (lane == 0 || !p.page_tiles))
+            copy_4b(smem_address(at + 16 + row * 4), p.table + ahead.r * p.table_stride + p.page.quotient(token + row));
+        const uint32_t skip = ahead.tokens.first > token ? ahead.tokens.first - token : 0;
+        if (lane == 0) {
+            Note& n = *reinterpret_cast<Note*>(at);
+            n.head = uint64_t(ahead.unit / p.chunks) * p.head_stride;
+            n.token = token;
+            n.mask = (0xffffu << skip) & (0xffffu >> (kTile - min(ahead.tokens.end - token, uint32_t(kTile))));
+        }
+        note_in = note_in + 1 == R::kNotes ? 0 : note_in + 1;
+        ++noted;
+        ahead_t += kWarps;
+        settle();
     };
     settle();
-    // lane's row of the tile (or the row that all have in common): its page and
-    // place in it, read ahead
-    int32_t id = -1;
-    uint32_t in_page = 0;
-    const auto look_up = [&] {
-        id = -1;
-        if (!more) return;
-        const uint32_t token = ahead.tokens.base() + ahead_t * kTile + (p.page_tiles ? 0 : lane % 16);
-        if (token < ahead.tokens.end) {
-            const uint32_t page = p.page.quotient(token);
-            in_page = token - page * p.page.d;
-            id = p.table[ahead.r * p.table_stride + page];
-        }
-    };
-    look_up();
+
+    // The copies: a noted tile's keys, and at the next call its values.
+    uint32_t* masks = reinterpret_cast<uint32_t*>(smem + R::kValid) + warp * R::kMasks;
     int slot_in = 0, mask_in = 0;
-    uint64_t row_offset = 0;
+    uint64_t row_offset = 0;  // of the lane's row, or of the first of all
     uint32_t mask = 0;
     bool values_next = false;
     const auto copy_rows = [&](const T* from) {
         unsigned char* to = ring + slot_in * R::kSlotBytes;
         if (kWide) {
             const uint32_t address = smem_address(to);
-            constexpr int kIn = 16 / int(sizeof(T)), kCopies = kTile * kChunks / kWarp;
+            constexpr int kCopies = kTile * kChunks / kWarp;
             if (p.page_tiles && kWarp % kChunks == 0) {
                 // a lane's rows are so many apart
                 constexpr int kApart = kWarp % kChunks == 0 ? kWarp / kChunks : 1;
@@ -700,8 +769,6 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
                 }
             }
         } else {
-            __syncwarp();  // the slot's last use is over
-            constexpr int kIn = 16 / int(sizeof(T));
             for (int row = 0; row < kTile; ++row) {
                 const uint64_t offset = p.page_tiles ? row_offset + row * p.token_stride : __shfl_sync(~0u, row_offset, row);
                 const bool live = mask >> row & 1;
@@ -712,87 +779,50 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
             }
         }
     };
-    // A tile's keys, and at the next call its values.
     const auto copy_next = [&] {
-        if (more) {
+        if (noted) {
             if (!values_next) {
-                const bool valid = uint32_t(id) < p.num_pages;
-                // rows of the window, and of pages that there are
-                const uint32_t token = ahead.tokens.base() + ahead_t * kTile;
-                const uint32_t skip = ahead.tokens.first > token ? ahead.tokens.first - token : 0;
-                mask = (0xffffu << skip) & (0xffffu >> (kTile - min(ahead.tokens.end - token, uint32_t(kTile))));
-                mask &= __ballot_sync(~0u, valid);
+                const unsigned char* at = notes + note_out * R::kNoteBytes;
+                const Note n = *reinterpret_cast<const Note*>(at);
+                const uint32_t row = p.page_tiles ? 0 : lane % kTile, token = n.token + row;
+                const uint32_t id = reinterpret_cast<const uint32_t*>(at + 16)[row];
+                const bool live = id < p.num_pages && (p.page_tiles || (n.mask >> row & 1));
+                mask = n.mask & __ballot_sync(~0u, live);
                 if (lane == 0) masks[mask_in] = mask;
                 mask_in = mask_in + 1 == R::kMasks ? 0 : mask_in + 1;
-                row_offset = valid ? uint64_t(uint32_t(id)) * p.page_stride + in_page * p.token_stride +
-                                         uint64_t(ahead.unit / p.chunks) * p.head_stride
-                                   : 0;
+                row_offset = live ? uint64_t(id) * p.page_stride + (token - p.page.quotient(token) * p.page.d) * p.token_stride + n.head : 0;
                 copy_rows(static_cast<const T*>(p.k));
             } else {
                 copy_rows(static_cast<const T*>(p.v));
-                ahead_t += kWarps;
-                settle();
-                look_up();
+                note_out = note_out + 1 == R::kNotes ? 0 : note_out + 1;
+                --noted;
+                note_next();
             }
             values_next = !values_next;
         }
         commit_copies();
         slot_in = slot_in + 1 == SLOTS ? 0 : slot_in + 1;
     };
+
+    load_queries(now, 0);
+#pragma unroll
+    for (int i = 0; i < R::kNotes; ++i) note_next();
+    commit_copies();
+    wait_copies<0>();
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < SLOTS - 1; ++i) copy_next();
-
     clear_empty<T>(p);
+    __syncthreads();
 
-    float* sum = reinterpret_cast<float*>(smem + R::kSum);
     float* m_all = reinterpret_cast<float*>(smem + R::kStats);
     float* l_all = m_all + kWarps * H;
     float* unit_m = l_all + kWarps * H;
     float* unit_l = unit_m + H;
-    int slot = 0, mask_out = 0;
+    int* free_slot = reinterpret_cast<int*>(smem + R::kFree);
+    int slot = 0, mask_out = 0, buffer = 0;
     long long first_tile = begin;  // number of the part's first tile
     Work work;
-    // A part's queries, [head] rows swizzled like the keys': on their way in
-    // registers, then in shared memory.
-    constexpr int kQueryLoads = (R::kQueryBytes / 16 + kThreads - 1) / kThreads;
-    uint4 queries[kQueryLoads];
-    const auto load_queries = [&](const Walk& w) {
-        const uint32_t kv_head = w.unit / p.chunks, head0 = (w.unit - kv_head * p.chunks) * p.per_unit;
-        const uint32_t heads = min(p.per_unit, p.group - head0);
-        const T* q = static_cast<const T*>(p.q) + w.r * p.q_request + (kv_head * p.group + head0) * p.q_head;
-        constexpr int kIn = 16 / int(sizeof(T));
-#pragma unroll
-        for (int i = 0; i < kQueryLoads; ++i) {
-            const uint32_t at = i * kThreads + threadIdx.x, head = at / kChunks, column = at % kChunks * kIn;
-            queries[i] = make_uint4(0, 0, 0, 0);
-            if (head >= heads || column >= p.dim) continue;
-            const T* from = q + head * p.q_head + column;
-            if (p.wide_q) {
-                queries[i] = *reinterpret_cast<const uint4*>(from);
-            } else {
-                uint32_t words[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int c = 0; c < kIn; ++c) {
-                    if (column + c >= p.dim) continue;
-                    if constexpr (sizeof(T) == 4) words[c] = __float_as_uint(from[c]);
-                    else words[c / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(from)[c]) << (c % 2 * 16);
-                }
-                queries[i] = make_uint4(words[0], words[1], words[2], words[3]);
-            }
-        }
-    };
-    const auto keep_queries = [&] {
-#pragma unroll
-        for (int i = 0; i < kQueryLoads; ++i) {
-            const int at = i * kThreads + threadIdx.x, head = at / kChunks, chunk = at % kChunks;
-            if (at < R::kQueryBytes / 16)
-                *reinterpret_cast<uint4*>(smem + R::kQueries + head * kRowBytes + swizzled(head, chunk) * 16) = queries[i];
-        }
-    };
-    load_queries(now);
-    keep_queries();
-    __syncthreads();
     // The oldest slot, once its copies have come; the newest is filled meanwhile.
     const auto next_slot = [&] {
         wait_copies<SLOTS - 2>();
@@ -803,29 +833,33 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
         return rows;
     };
     while (true) {
-        const uint32_t kv_head = now.unit / p.chunks, chunk = now.unit - kv_head * p.chunks;
-        const uint32_t head0 = chunk * p.per_unit, heads = min(p.per_unit, p.group - head0);
-        const uint32_t head = kv_head * p.group + head0;
+        const uint32_t kv_head = now.unit / p.chunks, head0 = (now.unit - kv_head * p.chunks) * p.per_unit;
+        const uint32_t heads = min(p.per_unit, p.group - head0), head = kv_head * p.group + head0;
+        Walk then = now;
+        const bool again = then.next(p);
+        if (again) load_queries(then, buffer ^ 1);
         work.clear();
-        for (uint32_t t = now.t + warp; t < now.t_end; t += kWarps) {
+        uint32_t own_tiles = 0;
+        for (uint32_t t = now.t + ((warp - uint32_t(first_tile - begin)) & (kWarps - 1)); t < now.t_end; t += kWarps) {
             const long long number = first_tile + (t - now.t);
             float* logits = p.logits && number < p.logit_tiles ? p.logits + number * p.per_unit * kTile : nullptr;
             void* own = smem + R::kOwn + warp * Work::kWarpBytes;
             const unsigned char* keys = next_slot();
-            work.keys(p, keys, smem + R::kQueries, own, masks[mask_out], logits, heads);
+            work.keys(p, keys, smem + R::kQueries + buffer * R::kQueryBytes, own, masks[mask_out], logits, heads);
             mask_out = mask_out + 1 == R::kMasks ? 0 : mask_out + 1;
             work.values(next_slot(), own);
+            ++own_tiles;
+        }
+        if (own_tiles * 2 < SLOTS) {  // else the next queries' copies have been waited for
+            commit_copies();
+            wait_copies<0>();
         }
 
-        // The warps' parts add up in shared memory, each warp a piece of its vectors at
-        // a time, every piece in an order of its own that never changes.  The next
-        // part's queries are on their way meanwhile.
-        Walk then = now;
-        const bool again = then.next(p);
-        if (again) load_queries(then);
+        // The warps' parts add up in their order.  Each puts its vectors into its slot
+        // that is filled next, relative to the largest of the warps' references.
         work.put_sums(m_all + warp * H, l_all + warp * H);
+        if (lane == 0) free_slot[warp] = slot_in;
         __syncthreads();
-        if (again) keep_queries();
         work.template rescale<kWarps>(m_all);
         if (threadIdx.x < H) {
             float top = -INFINITY, all = 0.f;
@@ -839,121 +873,97 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
             unit_m[threadIdx.x] = top;
             unit_l[threadIdx.x] = all;
         }
+        const bool whole = now.t == 0 && now.t_end == now.tiles;
+        const uint32_t part_of = blockIdx.x * 2 + (now.t ? 0 : 1);
 #pragma unroll
-        for (int round = 0; round < kWarps; ++round) {
-            if (Work::kPieces == 1) {
-                if (warp == round) work.put(sum, 0, round == 0);
-            } else {
-                static_assert(Work::kPieces == 1 || Work::kPieces % kWarps == 0, "");
-                constexpr int kEach = Work::kPieces / kWarps > 0 ? Work::kPieces / kWarps : 1;
+        for (int pass = 0; pass < H / Work::kPass; ++pass) {
+            work.put(reinterpret_cast<float*>(ring + slot_in * R::kSlotBytes), pass);
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < Work::kPass * D / 4; i += kThreads) {
+                const uint32_t in_pass = i / (D / 4), h = pass * Work::kPass + in_pass, column = i % (D / 4) * 4;
+                if (h >= heads) break;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < kEach; ++i) work.put(sum, (warp + round) % kWarps * kEach + i, round == 0);
+                for (int w = 0; w < kWarps; ++w) {
+                    const float* from = reinterpret_cast<const float*>(smem + w * R::kRing + free_slot[w] * R::kSlotBytes);
+                    const float4 y = *reinterpret_cast<const float4*>(from + Work::place(in_pass, column));
+                    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+                }
+                if (!whole) {
+                    *reinterpret_cast<float4*>(p.part + (uint64_t(part_of) * H + h) * D + column) = x;
+                } else if (column < p.dim) {
+                    const float all = unit_l[h], by = all == 0.f ? 0.f : 1.f / all;
+                    store_4(static_cast<T*>(p.out) + now.r * p.out_request + (head + h) * p.out_head + column,
+                            make_float4(x.x * by, x.y * by, x.z * by, x.w * by), p.wide_out, p.dim - column);
+                }
+            }
+            if (pass == 0 && threadIdx.x < heads) {
+                if (whole) {
+                    put_lse(p, uint64_t(now.r) * p.heads + head + threadIdx.x, unit_m[threadIdx.x], unit_l[threadIdx.x]);
+                } else {
+                    float2* stats = reinterpret_cast<float2*>(p.part + uint64_t(gridDim.x) * 2 * H * D);
+                    stats[uint64_t(part_of) * H + threadIdx.x] = make_float2(unit_m[threadIdx.x], unit_l[threadIdx.x]);
+                }
             }
             __syncthreads();
         }
-        if (now.t == 0 && now.t_end == now.tiles) {
-            T* out = static_cast<T*>(p.out) + now.r * p.out_request + head * p.out_head;
-            for (uint32_t i = threadIdx.x; i < heads * D; i += kThreads) {
-                const uint32_t h = i / D, c = i % D;
-                const float all = unit_l[h];
-                if (c < p.dim) out[h * p.out_head + c] = from_float<T>(all == 0.f ? 0.f : sum[h * (D + 4) + c] / all);
-            }
-            if (threadIdx.x < heads)
-                put_lse(p, uint64_t(now.r) * p.heads + head + threadIdx.x, unit_m[threadIdx.x], unit_l[threadIdx.x]);
-        } else {
-            const uint32_t place_of = blockIdx.x * 2 + (now.t ? 0 : 1);
-            float* part = p.part + uint64_t(place_of) * H * D;
-            for (uint32_t i = threadIdx.x; i < heads * D; i += kThreads) part[i] = sum[i / D * (D + 4) + i % D];
-            float2* stats = reinterpret_cast<float2*>(p.part + uint64_t(gridDim.x) * 2 * H * D) + uint64_t(place_of) * H;
-            if (threadIdx.x < heads) stats[threadIdx.x] = make_float2(unit_m[threadIdx.x], unit_l[threadIdx.x]);
+        if (p.dim < D) {  // and the slot's last columns are zeros again
+            uint4* to = reinterpret_cast<uint4*>(ring + slot_in * R::kSlotBytes);
+            for (int i = lane; i < R::kSlotBytes / 16; i += kWarp) to[i] = make_uint4(0, 0, 0, 0);
         }
-        if (p.first && now.unit == 0 && now.t == 0 && threadIdx.x == 0) p.first[now.r] = first_tile;
+        if (threadIdx.x == 0) {
+            if (p.first && now.unit == 0 && now.t == 0) p.first[now.r] = first_tile;
+            if (!again) {
+                const long long per = run_of(total, gridDim.x, kWarps), unit_begin = first_tile - now.t;
+                const int32_t from = int32_t(unit_begin / per), to = int32_t((unit_begin + now.tiles - 1) / per);
+                *split = make_int4(int32_t(now.r), int32_t(now.unit), from, now.t_end < now.tiles ? to - from : 0);
+            }
+        }
         if (!again) break;
-        // the next part writes what this one reads behind a barrier of its own
         first_tile += now.t_end - now.t;
         now = then;
+        buffer ^= 1;
     }
     wait_copies<0>();
 }
 
-// A unit whose tiles lie in several blocks' runs: the last part of the first of
-// them and the first parts of the next `count` join, in order; every warp takes a
-// head and each so-many-th part of it.  Which unit is worked out from the lengths
-// while the decode kernel still runs.  Where the call has fewer units than the
-// decode kernel has blocks (and a unit many parts), block (u, h) takes head h of
-// unit u; else (and mostly two) block b all heads of the one that b's run ends in.
-template <int H, bool kByUnit>
-struct Join {
-    static constexpr int kWarps = kByUnit ? 8 : 16, kThreads = kWarps * kWarp;
-    static constexpr int kHeads = kByUnit ? 1 : H < kWarps ? H : kWarps;  // at once
-    static constexpr int kGroups = kWarps / kHeads;
-};
-template <typename T, int D, int H, bool kByUnit>
-__global__ void __launch_bounds__(Join<H, kByUnit>::kThreads) join_kernel(const Params p, uint32_t decode_blocks, int decode_warps)
+// A unit whose tiles lie in the runs of `count` + 1 blocks: the last part of the
+// first of them and the first parts of the others join, in order.  The first `count`
+// blocks here share its heads; a block's warps take a head each, or where it has
+// fewer, every so-many-th part of one.
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * kWarp;
+template <typename T, int D, int H>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
 {
-    using J = Join<H, kByUnit>;
-    constexpr int kThreads = J::kThreads, kGroups = J::kGroups;
-    __shared__ float sums[J::kHeads][kGroups > 1 ? D : 1];
-    __shared__ float2 stats_of[J::kHeads][kGroups];
+    __shared__ float sums[kJoinWarps / 2][D];
+    __shared__ float2 stats_of[kJoinWarps];
     let_next_start();
-    const uint32_t units = p.kv_heads * p.chunks;
-    const auto weight = [&](uint32_t i) { return (long long)(tokens_of(p, i).tiles()) * units; };
-    uint32_t r = 0, unit = 0, block = 0, count = 0;
-    if (kByUnit) {
-        r = blockIdx.x / units;
-        unit = blockIdx.x - r * units;
-        long long total;
-        const long long before = sum_before<kThreads>(p.requests, r, weight, total);
-        const uint32_t tiles = tokens_of(p, r).tiles();
-        const long long per = run_of(total, decode_blocks, decode_warps), first = before + (long long)unit * tiles;
-        block = uint32_t(first / per);
-        if (tiles) count = uint32_t((first + tiles - 1) / per) - block;
-    } else {
-        long long per = 1, begin = 0, end = 0;
-        Place place;
-        block = blockIdx.x;
-        const long long total = share_of<kThreads>(
-            p.requests, weight,
-            [&](long long all) {
-                per = run_of(all, decode_blocks, decode_warps);
-                begin = block * per;
-                end = min(all, begin + per);
-                return begin < all ? end - 1 : -1;
-            },
-            place);
-        if (begin < total) {
-            r = place.item;
-            const uint32_t tiles = tokens_of(p, r).tiles();
-            unit = uint32_t((end - 1 - place.first) / tiles);
-            const long long unit_begin = place.first + (long long)unit * tiles, unit_end = unit_begin + tiles;
-            if (unit_begin >= begin && unit_end > end) count = uint32_t((unit_end - 1) / per - block);
-        }
-    }
-    const uint32_t kv_head = unit / p.chunks, head0 = unit % p.chunks * p.per_unit;
-    const uint32_t heads = min(p.per_unit, p.group - head0);
-    if (count == 0 || blockIdx.y >= heads) {
-        // this launch ends after the one before, for whatever comes after it
-        if (blockIdx.x == 0 && blockIdx.y == 0) wait_for_previous();
-        return;
-    }
-    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-    const int place_in = warp % J::kHeads, group = warp / J::kHeads;
-    const float2* stats = reinterpret_cast<const float2*>(p.part + uint64_t(decode_blocks) * 2 * H * D);
     wait_for_previous();
+    const int4 split = reinterpret_cast<const int4*>(p.split)[blockIdx.x];
+    const uint32_t r = uint32_t(split.x), unit = uint32_t(split.y), block = uint32_t(split.z), count = uint32_t(split.w);
+    const uint32_t kv_head = unit / p.chunks, head0 = unit % p.chunks * p.per_unit;
+    const uint32_t heads = min(p.per_unit, p.group - head0), turn = blockIdx.x - block;
+    if (count == 0 || turn >= heads) return;
+    const uint32_t mine = (heads - turn + count - 1) / count;  // the heads turn, turn + count, ...
+    uint32_t at_once = 1;
+    while (at_once < mine && at_once < kJoinWarps) at_once *= 2;
+    const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    const uint32_t groups = kJoinWarps / at_once, place_in = warp % at_once, group = warp / at_once;
+    const float2* stats = reinterpret_cast<const float2*>(p.part + uint64_t(gridDim.x) * 2 * H * D);
 
-    for (uint32_t h0 = kByUnit ? blockIdx.y : 0; h0 < heads; h0 += kByUnit ? heads : J::kHeads) {
-        const uint32_t h = h0 + place_in;
-        const bool live = h < heads;
-        constexpr int kPer = D / kWarp, kAhead = 4;
+    constexpr int kPer = D / kWarp, kAhead = 4;
+    for (uint32_t i0 = 0; i0 < mine; i0 += at_once) {
+        const bool live = i0 + place_in < mine;
+        const uint32_t h = turn + (i0 + place_in) * count;
         float o[kPer], top = -INFINITY, all = 0.f;
 #pragma unroll
         for (int c = 0; c < kPer; ++c) o[c] = 0.f;
-        for (uint32_t i = live ? group : count + 1; i <= count; i += kGroups * kAhead) {
+        for (uint32_t i = live ? group : count + 1; i <= count; i += groups * kAhead) {
             float2 s[kAhead];
             float x[kAhead][kPer];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                const uint32_t at = i + u * kGroups;
+                const uint32_t at = i + u * groups;
                 s[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
                 for (int c = 0; c < kPer; ++c) x[u][c] = 0.f;
@@ -980,23 +990,20 @@ __global__ void __launch_bounds__(Join<H, kByUnit>::kThreads) join_kernel(const 
             }
             top = to;
         }
-        if (kGroups > 1) {
-            if (lane == 0) stats_of[place_in][group] = make_float2(top, all);
+        if (groups > 1) {
+            if (lane == 0) stats_of[warp] = make_float2(top, all);
             __syncthreads();
             const float own = all;
             float to = -INFINITY;
             all = 0.f;
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) to = fmaxf(to, stats_of[place_in][g].x);
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                const float2 of = stats_of[place_in][g];
+            for (uint32_t g = 0; g < groups; ++g) to = fmaxf(to, stats_of[g * at_once + place_in].x);
+            for (uint32_t g = 0; g < groups; ++g) {
+                const float2 of = stats_of[g * at_once + place_in];
                 all += share(of.x, of.y, to) * of.y;
             }
             const float factor = share(top, own, to);
             top = to;
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
+            for (uint32_t g = 0; g < groups; ++g) {
                 if (group == g) {
 #pragma unroll
                     for (int c = 0; c < kPer; ++c) {
@@ -1008,12 +1015,13 @@ __global__ void __launch_bounds__(Join<H, kByUnit>::kThreads) join_kernel(const 
                 __syncthreads();
             }
         }
-        if (live && group == kGroups - 1) {
+        if (live && group == groups - 1) {
             const uint32_t head = kv_head * p.group + head0 + h;
             T* out = static_cast<T*>(p.out) + r * p.out_request + head * p.out_head;
+            const float by = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll
             for (int c = 0; c < kPer; ++c)
-                if (c * kWarp + lane < p.dim) out[c * kWarp + lane] = from_float<T>(all == 0.f ? 0.f : o[c] / all);
+                if (c * kWarp + lane < p.dim) out[c * kWarp + lane] = from_float<T>(o[c] * by);
             if (lane == 0) put_lse(p, uint64_t(r) * p.heads + head, top, all);
         }
     }
@@ -1042,16 +1050,9 @@ lcpp_status launch(const Params& base, bool wide, size_t part_bytes_at_most, cud
     config.stream = s;
     config.attrs = &early;
     config.numAttrs = 1;
-    const uint64_t units = uint64_t(p.requests) * p.kv_heads * p.chunks;
-    if (units < blocks) {
-        config.gridDim = dim3(unsigned(units), std::min<uint32_t>(p.per_unit, H));
-        config.blockDim = dim3(Join<H, true>::kThreads);
-        LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H, true>, p, uint32_t(blocks), WARPS));
-    } else {
-        config.gridDim = dim3(blocks);
-        config.blockDim = dim3(Join<H, false>::kThreads);
-        LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H, false>, p, uint32_t(blocks), WARPS));
-    }
+    config.gridDim = dim3(blocks);
+    config.blockDim = dim3(kJoinThreads);
+    LCPP_CUDA_TRY(cudaLaunchKernelEx(&config, join_kernel<T, D, H>, p));
     return LCPP_OK;
 }
 
@@ -1083,17 +1084,17 @@ lcpp_status run_16bit(const Params& p, const Choice& c, bool wide, size_t part_b
 {
     switch (c.columns) {
     case 64:
-        return c.heads == 8    ? launch<T, 64, 8, 4, 4, 4>(p, wide, part_bytes, s)
+        return c.heads == 8    ? launch<T, 64, 8, 4, 4, 5>(p, wide, part_bytes, s)
                : c.heads == 16 ? launch<T, 64, 16, 4, 4, 4>(p, wide, part_bytes, s)
                                : launch<T, 64, 32, 4, 4, 2>(p, wide, part_bytes, s);
     case 128:
-        return c.heads == 8    ? launch<T, 128, 8, 3, 4, 4>(p, wide, part_bytes, s)
+        return c.heads == 8    ? launch<T, 128, 8, 2, 4, 4>(p, wide, part_bytes, s)
                : c.heads == 16 ? launch<T, 128, 16, 3, 4, 3>(p, wide, part_bytes, s)
                                : launch<T, 128, 32, 4, 4, 2>(p, wide, part_bytes, s);
     case 192:
         return c.heads == 8 ? launch<T, 192, 8, 3, 4, 2>(p, wide, part_bytes, s) : launch<T, 192, 16, 3, 4, 2>(p, wide, part_bytes, s);
     default:
-        return c.heads == 8 ? launch<T, 256, 8, 3, 4, 2>(p, wide, part_bytes, s) : launch<T, 256, 16, 2, 4, 2>(p, wide, part_bytes, s);
+        return c.heads == 8 ? launch<T, 256, 8, 2, 4, 3>(p, wide, part_bytes, s) : launch<T, 256, 16, 2, 4, 2>(p, wide, part_bytes, s);
     }
 }
 

@@ -19,9 +19,9 @@ lcpp_status run_f32(const Params& p, const Choice& c, bool wide, size_t part_byt
                : c.heads == 4 ? launch<float, 128, 4, 3, 4, 2>(p, wide, part_bytes, s)
                               : launch<float, 128, 8, 3, 4, 2>(p, wide, part_bytes, s);
     default:
-        return c.heads == 1   ? launch<float, 256, 1, 3, 2, 2>(p, wide, part_bytes, s)
-               : c.heads == 2 ? launch<float, 256, 2, 3, 2, 2>(p, wide, part_bytes, s)
-                              : launch<float, 256, 4, 3, 2, 2>(p, wide, part_bytes, s);
+        return c.heads == 1   ? launch<float, 256, 1, 2, 2, 3>(p, wide, part_bytes, s)
+               : c.heads == 2 ? launch<float, 256, 2, 2, 2, 3>(p, wide, part_bytes, s)
+                              : launch<float, 256, 4, 2, 2, 3>(p, wide, part_bytes, s);
     }
 }
 
