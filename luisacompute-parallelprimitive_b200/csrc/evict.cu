@@ -26,7 +26,8 @@ namespace {
 constexpr int kThreads = 1024, kWarps = kThreads / kWarp;
 constexpr int kMostCluster = 8;
 constexpr int kAhead = 4;              // tokens whose loads a thread has under way
-constexpr uint32_t kKeys = 40 * 1024;  // keys of a block that stay in shared memory; others are read again
+constexpr uint32_t kPages = 2048;      // page ids of a block's run that come into shared memory; others are read where needed
+constexpr uint32_t kKeys = 38 * 1024;  // keys of a block that stay in shared memory; others are read again
 constexpr uint32_t kProtected = 0xffffffffu, kNaN = 0xfffffffeu;
 
 struct Params {
@@ -50,6 +51,7 @@ struct Params {
 constexpr int kBins = 2048, kCopies = 4;
 struct alignas(16) Shared {
     uint32_t histogram[2][kBins];  // from the largest digit down
+    uint32_t groups[2][kWarps];    // sums of so many bins each
     uint32_t broken;            // a page id out of range
     uint32_t holes, fillers;    // of the block's tokens
 };
@@ -98,14 +100,15 @@ __device__ __noinline__ uint32_t key_again(const Params& p, const int32_t* row, 
     return at < p.first || at >= recent ? kProtected : key_of(p.scores[slot]);
 }
 
-__global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
+__global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ Params p)
 {
     extern __shared__ uint32_t dynamic[];
     uint32_t* copies = dynamic;  // [kBins][kCopies], from the largest digit down
-    uint32_t* keys = dynamic + kBins * kCopies;
+    uint32_t* pages = dynamic + kBins * kCopies;
+    uint32_t* keys = pages + kPages;
     __shared__ Shared shared;
     __shared__ uint32_t warps[3][kWarps];
-    __shared__ uint32_t found[4];  // digit, keys above it, keys of it in the blocks before and in all
+    __shared__ uint32_t found[5];  // digit, keys above it, keys of it in the blocks before and in all; a broken page
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t r = blockIdx.x / blocks;
@@ -129,11 +132,6 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
     const uint32_t run = (n + blocks - 1) / blocks, lo = min(n, rank * run), count = min(n - lo, run);
     const int32_t* row = p.table + r * p.table_stride;
     const int64_t recent = int64_t(n) + before - p.recent;
-    const auto slot_of = [&](uint32_t token, uint32_t& id) {
-        const uint32_t page = p.page.quotient(token);
-        id = uint32_t(row[page]);
-        return uint64_t(id) * p.page.d + (token - page * p.page.d);
-    };
     // four tokens' keys; 0, which no token has, past the last one
     const auto keys_at = [&](uint32_t i) {
         if (i + 3 < kKeys) return *reinterpret_cast<const uint4*>(keys + i);
@@ -141,35 +139,31 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         return make_uint4(one(i), one(i + 1), one(i + 2), one(i + 3));
     };
 
+    // the pages of the run
+    const uint32_t first_page = p.page.quotient(lo), end_page = count ? p.page.quotient(lo + count - 1) + 1 : first_page;
+    const bool staged = end_page - first_page <= kPages;
+    if (staged)
+        for (uint32_t i = threadIdx.x; i < end_page - first_page; i += kThreads) pages[i] = uint32_t(row[first_page + i]);
+    const auto page_id = [&](uint32_t page) { return staged ? pages[page - first_page] : uint32_t(row[page]); };
+
     if (threadIdx.x == 0) shared.broken = 0;
     if (threadIdx.x < 3 && count + threadIdx.x < kKeys) keys[count + threadIdx.x] = 0;
     for (int i = threadIdx.x; i < kBins * kCopies; i += kThreads) copies[i] = 0;
     __syncthreads();
     bool broken = false;
-    // kAhead tokens at a time, whose loads are under way together; the page ids of
-    // the next ones come meanwhile
-    uint32_t id[kAhead];
-    const auto look_up = [&](uint32_t i) {
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const uint32_t at = i + u * kThreads;
-            id[u] = at < count ? uint32_t(row[p.page.quotient(lo + at)]) : 0;
-        }
-    };
-    look_up(threadIdx.x);
-    for (uint32_t i = threadIdx.x; i < count; i += kThreads * kAhead) {
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads * kAhead) {  // whose loads are under way together
         float score[kAhead];
         int32_t position[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const uint32_t at = i + u * kThreads, token = lo + at;
-            const bool in = at < count && id[u] < p.num_pages;
+            const uint32_t at = i + u * kThreads, token = lo + at, page = p.page.quotient(token);
+            const uint32_t id = at < count ? page_id(page) : 0;
+            const bool in = at < count && id < p.num_pages;
             broken |= at < count && !in;
-            const uint64_t slot = uint64_t(id[u]) * p.page.d + (token - p.page.quotient(token) * p.page.d);
+            const uint64_t slot = uint64_t(id) * p.page.d + (token - page * p.page.d);
             score[u] = in ? p.scores[slot] : 0.f;
             position[u] = in && p.positions ? p.positions[slot] : int32_t(token);
         }
-        look_up(i + kThreads * kAhead);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const uint32_t at = i + u * kThreads;
@@ -208,44 +202,57 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         uint4* bin = reinterpret_cast<uint4*>(copies) + threadIdx.x * 2;
         const uint4 x = bin[0], y = bin[1];
         bin[0] = bin[1] = make_uint4(0, 0, 0, 0);  // for the next pass
-        uint2 mine = make_uint2(x.x + x.y + x.z + x.w, y.x + y.y + y.z + y.w), earlier = make_uint2(0, 0);
-        if (blocks > 1) {
-            reinterpret_cast<uint2*>(shared.histogram[pass & 1])[threadIdx.x] = mine;
-            cluster.sync();  // the other buffer is free again, too
-            uint2 of[kMostCluster];
-#pragma unroll
-            for (uint32_t b = 0; b < kMostCluster; ++b)
-                of[b] = b < blocks ? reinterpret_cast<const uint2*>(
-                                         cluster.map_shared_rank(&shared, b)->histogram[pass & 1])[threadIdx.x]
-                                   : make_uint2(0, 0);
-            mine = make_uint2(0, 0);
-#pragma unroll
-            for (uint32_t b = 0; b < kMostCluster; ++b) {
-                mine.x += of[b].x, mine.y += of[b].y;
-                if (b < rank) earlier.x += of[b].x, earlier.y += of[b].y;
-            }
-        }
-        if (pass == 0) {
-            uint32_t any = 0;
-            for (uint32_t b = 0; b < blocks; ++b) any |= cluster.map_shared_rank(&shared, b)->broken;
-            if (any) {
-                leave();
-                meet();  // nobody leaves while others read
-                return;
-            }
-        }
-        uint32_t of_warp, all;
-        uint32_t above = lanes_before(mine.x + mine.y, of_warp);
-        above += warps_before(of_warp, warps[0], all);
-        // one thread finds the bin: there are at least `need` such keys
-        if (above < need && above + mine.x + mine.y >= need) {
-            const bool second = above + mine.x < need;
-            found[0] = kBins - 1 - 2 * threadIdx.x - second;
-            found[1] = above + (second ? mine.x : 0);
+        const uint2 mine = make_uint2(x.x + x.y + x.z + x.w, y.x + y.y + y.z + y.w);
+        // The bin of the last kept key: there are at least `need` such keys.
+        const auto look_in = [&](uint32_t above, uint2 in_bin, uint2 earlier, uint32_t bin_pair) {
+            if (above >= need || above + in_bin.x + in_bin.y < need) return;
+            const bool second = above + in_bin.x < need;
+            found[0] = kBins - 1 - 2 * bin_pair - second;
+            found[1] = above + (second ? in_bin.x : 0);
             found[2] = second ? earlier.y : earlier.x;
-            found[3] = second ? mine.y : mine.x;
+            found[3] = second ? in_bin.y : in_bin.x;
+        };
+        uint32_t of_warp, all;
+        if (blocks == 1) {
+            uint32_t above = lanes_before(mine.x + mine.y, of_warp);
+            above += warps_before(of_warp, warps[0], all);
+            look_in(above, mine, make_uint2(0, 0), threadIdx.x);
+            if (threadIdx.x == 0) found[4] = shared.broken;
+        } else {
+            reinterpret_cast<uint2*>(shared.histogram[pass & 1])[threadIdx.x] = mine;
+            of_warp = __reduce_add_sync(~0u, mine.x + mine.y);
+            if (lane == 0) shared.groups[pass & 1][warp] = of_warp;
+            cluster.sync();  // the other buffer is free again, too
+            if (warp == 0) {
+                // first the group of 64 bins over all blocks, then the bin: little is read from the others
+                uint32_t sum = 0, any = 0;
+#pragma unroll
+                for (uint32_t b = 0; b < kMostCluster; ++b) {
+                    const Shared* other = cluster.map_shared_rank(&shared, b < blocks ? b : 0);
+                    sum += b < blocks ? other->groups[pass & 1][lane] : 0;
+                    any |= other->broken;
+                }
+                const uint32_t above = lanes_before(sum, all);
+                const int at = __ffs(__ballot_sync(~0u, above < need && above + sum >= need)) - 1;
+                uint2 in_bin = make_uint2(0, 0), earlier = make_uint2(0, 0);
+#pragma unroll
+                for (uint32_t b = 0; b < kMostCluster; ++b) {
+                    const Shared* other = cluster.map_shared_rank(&shared, b < blocks ? b : 0);
+                    const uint2 c = b < blocks ? reinterpret_cast<const uint2*>(other->histogram[pass & 1])[at * kWarp + lane]
+                                               : make_uint2(0, 0);
+                    in_bin.x += c.x, in_bin.y += c.y;
+                    if (b < rank) earlier.x += c.x, earlier.y += c.y;
+                }
+                look_in(__shfl_sync(~0u, above, at) + lanes_before(in_bin.x + in_bin.y, all), in_bin, earlier, at * kWarp + lane);
+                if (lane == 0) found[4] = any;
+            }
         }
         __syncthreads();
+        if (pass == 0 && found[4]) {
+            leave();
+            meet();  // nobody leaves while others read
+            return;
+        }
         top |= found[0] << shift;
         need -= found[1];
         equal_before = found[2];
@@ -312,15 +319,11 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
     uint32_t filler = __shfl_sync(~0u, lanes_before(warps[2][lane], total), warp);
     if (threadIdx.x == 0) shared.fillers = total;
     meet();
-    uint32_t moves = 0;
-    for (uint32_t b = 0; b < blocks; ++b) {
-        const Shared* other = cluster.map_shared_rank(&shared, b);
-        if (b < rank) {
-            hole += other->holes;
-            filler += other->fillers;
-        }
-        moves += other->fillers;
-    }
+    const Shared* other = cluster.map_shared_rank(&shared, lane < blocks ? lane : 0);
+    const uint32_t others_holes = lane < blocks ? other->holes : 0, others_fillers = lane < blocks ? other->fillers : 0;
+    hole += __reduce_add_sync(~0u, lane < rank ? others_holes : 0);
+    filler += __reduce_add_sync(~0u, lane < rank ? others_fillers : 0);
+    const uint32_t moves = __reduce_add_sync(~0u, others_fillers);
     meet();  // nobody leaves while others read
     if (moves > p.max_moves) {
         leave();
@@ -334,13 +337,17 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const Params p)
         hole += in_warp;
         uint32_t to_filler = filler + lanes_before(__popc(filler_mask), in_warp);
         filler += in_warp;
+        int64_t slot[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (!((hole_mask | filler_mask) >> u & 1)) continue;
-            uint32_t id;
-            const int64_t slot = int64_t(slot_of(lo + i + u, id));
-            if (filler_mask >> u & 1) out[to_filler++].x = slot;
-            else out[to_hole++].y = slot;
+            const uint32_t token = lo + i + u, page = p.page.quotient(token);
+            const uint32_t id = (hole_mask | filler_mask) >> u & 1 ? page_id(page) : 0;
+            slot[u] = int64_t(uint64_t(id) * p.page.d + (token - page * p.page.d));
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (filler_mask >> u & 1) out[to_filler++].x = slot[u];
+            else if (hole_mask >> u & 1) out[to_hole++].y = slot[u];
         }
     });
     if (rank == 0 && threadIdx.x == 0) {
@@ -522,8 +529,8 @@ lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
         // room in a few steps, so that few launch shapes are set up
         uint32_t room = 4096;
         while (room < kKeys && room < run) room *= 2;
-        const size_t smem = (kBins * kCopies + std::min(room, kKeys)) * 4;
-        set_max_dynamic_smem(reinterpret_cast<const void*>(plan_kernel), (kBins * kCopies + kKeys) * 4);
+        const size_t smem = (kBins * kCopies + kPages + std::min(room, kKeys)) * 4;
+        set_max_dynamic_smem(reinterpret_cast<const void*>(plan_kernel), (kBins * kCopies + kPages + kKeys) * 4);
         cudaLaunchAttribute shape{};
         shape.id = cudaLaunchAttributeClusterDimension;
         shape.val.clusterDim.x = cluster;
