@@ -255,13 +255,13 @@ def lib() -> ctypes.CDLL:
         "lcpp_dispatch_combine_backward": ([vp, u64, vp, u64, vp, vp, vp, vp, vp, u64, vp, u64, u32, u32, u64, u64,
                                             i, vp], i),
         "lcpp_rotary_frequencies": ([vp, u32, f64, i, f64, f64, f64, f64], i),
-        "lcpp_rotary_forward": ([ctypes.POINTER(RotaryArgs), vp], i),
-        "lcpp_rotary_backward": ([ctypes.POINTER(RotaryArgs), vp], i),
-        "lcpp_rotary_append": ([ctypes.POINTER(RotaryArgs), ctypes.POINTER(CacheAppendArgs), vp], i),
+        "lcpp_rotary_forward": ([vp, vp], i),
+        "lcpp_rotary_backward": ([vp, vp], i),
+        "lcpp_rotary_append": ([vp, vp, vp], i),
         "lcpp_paged_attention_temp_bytes": ([u32, u32, u32, u32, u64, szp], i),
-        "lcpp_paged_attention_decode": ([vp, sz, ctypes.POINTER(PagedAttentionArgs), vp], i),
-        "lcpp_cache_evict_plan": ([ctypes.POINTER(CacheEvictArgs), vp], i),
-        "lcpp_cache_evict_move": ([ctypes.POINTER(KVCache), vp, u64, u32, vp, u32, vp, vp, vp], i),
+        "lcpp_paged_attention_decode": ([vp, sz, vp, vp], i),
+        "lcpp_cache_evict_plan": ([vp, vp], i),
+        "lcpp_cache_evict_move": ([vp, vp, u64, u32, vp, u32, vp, vp, vp], i),
         "lcpp_diag_timing_enable": ([i], i),
         "lcpp_diag_launch_shapes": ([ctypes.POINTER(u64)], i),
         "lcpp_diag_wait_timeout_probe": ([vp, sz, u64, vp], i),
@@ -283,9 +283,15 @@ def check(status: int, what: str) -> None:
 # ---------------------------------------------------------------------------
 # torch helpers (plumbing only)
 # ---------------------------------------------------------------------------
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def dtype_code(t) -> int:
@@ -985,72 +991,116 @@ def _rows(t, rows, columns, code, name):
 _raw_stream = None
 
 
-def _queue(stream):
+def _queue(stream, device=None):
     """Handle of the stream to enqueue on: the one given, else torch's current one."""
     global _raw_stream
     if stream is not None:
         return stream.cuda_stream
-    torch = _torch()
     if _raw_stream is None:
+        torch = _torch()
         # the handle without a Stream object around it, where torch offers it
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                               lambda device: torch.cuda.current_stream(device).cuda_stream)
-    return _raw_stream(torch.cuda.current_device())
+    return _raw_stream(_torch().cuda.current_device() if device is None else device)
 
 
-def _here(t, name):
-    """Refuses a tensor of another device than the current one: its memory is not the kernels' to use."""
-    if t.get_device() != _torch().cuda.current_device():
-        raise LcppError(ERR_INVALID_ARG, f"{name}: a tensor of the current device")
+_FORMATS = {ctypes.c_void_p: "Q", ctypes.c_uint64: "Q", ctypes.c_uint32: "I", ctypes.c_int: "i", ctypes.c_float: "f"}
 
 
-def _heads(t, tokens, heads, dim, code, name):
+def _packer(structure):
+    """struct.Struct.pack for a ctypes structure's fields, those of nested ones in their place: a call's arguments
+    are put together several times faster than by the structure itself."""
+    import struct
+
+    def fields(kind, at):
+        for name, field in kind._fields_:
+            offset = at + getattr(kind, name).offset
+            if issubclass(field, ctypes.Structure):
+                yield from fields(field, offset)
+            else:
+                yield offset, ctypes.sizeof(field), _FORMATS[field]
+
+    text, end = "=", 0
+    for offset, size, code in fields(structure, 0):
+        text += f"{offset - end}x{code}"
+        end = offset + size
+    return struct.Struct(text + f"{ctypes.sizeof(structure) - end}x").pack
+
+
+_pack_rotary, _pack_append = _packer(RotaryArgs), _packer(CacheAppendArgs)
+_pack_attention, _pack_evict, _pack_cache = _packer(PagedAttentionArgs), _packer(CacheEvictArgs), _packer(KVCache)
+
+
+_current_device = None
+
+
+def _device():
+    """The current device, whose memory alone the kernels use (-2 without one, where no tensor is)."""
+    global _current_device
+    if _current_device is None:
+        torch = _torch()
+        if not torch.cuda.is_available():
+            return -2
+        torch.cuda.current_device()  # starts CUDA
+        # the number without the checks around it, where torch offers it
+        _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    return _current_device()
+
+
+def _array(t, dtype, count, name, device):
+    """Pointer of a contiguous tensor of `dtype` with at least `count` elements on the device (None: 0)."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.numel() < count or not t.is_contiguous():
+        raise LcppError(ERR_INVALID_ARG, f"{name}: contiguous {dtype} with at least {count} elements")
+    if t.get_device() != device:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a CUDA tensor of the current device")
+    return t.data_ptr()
+
+
+def _heads(t, tokens, heads, dim, dtype, name, device):
     """(pointer, token stride, head stride) of a [tokens, heads, dim] tensor whose columns are adjacent."""
-    shape = t.shape
-    if _row_code(t) != code or len(shape) != 3 or shape[0] < tokens or shape[1] != heads or shape[2] != dim:
-        raise LcppError(ERR_INVALID_ARG, f"{name}: one dtype, at least {tokens} x {heads} x {dim}")
-    a, b, c = t.stride()
-    if c != 1 and dim > 1 and shape[0]:
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not dtype or len(shape) != 3 or shape[0] < tokens or shape[1] != heads or shape[2] != dim:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: {dtype}, at least {tokens} x {heads} x {dim}")
+    if stride[2] != 1 and dim > 1 and tokens:
         raise LcppError(ERR_INVALID_ARG, f"{name}: a head's columns have to be adjacent")
-    if not t.is_cuda:
-        raise LcppError(ERR_INVALID_ARG, f"{name}: a CUDA tensor")
-    return t.data_ptr(), a, b
+    if t.get_device() != device:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a CUDA tensor of the current device")
+    return t.data_ptr(), stride[0], stride[1]
 
 
-def _kv_cache(k, v):
-    """The lcpp_kv_cache of two [pages, block_size, heads, dim] tensors of equal strides."""
-    shape, stride, code = k.shape, k.stride(), _row_code(k)
-    if len(shape) != 4 or v.shape != shape or v.stride() != stride or _row_code(v) != code:
+def _kv_cache(k, v, device):
+    """The lcpp_kv_cache's fields of two [pages, block_size, heads, dim] tensors of equal strides."""
+    shape, stride, dtype = k.shape, k.stride(), k.dtype
+    if len(shape) != 4 or v.shape != shape or v.stride() != stride or v.dtype is not dtype:
         raise LcppError(ERR_INVALID_ARG, "keys and values: [pages, block_size, heads, dim] of one dtype, shape and layout")
     if stride[3] != 1 and shape[3] > 1:
         raise LcppError(ERR_INVALID_ARG, "keys and values: a head's columns have to be adjacent")
-    if not k.is_cuda or not v.is_cuda:
-        raise LcppError(ERR_INVALID_ARG, "keys and values: CUDA tensors")
-    _here(k, "keys")
-    return KVCache(k.data_ptr(), v.data_ptr(), stride[0], stride[1], stride[2], shape[0], shape[1], shape[2], shape[3],
-                   code)
+    if k.get_device() != device or v.get_device() != device:
+        raise LcppError(ERR_INVALID_ARG, "keys and values: CUDA tensors of the current device")
+    return k.data_ptr(), v.data_ptr(), stride[0], stride[1], stride[2], *shape, _row_code(k)
 
 
-def _table(t, rows):
+def _table(t, rows, device):
     """(pointer, row stride, width) of an int32 block table of at least `rows` rows."""
-    if t.dtype != _torch().int32 or t.dim() != 2 or t.shape[0] < rows or \
-            (t.stride(1) != 1 and t.shape[1] > 1 and rows):
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not _torch().int32 or len(shape) != 2 or shape[0] < rows or (stride[1] != 1 and shape[1] > 1 and rows):
         raise LcppError(ERR_INVALID_ARG, "d_block_table: int32 [num_requests, width], columns adjacent")
-    if not t.is_cuda:
-        raise LcppError(ERR_INVALID_ARG, "d_block_table: a CUDA tensor")
-    width = t.shape[1]
-    return t.data_ptr(), (t.stride(0) if rows > 1 else max(t.stride(0), width)), width
+    if t.get_device() != device:
+        raise LcppError(ERR_INVALID_ARG, "d_block_table: a CUDA tensor of the current device")
+    return t.data_ptr(), (stride[0] if rows > 1 else max(stride[0], shape[1])), shape[1]
 
 
-def _moves(t, requests, name):
+def _moves(t, requests, name, device):
     """(pointer, pairs from request to request, pairs of a request) of an int64 [requests, moves, 2] tensor."""
     shape, stride = t.shape, t.stride()
-    if t.dtype != _torch().int64 or len(shape) != 3 or shape[2] != 2 or shape[0] < requests or stride[2] != 1 or \
+    if t.dtype is not _torch().int64 or len(shape) != 3 or shape[2] != 2 or shape[0] < requests or stride[2] != 1 or \
             (stride[1] != 2 and shape[1] > 1) or (stride[0] % 2 and shape[0] > 1):
         raise LcppError(ERR_INVALID_ARG, f"{name}: int64 [num_requests, max_moves, 2], pairs adjacent")
-    if not t.is_cuda:
-        raise LcppError(ERR_INVALID_ARG, f"{name}: a CUDA tensor")
-    return t.data_ptr(), (stride[0] // 2 if shape[0] > 1 else shape[1]), shape[1]
+    if t.get_device() != device:
+        raise LcppError(ERR_INVALID_ARG, f"{name}: a CUDA tensor of the current device")
+    return t.data_ptr(), (stride[0] // 2 if requests > 1 else max(stride[0] // 2, shape[1])), shape[1]
 
 
 def _scratch(temp):
@@ -1238,31 +1288,30 @@ class DeviceRotary:
         return torch.tensor(list(out)[:rotary_dim // 2], dtype=torch.float64, device=device or "cuda")
 
     @staticmethod
-    def _args(q, k, q_out, k_out, positions, frequencies, tokens, layout, scale, token_request, position_offset):
+    def _args(device, q, k, q_out, k_out, positions, frequencies, tokens, layout, scale, token_request,
+              position_offset, append=False):
+        """The fields of lcpp_rotary_args."""
         torch = _torch()
-        some = q if q is not None else k
-        if some is None:
-            raise LcppError(ERR_INVALID_ARG, "d_q or d_k: a tensor")
-        if some.dim() != 3:
+        some = k if q is None else q
+        if some is None or some.dim() != 3:
             raise LcppError(ERR_INVALID_ARG, "d_q, d_k: [tokens, heads, dim]")
-        code, dim = _row_code(some), some.shape[2]
-        rows = []
+        dtype, code, dim = some.dtype, _row_code(some), some.shape[2]
+        fields = []
         for x, out, name in ((q, q_out, "d_q"), (k, k_out, "d_k")):
             if x is None:
-                rows.append(HeadRows())
+                fields += (0, 0, 0, 0, 0, 0, 0)
                 continue
             heads = x.shape[1] if x.dim() == 3 else 0
-            at, a, b = _heads(x, tokens, heads, dim, code, name)
-            to, c, d = (None, 0, 0) if out is None else _heads(out, tokens, heads, dim, code, name + "_out")
-            rows.append(HeadRows(at, to, a, b, c, d, heads))
-        _here(some, "d_q, d_k")
-        requests = 0 if token_request is None else (1 << 31) - 1 if position_offset is None else position_offset.numel()
-        return RotaryArgs(
-            rows[0], rows[1], _flat(positions, torch.int32, tokens, "d_positions"),
-            _flat(token_request, torch.int32, tokens, "d_token_request"),
-            _flat(position_offset, torch.int32, 0, "d_position_offset"),
-            _flat(frequencies, torch.float64, 0, "d_frequencies"), tokens, requests, dim, 2 * frequencies.numel(),
-            layout, scale, code)
+            at, a, b = _heads(x, tokens, heads, dim, dtype, name, device)
+            to, c, d = (0, 0, 0) if append and x is k else _heads(out, tokens, heads, dim, dtype, name + "_out", device)
+            fields += (at, to, a, b, c, d, heads)
+        requests = 0 if token_request is None else 0x7fffffff if position_offset is None else position_offset.numel()
+        turned = frequencies.numel()
+        return (*fields, _array(positions, torch.int32, tokens, "d_positions", device),
+                _array(token_request, torch.int32, tokens, "d_token_request", device),
+                _array(position_offset, torch.int32, 0, "d_position_offset", device),
+                _array(frequencies, torch.float64, 0, "d_frequencies", device), tokens, requests, dim, 2 * turned,
+                layout, scale, code)
 
     def Forward(self, d_q, d_k, d_q_out, d_k_out, d_positions, d_frequencies, num_tokens, layout=ROTARY_HALF, scale=1.0,
                 d_token_request=None, d_position_offset=None, stream=None):
@@ -1270,16 +1319,18 @@ class DeviceRotary:
         with any strides of tokens and heads, in place where the output is the input; positions int32; as many
         columns as twice the frequencies (float64) are turned.  Tokens whose request (int32) is negative are left
         out; a request's offset (int32) is added to its tokens' positions."""
-        args = self._args(d_q, d_k, d_q_out, d_k_out, d_positions, d_frequencies, num_tokens, layout, scale,
+        device = _device()
+        args = self._args(device, d_q, d_k, d_q_out, d_k_out, d_positions, d_frequencies, num_tokens, layout, scale,
                           d_token_request, d_position_offset)
-        check(lib().lcpp_rotary_forward(args, _queue(stream)), "Forward")
+        check(lib().lcpp_rotary_forward(_pack_rotary(*args), _queue(stream, device)), "Forward")
 
     def Backward(self, d_grad_q, d_grad_k, d_grad_q_out, d_grad_k_out, d_positions, d_frequencies, num_tokens,
                  layout=ROTARY_HALF, scale=1.0, d_token_request=None, d_position_offset=None, stream=None):
         """Gradients of Forward's inputs from those of its outputs (lcpp_rotary_backward)."""
-        args = self._args(d_grad_q, d_grad_k, d_grad_q_out, d_grad_k_out, d_positions, d_frequencies, num_tokens,
-                          layout, scale, d_token_request, d_position_offset)
-        check(lib().lcpp_rotary_backward(args, _queue(stream)), "Backward")
+        device = _device()
+        args = self._args(device, d_grad_q, d_grad_k, d_grad_q_out, d_grad_k_out, d_positions, d_frequencies,
+                          num_tokens, layout, scale, d_token_request, d_position_offset)
+        check(lib().lcpp_rotary_backward(_pack_rotary(*args), _queue(stream, device)), "Backward")
 
     def Append(self, d_q, d_k, d_v, d_q_out, d_k_cache, d_v_cache, d_slots, d_positions, d_frequencies, num_tokens,
                layout=ROTARY_HALF, scale=1.0, d_token_request=None, d_position_offset=None, d_slot_positions=None,
@@ -1288,16 +1339,17 @@ class DeviceRotary:
         (lcpp_rotary_append): caches [pages, block_size, heads, dim] with any strides, slots int64 as
         DeviceBlockTable.Extend gives them.  d_slot_positions (int32, one per slot) gets the tokens' positions,
         d_slot_scores (float32) zeros."""
-        torch = _torch()
-        args = self._args(d_q, d_k, d_q_out, None, d_positions, d_frequencies, num_tokens, layout, scale,
-                          d_token_request, d_position_offset)
-        cache = _kv_cache(d_k_cache, d_v_cache)
-        slots = cache.num_pages * cache.block_size
-        v, v_token, v_head = _heads(d_v, num_tokens, cache.num_kv_heads, cache.head_dim, cache.dtype, "d_v")
-        append = CacheAppendArgs(cache, v, v_token, v_head, _flat(d_slots, torch.int64, num_tokens, "d_slots"),
-                                 _flat(d_slot_positions, torch.int32, slots, "d_slot_positions"),
-                                 _flat(d_slot_scores, torch.float32, slots, "d_slot_scores"))
-        check(lib().lcpp_rotary_append(args, append, _queue(stream)), "Append")
+        torch, device = _torch(), _device()
+        args = self._args(device, d_q, d_k, d_q_out, None, d_positions, d_frequencies, num_tokens, layout, scale,
+                          d_token_request, d_position_offset, append=True)
+        cache = _kv_cache(d_k_cache, d_v_cache, device)
+        pages, block, heads, dim = cache[5:9]
+        append = _pack_append(
+            *cache, *_heads(d_v, num_tokens, heads, dim, d_k_cache.dtype, "d_v", device),
+            _array(d_slots, torch.int64, num_tokens, "d_slots", device),
+            _array(d_slot_positions, torch.int32, pages * block, "d_slot_positions", device),
+            _array(d_slot_scores, torch.float32, pages * block, "d_slot_scores", device))
+        check(lib().lcpp_rotary_append(_pack_rotary(*args), append, _queue(stream, device)), "Append")
 
 
 class DevicePagedAttention:
@@ -1318,19 +1370,17 @@ class DevicePagedAttention:
         with any strides, block table and lengths int32 as DeviceBlockTable.Extend leaves them.  scale None:
         dim ** -0.5.  d_lse_out float32 [requests, heads]; scores float32, one per slot: the outputs are
         score_decay * d_scores (None: zeros) plus each token's attention weight, summed over the heads."""
-        torch = _torch()
-        cache = _kv_cache(d_k_cache, d_v_cache)
-        heads, dim, n, f32 = d_q.shape[1] if d_q.dim() == 3 else 0, cache.head_dim, num_requests, torch.float32
-        slots = cache.num_pages * cache.block_size
-        q, q_request, q_head = _heads(d_q, n, heads, dim, cache.dtype, "d_q")
-        out, out_request, out_head = _heads(d_out, n, heads, dim, cache.dtype, "d_out")
-        table, table_stride, width = _table(d_block_table, n)
-        args = PagedAttentionArgs(
-            cache, q, q_request, q_head, out, out_request, out_head, table, table_stride, width, n,
-            _flat(d_seq_lens, torch.int32, n, "d_seq_lens"), heads, window, dim ** -0.5 if scale is None else scale,
-            softcap, _flat(d_lse_out, f32, n * heads, "d_lse_out"), _flat(d_scores, f32, slots, "d_scores"),
-            _flat(d_scores_out, f32, slots, "d_scores_out"), score_decay)
-        check(lib().lcpp_paged_attention_decode(*_scratch(temp), args, _queue(stream)), "Decode")
+        device, n, f32 = _device(), num_requests, _torch().float32
+        cache = _kv_cache(d_k_cache, d_v_cache, device)
+        slots, dim, dtype, heads = cache[5] * cache[6], cache[8], d_k_cache.dtype, d_q.shape[1] if d_q.dim() == 3 else 0
+        table, table_stride, width = _table(d_block_table, n, device)
+        args = _pack_attention(
+            *cache, *_heads(d_q, n, heads, dim, dtype, "d_q", device), *_heads(d_out, n, heads, dim, dtype, "d_out", device),
+            table, table_stride, width, n, _array(d_seq_lens, _torch().int32, n, "d_seq_lens", device), heads, window,
+            dim ** -0.5 if scale is None else scale, softcap, _array(d_lse_out, f32, n * heads, "d_lse_out", device),
+            _array(d_scores, f32, slots, "d_scores", device), _array(d_scores_out, f32, slots, "d_scores_out", device),
+            score_decay)
+        check(lib().lcpp_paged_attention_decode(*_scratch(temp), args, _queue(stream, device)), "Decode")
 
 
 class DeviceCacheEviction:
@@ -1343,35 +1393,36 @@ class DeviceCacheEviction:
         budget tokens, by d_scores (float32, one per slot).  d_moves_out int64 [requests, max_moves, 2]; the lengths
         and counts int32.  With the free list that DeviceBlockTable.Extend takes pages from, pages that are not
         needed any more go back to it."""
-        torch = _torch()
-        i32, n = torch.int32, num_requests
-        table, table_stride, width = _table(d_block_table, n)
-        moves, moves_stride, max_moves = _moves(d_moves_out, n, "d_moves_out")
+        torch, device, n = _torch(), _device(), num_requests
+        i32 = torch.int32
+        table, table_stride, width = _table(d_block_table, n, device)
+        moves, moves_stride, max_moves = _moves(d_moves_out, n, "d_moves_out", device)
         if block_size < 1:
             raise LcppError(ERR_INVALID_ARG, "block_size: at least 1")
         pages = d_scores.numel() // block_size
-        args = CacheEvictArgs(
-            _flat(d_seq_lens, i32, n, "d_seq_lens"), table, table_stride, width, n, pages, block_size,
-            _flat(d_scores, torch.float32, 0, "d_scores"),
-            _flat(d_positions, i32, pages * block_size, "d_positions"), _flat(d_evicted, i32, n, "d_evicted"), budget,
-            budget if trigger is None else trigger, keep_first, keep_recent, max_moves,
-            _flat(d_seq_lens_out, i32, n, "d_seq_lens_out"), _flat(d_evicted_out, i32, n, "d_evicted_out"),
-            _flat(d_move_counts_out, i32, n, "d_move_counts_out"),
-            moves, moves_stride,
-            _flat(d_free_blocks, i32, 0, "d_free_blocks"), _flat(d_free_used, i32, 1, "d_free_used"),
-            _flat(d_free_used_out, i32, 1, "d_free_used_out"), 0 if d_free_blocks is None else d_free_blocks.numel())
-        _here(d_scores, "d_scores")
-        check(lib().lcpp_cache_evict_plan(args, _queue(stream)), "Plan")
+        args = _pack_evict(
+            _array(d_seq_lens, i32, n, "d_seq_lens", device), table, table_stride, width, n, pages, block_size,
+            _array(d_scores, torch.float32, 0, "d_scores", device),
+            _array(d_positions, i32, pages * block_size, "d_positions", device),
+            _array(d_evicted, i32, n, "d_evicted", device), budget, budget if trigger is None else trigger, keep_first,
+            keep_recent, max_moves, _array(d_seq_lens_out, i32, n, "d_seq_lens_out", device),
+            _array(d_evicted_out, i32, n, "d_evicted_out", device),
+            _array(d_move_counts_out, i32, n, "d_move_counts_out", device), moves, moves_stride,
+            _array(d_free_blocks, i32, 0, "d_free_blocks", device), _array(d_free_used, i32, 1, "d_free_used", device),
+            _array(d_free_used_out, i32, 1, "d_free_used_out", device),
+            0 if d_free_blocks is None else d_free_blocks.numel())
+        check(lib().lcpp_cache_evict_plan(args, _queue(stream, device)), "Plan")
 
     def Move(self, d_moves, d_move_counts, d_k_cache, d_v_cache, num_requests, d_scores=None, d_positions=None,
              stream=None):
         """Moves a layer's keys and values as a plan says (lcpp_cache_evict_move), and where given the scores and
         positions, which belong in one call only."""
-        torch = _torch()
-        cache = _kv_cache(d_k_cache, d_v_cache)
-        slots = cache.num_pages * cache.block_size
-        moves, moves_stride, max_moves = _moves(d_moves, num_requests, "d_moves")
+        torch, device, n = _torch(), _device(), num_requests
+        cache = _kv_cache(d_k_cache, d_v_cache, device)
+        slots = cache[5] * cache[6]
+        moves, moves_stride, max_moves = _moves(d_moves, n, "d_moves", device)
         check(lib().lcpp_cache_evict_move(
-            cache, moves, moves_stride, max_moves, _flat(d_move_counts, torch.int32, num_requests, "d_move_counts"), num_requests,
-            _flat(d_scores, torch.float32, slots, "d_scores"), _flat(d_positions, torch.int32, slots, "d_positions"),
-            _queue(stream)), "Move")
+            _pack_cache(*cache), moves, moves_stride, max_moves,
+            _array(d_move_counts, torch.int32, n, "d_move_counts", device), n,
+            _array(d_scores, torch.float32, slots, "d_scores", device),
+            _array(d_positions, torch.int32, slots, "d_positions", device), _queue(stream, device)), "Move")
