@@ -57,6 +57,180 @@ public:
     }
 };
 
+/// A tensor of heads: element (token, head, column) is ptr[token * token_stride
+/// + head * head_stride + column]; an empty one (no heads) is left out.
+template <typename Void>
+struct BasicHeadsView {
+    Void* ptr = nullptr;
+    uint64_t tokens = 0, token_stride = 0, head_stride = 0;
+    uint32_t heads = 0, dim = 0;
+    lcpp_dtype dtype = LCPP_NONE;
+
+    BasicHeadsView() = default;
+    BasicHeadsView(Void* p, uint64_t num_tokens, uint32_t num_heads, uint32_t head_dim, lcpp_dtype type,
+                   uint64_t stride_of_tokens = 0, uint64_t stride_of_heads = 0) noexcept
+        : ptr(p), tokens(num_tokens),
+          token_stride(stride_of_tokens ? stride_of_tokens : uint64_t(num_heads) * head_dim),
+          head_stride(stride_of_heads ? stride_of_heads : head_dim), heads(num_heads), dim(head_dim), dtype(type)
+    {
+    }
+    template <typename Other>
+    BasicHeadsView(const BasicHeadsView<Other>& o) noexcept
+        : ptr(o.ptr), tokens(o.tokens), token_stride(o.token_stride), head_stride(o.head_stride), heads(o.heads),
+          dim(o.dim), dtype(o.dtype)
+    {
+    }
+};
+using HeadsView = BasicHeadsView<void>;
+using ConstHeadsView = BasicHeadsView<const void>;
+
+/// How a call turns its tokens: positions and frequencies, pair layout, scale,
+/// and (empty: none) the tokens' requests with their position offsets.
+struct Rotation {
+    BufferView<const int32_t> positions;
+    BufferView<const double> frequencies;
+    lcpp_rotary_layout layout = LCPP_ROTARY_HALF;
+    float scale = 1.f;
+    BufferView<const int32_t> token_request, position_offset;
+};
+
+/// Rotary positions of queries and keys, with the gradient and the write of
+/// keys and values into a paged cache.
+class DeviceRotary {
+public:
+    /// rotary_dim / 2 frequencies to host memory (lcpp_rotary_frequencies).
+    static void Frequencies(double* frequencies_out, uint32_t rotary_dim, double base = 10000.0,
+                            lcpp_rotary_scaling scaling = LCPP_ROTARY_PLAIN, double factor = 1.0,
+                            double original_context = 0.0, double low = 1.0, double high = 4.0)
+    {
+        detail::check(lcpp_rotary_frequencies(frequencies_out, rotary_dim, base, scaling, factor, original_context, low,
+                                              high),
+                      "Frequencies");
+    }
+
+    /// lcpp_rotary_forward; an empty q or k is left out.
+    void Forward(lcpp_stream_t stream, ConstHeadsView q, ConstHeadsView k, HeadsView q_out, HeadsView k_out,
+                 const Rotation& rotation, uint64_t num_tokens)
+    {
+        const lcpp_rotary_args args = make(q, k, q_out, k_out, true, rotation, num_tokens);
+        detail::check(lcpp_rotary_forward(&args, stream), "Forward");
+    }
+
+    /// lcpp_rotary_backward: gradients of Forward's inputs from those of its outputs.
+    void Backward(lcpp_stream_t stream, ConstHeadsView grad_q, ConstHeadsView grad_k, HeadsView grad_q_out,
+                  HeadsView grad_k_out, const Rotation& rotation, uint64_t num_tokens)
+    {
+        const lcpp_rotary_args args = make(grad_q, grad_k, grad_q_out, grad_k_out, true, rotation, num_tokens);
+        detail::check(lcpp_rotary_backward(&args, stream), "Backward");
+    }
+
+    /// lcpp_rotary_append: keys and values go to their slots of the cache; empty
+    /// `slot_positions` and `slot_scores` views: not wanted.
+    void Append(lcpp_stream_t stream, ConstHeadsView q, ConstHeadsView k, ConstHeadsView v, HeadsView q_out,
+                const lcpp_kv_cache& cache, BufferView<const int64_t> slots, const Rotation& rotation,
+                uint64_t num_tokens, BufferView<int32_t> slot_positions = {}, BufferView<float> slot_scores = {})
+    {
+        const lcpp_rotary_args args = make(q, k, q_out, {}, false, rotation, num_tokens);
+        const uint64_t all = uint64_t(cache.num_pages) * cache.block_size;
+        detail::require(v.tokens >= num_tokens && v.heads == k.heads && v.dim == k.dim && v.dtype == k.dtype &&
+                            slots.size() >= num_tokens && (!slot_positions.data() || slot_positions.size() >= all) &&
+                            (!slot_scores.data() || slot_scores.size() >= all),
+                        "Append: a view is too short, or of another shape");
+        lcpp_cache_append_args append{};
+        append.cache = cache;
+        append.v = v.ptr;
+        append.v_token_stride = v.token_stride;
+        append.v_head_stride = v.head_stride;
+        append.slots = slots.data();
+        append.slot_positions = slot_positions.data();
+        append.slot_scores = slot_scores.data();
+        detail::check(lcpp_rotary_append(&args, &append, stream), "Append");
+    }
+
+private:
+    static lcpp_head_rows rows(ConstHeadsView in, HeadsView out)
+    {
+        return {in.ptr, out.ptr, in.token_stride, in.head_stride, out.token_stride, out.head_stride, in.heads};
+    }
+    static lcpp_rotary_args make(ConstHeadsView q, ConstHeadsView k, HeadsView q_out, HeadsView k_out, bool both,
+                                 const Rotation& rotation, uint64_t num_tokens)
+    {
+        const ConstHeadsView& some = q.heads ? q : k;
+        const auto fits = [&](const ConstHeadsView& x) {
+            return !x.heads || (x.tokens >= num_tokens && x.dim == some.dim && x.dtype == some.dtype);
+        };
+        const auto takes = [&](const ConstHeadsView& x, const HeadsView& out) {
+            return !x.heads || (out.tokens >= num_tokens && out.heads == x.heads && out.dim == x.dim && out.dtype == x.dtype);
+        };
+        detail::require(fits(q) && fits(k) && takes(q, q_out) && (!both || takes(k, k_out)) &&
+                            rotation.positions.size() >= num_tokens &&
+                            (!rotation.token_request.data() || rotation.token_request.size() >= num_tokens),
+                        "DeviceRotary: a view is too short, or of another shape");
+        lcpp_rotary_args args{};
+        args.q = rows(q, q_out);
+        args.k = rows(k, k_out);
+        args.positions = rotation.positions.data();
+        args.token_request = rotation.token_request.data();
+        args.position_offset = rotation.position_offset.data();
+        args.frequencies = rotation.frequencies.data();
+        args.num_tokens = num_tokens;
+        args.num_requests = rotation.position_offset.data() ? uint32_t(rotation.position_offset.size()) : 0x7fffffffu;
+        args.head_dim = some.dim;
+        args.rotary_dim = uint32_t(2 * rotation.frequencies.size());
+        args.layout = rotation.layout;
+        args.scale = rotation.scale;
+        args.dtype = some.dtype;
+        return args;
+    }
+};
+
+/// Attention of one new token of each request over a paged cache.
+class DevicePagedAttention {
+public:
+    /// score_slots: num_pages * block_size when scores are wanted.
+    static size_t GetTempStorageBytes(uint32_t num_requests, uint32_t num_heads, uint32_t num_kv_heads,
+                                      uint32_t head_dim, uint64_t score_slots = 0)
+    {
+        size_t b = 0;
+        detail::check(lcpp_paged_attention_temp_bytes(num_requests, num_heads, num_kv_heads, head_dim, score_slots, &b),
+                      "GetTempStorageBytes");
+        return b;
+    }
+
+    /// lcpp_paged_attention_decode.
+    void Decode(lcpp_stream_t stream, BufferView<uint32_t> temp_storage, const lcpp_paged_attention_args& args)
+    {
+        detail::check(lcpp_paged_attention_decode(temp_storage.data(), detail::temp_bytes(temp_storage), &args, stream),
+                      "Decode");
+    }
+};
+
+/// Requests of a paged cache cut down to their heaviest tokens.
+class DeviceCacheEviction {
+public:
+    /// lcpp_cache_evict_plan: which tokens stay, and the pages that come back.
+    void Plan(lcpp_stream_t stream, const lcpp_cache_evict_args& args)
+    {
+        detail::check(lcpp_cache_evict_plan(&args, stream), "Plan");
+    }
+
+    /// lcpp_cache_evict_move: a layer's keys and values; empty `slot_scores` and
+    /// `slot_positions` views: not moved.
+    void Move(lcpp_stream_t stream, const lcpp_kv_cache& cache, BufferView<const int64_t> moves, uint64_t moves_stride,
+              uint32_t max_moves, BufferView<const int32_t> move_counts, uint32_t num_requests,
+              BufferView<float> slot_scores = {}, BufferView<int32_t> slot_positions = {})
+    {
+        const uint64_t all = uint64_t(cache.num_pages) * cache.block_size;
+        detail::require((!num_requests || moves.size() >= 2 * ((num_requests - 1) * moves_stride + max_moves)) &&
+                            move_counts.size() >= num_requests && (!slot_scores.data() || slot_scores.size() >= all) &&
+                            (!slot_positions.data() || slot_positions.size() >= all),
+                        "Move: a view is too short");
+        detail::check(lcpp_cache_evict_move(&cache, moves.data(), moves_stride, max_moves, move_counts.data(),
+                                            num_requests, slot_scores.data(), slot_positions.data(), stream),
+                      "Move");
+    }
+};
+
 /// Experts of each token, their weights, per-expert counts and the balance
 /// loss, with the gradient.
 class DeviceRouter {
