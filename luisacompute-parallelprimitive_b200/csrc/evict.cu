@@ -394,7 +394,9 @@ struct Moves {
     unsigned char* v;
     uint64_t page, token, head;  // strides in bytes
     Divider vectors;             // accesses of a head
-    uint32_t heads, block_size;
+    Divider block;               // slots of a page
+    bool small;                  // slots are counted in 31 bits
+    uint32_t heads;
     uint64_t num_slots;
     const longlong2* moves;
     uint64_t moves_stride;
@@ -404,10 +406,13 @@ struct Moves {
     int32_t* positions;
 };
 
-// A warp takes a move: all heads' keys and values of a token, V at a time, four
-// of them (or a head's last ones) under way in each lane.
+// Accesses are V bytes of a key and of a value, four of each under way in a thread.
+// kByWarp: a warp takes a move.  Else threads take all accesses in their order,
+// moves that have few for a warp side by side (256 bytes a token, 225 x 732 moves:
+// 61 us by warps, 29 us in order; 2048 bytes, 16 x 7600 moves: 151 and 202 us, for
+// every access finds its move anew).
 constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / kWarp, kMoveAhead = 4;
-template <typename V>
+template <typename V, bool kByWarp>
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Moves p)
 {
     const auto moves_of = [&](uint32_t r) { return (long long)min(uint32_t(max(p.counts[r], 0)), p.max_moves); };
@@ -423,41 +428,84 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Moves p)
         },
         place);
     if (begin >= total) return;
-    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     const uint32_t each = p.heads * p.vectors.d;
+    // the place of a slot
+    const auto place_of = [&](uint64_t slot) {
+        const uint64_t page = p.small ? p.block.quotient(uint32_t(slot)) : slot / p.block.d;
+        return page * p.page + (slot - page * p.block.d) * p.token;
+    };
     uint32_t r = place.item;
-    long long first = place.first;
-    for (long long i = begin + warp; i < end; i += kMoveWarps) {
-        while (i >= first + moves_of(r)) first += moves_of(r++);
-        const longlong2 move = p.moves[r * p.moves_stride + uint64_t(i - first)];
-        const uint64_t from = uint64_t(move.x), to = uint64_t(move.y);
-        if (from >= p.num_slots || to >= p.num_slots) continue;
-        const uint64_t from_page = from / p.block_size, to_page = to / p.block_size;
-        const uint64_t from_at = from_page * p.page + (from - from_page * p.block_size) * p.token;
-        const uint64_t to_at = to_page * p.page + (to - to_page * p.block_size) * p.token;
-        for (uint32_t at = lane; at < each; at += kWarp * kMoveAhead) {
-            V k[kMoveAhead], v[kMoveAhead];
-            uint64_t offset[kMoveAhead];
+    if (kByWarp) {
+        const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+        long long first = place.first;
+        for (long long i = begin + warp; i < end; i += kMoveWarps) {
+            while (i >= first + moves_of(r)) first += moves_of(r++);
+            const longlong2 move = p.moves[r * p.moves_stride + uint64_t(i - first)];
+            if (uint64_t(move.x) >= p.num_slots || uint64_t(move.y) >= p.num_slots) continue;
+            const uint64_t from = place_of(uint64_t(move.x)), to = place_of(uint64_t(move.y));
+            for (uint32_t at = lane; at < each; at += kWarp * kMoveAhead) {
+                V k[kMoveAhead], v[kMoveAhead];
+                uint64_t offset[kMoveAhead];
 #pragma unroll
-            for (int u = 0; u < kMoveAhead; ++u) {
-                const uint32_t x = at + u * kWarp;
-                if (x >= each) continue;
-                const uint32_t head = p.vectors.quotient(x);
-                offset[u] = head * p.head + (x - head * p.vectors.d) * sizeof(V);
-                k[u] = *reinterpret_cast<const V*>(p.k + from_at + offset[u]);
-                v[u] = *reinterpret_cast<const V*>(p.v + from_at + offset[u]);
+                for (int u = 0; u < kMoveAhead; ++u) {
+                    const uint32_t x = at + u * kWarp;
+                    if (x >= each) continue;
+                    const uint32_t head = p.vectors.quotient(x);
+                    offset[u] = head * p.head + (x - head * p.vectors.d) * sizeof(V);
+                    k[u] = *reinterpret_cast<const V*>(p.k + from + offset[u]);
+                    v[u] = *reinterpret_cast<const V*>(p.v + from + offset[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < kMoveAhead; ++u) {
+                    if (at + u * kWarp >= each) continue;
+                    *reinterpret_cast<V*>(p.k + to + offset[u]) = k[u];
+                    *reinterpret_cast<V*>(p.v + to + offset[u]) = v[u];
+                }
             }
-#pragma unroll
-            for (int u = 0; u < kMoveAhead; ++u) {
-                if (at + u * kWarp >= each) continue;
-                *reinterpret_cast<V*>(p.k + to_at + offset[u]) = k[u];
-                *reinterpret_cast<V*>(p.v + to_at + offset[u]) = v[u];
+            if (lane == 0) {
+                if (p.scores) p.scores[move.y] = p.scores[move.x];
+                if (p.positions) p.positions[move.y] = p.positions[move.x];
             }
         }
-        if (lane == 0) {
-            if (p.scores) p.scores[to] = p.scores[from];
-            if (p.positions) p.positions[to] = p.positions[from];
+        return;
+    }
+    long long first = place.first, i = begin;  // the access's move, and the first one of its request
+    uint32_t at = threadIdx.x;                 // the access in its move
+    while (true) {
+        V k[kMoveAhead], v[kMoveAhead];
+        uint64_t to[kMoveAhead];
+#pragma unroll
+        for (int u = 0; u < kMoveAhead; ++u) {
+            to[u] = ~0ull;
+            while (at >= each) {
+                at -= each;
+                ++i;
+            }
+            if (i < end) {
+                while (i >= first + moves_of(r)) first += moves_of(r++);
+                const longlong2 move = p.moves[r * p.moves_stride + uint64_t(i - first)];
+                if (uint64_t(move.x) < p.num_slots && uint64_t(move.y) < p.num_slots) {
+                    const uint32_t head = p.vectors.quotient(at);
+                    const uint64_t offset = head * p.head + (at - head * p.vectors.d) * sizeof(V);
+                    const uint64_t from = place_of(uint64_t(move.x)) + offset;
+                    to[u] = place_of(uint64_t(move.y)) + offset;
+                    k[u] = *reinterpret_cast<const V*>(p.k + from);
+                    v[u] = *reinterpret_cast<const V*>(p.v + from);
+                    if (at == 0) {
+                        if (p.scores) p.scores[move.y] = p.scores[move.x];
+                        if (p.positions) p.positions[move.y] = p.positions[move.x];
+                    }
+                }
+            }
+            at += kMoveThreads;
         }
+#pragma unroll
+        for (int u = 0; u < kMoveAhead; ++u) {
+            if (to[u] == ~0ull) continue;
+            *reinterpret_cast<V*>(p.k + to[u]) = k[u];
+            *reinterpret_cast<V*>(p.v + to[u]) = v[u];
+        }
+        if (i >= end) return;
     }
 }
 
@@ -588,7 +636,8 @@ lcpp_status move(const lcpp_kv_cache* c, const int64_t* moves, uint64_t moves_st
     p.head = c->head_stride * e;
     p.vectors = Divider(c->head_dim * e / access);
     p.heads = c->num_kv_heads;
-    p.block_size = c->block_size;
+    p.block = Divider(c->block_size);
+    p.small = slots < uint64_t(1) << 31;
     p.num_slots = slots;
     p.moves = reinterpret_cast<const longlong2*>(moves);
     p.moves_stride = moves_stride;
@@ -599,12 +648,15 @@ lcpp_status move(const lcpp_kv_cache* c, const int64_t* moves, uint64_t moves_st
     p.positions = positions;
     const auto launch = [&](auto kernel) {
         const uint64_t most = uint64_t(device_sm_count()) * resident_blocks(reinterpret_cast<const void*>(kernel), kMoveThreads, 0);
-        const unsigned blocks = unsigned(std::min<uint64_t>(most, ceil_div(n * max_moves, kMoveWarps)));
+        const uint64_t accesses = std::min<uint64_t>(n * max_moves, uint64_t(1) << 32) * (p.heads * p.vectors.d);
+        const unsigned blocks = unsigned(std::min<uint64_t>(most, ceil_div(accesses, kMoveThreads)));
         kernel<<<blocks, kMoveThreads, 0, s>>>(p);
         return launched();
     };
     diag::KernelTimer timer(kTimerEviction, n, s);
-    return wide ? launch(move_kernel<uint4>) : e == 4 ? launch(move_kernel<uint32_t>) : launch(move_kernel<unsigned short>);
+    if (p.heads * p.vectors.d >= 2 * kWarp)
+        return wide ? launch(move_kernel<uint4, true>) : e == 4 ? launch(move_kernel<uint32_t, true>) : launch(move_kernel<unsigned short, true>);
+    return wide ? launch(move_kernel<uint4, false>) : e == 4 ? launch(move_kernel<uint32_t, false>) : launch(move_kernel<unsigned short, false>);
 }
 
 }  // namespace

@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(kScoreThreads) scores_kernel(const Params p)
     const long long total = share_of<kScoreThreads>(
         p.requests, weight,
         [&](long long all) {
-            const long long per = run_of(all, gridDim.x, kScoreWarps);
+            const long long per = max((all + gridDim.x - 1) / gridDim.x, (long long)kScoreWarps);
             begin = blockIdx.x * per;
             end = min(all, begin + per);
             return begin < all ? begin : -1;

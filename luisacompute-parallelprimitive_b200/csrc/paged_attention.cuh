@@ -81,10 +81,12 @@ __device__ __forceinline__ Tokens tokens_of_length(const Params& p, int32_t leng
 }
 __device__ __forceinline__ Tokens tokens_of(const Params& p, uint32_t r) { return tokens_of_length(p, p.lens[r]); }
 
-// Tiles of a block's run: equal ones, of not less than a tile for each warp.
-__device__ __forceinline__ long long run_of(long long all, uint32_t blocks, int warps)
+// Tiles of a block's run: equal ones, of not less than a tile for each warp unless
+// units have fewer (a part's end costs a block a microsecond or two).
+__device__ __forceinline__ long long run_of(long long all, uint64_t units, uint32_t blocks, int warps)
 {
-    return max((all + blocks - 1) / blocks, (long long)warps);
+    const long long equal = (all + blocks - 1) / blocks;
+    return equal >= warps ? equal : max(equal, min((long long)warps, (all + (long long)units - 1) / (long long)units));
 }
 
 // The block's run of tiles, and the walk over the parts of units in it.
@@ -653,7 +655,7 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
     const long long total = share_of<kThreads>(
         p.requests, [&](uint32_t r) { return (long long)(tokens_of(p, r).tiles()) * units; },
         [&](long long all) {
-            const long long per = run_of(all, gridDim.x, kWarps);
+            const long long per = run_of(all, uint64_t(units) * p.requests, gridDim.x, kWarps);
             begin = blockIdx.x * per;
             end = min(all, begin + per);
             return begin < all ? begin : -1;
@@ -914,7 +916,7 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
         if (threadIdx.x == 0) {
             if (p.first && now.unit == 0 && now.t == 0) p.first[now.r] = first_tile;
             if (!again) {
-                const long long per = run_of(total, gridDim.x, kWarps), unit_begin = first_tile - now.t;
+                const long long per = run_of(total, uint64_t(units) * p.requests, gridDim.x, kWarps), unit_begin = first_tile - now.t;
                 const int32_t from = int32_t(unit_begin / per), to = int32_t((unit_begin + now.tiles - 1) / per);
                 *split = make_int4(int32_t(now.r), int32_t(now.unit), from, now.t_end < now.tiles ? to - from : 0);
             }

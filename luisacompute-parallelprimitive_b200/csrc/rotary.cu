@@ -119,8 +119,9 @@ __device__ __forceinline__ void turn_pair(float2 cs, float& a, float& b)
     b = fmaf(y, cs.x, __fmul_rn(x, cs.y));
 }
 
-template <typename T, int N, bool kHalf, bool kAppend>
-__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const Params p)
+// kValues: elements of an access to values that are copied.
+template <typename T, int N, bool kHalf, bool kAppend, int kValues>
+__global__ void __launch_bounds__(kThreads, kHalf && kAppend ? 3 : 4) rotary_kernel(const Params p)
 {
     // kHalf: vectors of N pairs (i, i + half) in two places; else of N / 2 adjacent
     // pairs, or for N = 1 of one pair as two elements
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const Params p)
         }
         // The first vectors of q, or of k, are loaded before the angles are worked out.
         bool ready = false;
-        const auto section = [&](const Section& c, uint64_t to, bool turns) {
+        const auto section = [&](const Section& c, uint64_t to) {
             const uint32_t head = start / c.per_head;
             uint32_t j = start - head * c.per_head;
             const T* in = static_cast<const T*>(c.in) + t * c.in_token + head * c.in_head + j * N;
@@ -172,10 +173,10 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const Params p)
                 for (int u = 0; u < kAhead; ++u) {
                     at[u] = nullptr;
                     angle[u] = -1;
-                    const bool turned = turns && j < p.turned;
+                    const bool turned = j < p.turned;
                     if (v < c.vectors && (turned || c.copied)) {
                         // from a vector's number to its column: past the turned ones for those that are copied
-                        const int64_t more = !turns ? 0 : kHalf ? (turned ? 0 : p.half) : N > 1 ? 0 : turned ? j : p.half;
+                        const int64_t more = kHalf ? (turned ? 0 : p.half) : N > 1 ? 0 : turned ? j : p.half;
                         at[u] = out + more;
                         load(a[u], in + more);
                         if (turned) {
@@ -242,9 +243,39 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const Params p)
                 }
             }
         };
-        section(p.s[0], t * p.s[0].out_token, true);
-        section(p.s[1], kAppend ? uint64_t(place) : t * p.s[1].out_token, true);
-        if (kAppend) section(p.s[2], uint64_t(place), false);
+        section(p.s[0], t * p.s[0].out_token);
+        section(p.s[1], kAppend ? uint64_t(place) : t * p.s[1].out_token);
+        if (kAppend) {
+            const Section& c = p.s[2];
+            const uint32_t head = start / c.per_head, j = start - head * c.per_head;
+            const T* in = static_cast<const T*>(c.in) + t * c.in_token + head * c.in_head + j * kValues;
+            T* out = static_cast<T*>(c.out) + uint64_t(place) + head * c.out_head + j * kValues;
+            uint32_t v = start, at = j;
+            while (v < c.vectors) {
+                Pack<T, kValues> x[2];
+                T* to[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    to[u] = nullptr;
+                    if (v < c.vectors) {
+                        to[u] = out;
+                        load(x[u], in);
+                    }
+                    v += p.team * kWarp;
+                    in += c.in_step;
+                    out += c.out_step;
+                    at += c.step;
+                    if (at >= c.per_head) {
+                        at -= c.per_head;
+                        in += c.in_wrap;
+                        out += c.out_wrap;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (to[u]) store(to[u], x[u]);
+            }
+        }
         __syncwarp();  // the table is free
     }
 }
@@ -260,9 +291,11 @@ Strided rows_out(const lcpp_head_rows& r, uint64_t tokens, uint32_t dim, int e)
 Strided flat(const void* p, uint64_t n, int e) { return Strided(p, e, n, {}); }
 
 template <typename T, int N, bool kHalf>
-lcpp_status launch(const Params& p, bool append, cudaStream_t s)
+lcpp_status launch(const Params& p, bool append, bool wide_values, cudaStream_t s)
 {
-    auto kernel = append ? rotary_kernel<T, N, kHalf, true> : rotary_kernel<T, N, kHalf, false>;
+    constexpr int kWide = 16 / int(sizeof(T));
+    auto kernel = !append ? rotary_kernel<T, N, kHalf, false, N>
+                  : wide_values ? rotary_kernel<T, N, kHalf, true, kWide> : rotary_kernel<T, N, kHalf, true, N>;
     const size_t smem = size_t(kWarps) * align_up(p.half, 2) * sizeof(float2);
     // as for the longest tables, so that few launch shapes are looked up and kept
     const size_t room = size_t(kWarps) * (LCPP_MAX_HEAD_DIM / 2) * sizeof(float2);
@@ -273,15 +306,16 @@ lcpp_status launch(const Params& p, bool append, cudaStream_t s)
 }
 
 template <typename T, int N>
-lcpp_status launch(Params& p, const lcpp_rotary_args& a, bool append, cudaStream_t s)
+lcpp_status launch(Params& p, const lcpp_rotary_args& a, bool append, bool wide_values, cudaStream_t s)
 {
     const bool half = a.layout == LCPP_ROTARY_HALF;
     p.turned = (half ? p.half : 2 * p.half) / (half ? N : (N == 1 ? 2 : N));
     const uint32_t heads[3] = {a.q.num_heads, a.k.num_heads, append ? a.k.num_heads : 0};
-    // a head's vectors: of pairs, then of columns
+    // a head's vectors: of pairs, then of columns; of values as wide as those allow by themselves
+    const uint32_t in_value = wide_values ? 16 / sizeof(T) : N;
     const uint32_t per_head = p.turned + (a.head_dim - a.rotary_dim) / N;
     for (int i = 0; i < 3; ++i) {
-        p.s[i].per_head = i < 2 ? per_head : a.head_dim / N;
+        p.s[i].per_head = i < 2 ? per_head : a.head_dim / in_value;
         p.s[i].vectors = heads[i] * p.s[i].per_head;
     }
     // warps to a token until every SM has 32, but no more than have work for each lane
@@ -290,15 +324,15 @@ lcpp_status launch(Params& p, const lcpp_rotary_args& a, bool append, cudaStream
            p.s[0].vectors + p.s[1].vectors > p.team * kWarp)
         p.team *= 2;
     for (Section& c : p.s) {
-        const uint32_t step = p.team * kWarp;
+        const uint32_t step = p.team * kWarp, columns = &c == &p.s[2] ? in_value : N;
         c.step = step % c.per_head;
         const int64_t over = step / c.per_head;
-        c.in_step = over * int64_t(c.in_head) + int64_t(c.step) * N;
-        c.out_step = over * int64_t(c.out_head) + int64_t(c.step) * N;
-        c.in_wrap = int64_t(c.in_head) - int64_t(c.per_head) * N;
-        c.out_wrap = int64_t(c.out_head) - int64_t(c.per_head) * N;
+        c.in_step = over * int64_t(c.in_head) + int64_t(c.step) * columns;
+        c.out_step = over * int64_t(c.out_head) + int64_t(c.step) * columns;
+        c.in_wrap = int64_t(c.in_head) - int64_t(c.per_head) * columns;
+        c.out_wrap = int64_t(c.out_head) - int64_t(c.per_head) * columns;
     }
-    return half ? launch<T, N, true>(p, append, s) : launch<T, N, false>(p, append, s);
+    return half ? launch<T, N, true>(p, append, wide_values, s) : launch<T, N, false>(p, append, wide_values, s);
 }
 
 lcpp_status run(const lcpp_rotary_args* a, const lcpp_cache_append_args* c, float sign, cudaStream_t s)
@@ -428,7 +462,11 @@ lcpp_status run(const lcpp_rotary_args* a, const lcpp_cache_append_args* c, floa
                                        !rows_aligned(x.out, {x.out_token, x.out_head}, e, bytes)))
                 return false;
         }
-        return !c || (rows_aligned(p.s[2].in, {p.s[2].in_token, p.s[2].in_head}, e, bytes) &&
+        return true;
+    };
+    const auto values_fit = [&](int count) {
+        const size_t bytes = size_t(count) * e;
+        return !c || (a->head_dim % count == 0 && rows_aligned(p.s[2].in, {p.s[2].in_token, p.s[2].in_head}, e, bytes) &&
                       rows_aligned(p.s[2].out, {p.s[2].out_token, p.s[2].out_head}, e, bytes) &&
                       rows_aligned(nullptr, {p.page_stride}, e, bytes));
     };
@@ -436,10 +474,11 @@ lcpp_status run(const lcpp_rotary_args* a, const lcpp_cache_append_args* c, floa
     return with_row_type(a->dtype, [&](auto type) {
         using T = decltype(type);
         constexpr int kMost = 16 / int(sizeof(T));
-        if (kMost == 8 && fits(8)) return launch<T, kMost>(p, *a, c, s);
-        if (fits(4)) return launch<T, 4>(p, *a, c, s);
-        if (fits(2)) return launch<T, 2>(p, *a, c, s);
-        return launch<T, 1>(p, *a, c, s);
+        const bool wide = c && values_fit(kMost);
+        if (kMost == 8 && fits(8) && values_fit(8)) return launch<T, kMost>(p, *a, c, wide, s);
+        if (fits(4) && values_fit(4)) return launch<T, 4>(p, *a, c, wide, s);
+        if (fits(2) && values_fit(2)) return launch<T, 2>(p, *a, c, wide, s);
+        return launch<T, 1>(p, *a, c, wide, s);
     });
 }
 
