@@ -123,9 +123,16 @@ struct Walk {
 };
 
 __device__ __forceinline__ uint32_t smem_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+// L2 is asked for 64 bytes of a line: rows that begin in the middle of one would
+// bring in their neighbours' halves, which other blocks read at other times
+// (301 x 1500 tokens of 7 x 80 bfloat16 columns: 150 us with whole lines, 130).
 __device__ __forceinline__ void copy_16b(uint32_t to, const void* from, bool valid)
 {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::64B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_16b(uint32_t to, const void* from)
+{
+    asm volatile("cp.async.cg.shared.global.L2::64B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy_4b(uint32_t to, const void* from)
 {
@@ -205,9 +212,59 @@ __device__ __forceinline__ void multiply<__half>(float (&c)[4], const uint32_t (
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Swizzle of a row's 16-byte chunks: 8 rows of one chunk, or 8 chunks of one row,
-// lie in different banks.
-__device__ __forceinline__ int swizzled(int row, int chunk) { return chunk ^ (row & 7); }
+template <typename T>
+__device__ __forceinline__ void multiply_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void multiply_first<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+template <>
+__device__ __forceinline__ void multiply_first<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Two floats as 16-bit numbers in a word, and what their rounding left out in another.
+template <typename T>
+__device__ __forceinline__ void split_pair(float low, float high, uint32_t& word, uint32_t& rest);
+template <>
+__device__ __forceinline__ void split_pair<__nv_bfloat16>(float low, float high, uint32_t& word, uint32_t& rest)
+{
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(word) : "f"(high), "f"(low));
+    low -= __uint_as_float(word << 16);
+    high -= __uint_as_float(word & 0xffff0000u);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(rest) : "f"(high), "f"(low));
+}
+template <>
+__device__ __forceinline__ void split_pair<__half>(float low, float high, uint32_t& word, uint32_t& rest)
+{
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(word) : "f"(high), "f"(low));
+    low -= __half2float(__ushort_as_half(static_cast<unsigned short>(word)));
+    high -= __half2float(__ushort_as_half(static_cast<unsigned short>(word >> 16)));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(rest) : "f"(high), "f"(low));
+}
+
+// Swizzle of the 16-byte chunks of rows of CHUNKS: 8 rows of one chunk, or 8 chunks
+// of one row, lie in different banks.  Rows of an odd number of 64 bytes alternate
+// between the banks' halves by themselves.
+template <int CHUNKS>
+__device__ __forceinline__ int swizzled(int row, int chunk)
+{
+    static_assert(CHUNKS % 4 == 0, "");
+    return CHUNKS % 8 ? chunk ^ (row >> 1 & 3) : chunk ^ (row & 7);
+}
+// The address `even` chunks on from a swizzled one of chunk 0 or 1: an exclusive or,
+// and a constant.
+template <int CHUNKS>
+__device__ __forceinline__ uint32_t chunks_on(uint32_t address, int even)
+{
+    constexpr int kLow = CHUNKS % 8 ? 3 : 7;
+    return (address ^ ((even & kLow) * 16)) + (even & ~kLow) * 16;
+}
 
 template <typename T, int D, int H>
 struct Tile;
@@ -250,44 +307,63 @@ struct Tile16 {
         constexpr int kChains = kN == 1 ? 4 : 2;
         const int lane = threadIdx.x % kWarp;
         float c[kChains][kN][4];
-#pragma unroll
-        for (int i = 0; i < kChains; ++i)
-#pragma unroll
-            for (int n = 0; n < kN; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) c[i][n][j] = 0.f;
         const int row = lane % 16, head = lane % 8;
-        const uint32_t at = smem_address(rows) + row * (D * 2), q = smem_address(queries) + head * (D * 2);
+        const uint32_t at = smem_address(rows) + row * (D * 2) + swizzled<D / 8>(row, lane / 16) * 16;
+        // lane / 8 is a chunk of four: two pairs of even ones
+        const uint32_t q = smem_address(queries) + head * (D * 2) + chunks_on<D / 8>(swizzled<D / 8>(head, lane / 8 % 2) * 16, lane / 16 * 2);
 #pragma unroll
         for (int step = 0; step < D / 16; step += 2) {
             uint32_t a[2][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) load_matrices(a[i], at + swizzled(row, (step + i) * 2 + lane / 16) * 16);
+            for (int i = 0; i < 2; ++i) load_matrices(a[i], chunks_on<D / 8>(at, (step + i) * 2));
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
                 uint32_t b[4];  // the heads' next 32 columns
-                load_matrices(b, q + n * 8 * (D * 2) + swizzled(head, step * 2 + lane / 8) * 16);
-                multiply<T>(c[step % kChains][n], a[0], b[0], b[1]);
-                multiply<T>(c[(step + 1) % kChains][n], a[1], b[2], b[3]);
+                load_matrices(b, chunks_on<D / 8>(q, step * 2) + n * 8 * (D * 2));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (step + i < kChains) multiply_first<T>(c[(step + i) % kChains][n], a[i], b[2 * i], b[2 * i + 1]);
+                    else multiply<T>(c[(step + i) % kChains][n], a[i], b[2 * i], b[2 * i + 1]);
+                }
             }
         }
-        const bool valid0 = valid >> (lane / 4) & 1, valid1 = valid >> (lane / 4 + 8) & 1;
-        bool past = false;
         float s[kN][4];
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float dot = c[0][n][j] + c[1][n][j];
                 if (kChains == 4) dot += c[kChains - 2][n][j] + c[kChains - 1][n][j];
-                s[n][j] = (j < 2 ? valid0 : valid1) ? logit(p, dot) : -INFINITY;
-                past |= s[n][j] > m[n][j & 1] + (8.f + kShift);
-                if (logits) {
-                    const uint32_t head = n * 8 + lane % 4 * 2 + (j & 1);
-                    if (head < heads) logits[head * kTile + lane / 4 + (j < 2 ? 0 : 8)] = s[n][j];
-                }
+                s[n][j] = dot * p.scale;
             }
+        if (p.softcap > 0.f) {
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[n][j] = p.softcap * tanhf(s[n][j]);
         }
+        if (valid != 0xffffu) {
+            const bool valid0 = valid >> (lane / 4) & 1, valid1 = valid >> (lane / 4 + 8) & 1;
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!(j < 2 ? valid0 : valid1)) s[n][j] = -INFINITY;
+        }
+        if (logits) {
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t of = n * 8 + lane % 4 * 2 + (j & 1);
+                    if (of < heads) logits[of * kTile + lane / 4 + (j < 2 ? 0 : 8)] = s[n][j];
+                }
+        }
+        bool past = false;
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) past |= s[n][j] > m[n][j & 1] + (8.f + kShift);
         if (__any_sync(~0u, past)) {
 #pragma unroll
             for (int n = 0; n < kN; ++n)
@@ -308,25 +384,18 @@ struct Tile16 {
         }
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
+            const float reference[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
             float e[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float reference = m[n][j & 1] == -INFINITY ? 0.f : m[n][j & 1];
-                e[j] = exp2_fast(s[n][j] - reference);
-                l[n][j & 1] += e[j];
-            }
+            for (int j = 0; j < 4; ++j) e[j] = exp2_fast(s[n][j] - reference[j & 1]);
+            l[n][0] += e[0] + e[2];
+            l[n][1] += e[1] + e[3];
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                T hi[2], lo[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    hi[h] = from_float<T>(e[w * 2 + h]);
-                    lo[h] = from_float<T>(e[w * 2 + h] - to_float(hi[h]));
-                }
-                high[n][w] = transposed(*reinterpret_cast<const uint16_t*>(&hi[0]) |
-                                        uint32_t(*reinterpret_cast<const uint16_t*>(&hi[1])) << 16);
-                rest[n][w] = transposed(*reinterpret_cast<const uint16_t*>(&lo[0]) |
-                                        uint32_t(*reinterpret_cast<const uint16_t*>(&lo[1])) << 16);
+                uint32_t word, left;
+                split_pair<T>(e[w * 2], e[w * 2 + 1], word, left);
+                high[n][w] = transposed(word);
+                rest[n][w] = transposed(left);
             }
         }
     }
@@ -334,11 +403,11 @@ struct Tile16 {
     __device__ __forceinline__ void values(const unsigned char* rows, const void*)
     {
         const int lane = threadIdx.x % kWarp, row = lane % 8 + lane / 16 * 8;
-        const uint32_t at = smem_address(rows) + row * (D * 2);
+        const uint32_t at = smem_address(rows) + row * (D * 2) + swizzled<D / 8>(row, lane / 8 % 2) * 16;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             uint32_t a[4];
-            load_matrices_transposed(a, at + swizzled(row, i * 2 + lane / 8 % 2) * 16);
+            load_matrices_transposed(a, chunks_on<D / 8>(at, i * 2));
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
                 multiply<T>(o[i][n], a, high[n][0], high[n][1]);
@@ -448,10 +517,10 @@ struct Tile<float, D, H> {
 #pragma unroll 4
         for (int i = 0; i < half; ++i) {
             const int chunk = part * half + i;
-            const float4 a = k[swizzled(token, chunk)];
+            const float4 a = k[swizzled<kChunks>(token, chunk)];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                const float4 b = q[h * kChunks + swizzled(h, chunk)];
+                const float4 b = q[h * kChunks + swizzled<kChunks>(h, chunk)];
                 s[h] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s[h]))));
             }
         }
@@ -499,11 +568,17 @@ struct Tile<float, D, H> {
 #pragma unroll 4
         for (int t = lane / kLanes; t < kTile; t += kTokenStep) {
             float e[H];
+            if constexpr (H % 4 == 0) {
 #pragma unroll
-            for (int h = 0; h < H; ++h) e[h] = term[t * H + h];
+                for (int h = 0; h < H; h += 4)
+                    *reinterpret_cast<float4*>(e + h) = *reinterpret_cast<const float4*>(term + t * H + h);
+            } else {
+#pragma unroll
+                for (int h = 0; h < H; ++h) e[h] = term[t * H + h];
+            }
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                const float4 x = v[t * kChunks + swizzled(t, column + i * kLanes)];
+                const float4 x = v[t * kChunks + swizzled<kChunks>(t, column + i * kLanes)];
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     o[h][i].x = fmaf(e[h], x.x, o[h][i].x);
@@ -565,7 +640,7 @@ struct Tile<float, D, H> {
 
 // A tile that a warp will copy: what its rows' places are worked out from.
 struct alignas(16) Note {
-    uint64_t head;   // the kv head's offset
+    uint64_t head;   // the kv head's offset, with that of the tile in its page where it lies in one
     uint32_t token;  // the first one
     uint32_t mask;   // rows of the request and its window
 };
@@ -686,7 +761,7 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
         unsigned char* to = smem + R::kQueries + buffer * R::kQueryBytes;
         for (int at = threadIdx.x; at < H * kChunks; at += kThreads) {
             const uint32_t head = at / kChunks, chunk = at % kChunks, column = chunk * kIn;
-            unsigned char* into = to + head * kRowBytes + swizzled(head, chunk) * 16;
+            unsigned char* into = to + head * kRowBytes + swizzled<kChunks>(head, chunk) * 16;
             const bool live = head < heads && column < p.dim;
             const T* from = live ? q + head * p.q_head + column : q;
             if (p.wide_q) {
@@ -727,6 +802,7 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
         if (lane == 0) {
             Note& n = *reinterpret_cast<Note*>(at);
             n.head = uint64_t(ahead.unit / p.chunks) * p.head_stride;
+            if (p.page_tiles) n.head += (token - p.page.quotient(token) * p.page.d) * p.token_stride;
             n.token = token;
             n.mask = (0xffffu << skip) & (0xffffu >> (kTile - min(ahead.tokens.end - token, uint32_t(kTile))));
         }
@@ -749,17 +825,20 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
             const uint32_t address = smem_address(to);
             constexpr int kCopies = kTile * kChunks / kWarp;
             if (p.page_tiles && kWarp % kChunks == 0) {
-                // a lane's rows are so many apart
+                // a lane's rows are so many apart, their chunks an exclusive or
                 constexpr int kApart = kWarp % kChunks == 0 ? kWarp / kChunks : 1;
                 const int row0 = lane / kChunks, chunk = lane % kChunks;
                 const T* at = from + row_offset + row0 * p.token_stride + chunk * kIn;
-                if (chunk * kIn < p.dim) {
+                const uint32_t into = address + row0 * kRowBytes + swizzled<kChunks>(row0, chunk) * 16;
+                const auto to_row = [&](int i) { return (into ^ (i * kApart % 8 * 16)) + i * kApart * kRowBytes; };
+                if (chunk * kIn >= p.dim) {
+                } else if (mask == 0xffffu) {
 #pragma unroll
-                    for (int i = 0; i < kCopies; ++i) {
-                        const int row = row0 + i * kApart;
-                        copy_16b(address + row * kRowBytes + swizzled(row, chunk) * 16, at, mask >> row & 1);
-                        at += kApart * p.token_stride;
-                    }
+                    for (int i = 0; i < kCopies; ++i, at += kApart * p.token_stride) copy_16b(to_row(i), at);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kCopies; ++i, at += kApart * p.token_stride)
+                        copy_16b(to_row(i), at, mask >> (row0 + i * kApart) & 1);
                 }
             } else {
 #pragma unroll
@@ -767,7 +846,7 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
                     const int at = i * kWarp + lane, row = at / kChunks, chunk = at % kChunks;
                     const uint64_t offset = p.page_tiles ? row_offset + row * p.token_stride : __shfl_sync(~0u, row_offset, row);
                     if (chunk * kIn < p.dim)
-                        copy_16b(address + row * kRowBytes + swizzled(row, chunk) * 16, from + offset + chunk * kIn, mask >> row & 1);
+                        copy_16b(address + row * kRowBytes + swizzled<kChunks>(row, chunk) * 16, from + offset + chunk * kIn, mask >> row & 1);
                 }
             }
         } else {
@@ -775,7 +854,7 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
                 const uint64_t offset = p.page_tiles ? row_offset + row * p.token_stride : __shfl_sync(~0u, row_offset, row);
                 const bool live = mask >> row & 1;
                 for (uint32_t c = lane; c < p.dim; c += kWarp) {
-                    T* into = reinterpret_cast<T*>(to + row * kRowBytes + swizzled(row, c / kIn) * 16) + c % kIn;
+                    T* into = reinterpret_cast<T*>(to + row * kRowBytes + swizzled<kChunks>(row, c / kIn) * 16) + c % kIn;
                     *into = live ? from[offset + c] : from_float<T>(0.f);
                 }
             }
@@ -792,7 +871,9 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
                 mask = n.mask & __ballot_sync(~0u, live);
                 if (lane == 0) masks[mask_in] = mask;
                 mask_in = mask_in + 1 == R::kMasks ? 0 : mask_in + 1;
-                row_offset = live ? uint64_t(id) * p.page_stride + (token - p.page.quotient(token) * p.page.d) * p.token_stride + n.head : 0;
+                row_offset = id * p.page_stride + n.head;
+                if (!p.page_tiles) row_offset += (token - p.page.quotient(token) * p.page.d) * p.token_stride;
+                if (!live) row_offset = 0;
                 copy_rows(static_cast<const T*>(p.k));
             } else {
                 copy_rows(static_cast<const T*>(p.v));
@@ -1066,7 +1147,7 @@ struct Choice {
 inline Choice choose(uint32_t group, uint32_t dim, bool f32)
 {
     Choice c{};
-    c.columns = dim <= 64 ? 64 : dim <= 128 ? 128 : (f32 || dim > 192) ? 256 : 192;
+    c.columns = dim <= 64 ? 64 : !f32 && dim <= 96 ? 96 : dim <= 128 ? 128 : (f32 || dim > 192) ? 256 : 192;
     // what a warp's accumulators hold: 128 registers of them
     const uint32_t most = f32 ? (c.columns == 256 ? 4 : 8) : (c.columns <= 128 ? 32 : 16);
     c.chunks = (group + most - 1) / most;
@@ -1089,6 +1170,10 @@ lcpp_status run_16bit(const Params& p, const Choice& c, bool wide, size_t part_b
         return c.heads == 8    ? launch<T, 64, 8, 4, 4, 5>(p, wide, part_bytes, s)
                : c.heads == 16 ? launch<T, 64, 16, 4, 4, 4>(p, wide, part_bytes, s)
                                : launch<T, 64, 32, 4, 4, 2>(p, wide, part_bytes, s);
+    case 96:
+        return c.heads == 8    ? launch<T, 96, 8, 3, 4, 4>(p, wide, part_bytes, s)
+               : c.heads == 16 ? launch<T, 96, 16, 3, 4, 3>(p, wide, part_bytes, s)
+                               : launch<T, 96, 32, 4, 4, 2>(p, wide, part_bytes, s);
     case 128:
         return c.heads == 8    ? launch<T, 128, 8, 2, 4, 4>(p, wide, part_bytes, s)
                : c.heads == 16 ? launch<T, 128, 16, 3, 4, 3>(p, wide, part_bytes, s)
