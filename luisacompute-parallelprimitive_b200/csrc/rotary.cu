@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / kWarp;
 
+// Vectors of a token that are turned or copied: of all heads, per_head of each.
 struct Section {
     const void* in;
     void* out;
@@ -29,13 +30,13 @@ struct Section {
     // From a lane's vector to its next one, 32 * team on, in elements; and what
     // is added where that lies in the next head.
     int64_t in_step, in_wrap, out_step, out_wrap;
-    uint32_t vectors;             // of a token
-    uint32_t step, per_head;      // a lane's step past whole heads, and a head's vectors
-    uint32_t copied;              // 0: the columns past rotary_dim are in place already
+    uint32_t vectors;         // of a token
+    uint32_t step, per_head;  // a lane's step past whole heads, and a head's vectors
 };
 
 struct Params {
-    Section s[3];  // q, k, v
+    Section turn[2];  // of q and k
+    Section copy[3];  // their columns past rotary_dim, and v
     const int32_t* positions;
     const int32_t* token_request;
     const int32_t* position_offset;
@@ -48,7 +49,7 @@ struct Params {
     uint32_t block_size;
     uint32_t tokens, requests;
     uint32_t half;       // rotary_dim / 2
-    uint32_t turned;     // vectors (of pairs) of a head that are turned, the first ones
+    uint32_t turned;     // vectors of pairs of a head
     uint32_t team;       // warps that share a token, a power of two
     float scale, sign;
 };
@@ -119,22 +120,28 @@ __device__ __forceinline__ void turn_pair(float2 cs, float& a, float& b)
     b = fmaf(y, cs.x, __fmul_rn(x, cs.y));
 }
 
-// kValues: elements of an access to values that are copied.
-template <typename T, int N, bool kHalf, bool kAppend, int kValues>
-__global__ void __launch_bounds__(kThreads, kHalf && kAppend ? 3 : 4) rotary_kernel(const Params p)
+// N: elements of an access to pairs, kCopy: to columns that are copied.
+template <typename T, int N, bool kHalf, bool kAppend, int kCopy>
+__global__ void __launch_bounds__(kThreads, kHalf && kAppend && Pack<T, N>::kBytes < 16 ? 3 : 4) rotary_kernel(const Params p)
 {
     // kHalf: vectors of N pairs (i, i + half) in two places; else of N / 2 adjacent
     // pairs, or for N = 1 of one pair as two elements
     constexpr bool kTwo = kHalf || N == 1;  // a pair's second half is loaded by itself
     constexpr int kPairs = kHalf ? N : N == 1 ? 1 : N / 2;
-    constexpr int kAhead = 2;    // vectors that a lane has under way
+    constexpr int kColumns = kHalf ? N : N == 1 ? 2 : N;  // from vector to vector
+    // Vectors that a lane has under way: enough that loads cover the latency, few
+    // enough that nothing spills. 32768 tokens of 32 + 8 heads of 128 in bfloat16:
+    // halves 107 us with one (two loads each) and 118 with two; the first 42 columns
+    // by words 211 us with four and 242 with two; an interleaved append of 4096 tokens
+    // 38.5 us with two, 41 with one, 47 with four.
+    constexpr bool kWide = Pack<T, N>::kBytes == 16, kNarrow = !kAppend && Pack<T, N>::kBytes <= 4;
+    constexpr int kAhead = kHalf && kWide ? 1 : kNarrow ? 4 : 2, kCopies = kNarrow ? 4 : 2;
     extern __shared__ __align__(16) float2 tables[];  // [warp][half] cosine and sine with the scale
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     float2* turn = tables + warp * ((p.half + 1) / 2 * 2);
     const uint32_t worker = blockIdx.x * kWarps + warp, part = worker & (p.team - 1);
     const uint32_t teams = gridDim.x * kWarps / p.team;
     const uint32_t start = part * kWarp + lane;  // the lane's first vector
-    using P = Pack<T, N>;
 
     for (uint32_t t = worker / p.team; t < p.tokens; t += teams) {
         int64_t position = p.positions[t], place = 0;
@@ -144,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, kHalf && kAppend ? 3 : 4) rotary_ker
             live = uint64_t(slot) < p.num_slots;
             if (live) {
                 const uint64_t page = uint64_t(slot) / p.block_size;
-                place = int64_t(page * p.page_stride + (uint64_t(slot) - page * p.block_size) * p.s[1].out_token);
+                place = int64_t(page * p.page_stride + (uint64_t(slot) - page * p.block_size) * p.turn[1].out_token);
             }
         }
         if (p.token_request) {
@@ -160,29 +167,23 @@ __global__ void __launch_bounds__(kThreads, kHalf && kAppend ? 3 : 4) rotary_ker
         }
         // The first vectors of q, or of k, are loaded before the angles are worked out.
         bool ready = false;
-        const auto section = [&](const Section& c, uint64_t to) {
+        const auto turn_all = [&](const Section& c, uint64_t to) {
             const uint32_t head = start / c.per_head;
             uint32_t j = start - head * c.per_head;
-            const T* in = static_cast<const T*>(c.in) + t * c.in_token + head * c.in_head + j * N;
-            T* out = static_cast<T*>(c.out) + to + head * c.out_head + j * N;
-            for (uint32_t v = start; v - lane < c.vectors; ) {  // the warp's lanes together
-                P a[kAhead], b[kAhead];
+            const T* in = static_cast<const T*>(c.in) + t * c.in_token + head * c.in_head + j * kColumns;
+            T* out = static_cast<T*>(c.out) + to + head * c.out_head + j * kColumns;
+            for (uint32_t v = start; v - lane < c.vectors;) {  // the warp's lanes together
+                Pack<T, N> a[kAhead], b[kAhead];
                 T* at[kAhead];
-                int angle[kAhead];
+                uint32_t angle[kAhead];
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
                     at[u] = nullptr;
-                    angle[u] = -1;
-                    const bool turned = j < p.turned;
-                    if (v < c.vectors && (turned || c.copied)) {
-                        // from a vector's number to its column: past the turned ones for those that are copied
-                        const int64_t more = kHalf ? (turned ? 0 : p.half) : N > 1 ? 0 : turned ? j : p.half;
-                        at[u] = out + more;
-                        load(a[u], in + more);
-                        if (turned) {
-                            angle[u] = int(j);
-                            if (kTwo) load(b[u], in + more + (kHalf ? p.half : 1));
-                        }
+                    angle[u] = j;
+                    if (v < c.vectors) {
+                        at[u] = out;
+                        load(a[u], in);
+                        if (kTwo) load(b[u], in + (kHalf ? p.half : 1));
                     }
                     v += p.team * kWarp;
                     in += c.in_step;
@@ -210,10 +211,6 @@ __global__ void __launch_bounds__(kThreads, kHalf && kAppend ? 3 : 4) rotary_ker
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
                     if (!at[u]) continue;
-                    if (angle[u] < 0) {
-                        store(at[u], a[u]);
-                        continue;
-                    }
                     float x[N], y[N];
                     floats_of(a[u], x);
                     if constexpr (kTwo) floats_of(b[u], y);
@@ -243,39 +240,41 @@ __global__ void __launch_bounds__(kThreads, kHalf && kAppend ? 3 : 4) rotary_ker
                 }
             }
         };
-        section(p.s[0], t * p.s[0].out_token);
-        section(p.s[1], kAppend ? uint64_t(place) : t * p.s[1].out_token);
-        if (kAppend) {
-            const Section& c = p.s[2];
-            const uint32_t head = start / c.per_head, j = start - head * c.per_head;
-            const T* in = static_cast<const T*>(c.in) + t * c.in_token + head * c.in_head + j * kValues;
-            T* out = static_cast<T*>(c.out) + uint64_t(place) + head * c.out_head + j * kValues;
-            uint32_t v = start, at = j;
-            while (v < c.vectors) {
-                Pack<T, kValues> x[2];
-                T* to[2];
+        const auto copy_all = [&](const Section& c, uint64_t to) {
+            const uint32_t head = start / c.per_head;
+            uint32_t j = start - head * c.per_head;
+            const T* in = static_cast<const T*>(c.in) + t * c.in_token + head * c.in_head + j * kCopy;
+            T* out = static_cast<T*>(c.out) + to + head * c.out_head + j * kCopy;
+            for (uint32_t v = start; v < c.vectors;) {
+                Pack<T, kCopy> x[kCopies];
+                T* at[kCopies];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    to[u] = nullptr;
+                for (int u = 0; u < kCopies; ++u) {
+                    at[u] = nullptr;
                     if (v < c.vectors) {
-                        to[u] = out;
+                        at[u] = out;
                         load(x[u], in);
                     }
                     v += p.team * kWarp;
                     in += c.in_step;
                     out += c.out_step;
-                    at += c.step;
-                    if (at >= c.per_head) {
-                        at -= c.per_head;
+                    j += c.step;
+                    if (j >= c.per_head) {
+                        j -= c.per_head;
                         in += c.in_wrap;
                         out += c.out_wrap;
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    if (to[u]) store(to[u], x[u]);
+                for (int u = 0; u < kCopies; ++u)
+                    if (at[u]) store(at[u], x[u]);
             }
-        }
+        };
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) turn_all(p.turn[i], kAppend && i ? uint64_t(place) : t * p.turn[i].out_token);
+#pragma unroll 1
+        for (int i = 0; i < (kAppend ? 3 : 2); ++i)
+            copy_all(p.copy[i], kAppend && i ? uint64_t(place) : t * p.copy[i].out_token);
         __syncwarp();  // the table is free
     }
 }
@@ -290,12 +289,10 @@ Strided rows_out(const lcpp_head_rows& r, uint64_t tokens, uint32_t dim, int e)
 }
 Strided flat(const void* p, uint64_t n, int e) { return Strided(p, e, n, {}); }
 
-template <typename T, int N, bool kHalf>
-lcpp_status launch(const Params& p, bool append, bool wide_values, cudaStream_t s)
+template <typename T, int N, bool kHalf, int kCopy>
+lcpp_status launch(const Params& p, bool append, cudaStream_t s)
 {
-    constexpr int kWide = 16 / int(sizeof(T));
-    auto kernel = !append ? rotary_kernel<T, N, kHalf, false, N>
-                  : wide_values ? rotary_kernel<T, N, kHalf, true, kWide> : rotary_kernel<T, N, kHalf, true, N>;
+    auto kernel = append ? rotary_kernel<T, N, kHalf, true, kCopy> : rotary_kernel<T, N, kHalf, false, kCopy>;
     const size_t smem = size_t(kWarps) * align_up(p.half, 2) * sizeof(float2);
     // as for the longest tables, so that few launch shapes are looked up and kept
     const size_t room = size_t(kWarps) * (LCPP_MAX_HEAD_DIM / 2) * sizeof(float2);
@@ -306,33 +303,42 @@ lcpp_status launch(const Params& p, bool append, bool wide_values, cudaStream_t 
 }
 
 template <typename T, int N>
-lcpp_status launch(Params& p, const lcpp_rotary_args& a, bool append, bool wide_values, cudaStream_t s)
+lcpp_status launch(Params& p, const lcpp_rotary_args& a, int copy, bool append, cudaStream_t s)
 {
     const bool half = a.layout == LCPP_ROTARY_HALF;
-    p.turned = (half ? p.half : 2 * p.half) / (half ? N : (N == 1 ? 2 : N));
-    const uint32_t heads[3] = {a.q.num_heads, a.k.num_heads, append ? a.k.num_heads : 0};
-    // a head's vectors: of pairs, then of columns; of values as wide as those allow by themselves
-    const uint32_t in_value = wide_values ? 16 / sizeof(T) : N;
-    const uint32_t per_head = p.turned + (a.head_dim - a.rotary_dim) / N;
-    for (int i = 0; i < 3; ++i) {
-        p.s[i].per_head = i < 2 ? per_head : a.head_dim / in_value;
-        p.s[i].vectors = heads[i] * p.s[i].per_head;
+    const uint32_t columns = half ? N : N == 1 ? 2 : N, heads[2] = {a.q.num_heads, a.k.num_heads};
+    p.turned = (half ? p.half : 2 * p.half) / columns;
+    const uint32_t rest = (a.head_dim - a.rotary_dim) / copy;
+    for (int i = 0; i < 2; ++i) {
+        p.turn[i].per_head = std::max<uint32_t>(p.turned, 1);
+        p.turn[i].vectors = heads[i] * p.turned;
+        p.copy[i].per_head = std::max<uint32_t>(rest, 1);
+        p.copy[i].vectors = p.copy[i].in == p.copy[i].out ? 0 : heads[i] * rest;  // in place
     }
+    const uint32_t value = append ? a.head_dim / copy : 0;  // vectors of a head of v
+    p.copy[2].per_head = std::max<uint32_t>(value, 1);
+    p.copy[2].vectors = append ? a.k.num_heads * value : 0;
     // warps to a token until every SM has 32, but no more than have work for each lane
     p.team = 1;
     while (p.team < kWarps && p.team * p.tokens < uint64_t(device_sm_count()) * 32 &&
-           p.s[0].vectors + p.s[1].vectors > p.team * kWarp)
+           p.turn[0].vectors + p.turn[1].vectors + p.copy[0].vectors > p.team * kWarp)
         p.team *= 2;
-    for (Section& c : p.s) {
-        const uint32_t step = p.team * kWarp, columns = &c == &p.s[2] ? in_value : N;
+    const auto steps = [&](Section& c, uint32_t in_vector) {
+        const uint32_t step = p.team * kWarp;
         c.step = step % c.per_head;
         const int64_t over = step / c.per_head;
-        c.in_step = over * int64_t(c.in_head) + int64_t(c.step) * columns;
-        c.out_step = over * int64_t(c.out_head) + int64_t(c.step) * columns;
-        c.in_wrap = int64_t(c.in_head) - int64_t(c.per_head) * columns;
-        c.out_wrap = int64_t(c.out_head) - int64_t(c.per_head) * columns;
-    }
-    return half ? launch<T, N, true>(p, append, wide_values, s) : launch<T, N, false>(p, append, wide_values, s);
+        c.in_step = over * int64_t(c.in_head) + int64_t(c.step) * in_vector;
+        c.out_step = over * int64_t(c.out_head) + int64_t(c.step) * in_vector;
+        c.in_wrap = int64_t(c.in_head) - int64_t(c.per_head) * in_vector;
+        c.out_wrap = int64_t(c.out_head) - int64_t(c.per_head) * in_vector;
+    };
+    for (Section& c : p.turn) steps(c, columns);
+    for (Section& c : p.copy) steps(c, copy);
+    constexpr int kWide = 16 / int(sizeof(T));
+    if (copy == kWide) return half ? launch<T, N, true, kWide>(p, append, s) : launch<T, N, false, kWide>(p, append, s);
+    if (copy == 4 / int(sizeof(T)) && copy > 1)
+        return half ? launch<T, N, true, 4 / int(sizeof(T))>(p, append, s) : launch<T, N, false, 4 / int(sizeof(T))>(p, append, s);
+    return half ? launch<T, N, true, 1>(p, append, s) : launch<T, N, false, 1>(p, append, s);
 }
 
 lcpp_status run(const lcpp_rotary_args* a, const lcpp_cache_append_args* c, float sign, cudaStream_t s)
@@ -415,13 +421,12 @@ lcpp_status run(const lcpp_rotary_args* a, const lcpp_cache_append_args* c, floa
         p.num_slots = slots;
         p.page_stride = c->cache.page_stride;
         p.block_size = c->cache.block_size;
-        p.s[2].in = c->v;
-        p.s[2].out = c->cache.v;
-        p.s[2].in_token = c->v_token_stride;
-        p.s[2].in_head = c->v_head_stride;
-        p.s[2].out_token = c->cache.token_stride;
-        p.s[2].out_head = c->cache.head_stride;
-        p.s[2].copied = 1;
+        p.copy[2].in = c->v;
+        p.copy[2].out = c->cache.v;
+        p.copy[2].in_token = c->v_token_stride;
+        p.copy[2].in_head = c->v_head_stride;
+        p.copy[2].out_token = c->cache.token_stride;
+        p.copy[2].out_head = c->cache.head_stride;
     }
     for (size_t i = 0; i < out.size(); ++i) {
         for (const Strided& x : in)
@@ -433,13 +438,18 @@ lcpp_status run(const lcpp_rotary_args* a, const lcpp_cache_append_args* c, floa
     for (int i = 0; i < 2; ++i) {
         const lcpp_head_rows& r = *rows[i];
         const bool cached = c && i == 1;
-        p.s[i].in = r.in;
-        p.s[i].out = cached ? c->cache.k : r.out;
-        p.s[i].in_token = r.in_token_stride;
-        p.s[i].in_head = r.in_head_stride;
-        p.s[i].out_token = cached ? c->cache.token_stride : r.out_token_stride;
-        p.s[i].out_head = cached ? c->cache.head_stride : r.out_head_stride;
-        p.s[i].copied = cached || r.in != r.out;
+        Section& x = p.turn[i];
+        x.in = r.in;
+        x.out = cached ? c->cache.k : r.out;
+        x.in_token = r.in_token_stride;
+        x.in_head = r.in_head_stride;
+        x.out_token = cached ? c->cache.token_stride : r.out_token_stride;
+        x.out_head = cached ? c->cache.head_stride : r.out_head_stride;
+        p.copy[i] = x;
+        if (r.num_heads) {
+            p.copy[i].in = static_cast<const char*>(x.in) + size_t(a->rotary_dim) * e;
+            p.copy[i].out = static_cast<char*>(x.out) + size_t(a->rotary_dim) * e;
+        }
     }
     p.positions = a->positions;
     p.token_request = a->token_request;
@@ -451,34 +461,32 @@ lcpp_status run(const lcpp_rotary_args* a, const lcpp_cache_append_args* c, floa
     p.scale = a->scale;
     p.sign = sign * a->scale;
 
-    // the widest vectors that all rows, the turned part and the rest allow
-    const auto fits = [&](int count) {
-        const size_t bytes = size_t(count) * e;
-        const uint32_t unit = a->layout == LCPP_ROTARY_HALF ? p.half : a->rotary_dim;
-        if (unit % count || a->head_dim % count) return false;
-        for (int i = 0; i < 2; ++i) {
-            const Section& x = p.s[i];
-            if (rows[i]->num_heads && (!rows_aligned(x.in, {x.in_token, x.in_head}, e, bytes) ||
-                                       !rows_aligned(x.out, {x.out_token, x.out_head}, e, bytes)))
-                return false;
-        }
+    // the widest accesses that the rows of pairs allow, and those of the columns that are copied
+    const auto rows_fit = [&](const Section& x, size_t bytes) {
+        return rows_aligned(x.in, {x.in_token, x.in_head}, e, bytes) && rows_aligned(x.out, {x.out_token, x.out_head}, e, bytes) &&
+               (!c || rows_aligned(nullptr, {p.page_stride}, e, bytes));
+    };
+    const auto pairs_fit = [&](int count) {
+        if ((a->layout == LCPP_ROTARY_HALF ? p.half : a->rotary_dim) % count) return false;
+        for (int i = 0; i < 2; ++i)
+            if (rows[i]->num_heads && !rows_fit(p.turn[i], size_t(count) * e)) return false;
         return true;
     };
-    const auto values_fit = [&](int count) {
-        const size_t bytes = size_t(count) * e;
-        return !c || (a->head_dim % count == 0 && rows_aligned(p.s[2].in, {p.s[2].in_token, p.s[2].in_head}, e, bytes) &&
-                      rows_aligned(p.s[2].out, {p.s[2].out_token, p.s[2].out_head}, e, bytes) &&
-                      rows_aligned(nullptr, {p.page_stride}, e, bytes));
+    const auto copies_fit = [&](int count) {
+        if ((a->head_dim - a->rotary_dim) % count || (c && a->head_dim % count)) return false;
+        for (int i = 0; i < 2; ++i)
+            if (rows[i]->num_heads && a->head_dim > a->rotary_dim && !rows_fit(p.copy[i], size_t(count) * e)) return false;
+        return !c || rows_fit(p.copy[2], size_t(count) * e);
     };
     diag::KernelTimer timer(kTimerRotary, n, s);
     return with_row_type(a->dtype, [&](auto type) {
         using T = decltype(type);
-        constexpr int kMost = 16 / int(sizeof(T));
-        const bool wide = c && values_fit(kMost);
-        if (kMost == 8 && fits(8) && values_fit(8)) return launch<T, kMost>(p, *a, c, wide, s);
-        if (fits(4) && values_fit(4)) return launch<T, 4>(p, *a, c, wide, s);
-        if (fits(2) && values_fit(2)) return launch<T, 2>(p, *a, c, wide, s);
-        return launch<T, 1>(p, *a, c, wide, s);
+        constexpr int kMost = 16 / int(sizeof(T)), kWord = 4 / int(sizeof(T));
+        const int copy = copies_fit(kMost) ? kMost : copies_fit(kWord) ? kWord : 1;
+        if (kMost == 8 && pairs_fit(8)) return launch<T, kMost>(p, *a, copy, c, s);
+        if (pairs_fit(4)) return launch<T, 4>(p, *a, copy, c, s);
+        if (pairs_fit(2)) return launch<T, 2>(p, *a, copy, c, s);
+        return launch<T, 1>(p, *a, copy, c, s);
     });
 }
 
