@@ -254,10 +254,11 @@ typedef struct lcpp_cache_evict_args {
 
 /* Cuts every request longer than trigger to budget tokens: those whose position
  * is below keep_first or among the last keep_recent of its seq_lens + evicted
- * positions, then the heaviest by slot_scores, equal ones by their place in the
- * cache, earlier ones first (NaN counts as heavier than +inf, both zeros as
- * equal; should more than budget positions be protected, the earlier places are
- * kept).  The kept tokens come to lie in the first budget places: the i-th kept
+ * positions (without slot_positions: whose place is among the first keep_first
+ * or the last keep_recent of its seq_lens), then the heaviest by slot_scores,
+ * equal ones by their place in the cache, earlier ones first (NaN counts as
+ * heavier than +inf, both zeros as equal; should more than budget positions be
+ * protected, the earlier places are kept).  The kept tokens come to lie in the first budget places: the i-th kept
  * token past them goes to the i-th place among them whose token is not kept, so
  * at most as many move as leave.  moves_out holds the slots; entries past
  * move_counts_out are not written.  This call moves nothing:

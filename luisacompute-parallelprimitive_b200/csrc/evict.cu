@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ 
     // the block's run of tokens
     const uint32_t run = (n + blocks - 1) / blocks, lo = min(n, rank * run), count = min(n - lo, run);
     const int32_t* row = p.table + r * p.table_stride;
-    const int64_t recent = int64_t(n) + before - p.recent;
+    const int64_t recent = int64_t(n) + (p.positions ? before : 0) - p.recent;
     // four tokens' keys; 0, which no token has, past the last one
     const auto keys_at = [&](uint32_t i) {
         if (i + 3 < kKeys) return *reinterpret_cast<const uint4*>(keys + i);
@@ -147,7 +147,8 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ 
     const auto page_id = [&](uint32_t page) { return staged ? pages[page - first_page] : uint32_t(row[page]); };
 
     if (threadIdx.x == 0) shared.broken = 0;
-    if (threadIdx.x < 3 && count + threadIdx.x < kKeys) keys[count + threadIdx.x] = 0;
+    // keys are read by fours: the last ones are filled up, which the room, a multiple of four, allows
+    if (threadIdx.x < (4 - count % 4) % 4 && count < kKeys) keys[count + threadIdx.x] = 0;
     for (int i = threadIdx.x; i < kBins * kCopies; i += kThreads) copies[i] = 0;
     __syncthreads();
     bool broken = false;

@@ -1024,7 +1024,15 @@ def _packer(structure):
     for offset, size, code in fields(structure, 0):
         text += f"{offset - end}x{code}"
         end = offset + size
-    return struct.Struct(text + f"{ctypes.sizeof(structure) - end}x").pack
+    pack = struct.Struct(text + f"{ctypes.sizeof(structure) - end}x").pack
+
+    def packed(*values):
+        try:
+            return pack(*values)
+        except (struct.error, OverflowError) as error:  # a number that its field does not hold
+            raise LcppError(ERR_INVALID_ARG, str(error)) from None
+
+    return packed
 
 
 _pack_rotary, _pack_append = _packer(RotaryArgs), _packer(CacheAppendArgs)

@@ -201,6 +201,15 @@ def test_structures_are_packed_as_they_lie(lcpp):
         assert bytes(a) == packed
 
 
+def test_python_refuses_numbers(lcpp):
+    """Numbers that the call's fields do not hold."""
+    fields = [1, 1, 64, 64, 64, 2, 16, 1, 64, 0]
+    assert len(lcpp._pack_cache(*fields)) == ctypes.sizeof(lcpp.KVCache)
+    for at, value in ((5, -1), (6, 2 ** 32), (2, -64), (0, 2 ** 64), (8, 1.5)):
+        with pytest.raises(lcpp.LcppError):
+            lcpp._pack_cache(*(value if i == at else x for i, x in enumerate(fields)))
+
+
 def test_python_refuses_tensors(lcpp):
     """Tensors of the host, of other types, shapes and layouts."""
     L, bf, i32 = lcpp, torch.bfloat16, torch.int32

@@ -751,3 +751,80 @@ def test_serving_loop(lcpp, cache, order):
             assert len(set(free[int(used):].tolist()) |
                        {int(p) for r in range(n) for p in table[r, :-(-int(lens[r]) // block)]}) == pages
     assert max(int(x) for x in evicted) > 0
+
+
+@pytest.mark.parametrize("n", [4093, 4095, 4096, 8192, 16384, 32768])
+def test_plan_where_a_run_fills_its_room(lcpp, n):
+    """A block's keys take all of the shared memory that was asked for, and the last four are not always whole."""
+    table, pages, scores, positions, evicted = eviction_case(n, [n], 4096)
+    check_plan(lcpp, [n], table, scores, positions, evicted, n // 3, n // 2, 5, 100, 4096, pages, n // 3)
+
+
+def test_plan_of_places(lcpp):
+    """Without positions, places count: what left the requests before does not shift the last ones."""
+    lens = [100, 64, 65, 300]
+    table, pages, scores, _, _ = eviction_case(9, lens, 16)
+    kept = check_plan(lcpp, lens, table, scores, None, None, 50, 64, 3, 20, 16, pages, 50)
+    gone, gone_out, counts, cut = i32([7, 0, 900, 41]), i32([0] * 4), i32([0] * 4), i32([0] * 4)
+    moves = torch.full((4, 50, 2), -9, dtype=torch.int64, device="cuda")
+    lcpp.DeviceCacheEviction().Plan(i32(lens), i32(table), torch.tensor(scores, device="cuda"), cut, counts, moves, 4, 16,
+                                    50, trigger=64, keep_first=3, keep_recent=20, d_evicted=gone, d_evicted_out=gone_out)
+    assert torch.equal(moves, kept[0]) and torch.equal(counts, kept[1]) and torch.equal(cut, kept[2])
+    assert torch.equal(gone_out, gone + i32(lens) - cut)
+
+
+def test_steps_in_a_graph(lcpp):
+    """Append, Decode, Plan and Move captured together on a stream of their own and replayed on other lengths, slots and
+    values, next to the same calls one by one."""
+    L, n, h, kv, d, block, width, budget = lcpp, 3, 8, 2, 64, 16, 8, 60
+    pages = n * width
+    table = i32(np.random.default_rng(2).permutation(pages).reshape(n, width))
+    f = L.DeviceRotary.Frequencies(d)
+
+    def state():
+        kc, vc = make_cache("bf16", pages, block, kv, d, "tokens", 5)
+        return dict(kc=kc, vc=vc, rows=randn(7, torch.bfloat16, n, (h + 2 * kv) * d), lens=i32([100, 20, 128]),
+                    slots=torch.zeros(n, dtype=torch.int64, device="cuda"), positions=i32([99, 19, 127]),
+                    gone=i32([3, 0, 9]), held=i32(np.arange(pages * block) % 140),
+                    scores=randn(8, torch.float32, pages * block).abs(), q=torch.zeros(n, h, d, dtype=torch.bfloat16, device="cuda"),
+                    out=torch.zeros(n, h, d, dtype=torch.bfloat16, device="cuda"), cut=i32([0] * n), counts=i32([0] * n),
+                    gone_out=i32([0] * n), moves=torch.zeros(n, budget, 2, dtype=torch.int64, device="cuda"),
+                    temp=L.alloc_temp(L.DevicePagedAttention.GetTempStorageBytes(n, h, kv, d, pages * block)))
+
+    def step(s, stream=None):
+        q, k, v = (x.unflatten(1, (-1, d)) for x in s["rows"].split((h * d, kv * d, kv * d), 1))
+        L.DeviceRotary().Append(q, k, v, s["q"], s["kc"], s["vc"], s["slots"], s["positions"], f, n,
+                                d_token_request=i32_rows, d_position_offset=s["gone"], d_slot_positions=s["held"],
+                                d_slot_scores=s["scores"], stream=stream)
+        L.DevicePagedAttention().Decode(s["temp"], s["q"], s["kc"], s["vc"], table, s["lens"], s["out"], n,
+                                        d_scores=s["scores"], d_scores_out=s["scores"], stream=stream)
+        L.DeviceCacheEviction().Plan(s["lens"], table, s["scores"], s["cut"], s["counts"], s["moves"], n, block, budget,
+                                     keep_recent=8, d_positions=s["held"], d_evicted=s["gone"], d_evicted_out=s["gone_out"],
+                                     stream=stream)
+        L.DeviceCacheEviction().Move(s["moves"], s["counts"], s["kc"], s["vc"], n, d_scores=s["scores"],
+                                     d_positions=s["held"], stream=stream)
+
+    def other(s, lens, seed):
+        at = i32(lens).long() - 1
+        s["lens"].copy_(i32(lens))
+        s["positions"].copy_(at)
+        s["slots"].copy_(table.long().gather(1, (at // block)[:, None])[:, 0] * block + at % block)
+        s["rows"].copy_(randn(seed, torch.bfloat16, n, (h + 2 * kv) * d))
+
+    i32_rows = i32(np.arange(n))
+    one, two = state(), state()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    other(two, [100, 20, 128], 7)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        step(two, side)
+    for lens, seed in (([100, 20, 128], 11), ([61, 128, 1], 12), ([60, 60, 90], 13)):
+        other(one, lens, seed)
+        other(two, lens, seed)
+        step(one)
+        graph.replay()
+        torch.cuda.synchronize()
+        for name in one:
+            if name != "temp":
+                assert torch.equal(one[name], two[name]), name
+        assert one["cut"].tolist() == [min(x, budget) for x in lens]
