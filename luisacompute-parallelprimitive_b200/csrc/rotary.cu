@@ -318,11 +318,23 @@ lcpp_status launch(Params& p, const lcpp_rotary_args& a, int copy, bool append, 
     const uint32_t value = append ? a.head_dim / copy : 0;  // vectors of a head of v
     p.copy[2].per_head = std::max<uint32_t>(value, 1);
     p.copy[2].vectors = append ? a.k.num_heads * value : 0;
-    // warps to a token until every SM has 32, but no more than have work for each lane
-    p.team = 1;
-    while (p.team < kWarps && p.team * p.tokens < uint64_t(device_sm_count()) * 32 &&
-           p.turn[0].vectors + p.turn[1].vectors + p.copy[0].vectors > p.team * kWarp)
-        p.team *= 2;
+    // Warps to a token: of 1, 2, 4 and 8 the number that takes the shortest time, which
+    // is the rounds of 32 warps on every SM times what one takes: its vectors' turns
+    // and two more for the start and the table.  40 heads of 128 in bfloat16, 1 / 2 / 4
+    // / 8 warps: 64 tokens 7.9 / 5.6 / 4.7 / 4.2 us (with the append), 1024 tokens 6.8 /
+    // 5.6 / 5.5 / 7.5, 4096 tokens 17.7 / 17.8 / 19.6 / 25.4, 5003 tokens 26.0 / 22.9 /
+    // 23.5 / 30.0, 32768 tokens 107 / 108 / 123 / 180.
+    uint64_t least = ~0ull;
+    for (uint32_t team = 1; team <= kWarps; team *= 2) {
+        uint64_t turns = 2;
+        for (const Section& c : p.turn) turns += ceil_div(c.vectors, team * kWarp);
+        for (const Section& c : p.copy) turns += ceil_div(c.vectors, team * kWarp);
+        const uint64_t time = ceil_div(uint64_t(p.tokens) * team, uint64_t(device_sm_count()) * 32) * turns;
+        if (time < least) {
+            least = time;
+            p.team = team;
+        }
+    }
     const auto steps = [&](Section& c, uint32_t in_vector) {
         const uint32_t step = p.team * kWarp;
         c.step = step % c.per_head;
