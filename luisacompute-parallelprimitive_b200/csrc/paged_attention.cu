@@ -38,53 +38,72 @@ __global__ void __launch_bounds__(kScoreThreads) scores_kernel(const Params p)
         if (blockIdx.x == 0) wait_for_previous();  // this launch ends after the ones before
         return;
     }
-    wait_for_previous();
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp, quad = lane % 4, part = lane / 4;
     const uint32_t units = p.kv_heads * p.chunks;
     uint32_t r = place.item;
     long long first = place.first;
-    for (long long at = begin + warp; at < end; at += kScoreWarps) {
-        while (at >= first + weight(r)) first += weight(r++);
-        const Tokens seen = tokens_of(p, r);
+    bool waited = false;
+    for (long long at = begin + warp; at < end || !waited; at += kScoreWarps) {
+        const bool live = at < end;
+        float before_score = 0.f;  // of the token that the lane writes: 4 quad + part of the tile
+        int64_t slot = -1;
+        Tokens seen{};
+        if (live) {
+            while (at >= first + weight(r)) first += weight(r++);
+            seen = tokens_of(p, r);
+            const uint32_t token = uint32_t(at - first) * kTile + quad * 4 + part;
+            if (part < 4 && token < seen.end) {
+                const uint32_t page = p.page.quotient(token), id = uint32_t(p.table[r * p.table_stride + page]);
+                if (id < p.num_pages) {
+                    slot = int64_t(uint64_t(id) * p.page.d + (token - page * p.page.d));
+                    if (p.scores) before_score = p.scores[slot];
+                }
+            }
+        }
+        // up to here nothing is read that the launches before this one write
+        if (!waited) wait_for_previous();
+        waited = true;
+        if (!live) break;
         const uint32_t before = seen.base() / kTile, tiles = seen.tiles();
         const long long number = p.first[r];
         if (number + (long long)tiles * units > p.logit_tiles) continue;
-        uint32_t token = uint32_t(at - first) * kTile;
         float mass[4] = {0.f, 0.f, 0.f, 0.f};
         if (at - first >= before) {
             const uint32_t t = uint32_t(at - first) - before;
-            token = seen.base() + t * kTile;
             const float* lse = p.lse2 + uint64_t(r) * p.heads;
             const float4* x = reinterpret_cast<const float4*>(p.logits) + (number + t) * p.per_unit * (kTile / 4) + quad;
             const long long pitch = (long long)tiles * p.per_unit * (kTile / 4);
-#pragma unroll 4
-            for (uint32_t head = part; head < p.heads; head += kWarp / 4) {
-                // the head's unit, and its place in it
-                const uint32_t kv_head = p.by_group.quotient(head), in_group = head - kv_head * p.group;
-                const uint32_t chunk = p.by_unit.quotient(in_group), h = in_group - chunk * p.per_unit;
-                const float of = lse[head];
-                const float4 logits = x[(kv_head * p.chunks + chunk) * pitch + h * (kTile / 4)];
-                if (of == -INFINITY) continue;
-                mass[0] += exp2_fast(logits.x - of);
-                mass[1] += exp2_fast(logits.y - of);
-                mass[2] += exp2_fast(logits.z - of);
-                mass[3] += exp2_fast(logits.w - of);
+            constexpr int kAhead = 5;  // heads of a lane under way
+            for (uint32_t h0 = part; h0 < p.heads; h0 += kAhead * (kWarp / 4)) {
+                float of[kAhead];
+                float4 logits[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const uint32_t head = h0 + u * (kWarp / 4);
+                    of[u] = -INFINITY;
+                    if (head >= p.heads) continue;
+                    // the head's unit, and its place in it
+                    const uint32_t kv_head = p.by_group.quotient(head), in_group = head - kv_head * p.group;
+                    const uint32_t chunk = p.by_unit.quotient(in_group), h = in_group - chunk * p.per_unit;
+                    of[u] = lse[head];
+                    logits[u] = x[(kv_head * p.chunks + chunk) * pitch + h * (kTile / 4)];
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    if (of[u] == -INFINITY) continue;
+                    mass[0] += exp2_fast(logits[u].x - of[u]);
+                    mass[1] += exp2_fast(logits[u].y - of[u]);
+                    mass[2] += exp2_fast(logits[u].z - of[u]);
+                    mass[3] += exp2_fast(logits[u].w - of[u]);
+                }
             }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int d = 4; d < kWarp; d *= 2) mass[i] += __shfl_xor_sync(~0u, mass[i], d);
-        // lane 4 i + quad writes token 4 quad + i
         const float own = part == 0 ? mass[0] : part == 1 ? mass[1] : part == 2 ? mass[2] : mass[3];
-        token += quad * 4 + part;
-        if (part < 4 && token < seen.end) {
-            const uint32_t page = p.page.quotient(token), id = uint32_t(p.table[r * p.table_stride + page]);
-            if (id < p.num_pages) {
-                const uint64_t slot = uint64_t(id) * p.page.d + (token - page * p.page.d);
-                p.scores_out[slot] = (p.scores ? p.decay * p.scores[slot] : 0.f) + own;
-            }
-        }
+        if (slot >= 0) p.scores_out[slot] = p.decay * before_score + own;
     }
 }
 
