@@ -5,7 +5,9 @@
 // known when all of the head's tokens are: where scores are wanted the decode
 // kernel leaves its logits, 4 bytes for each token and head against the 4 D / g
 // (16 bits, g query heads to a kv head) that it reads for them, and scores_kernel
-// sums them for each token in the order of the heads.
+// sums them for each token in the order of the heads.  The logits stay in L2; their
+// writes, the third launch and its dependent loads are what scores cost (48 requests of
+// 4096 tokens and fewer, 40 heads: 98 us with them, 86 without).
 #include "paged_attention.cuh"
 
 using namespace lcpp;
@@ -16,7 +18,9 @@ namespace {
 
 constexpr int kScoreThreads = 256, kScoreWarps = kScoreThreads / kWarp;
 
-// A warp takes 16 tokens: a lane four of them under every eighth head.
+// A warp takes 16 tokens: a lane four of them under every eighth head.  Bound by the
+// latency of page id, score, log-sum and logits, of which the first two are loaded
+// before the wait and the others together (102.6 -> 97.9 us for the call above).
 __global__ void __launch_bounds__(kScoreThreads) scores_kernel(const Params p)
 {
     const auto weight = [&](uint32_t r) {  // tiles before the window, then those of the logits

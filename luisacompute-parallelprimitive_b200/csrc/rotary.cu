@@ -12,7 +12,12 @@
 // are on their way, and turns its share of the vectors.  No warp waits for
 // another.
 //
-// Bound by memory: every element is read once and written once.
+// Bound by memory: every element is read once and written once.  Turned columns and
+// copied ones are walked one after the other, each with the widest access that its
+// own start allows (together with the narrower one's: 32768 tokens of 40 heads of
+// 128 whose first 42 columns are turned 444 us, apart 211).  32768 tokens of 40 heads
+// of 128 in bfloat16: 107 us, 6.3 TB/s (a copy reaches 6.5); queries and the append
+// of keys and values of as many tokens: 82 us for 537 MB; 64 tokens: 4.1 us.
 #include "cache.cuh"
 
 using namespace lcpp;

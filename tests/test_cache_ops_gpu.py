@@ -828,3 +828,12 @@ def test_steps_in_a_graph(lcpp):
             if name != "temp":
                 assert torch.equal(one[name], two[name]), name
         assert one["cut"].tolist() == [min(x, budget) for x in lens]
+
+
+@pytest.mark.parametrize("ties", [False, True])
+def test_plan_of_more_tokens_than_a_cluster_holds(lcpp, ties):
+    """Keys that no block of the largest cluster has room for are read again."""
+    lens = [350_001, 3, 320_000]
+    table, pages, scores, positions, evicted = eviction_case(11, lens, 128, ties)
+    check_plan(lcpp, lens, table, scores, positions, evicted, 100_000, 100_000, 5, 300, 128, pages, 100_000)
+    check_plan(lcpp, lens, table, scores, None, None, 330_000, 330_000, 0, 0, 128, pages, 20_001)
