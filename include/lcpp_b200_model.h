@@ -214,7 +214,9 @@ lcpp_status lcpp_paged_attention_temp_bytes(uint32_t num_requests, uint32_t num_
  * outside the request are never used, whatever they hold.  Tokens before the
  * window keep score_decay * slot_scores; slots of no request are not written.
  * Requests may share pages unless scores are wanted: then a shared slot gets
- * the score of one of them.  A request's bits depend on the lengths of the
+ * the score of one of them, and where the requests have more tokens in all than
+ * score_slots, those whose logits find no room in temp storage leave the scores
+ * of their slots as they are.  A request's bits depend on the lengths of the
  * call's requests, which the work is divided by, not on their values.
  * out, lse_out, slot_scores_out and temp storage must not overlap one another
  * or the inputs (slot_scores_out may be slot_scores). */

@@ -837,3 +837,27 @@ def test_plan_of_more_tokens_than_a_cluster_holds(lcpp, ties):
     table, pages, scores, positions, evicted = eviction_case(11, lens, 128, ties)
     check_plan(lcpp, lens, table, scores, positions, evicted, 100_000, 100_000, 5, 300, 128, pages, 100_000)
     check_plan(lcpp, lens, table, scores, None, None, 330_000, 330_000, 0, 0, 128, pages, 20_001)
+
+
+def test_decode_of_more_tokens_than_slots(lcpp):
+    """Lengths far past the pages there are: outputs hold, scores of the requests in front too, no memory is left."""
+    rng = np.random.default_rng(3)
+    pages, block = 30, 16
+    kc, vc = make_cache("bf16", pages, block, 2, 64, "tokens")
+    table = np.full((3, 4000), -1, np.int32)
+    ids = rng.permutation(pages)
+    table[0, :7], table[1, :9], table[2, 3990:3996] = ids[:7], ids[7:16], ids[16:22]
+    lens, q = [100, 60_000, 64_000], randn(1, torch.bfloat16, 3, 8, 64)
+    out, lse, after = decode(lcpp, q, kc, vc, i32(table), i32(lens), scores=torch.zeros(pages * block, device="cuda"))
+    plain = decode(lcpp, q, kc, vc, i32(table), i32(lens))
+    assert torch.equal(out, plain[0]) and torch.equal(lse, plain[1])
+    want, want_lse, _ = decode(lcpp, q[:1], kc, vc, i32(table[:1, :7]), i32(lens[:1]))
+    assert ((out[0].float() - want[0].float()).abs() <= 6e-5 + 2 ** -7 * want[0].float().abs()).all()
+    assert ((lse[0] - want_lse[0]).abs() <= 4e-5 * (1 + want_lse[0].abs())).all()
+    first = torch.tensor(ids[:7].astype(np.int64), device="cuda")[:, None] * block + torch.arange(block, device="cuda")
+    first = first.view(-1)[:100]
+    total = float(after[first].double().sum())
+    assert abs(total - 8) <= 8 * 4e-5  # each head hands out 1
+    rest = torch.ones(pages * block, dtype=torch.bool, device="cuda")
+    rest[first] = False
+    assert (after[rest] == -8).all()
