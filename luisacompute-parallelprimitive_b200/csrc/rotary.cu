@@ -137,10 +137,12 @@ __global__ void __launch_bounds__(kThreads, kHalf && kAppend && Pack<T, N>::kByt
     // Vectors that a lane has under way: enough that loads cover the latency, few
     // enough that nothing spills. 32768 tokens of 32 + 8 heads of 128 in bfloat16:
     // halves 107 us with one (two loads each) and 118 with two; the first 42 columns
-    // by words 211 us with four and 242 with two; an interleaved append of 4096 tokens
-    // 38.5 us with two, 41 with one, 47 with four.
+    // by elements 211 us with four and 242 with two; an interleaved append of 8191 tokens
+    // 38.5 us with two, 41 with one, 47 with four.  Copied columns of 32768 appended
+    // tokens of 192 columns, 64 turned: 134 us with two, 127.5 with three; without the
+    // append (32 of 128 turned) 119 with two, 129 with three.
     constexpr bool kWide = Pack<T, N>::kBytes == 16, kNarrow = !kAppend && Pack<T, N>::kBytes <= 4;
-    constexpr int kAhead = kHalf && kWide ? 1 : kNarrow ? 4 : 2, kCopies = kNarrow ? 4 : 2;
+    constexpr int kAhead = kHalf && kWide ? 1 : kNarrow ? 4 : 2, kCopies = kNarrow ? 4 : kAppend ? 3 : 2;
     extern __shared__ __align__(16) float2 tables[];  // [warp][half] cosine and sine with the scale
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     float2* turn = tables + warp * ((p.half + 1) / 2 * 2);
