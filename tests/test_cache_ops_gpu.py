@@ -861,3 +861,76 @@ def test_decode_of_more_tokens_than_slots(lcpp):
     rest = torch.ones(pages * block, dtype=torch.bool, device="cuda")
     rest[first] = False
     assert (after[rest] == -8).all()
+
+
+def test_broadcast_inputs(lcpp):
+    """Inputs whose heads or tokens are one row repeated (stride 0); as outputs and as a written cache they are refused."""
+    t, d = 37, 128
+    x, f = randn(1, torch.bfloat16, t, 1, d), lcpp.DeviceRotary.Frequencies(d)
+    positions = np.arange(t) * 3
+    out = torch.zeros(t, 6, d, dtype=torch.bfloat16, device="cuda")
+    lcpp.DeviceRotary().Forward(x.expand(t, 6, d), None, out, None, i32(positions), f, t)
+    check_turn(out, x.expand(t, 6, d).contiguous(), positions, f, ref.HALF, 1.0)
+    row = x[:1, :1].expand(t, 2, d)
+    same = torch.zeros(t, 2, d, dtype=torch.bfloat16, device="cuda")
+    lcpp.DeviceRotary().Backward(None, row, None, same, i32(positions), f, t)
+    check_turn(same, row.contiguous(), positions, f, ref.HALF, 1.0, inverse=True)
+    with pytest.raises(lcpp.LcppError):
+        lcpp.DeviceRotary().Forward(out, None, x.expand(t, 6, d), None, i32(positions), f, t)
+
+    rng = np.random.default_rng(0)
+    lens = [100, 1, 60]
+    table, pages = make_table(rng, lens, 10, 16)
+    kc, vc = make_cache("bf16", pages, 16, 1, d, "tokens")
+    shared = [c.expand(pages, 16, 4, d) for c in (kc, vc)]
+    q = randn(2, torch.bfloat16, 3, 8, d)
+    got = decode(lcpp, q, *shared, i32(table), i32(lens))
+    want = decode(lcpp, q, *(c.contiguous() for c in shared), i32(table), i32(lens))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    check_decode(lcpp, randn(3, torch.bfloat16, 1, 8, d).expand(3, 8, d), kc, vc, table, lens)
+    one = randn(4, torch.bfloat16, 3, 4, d)
+    slots = torch.tensor([0, 1, 2], device="cuda")
+    with pytest.raises(lcpp.LcppError):
+        lcpp.DeviceRotary().Append(None, one, one, None, *shared, slots, i32([0, 1, 2]), f, 3)
+    with pytest.raises(lcpp.LcppError):
+        lcpp.DeviceCacheEviction().Move(torch.zeros(3, 1, 2, dtype=torch.int64, device="cuda"), i32([0] * 3), *shared, 3)
+
+
+def test_plan_without_room_for_moves(lcpp):
+    """No moves at all fit: requests whose tokens happen to lie in front are cut, the others stay."""
+    lens, budget, block = [90, 90], 40, 16
+    table, pages, _, _, _ = eviction_case(12, lens, block)
+    scores = np.zeros(pages * block, np.float32)
+    for r in range(2):
+        slot = table[r, np.arange(90) // block].astype(np.int64) * block + np.arange(90) % block
+        scores[slot] = np.arange(90)[::-1] if r == 0 else np.arange(90)
+    cut, counts = i32([-7, -7]), i32([-7, -7])
+    moves = torch.zeros(2, 0, 2, dtype=torch.int64, device="cuda")
+    lcpp.DeviceCacheEviction().Plan(i32(lens), i32(table), torch.tensor(scores, device="cuda"), cut, counts, moves, 2, block,
+                                    budget)
+    assert cut.tolist() == [budget, 90] and counts.tolist() == [0, 0]
+
+
+def test_two_streams_at_once(lcpp):
+    """Calls on two streams with temp storage of their own do not disturb one another."""
+    rng = np.random.default_rng(4)
+    lens = [3000, 700, 41, 1800]
+    table, pages = make_table(rng, lens, 200, 16)
+    kc, vc = make_cache("bf16", pages, 16, 2, 128, "tokens")
+    qs = [randn(s, torch.bfloat16, 4, 16, 128) for s in range(2)]
+    want = [decode(lcpp, q, kc, vc, i32(table), i32(lens), scores=torch.zeros(pages * 16, device="cuda")) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    d_table, d_lens, f = i32(table), i32(lens), lcpp.DeviceRotary.Frequencies(128)
+    temps = [lcpp.alloc_temp(lcpp.DevicePagedAttention.GetTempStorageBytes(4, 16, 2, 128, pages * 16)) for _ in qs]
+    outs, scores = [torch.zeros_like(q) for q in qs], [torch.full((pages * 16,), -8.0, device="cuda") for _ in qs]
+    turned = [torch.zeros_like(q) for q in qs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            lcpp.DevicePagedAttention().Decode(temps[i], qs[i], kc, vc, d_table, d_lens, outs[i], 4, d_scores_out=scores[i],
+                                               stream=s)
+            lcpp.DeviceRotary().Forward(qs[i], None, turned[i], None, d_lens, f, 4, stream=s)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(outs[i], want[i][0]) and torch.equal(scores[i], want[i][2])
+        check_turn(turned[i], qs[i], np.array(lens), f, ref.HALF, 1.0)
