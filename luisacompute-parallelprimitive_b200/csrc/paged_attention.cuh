@@ -39,6 +39,7 @@ namespace attention {
 
 constexpr int kTile = 16;              // tokens of a tile
 constexpr uint32_t kMostBlocks = 800;  // the partial results' room
+constexpr int32_t kLost = 1 << 30;     // beside a request in `split`: the run wrote a row that is to be computed again
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -66,7 +67,8 @@ struct Params {
     float softcap;        // with log2 e; 0: none
     float* lse;
     float* part;          // [block][2][heads of a unit][columns] and, behind them, [block][2][heads of a unit][2]
-    int32_t* split;       // [block][4]: request, unit, first block and further blocks of the unit that its run ends in
+    int32_t* split;       // [block][4]: request (and kLost), unit, first block and further blocks of the unit that its run ends in
+    uint32_t warps;       // of a block of the decode kernel
     Divider by_group, by_unit;  // by `group` and `per_unit`, for the scores
     float* logits;        // [tile][per_unit][16] in base 2, or NULL
     long long logit_tiles;
@@ -113,6 +115,18 @@ struct Walk {
         left = room - (t_end - t);
     }
     __device__ __forceinline__ void read_ahead(const Params& p) { next_length = r + 1 < p.requests ? p.lens[r + 1] : 0; }
+    // At tile `begin` of all, which lies in request `place`, for a run up to `end`.
+    __device__ __forceinline__ void start(const Params& p, const Place& place, long long begin, long long end)
+    {
+        r = place.item;
+        tokens = tokens_of(p, r);
+        read_ahead(p);
+        tiles = tokens.tiles();
+        unit = uint32_t((begin - place.first) / tiles);
+        t = uint32_t((begin - place.first) - (long long)unit * tiles);
+        left = end - begin;
+        part();
+    }
     // To the part after this one; false: the run has ended.
     __device__ __forceinline__ bool next(const Params& p)
     {
@@ -672,10 +686,21 @@ struct Room {
     static constexpr int kStats = kOwn + WARPS * Work::kWarpBytes;  // m, l [warp][head], then of the unit [head]
     static constexpr int kValid = kStats + (2 * WARPS + 2) * H * 4;
     static constexpr int kFree = kValid + WARPS * kMasks * 4;
-    static constexpr int kBytes = kFree + WARPS * 4;
+    static constexpr int kLostRows = kFree + WARPS * 4;   // whether the run has any
+    static constexpr int kBytes = kLostRows + 4;
     static_assert(Work::kPass * D * 4 <= kSlotBytes, "a warp's vectors fit its free slot");
     static_assert(SLOTS <= 2 * kNotes, "page ids have come when they are needed");
 };
+
+__device__ __forceinline__ bool finite(float x) { return x - x == 0.f; }
+// Terms of up to 2^8 (float16: 2^15) times a value may pass what 32 bits hold where the
+// mean does not, and two parts of a term make NaN of an infinite value.  Neither comes
+// back to a finite number on its way, so a row with weights whose vector has ended as
+// one is right; the others are computed again (mend_row).
+__device__ __forceinline__ bool lost(float weights, float4 x)
+{
+    return weights != 0.f && finite(weights) && !(finite(x.x) && finite(x.y) && finite(x.z) && finite(x.w));
+}
 
 // Zeros for the requests without tokens, divided among the blocks.
 template <typename T>
@@ -754,14 +779,7 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
     }
 
     Walk now;
-    now.r = place.item;
-    now.tokens = tokens_of(p, now.r);
-    now.read_ahead(p);
-    now.tiles = now.tokens.tiles();
-    now.unit = uint32_t((begin - place.first) / now.tiles);
-    now.t = uint32_t((begin - place.first) - (long long)now.unit * now.tiles);
-    now.left = end - begin;
-    now.part();
+    now.start(p, place, begin, end);
 
     // A part's queries, [head] rows swizzled like the keys'.
     const auto load_queries = [&](const Walk& w, int buffer) {
@@ -897,6 +915,8 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
         slot_in = slot_in + 1 == SLOTS ? 0 : slot_in + 1;
     };
 
+    int* any_lost = reinterpret_cast<int*>(smem + R::kLostRows);
+    if (threadIdx.x == 0) *any_lost = 0;
     load_queries(now, 0);
 #pragma unroll
     for (int i = 0; i < R::kNotes; ++i) note_next();
@@ -986,8 +1006,10 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
                     *reinterpret_cast<float4*>(p.part + (uint64_t(part_of) * H + h) * D + column) = x;
                 } else if (column < p.dim) {
                     const float all = unit_l[h], by = all == 0.f ? 0.f : 1.f / all;
-                    store_4(static_cast<T*>(p.out) + now.r * p.out_request + (head + h) * p.out_head + column,
-                            make_float4(x.x * by, x.y * by, x.z * by, x.w * by), p.wide_out, p.dim - column);
+                    const float4 y = make_float4(x.x * by, x.y * by, x.z * by, x.w * by);
+                    if (lost(all, y)) *any_lost = 1;
+                    store_4(static_cast<T*>(p.out) + now.r * p.out_request + (head + h) * p.out_head + column, y, p.wide_out,
+                            p.dim - column);
                 }
             }
             if (pass == 0 && threadIdx.x < heads) {
@@ -1009,7 +1031,7 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
             if (!again) {
                 const long long per = run_of(total, uint64_t(units) * p.requests, gridDim.x, kWarps), unit_begin = first_tile - now.t;
                 const int32_t from = int32_t(unit_begin / per), to = int32_t((unit_begin + now.tiles - 1) / per);
-                *split = make_int4(int32_t(now.r), int32_t(now.unit), from, now.t_end < now.tiles ? to - from : 0);
+                *split = make_int4(int32_t(now.r) | (*any_lost ? kLost : 0), int32_t(now.unit), from, now.t_end < now.tiles ? to - from : 0);
             }
         }
         if (!again) break;
@@ -1020,25 +1042,114 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
     wait_copies<0>();
 }
 
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * kWarp;
+
+// 2^x for x <= 0 in the range of 64 bits, with the digits of 32.
+__device__ __forceinline__ double exp2_wide(float x)
+{
+    if (x < -1000.f) return 0.0;
+    const float whole = rintf(x);
+    return double(exp2_fast(x - whole)) * __hiloint2double((1023 + int(whole)) << 20, 0);
+}
+
+// One row of the output by one block, its sums in 64 bits, where none of 32-bit values
+// ends, and its terms one number each: sum_t p_t v_t as it stands, infinities and NaN
+// among the values.  Slow (every eighth token a warp's, one after the other): no
+// ordinary call has such a row.  room: [4][D].
+template <typename T, int D>
+__device__ __forceinline__ void mend_row(const Params& p, uint32_t r, uint32_t head, float* room, double2* stats)
+{
+    constexpr int kPer = D / kWarp;
+    const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    const Tokens seen = tokens_of(p, r);
+    const uint64_t kv_offset = head / p.group * p.head_stride;
+    double* sums = reinterpret_cast<double*>(room);  // [D]
+    float* q = room + 2 * D;
+    __syncthreads();  // the room is free
+    for (uint32_t column = threadIdx.x; column < D; column += kJoinThreads)
+        q[column] = column < p.dim ? to_float((static_cast<const T*>(p.q) + r * p.q_request + head * p.q_head)[column]) : 0.f;
+    __syncthreads();
+    double o[kPer], l = 0.0;
+    float m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) o[c] = 0.0;
+#pragma unroll 1
+    for (uint32_t t = seen.first + warp; t < seen.end; t += kJoinWarps) {
+        const uint32_t page = p.page.quotient(t), id = uint32_t(p.table[r * p.table_stride + page]);
+        if (id >= p.num_pages) continue;
+        const uint64_t at = id * p.page_stride + (t - page * p.page.d) * p.token_stride + kv_offset + lane;
+        const T* k_row = static_cast<const T*>(p.k) + at;
+        const T* v_row = static_cast<const T*>(p.v) + at;
+        float v[kPer], x = 0.f;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) {
+            const bool in = c * kWarp + lane < p.dim;
+            v[c] = in ? to_float(v_row[c * kWarp]) : 0.f;
+            x = fmaf(q[c * kWarp + lane], in ? to_float(k_row[c * kWarp]) : 0.f, x);
+        }
+#pragma unroll
+        for (int d = 1; d < kWarp; d *= 2) x += __shfl_xor_sync(~0u, x, d);
+        x = logit(p, x);
+        if (x > m) {
+            const double f = m == -INFINITY ? 1.0 : exp2_wide(m - x);  // before the first one there is nothing but zeros and NaN
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) o[c] *= f;
+            m = x;
+        }
+        const double e = x == -INFINITY ? 0.0 : exp2_wide(x - m);
+        l += e;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) o[c] += e * v[c];
+    }
+    // the warps' parts, in their order
+    if (lane == 0) stats[warp] = make_double2(m, l);
+    __syncthreads();
+    double all = 0.0;
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, float(stats[w].x));
+    const auto factor = [&](float from) { return from == -INFINITY ? 1.0 : exp2_wide(from - top); };
+#pragma unroll 1
+    for (uint32_t w = 0; w < kJoinWarps; ++w) {
+        all += factor(float(stats[w].x)) * stats[w].y;
+        if (warp == w) {
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) {
+                double& sum = sums[c * kWarp + lane];
+                sum = factor(m) * o[c] + (w ? sum : 0.0);
+            }
+        }
+        __syncthreads();
+    }
+    T* out = static_cast<T*>(p.out) + r * p.out_request + head * p.out_head;
+    for (uint32_t column = threadIdx.x; column < p.dim; column += kJoinThreads)
+        out[column] = from_float<T>(float(all == 0.0 ? 0.0 : sums[column] / all));
+}
+
 // A unit whose tiles lie in the runs of `count` + 1 blocks: the last part of the
 // first of them and the first parts of the others join, in order.  The first `count`
 // blocks here share its heads; a block's warps take a head each, or where it has
 // fewer, every so-many-th part of one.  Few numbers, so latency: one block of 1024
 // threads for a unit measured slower.
-constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * kWarp;
 template <typename T, int D, int H>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
+__global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const __grid_constant__ Params p)
 {
-    __shared__ float sums[kJoinWarps / 2][D];
+    __shared__ __align__(16) float sums[kJoinWarps / 2][D];
     __shared__ float2 stats_of[kJoinWarps];
+    __shared__ double2 mend_stats[kJoinWarps];
+    __shared__ uint32_t lost_heads;  // of the unit that is joined here
     let_next_start();
+    if (threadIdx.x == 0) lost_heads = 0;
+    __syncthreads();
     wait_for_previous();
     const int4 split = reinterpret_cast<const int4*>(p.split)[blockIdx.x];
-    const uint32_t r = uint32_t(split.x), unit = uint32_t(split.y), block = uint32_t(split.z), count = uint32_t(split.w);
+    const uint32_t r = uint32_t(split.x & ~kLost), unit = uint32_t(split.y), block = uint32_t(split.z), count = uint32_t(split.w);
     const uint32_t kv_head = unit / p.chunks, head0 = unit % p.chunks * p.per_unit;
     const uint32_t heads = min(p.per_unit, p.group - head0), turn = blockIdx.x - block;
-    if (count == 0 || turn >= heads) return;
-    const uint32_t mine = (heads - turn + count - 1) / count;  // the heads turn, turn + count, ...
+    const bool joins = count != 0 && turn < heads;
+    if (!joins && !(split.x & kLost)) return;
+    const uint32_t mine = joins ? (heads - turn + count - 1) / count : 0;  // the heads turn, turn + count, ...
     uint32_t at_once = 1;
     while (at_once < mine && at_once < kJoinWarps) at_once *= 2;
     const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
@@ -1113,11 +1224,58 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
             const uint32_t head = kv_head * p.group + head0 + h;
             T* out = static_cast<T*>(p.out) + r * p.out_request + head * p.out_head;
             const float by = all == 0.f ? 0.f : 1.f / all;
+            bool none = false;
 #pragma unroll
-            for (int c = 0; c < kPer; ++c)
+            for (int c = 0; c < kPer; ++c) {
+                none |= lost(all, make_float4(o[c] * by, 0.f, 0.f, 0.f));
                 if (c * kWarp + lane < p.dim) out[c * kWarp + lane] = from_float<T>(o[c] * by);
+            }
+            if (__any_sync(~0u, none) && lane == 0) atomicOr(&lost_heads, 1u << h);
             if (lane == 0) put_lse(p, uint64_t(r) * p.heads + head, top, all);
         }
+    }
+    __syncthreads();
+    if (!lost_heads && !(split.x & kLost)) return;
+
+    // rows that are computed again: of this unit, then of the units that lie whole in the block's run of tiles
+    uint32_t again = lost_heads, row_r = r, first_head = kv_head * p.group + head0;
+    Walk now;
+    bool more = split.x & kLost, started = false;
+    while (true) {
+        while (!again && more) {
+            if (!started) {
+                const uint32_t units = p.kv_heads * p.chunks;
+                long long begin = -1, end = -1;
+                Place place;
+                share_of<kJoinThreads>(
+                    p.requests, [&](uint32_t i) { return (long long)(tokens_of(p, i).tiles()) * units; },
+                    [&](long long all) {
+                        const long long per = run_of(all, uint64_t(units) * p.requests, gridDim.x, int(p.warps));
+                        begin = blockIdx.x * per;
+                        end = min(all, begin + per);
+                        return begin < all ? begin : -1;
+                    },
+                    place);
+                now.start(p, place, begin, end);
+                started = true;
+            } else if (!now.next(p)) {
+                more = false;
+                break;
+            }
+            if (now.t || now.t_end != now.tiles) continue;
+            const uint32_t kv = now.unit / p.chunks, h0 = (now.unit - kv * p.chunks) * p.per_unit;
+            row_r = now.r;
+            first_head = kv * p.group + h0;
+            for (uint32_t h = 0; h < min(p.per_unit, p.group - h0); ++h) {
+                const T* row = static_cast<const T*>(p.out) + row_r * p.out_request + (first_head + h) * p.out_head;
+                bool none = false;
+                for (uint32_t column = threadIdx.x; column < p.dim; column += kJoinThreads) none |= !finite(to_float(row[column]));
+                if (__syncthreads_or(none)) again |= 1u << h;
+            }
+        }
+        if (!again) return;
+        mend_row<T, D>(p, row_r, first_head + __ffs(again) - 1, &sums[0][0], mend_stats);
+        again &= again - 1;
     }
 }
 
@@ -1134,6 +1292,7 @@ lcpp_status launch(const Params& base, bool wide, size_t part_bytes_at_most, cud
     const unsigned blocks = std::min<unsigned>(
         kMostBlocks, unsigned(device_sm_count()) * resident_blocks(reinterpret_cast<const void*>(kernel), kThreads, R::kBytes));
     if (uint64_t(blocks) * 2 * H * (D + 2) * 4 > part_bytes_at_most) return LCPP_ERR_INTERNAL;
+    p.warps = WARPS;
     kernel<<<blocks, kThreads, R::kBytes, s>>>(p);
     const lcpp_status status = launched();
     if (status != LCPP_OK) return status;

@@ -1,0 +1,79 @@
+"""The paged cache's operators where numbers end: infinite values and sums beyond 32 bits.  References and tolerances as in tests/test_cache_ops_gpu.py."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+import cache_ref as ref
+from test_cache_ops_gpu import KINDS, TYPES, decode, i32, make_cache, make_table, randn
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+MIXES = {
+    # units that a block has whole and units that blocks divide; some empty ones
+    "ragged": [int(n) for n in np.random.default_rng(0).integers(0, 90, 220)] + [900, 0, 2500],
+    "one": [70],
+    "long": [20_000],
+}
+
+
+def compare(out, lse, q, kc, vc, table, lens, **options):
+    """Infinities and NaN where the formula has them, and its numbers elsewhere."""
+    want, size, want_lse, _ = ref.attend(q.double(), kc.double(), vc.double(), torch.tensor(table), lens,
+                                         options.pop("scale", q.shape[2] ** -0.5), **options)
+    out = out.double()
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(torch.where(out.isinf(), out, 0), torch.where(want.isinf(), want, 0))
+    sure = want.isfinite()
+    error = (out - want)[sure].abs()
+    assert (error <= (3e-5 * size + torch.finfo(q.dtype).eps / 2 * want.abs())[sure] + 2.0 ** -25).all()
+    assert ((lse.double() - want_lse)[want_lse.isfinite()].abs() <= 2e-5 * (1 + want_lse[want_lse.isfinite()].abs())).all()
+    return want
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("mix", MIXES)
+@pytest.mark.parametrize("h,kv,d,block,options", [(8, 2, 64, 16, {}), (3, 1, 128, 24, {"window": 60}),
+                                                  (40, 1, 128, 16, {"softcap": 3.0}), (6, 3, 250, 7, {})])
+def test_decode_of_infinite_values(lcpp, kind, mix, h, kv, d, block, options):
+    """A value of +inf or -inf that is looked at gives its column that infinity, both of them or a NaN give NaN; other
+    columns, heads and requests keep their numbers."""
+    lens = MIXES[mix]
+    rng = np.random.default_rng(d + len(lens))
+    table, pages = make_table(rng, lens, max(lens) // block + 2, block)
+    kc, vc = make_cache(kind, pages, block, kv, d, "tokens", seed=d)
+    for r, n in enumerate(lens):
+        if not n or (r % 3 and mix == "ragged"):
+            continue
+        # columns 0, 1 and 5 of several tokens: inf, -inf, NaN; column 3: both infinities; the last: inf in the first token
+        for column, token, value in ((0, n - 1, math.inf), (0, n // 2, math.inf), (1, n - 1, -math.inf),
+                                     (3, n - 1, math.inf), (3, n // 3, -math.inf), (5, n // 2, math.nan),
+                                     (d - 1, 0, math.inf)):
+            vc[table[r, token // block], token % block, (r + column) % kv, column] = value
+    q = randn(d + 1, TYPES[kind], len(lens), h, d)
+    out, lse, _ = decode(lcpp, q, kc, vc, i32(table), i32(lens), **options)
+    want = compare(out, lse, q, kc, vc, table, lens, **options)
+    assert want.isinf().any() and want.isfinite().any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("mix", MIXES)
+def test_decode_of_the_largest_values(lcpp, kind, mix):
+    """The mean of the type's largest numbers is a number, although their sum is none in 32 bits; equal ones give
+    themselves."""
+    lens, h, kv, d, block = MIXES[mix], 8, 2, 64, 16
+    table, pages = make_table(np.random.default_rng(1), lens, max(lens) // block + 2, block)
+    kc, vc = make_cache(kind, pages, block, kv, d, "tokens", seed=3)
+    top = torch.finfo(TYPES[kind]).max
+    vc[..., 0], vc[..., 1] = top, -top
+    vc[..., 2] = torch.where(vc[..., 2] > 0, top, -top)
+    vc[..., 3] *= top / 8
+    q = randn(4, TYPES[kind], len(lens), h, d)
+    out, lse, _ = decode(lcpp, q, kc, vc, i32(table), i32(lens))
+    live = torch.tensor(lens, device="cuda") > 0
+    assert (out[live][..., 0] == top).all() and (out[live][..., 1] == -top).all() and out.isfinite().all()
+    compare(out, lse, q, kc, vc, table, lens)
