@@ -1005,8 +1005,9 @@ __global__ void __launch_bounds__(WARPS * kWarp, BLOCKS) decode_kernel(const Par
                 if (!whole) {
                     *reinterpret_cast<float4*>(p.part + (uint64_t(part_of) * H + h) * D + column) = x;
                 } else if (column < p.dim) {
-                    const float all = unit_l[h], by = all == 0.f ? 0.f : 1.f / all;
-                    const float4 y = make_float4(x.x * by, x.y * by, x.z * by, x.w * by);
+                    const float all = unit_l[h], by = 1.f / all;
+                    float4 y = make_float4(x.x * by, x.y * by, x.z * by, x.w * by);
+                    if (all == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);  // whatever the values were
                     if (lost(all, y)) *any_lost = 1;
                     store_4(static_cast<T*>(p.out) + now.r * p.out_request + (head + h) * p.out_head + column, y, p.wide_out,
                             p.dim - column);
@@ -1223,12 +1224,13 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const __grid_cons
         if (live && group == groups - 1) {
             const uint32_t head = kv_head * p.group + head0 + h;
             T* out = static_cast<T*>(p.out) + r * p.out_request + head * p.out_head;
-            const float by = all == 0.f ? 0.f : 1.f / all;
+            const float by = 1.f / all;
             bool none = false;
 #pragma unroll
             for (int c = 0; c < kPer; ++c) {
-                none |= lost(all, make_float4(o[c] * by, 0.f, 0.f, 0.f));
-                if (c * kWarp + lane < p.dim) out[c * kWarp + lane] = from_float<T>(o[c] * by);
+                const float y = all == 0.f ? 0.f : o[c] * by;  // without weights zeros, whatever the values were
+                none |= lost(all, make_float4(y, 0.f, 0.f, 0.f));
+                if (c * kWarp + lane < p.dim) out[c * kWarp + lane] = from_float<T>(y);
             }
             if (__any_sync(~0u, none) && lane == 0) atomicOr(&lost_heads, 1u << h);
             if (lane == 0) put_lse(p, uint64_t(r) * p.heads + head, top, all);

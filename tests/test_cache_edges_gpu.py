@@ -1,4 +1,5 @@
-"""The paged cache's operators where numbers end: infinite values and sums beyond 32 bits.  References and tolerances as in tests/test_cache_ops_gpu.py."""
+"""The paged cache's operators where numbers end: infinite values, sums beyond 32 bits, rows that are empty by their
+logits.  References and tolerances as in tests/test_cache_ops_gpu.py."""
 from __future__ import annotations
 
 import math
@@ -77,3 +78,22 @@ def test_decode_of_the_largest_values(lcpp, kind, mix):
     live = torch.tensor(lens, device="cuda") > 0
     assert (out[live][..., 0] == top).all() and (out[live][..., 1] == -top).all() and out.isfinite().all()
     compare(out, lse, q, kc, vc, table, lens)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("mix", MIXES)
+def test_decode_of_rows_without_weight(lcpp, kind, mix):
+    """A row whose logits are all -inf gets zeros and lse -inf, whatever its values hold."""
+    lens, d, block = MIXES[mix], 64, 16
+    table, pages = make_table(np.random.default_rng(2), lens, max(lens) // block + 2, block)
+    kc, vc = make_cache(kind, pages, block, 2, d, "tokens", seed=5)
+    q = randn(6, TYPES[kind], len(lens), 4, d)
+    kc[..., 0, 0] = -math.inf  # of the first kv head
+    q[..., 0] = 1
+    plain = vc.clone()
+    for i, bad in enumerate((math.inf, -math.inf, math.nan)):
+        vc[..., 0, i::4] = bad
+    out, lse, _ = decode(lcpp, q, kc, vc, i32(table), i32(lens))
+    assert (out[:, :2] == 0).all() and (lse[:, :2] == -math.inf).all()
+    other, other_lse, _ = decode(lcpp, q, kc, plain, i32(table), i32(lens))
+    assert torch.equal(out[:, 2:], other[:, 2:]) and torch.equal(lse, other_lse)
