@@ -1388,6 +1388,8 @@ class DevicePagedAttention:
             dim ** -0.5 if scale is None else scale, softcap, _array(d_lse_out, f32, n * heads, "d_lse_out", device),
             _array(d_scores, f32, slots, "d_scores", device), _array(d_scores_out, f32, slots, "d_scores_out", device),
             score_decay)
+        if temp is not None and (temp.get_device() != device or not temp.is_contiguous()):
+            raise LcppError(ERR_INVALID_ARG, "temp: contiguous, a CUDA tensor of the current device")
         check(lib().lcpp_paged_attention_decode(*_scratch(temp), args, _queue(stream, device)), "Decode")
 
 

@@ -1,0 +1,65 @@
+"""What the paged cache's Python classes and entry points refuse or hand on, beyond tests/test_cache_ops.py; no device
+needed: a stand-in takes the library's calls."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class Recorder:
+    """Stands in for the library and keeps its calls."""
+
+    def __init__(self):
+        self.calls = []
+
+    def lcpp_status_string(self, status):
+        return b""
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+        return call
+
+
+class Elsewhere:
+    """A tensor that says it lies on another device."""
+
+    def __init__(self, tensor):
+        self.tensor = tensor
+
+    def get_device(self):
+        return 3
+
+    def __getattr__(self, name):
+        return getattr(self.tensor, name)
+
+
+@pytest.fixture
+def recorder(lcpp, monkeypatch):
+    """CPU tensors pass as the current device's, whose number is theirs."""
+    lib = Recorder()
+    monkeypatch.setattr(lcpp, "lib", lambda: lib)
+    monkeypatch.setattr(lcpp, "_device", lambda: -1)
+    monkeypatch.setattr(lcpp, "_queue", lambda stream, device=None: 0)
+    return lib
+
+
+def decode_args():
+    i32 = torch.int32
+    q = torch.zeros(4, 4, 64)
+    return [q, torch.zeros(10, 16, 2, 64), torch.zeros(10, 16, 2, 64), torch.zeros(4, 8, dtype=i32),
+            torch.zeros(4, dtype=i32), torch.zeros_like(q), 4]
+
+
+def test_decode_takes_temp_of_its_device(lcpp, recorder):
+    """Temp storage of the host or of another device would be written by the kernels all the same."""
+    temp, call = torch.zeros(1024, dtype=torch.uint8), lcpp.DevicePagedAttention().Decode
+    call(temp, *decode_args())
+    assert [name for name, _ in recorder.calls] == ["lcpp_paged_attention_decode"]
+    assert recorder.calls[0][1][:2] == (temp.data_ptr(), 1024)
+    for bad in (Elsewhere(temp), torch.zeros(1, dtype=torch.uint8).expand(1 << 30)):
+        with pytest.raises(lcpp.LcppError):
+            call(bad, *decode_args())
+    assert len(recorder.calls) == 1
