@@ -1079,9 +1079,11 @@ def _heads(t, tokens, heads, dim, dtype, name, device):
 
 
 def _kv_cache(k, v, device):
-    """The lcpp_kv_cache's fields of two [pages, block_size, heads, dim] tensors of equal strides."""
+    """The lcpp_kv_cache's fields of two [pages, block_size, heads, dim] tensors of equal strides (those along a single
+    entry do not matter)."""
     shape, stride, dtype = k.shape, k.stride(), k.dtype
-    if len(shape) != 4 or v.shape != shape or v.stride() != stride or v.dtype is not dtype:
+    if len(shape) != 4 or v.shape != shape or v.dtype is not dtype or \
+            (v.stride() != stride and any(a != b and n > 1 for a, b, n in zip(stride, v.stride(), shape))):
         raise LcppError(ERR_INVALID_ARG, "keys and values: [pages, block_size, heads, dim] of one dtype, shape and layout")
     if stride[3] != 1 and shape[3] > 1:
         raise LcppError(ERR_INVALID_ARG, "keys and values: a head's columns have to be adjacent")

@@ -63,3 +63,28 @@ def test_decode_takes_temp_of_its_device(lcpp, recorder):
         with pytest.raises(lcpp.LcppError):
             call(bad, *decode_args())
     assert len(recorder.calls) == 1
+
+
+@pytest.mark.parametrize("k,v", [
+    # one kv head: heads first in the page, and tokens first
+    (torch.zeros(10, 1, 16, 64).transpose(1, 2), torch.zeros(10, 16, 1, 64)),
+    # one page, and the first of several that lie further apart
+    (torch.zeros(1, 16, 2, 64), torch.zeros(3, 20, 2, 64)[:1, :16]),
+    # pages of one token
+    (torch.zeros(10, 2, 64)[:, None], torch.zeros(10, 1, 2, 64)),
+    (torch.zeros(10, 16, 2, 1), torch.zeros(10, 16, 2, 3)[..., :1].contiguous()),
+])
+def test_strides_of_single_entries_do_not_matter(lcpp, k, v):
+    """Keys and values need equal strides where there is a second entry to step to."""
+    fields = lcpp._kv_cache(k, v, -1)
+    assert fields[:2] == (k.data_ptr(), v.data_ptr()) and fields[5:9] == tuple(k.shape)
+    for i in range(3):
+        assert k.shape[i] == 1 or fields[2 + i] == k.stride(i) == v.stride(i)
+
+
+def test_strides_of_keys_and_values_agree(lcpp):
+    k = torch.zeros(10, 16, 2, 64)
+    for v in (torch.zeros(10, 2, 16, 64).transpose(1, 2), torch.zeros(10, 17, 2, 64)[:, :16], torch.zeros(10, 16, 2, 65)[..., :64],
+              torch.zeros(10, 16, 2, 64, dtype=torch.float16), torch.zeros(9, 16, 2, 64)):
+        with pytest.raises(lcpp.LcppError):
+            lcpp._kv_cache(k, v, -1)
