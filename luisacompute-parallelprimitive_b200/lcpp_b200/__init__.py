@@ -1313,7 +1313,7 @@ class DeviceRotary:
                 continue
             heads = x.shape[1] if x.dim() == 3 else 0
             at, a, b = _heads(x, tokens, heads, dim, dtype, name, device)
-            to, c, d = (0, 0, 0) if append and x is k else _heads(out, tokens, heads, dim, dtype, name + "_out", device)
+            to, c, d = (0, 0, 0) if append and name == "d_k" else _heads(out, tokens, heads, dim, dtype, name + "_out", device)
             fields += (at, to, a, b, c, d, heads)
         requests = 0 if token_request is None else 0x7fffffff if position_offset is None else position_offset.numel()
         turned = frequencies.numel()

@@ -88,3 +88,13 @@ def test_strides_of_keys_and_values_agree(lcpp):
               torch.zeros(10, 16, 2, 64, dtype=torch.float16), torch.zeros(9, 16, 2, 64)):
         with pytest.raises(lcpp.LcppError):
             lcpp._kv_cache(k, v, -1)
+
+
+def test_append_of_one_tensor_as_queries_and_keys(lcpp, recorder):
+    """Queries that are the keys' own tensor are turned into their output, as those of an equal tensor are."""
+    x, out, cache = torch.zeros(8, 2, 64), torch.zeros(8, 2, 64), torch.zeros(2, 10, 16, 2, 64)
+    slots, positions, f = torch.zeros(8, dtype=torch.int64), torch.zeros(8, dtype=torch.int32), torch.zeros(32, dtype=torch.float64)
+    for keys in (x, x[:]):
+        lcpp.DeviceRotary().Append(x, keys, x, out, cache[0], cache[1], slots, positions, f, 8)
+    (_, (one, *_)), (_, (two, *_)) = recorder.calls
+    assert lcpp.RotaryArgs.from_buffer_copy(two).q.out == out.data_ptr() and one == two
