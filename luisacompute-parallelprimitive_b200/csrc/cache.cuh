@@ -57,18 +57,30 @@ struct Strided {
     }
 };
 
-// Whether a and b may share memory.  Apart, or rows of one pitch of which each
-// fits beside the other's: sure not to; everything else counts as shared.
+// Whether the innermost dims_a and dims_b dimensions of a and b may share memory where
+// b's first element lies `at` bytes behind a's.
+inline bool may_meet(const Strided& a, int dims_a, const Strided& b, int dims_b, uint64_t at)
+{
+    if (static_cast<unsigned __int128>(at) >= a.extent(dims_a) * a.element) return false;
+    while (dims_a && a.dim[dims_a - 1].n == 1) --dims_a;  // there is no second entry to step to
+    while (dims_b && b.dim[dims_b - 1].n == 1) --dims_b;
+    if (!dims_a && !dims_b) return true;
+    const auto step = [](const Strided& x, int dims) { return dims ? x.dim[dims - 1].stride * x.element : uint64_t(0); };
+    const uint64_t pitch = std::max(step(a, dims_a), step(b, dims_b)), within = pitch ? at % pitch : 0;
+    if (!pitch) return true;
+    if (step(a, dims_a) == pitch) --dims_a;  // else all of it is one row
+    if (step(b, dims_b) == pitch) --dims_b;
+    if (a.extent(dims_a) * a.element > pitch || within + b.extent(dims_b) * b.element > pitch) return true;
+    return may_meet(a, dims_a, b, dims_b, within);  // one's row lies in the pitch of one row of the other's
+}
+// Whether a and b may share memory.  Apart, or rows of one pitch (and in these rows of
+// one pitch again) of which each fits beside the other's: sure not to; everything else
+// counts as shared.
 inline bool may_share(const Strided& a, const Strided& b)
 {
     if (!overlap(a.p, a.bytes(), b.p, b.bytes())) return false;
-    if (!a.dims || !b.dims) return true;
-    const uint64_t pitch = a.dim[a.dims - 1].stride * a.element;
-    if (b.dim[b.dims - 1].stride * b.element != pitch || !pitch) return true;
-    const uint64_t in_a = uint64_t(a.extent(a.dims - 1)) * a.element, in_b = uint64_t(b.extent(b.dims - 1)) * b.element;
     const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-    const uint64_t at = y >= x ? (y - x) % pitch : (pitch - (x - y) % pitch) % pitch;
-    return at < in_a || at + in_b > pitch;
+    return x <= y ? may_meet(a, a.dims, b, b.dims, y - x) : may_meet(b, b.dims, a, a.dims, x - y);
 }
 
 // v / d for v < 2^31 through a multiplication: with l = ceil(log2 d) and

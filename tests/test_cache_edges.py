@@ -98,3 +98,14 @@ def test_append_of_one_tensor_as_queries_and_keys(lcpp, recorder):
         lcpp.DeviceRotary().Append(x, keys, x, out, cache[0], cache[1], slots, positions, f, 8)
     (_, (one, *_)), (_, (two, *_)) = recorder.calls
     assert lcpp.RotaryArgs.from_buffer_copy(two).q.out == out.data_ptr() and one == two
+
+
+@pytest.mark.parametrize("shift", [64 - 32, 128 + 32, 192 - 2, 192 * 3, 768 - 32, 192 + 32])
+def test_rows_inside_each_head_that_overlap_are_refused(lcpp, shift):
+    """Heads of [tokens, 4, 3, 64]: an output that is not one of the three in every head shares memory with the queries
+    (or, behind the third, with those of the next head or token)."""
+    at = 0x10000000
+    q = lcpp.HeadRows(at, at, 768, 192, 768, 192, 4)
+    k = lcpp.HeadRows(0x50000000, at + 2 * shift, 128, 64, 768, 192, 2)
+    args = lcpp.RotaryArgs(q, k, 0x60000000, None, None, 0x70000000, 8, 0, 64, 64, 0, 1.0, lcpp.BF16)
+    assert lcpp.lib().lcpp_rotary_forward(bytes(args), None) == lcpp.ERR_INVALID_ARG

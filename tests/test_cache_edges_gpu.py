@@ -97,3 +97,32 @@ def test_decode_of_rows_without_weight(lcpp, kind, mix):
     assert (out[:, :2] == 0).all() and (lse[:, :2] == -math.inf).all()
     other, other_lse, _ = decode(lcpp, q, kc, plain, i32(table), i32(lens))
     assert torch.equal(out[:, 2:], other[:, 2:]) and torch.equal(lse, other_lse)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_heads_side_by_side_in_each_head(lcpp, kind):
+    """Queries, keys and values of a head next to one another: outputs beside inputs and beside one another."""
+    t, h, d = 33, 4, 64
+    rows = randn(1, TYPES[kind], t, h, 3, d)
+    before, positions, f = rows.clone(), i32(np.arange(t) * 7), lcpp.DeviceRotary.Frequencies(d)
+    want_q, want_k = (before[:, :, i].contiguous() for i in range(2))
+    lcpp.DeviceRotary().Forward(want_q, want_k, want_q, want_k, positions, f, t)
+    lcpp.DeviceRotary().Forward(rows[:, :, 0], rows[:, :, 1], rows[:, :, 0], rows[:, :, 1], positions, f, t)
+    assert torch.equal(rows[:, :, 0], want_q) and torch.equal(rows[:, :, 1], want_k)
+    assert torch.equal(rows[:, :, 2], before[:, :, 2])
+    # the turned queries into the place of the values
+    lcpp.DeviceRotary().Forward(before[:, :, 0], None, before[:, :, 2], None, positions, f, t)
+    assert torch.equal(before[:, :, 2], want_q)
+
+    lens, block = [70, 0, 9], 16
+    table, pages = make_table(np.random.default_rng(0), lens, 6, block)
+    kc, vc = make_cache(kind, pages, block, 2, d, "tokens")
+    both = randn(3, TYPES[kind], 3, h, 2, d)
+    q = both[:, :, 0].contiguous()
+    want, lse, _ = decode(lcpp, q, kc, vc, i32(table), i32(lens))
+    temp = lcpp.alloc_temp(lcpp.DevicePagedAttention.GetTempStorageBytes(3, h, 2, d))
+    lcpp.DevicePagedAttention().Decode(temp, both[:, :, 0], kc, vc, i32(table), i32(lens), both[:, :, 1], 3)
+    assert torch.equal(both[:, :, 1], want) and torch.equal(both[:, :, 0], q)
+    for bad in (both.view(3, h, 2 * d)[..., d // 2:d // 2 + d], both.view(3, 2 * h, d)[:, h - 1:2 * h - 1]):
+        with pytest.raises(lcpp.LcppError):
+            lcpp.DevicePagedAttention().Decode(temp, both[:, :, 0], kc, vc, i32(table), i32(lens), bad, 3)
