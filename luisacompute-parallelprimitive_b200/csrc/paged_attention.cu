@@ -206,7 +206,8 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_paged_attention_args* 
     p.table_stride = a->table_stride;
     p.lens = a->seq_lens;
     p.page = Divider(cache.block_size);
-    p.longest = uint32_t(std::min<uint64_t>(uint64_t(a->table_width) * cache.block_size, 0x7fffffffu));
+    // without pages every row is empty: nothing asks for an address in them
+    p.longest = slots ? uint32_t(std::min<uint64_t>(uint64_t(a->table_width) * cache.block_size, 0x7fffffffu)) : 0u;
     p.page_tiles = cache.block_size % kTile == 0;
     p.wide_q = rows_aligned(a->q, {a->q_request_stride, a->q_head_stride}, e, 16) && cache.head_dim * e % 16 == 0;
     p.wide_out = rows_aligned(a->out, {a->out_request_stride, a->out_head_stride}, e, 4 * e) && cache.head_dim % 4 == 0;

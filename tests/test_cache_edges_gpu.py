@@ -126,3 +126,24 @@ def test_heads_side_by_side_in_each_head(lcpp, kind):
     for bad in (both.view(3, h, 2 * d)[..., d // 2:d // 2 + d], both.view(3, 2 * h, d)[:, h - 1:2 * h - 1]):
         with pytest.raises(lcpp.LcppError):
             lcpp.DevicePagedAttention().Decode(temp, both[:, :, 0], kc, vc, i32(table), i32(lens), bad, 3)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("block", [16, 7])
+def test_cache_without_pages(lcpp, kind, block):
+    """No page at all, whatever the tables and lengths say: rows are empty, nothing is written, nothing moves."""
+    kc, vc = (torch.zeros(0, block, 2, 64, dtype=TYPES[kind], device="cuda") for _ in range(2))
+    table, lens = i32([[0, 3, -1], [5, 1, 0]]), i32([40, 9])
+    none = torch.zeros(0, device="cuda")
+    for scores in (None, none):
+        out, lse, _ = decode(lcpp, randn(1, TYPES[kind], 2, 4, 64), kc, vc, table, lens, scores=scores)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    x, f = randn(2, TYPES[kind], 3, 2, 64), lcpp.DeviceRotary.Frequencies(64)
+    q = torch.full_like(x, 5)
+    lcpp.DeviceRotary().Append(x, x, x, q, kc, vc, torch.tensor([0, 1, -1], device="cuda"), i32([0, 1, 2]), f, 3)
+    assert (q == 5).all()  # tokens whose slot lies outside the cache are left out
+    lcpp.DeviceCacheEviction().Move(torch.zeros(2, 1, 2, dtype=torch.int64, device="cuda"), i32([1, 1]), kc, vc, 2)
+    cut, counts = i32([-7, -7]), i32([-7, -7])
+    lcpp.DeviceCacheEviction().Plan(i32([20, 9]), table, none, cut, counts,
+                                    torch.zeros(2, 4, 2, dtype=torch.int64, device="cuda"), 2, block, 4)
+    assert cut.tolist() == [20, 9] and counts.tolist() == [0, 0]
