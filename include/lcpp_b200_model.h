@@ -191,7 +191,8 @@ typedef struct lcpp_paged_attention_args {
     uint32_t num_heads;         /* a multiple of num_kv_heads: query head h reads kv head h / (num_heads / num_kv_heads) */
     uint32_t window;            /* only the last `window` tokens are looked at; 0: all */
     float scale;                /* factor of the dot products */
-    float softcap;              /* above 0: logits x become softcap * tanh(x / softcap) */
+    float softcap;              /* above 0: logits x become softcap * tanh(x / softcap); scale / softcap has to be finite, and
+                                   1.45 times scale and softcap */
     float* lse_out;             /* [num_requests][num_heads] logarithm of the sum of exponentials, or NULL */
     const float* slot_scores;   /* [num_pages * block_size]; NULL: zeros */
     float* slot_scores_out;     /* the same after this step, may be slot_scores itself; NULL: not wanted */

@@ -222,6 +222,8 @@ lcpp_status run(void* temp, size_t temp_bytes, const lcpp_paged_attention_args* 
     p.window = a->window;
     p.scale = a->softcap > 0.f ? a->scale / a->softcap : a->scale * kLog2e;
     p.softcap = a->softcap * kLog2e;
+    // products of factors that are numbers and may be none: 0 * inf would make NaN of logits of 0
+    if (!std::isfinite(p.scale) || !std::isfinite(p.softcap)) return LCPP_ERR_INVALID_ARG;
     p.lse = a->lse_out;
     p.part = reinterpret_cast<float*>(t + l.part);
     p.split = reinterpret_cast<int32_t*>(t + l.split);

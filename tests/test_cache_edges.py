@@ -109,3 +109,12 @@ def test_rows_inside_each_head_that_overlap_are_refused(lcpp, shift):
     k = lcpp.HeadRows(0x50000000, at + 2 * shift, 128, 64, 768, 192, 2)
     args = lcpp.RotaryArgs(q, k, 0x60000000, None, None, 0x70000000, 8, 0, 64, 64, 0, 1.0, lcpp.BF16)
     assert lcpp.lib().lcpp_rotary_forward(bytes(args), None) == lcpp.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("scale,softcap", [(1.0, 1e-40), (3e38, 0.0), (-3e38, 0.0), (1.0, 3e38), (1e30, 1e-10)])
+def test_decode_refuses_factors_beyond_32_bits(lcpp, scale, softcap):
+    """Factors that are no numbers where the kernel multiplies by them."""
+    cache = lcpp.KVCache(0xA0000000, 0xB0000000, 2048, 128, 64, 10, 16, 2, 64, lcpp.BF16)
+    args = lcpp.PagedAttentionArgs(cache, 0x10000000, 256, 64, 0x20000000, 256, 64, 0x30000000, 8, 8, 4, 0x40000000, 4, 0,
+                                   scale, softcap, 0x50000000, 0x60000000, 0x70000000, 1.0)
+    assert lcpp.lib().lcpp_paged_attention_decode(0x100000000, 1 << 30, bytes(args), None) == lcpp.ERR_INVALID_ARG
