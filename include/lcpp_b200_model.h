@@ -146,8 +146,8 @@ typedef struct lcpp_rotary_args {
 
 /* For the pairs (a, b) of every head, with angle = position * f_i:
  *   a' = scale * (a cos(angle) - b sin(angle)),  b' = scale * (b cos(angle) + a sin(angle));
- * columns from rotary_dim on are copied.  Computed in 32 bits (angles in 64),
- * rounded once.  `out` may be `in` itself with the same strides; else outputs
+ * columns from rotary_dim on are copied.  Computed in 32 bits (an angle's fraction
+ * of a turn in 64, cosine and sine of it in 32), rounded once.  `out` may be `in` itself with the same strides; else outputs
  * must not overlap inputs or one another.  Tokens that are left out are neither
  * read nor written. */
 lcpp_status lcpp_rotary_forward(const lcpp_rotary_args* args, lcpp_stream_t stream);
@@ -199,7 +199,9 @@ typedef struct lcpp_paged_attention_args {
     float score_decay;          /* factor of slot_scores */
 } lcpp_paged_attention_args;
 
-/* score_slots: num_pages * block_size when slot_scores_out is wanted, else 0. */
+/* score_slots: num_pages * block_size when slot_scores_out is wanted, else 0.
+ * Scores take 4 bytes for each of these slots and each query head (rounded up to
+ * whole units of the kernel): they are the logits of the call's tokens. */
 lcpp_status lcpp_paged_attention_temp_bytes(uint32_t num_requests, uint32_t num_heads, uint32_t num_kv_heads,
                                             uint32_t head_dim, uint64_t score_slots, size_t* temp_bytes);
 
@@ -208,7 +210,9 @@ lcpp_status lcpp_paged_attention_temp_bytes(uint32_t num_requests, uint32_t num_
  *   x_t = scale * q . k_t,  p = softmax of x,  out = sum_t p_t v_t,
  *   slot_scores_out[slot of t] = score_decay * slot_scores[slot of t] + sum_h p_t.
  * Statistics and sums are held in 32 bits, p as two numbers of the cache's
- * type where that has 16 bits; the output is rounded once.  A row that has
+ * type where that has 16 bits (bfloat16: 16 digits; float16: 22, but to 2^-32
+ * of the row's largest p, below which p counts as 0); the output is rounded
+ * once.  A row that has
  * weights but did not end as finite numbers that way is computed again with p
  * as one number and sums in 64 bits: large values whose mean is a number give
  * that number, infinities and NaN among the values act as in the formula (a
@@ -218,10 +222,10 @@ lcpp_status lcpp_paged_attention_temp_bytes(uint32_t num_requests, uint32_t num_
  * tokens, or whose logits are all -inf, gets zeros and lse -inf; keys and values
  * outside the request are never used, whatever they hold.  Tokens before the
  * window keep score_decay * slot_scores; slots of no request are not written.
- * Requests may share pages unless scores are wanted: then a shared slot gets
- * the score of one of them, and where the requests have more tokens in all than
- * score_slots, those whose logits find no room in temp storage leave the scores
- * of their slots as they are.  A request's bits depend on the lengths of the
+ * Requests may share pages unless scores are wanted: the score of a shared slot
+ * would depend on which request came first, and where the requests have more
+ * tokens in all than num_pages * block_size, those whose logits find no room in
+ * temp storage leave the scores of their slots as they are.  A request's bits depend on the lengths of the
  * call's requests, which the work is divided by, not on their values.
  * out, lse_out, slot_scores_out and temp storage must not overlap one another
  * or the inputs (slot_scores_out may be slot_scores). */
@@ -271,6 +275,9 @@ typedef struct lcpp_cache_evict_args {
  * move_counts_out are not written.  This call moves nothing:
  * lcpp_cache_evict_move does, for each layer's cache.  Attention does not mind
  * the order of the tokens (a window does: it counts places).
+ *
+ * No page may belong to two requests: its tokens would be moved and its page given
+ * back for one of them while the other still uses it.
  *
  * A request whose row holds a page id outside [0, num_pages), or that has more
  * moves than max_moves, is left as it is (0 moves, its length).  Lengths count as
