@@ -8,7 +8,8 @@ import numpy as np
 import pytest
 
 import cache_ref as ref
-from test_cache_ops_gpu import KINDS, TYPES, decode, i32, make_cache, make_table, randn
+from test_cache_ops_gpu import (KINDS, TYPES, check_decode, check_plan, decode, eviction_case, i32, make_cache, make_table,
+                                randn)
 
 pytestmark = pytest.mark.gpu
 
@@ -147,3 +148,35 @@ def test_cache_without_pages(lcpp, kind, block):
     lcpp.DeviceCacheEviction().Plan(i32([20, 9]), table, none, cut, counts,
                                     torch.zeros(2, 4, 2, dtype=torch.int64, device="cuda"), 2, block, 4)
     assert cut.tolist() == [20, 9] and counts.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("block", [1, 7, 24])
+def test_windows_that_begin_inside_pages(lcpp, kind, block):
+    """A window's first tile has rows before it, and rows in several pages; with scores."""
+    lens = [300, 1, 9, 0, 158, 33, 64]
+    table, pages = make_table(np.random.default_rng(block), lens, max(lens) // block + 2, block)
+    kc, vc = make_cache(kind, pages, block, 2, 80, "heads", seed=block)
+    q, scores = randn(block, TYPES[kind], len(lens), 6, 80), torch.rand(pages * block, device="cuda")
+    for window in (1, 9, 17, 23, 100, 299):
+        check_decode(lcpp, q, kc, vc, table, lens, scores=scores, window=window, decay=0.5)
+
+
+@pytest.mark.parametrize("ties", [False, True])
+@pytest.mark.parametrize("lens", [[2048, 2049, 4096, 3], [5000, 4999], [50_000, 20_000]])
+def test_plan_of_pages_of_one_token(lcpp, lens, ties):
+    """Runs of more pages than a block keeps the ids of, which are then read where they are needed, and of just as many."""
+    table, pages, scores, positions, evicted = eviction_case(len(lens), lens, 1, ties)
+    n = min(x for x in lens if x > 3)
+    check_plan(lcpp, lens, table, scores, positions, evicted, n // 2, n - 1, 5, 100, 1, pages, max(lens), 2 * pages,
+               np.arange(2 * pages + 1))
+    table[0, lens[0] - 2] = -1  # a request with a broken page stays as it is
+    check_plan(lcpp, lens, table, scores, None, None, n // 2, n - 1, 5, 100, 1, pages, max(lens))
+
+
+@pytest.mark.parametrize("ties", [False, True])
+def test_plan_of_more_keys_than_a_block_holds(lcpp, ties):
+    """A long request among many short ones: keys past what the largest cluster's blocks have room for are read again."""
+    lens = [330_000] + [3] * 200
+    table, pages, scores, positions, evicted = eviction_case(1, lens, 64, ties)
+    check_plan(lcpp, lens, table, scores, positions, evicted, 70_000, 70_000, 5, 300, 64, pages, 70_000)
