@@ -14,10 +14,11 @@
 // counts there.  A histogram has four copies, for every fourth lane one: equal
 // scores would serialise on a single one.
 //
-// Bound by latency: a pass over the keys costs about 1.4 us of barriers and dependent
-// steps.  64 requests of 2100 tokens and fewer cut to 2048, with the pages' release:
-// 14.3 us; 16 of 131072 to 8192: 33.7 us (39.4 with page ids read token by token from
-// L2 and every bin of the other blocks read by all).
+// Bound by latency: of 2100 tokens a pass over the keys costs about 1.4 us of barriers and
+// dependent steps, beside the start, the keys' loads and the sorting out.  64 requests of
+// 2100 tokens and fewer cut to 2048, with the pages' release: 14.4 us; 16 of 131072 to
+// 8192: 33.7 us (39.4 with page ids read token by token from L2 and every bin of the other
+// blocks read by all), of which the release, a block a request, takes 4.
 #include <cooperative_groups.h>
 
 #include "cache.cuh"
@@ -576,8 +577,10 @@ lcpp_status plan(const lcpp_cache_evict_args* a, cudaStream_t s)
 
     diag::KernelTimer timer(kTimerEviction, n, s);
     if (n) {
-        // Blocks of 2048 tokens and more, as long as the requests leave SMs for them; and
-        // of no more than have room for their keys.  Clusters of 1 / 2 / 4 / 8: 16 requests
+        // Blocks for 2048 tokens and more of what a row of the table holds (the lengths are on
+        // the device; 64 requests of 2100 tokens with their release 11.5 us under a table as
+        // wide, 23.7 under one for 131072), as long as the requests leave SMs for them; and of
+        // no more than have room for their keys.  Clusters of 1 / 2 / 4 / 8: 16 requests
         // of 4096 tokens 13.5 / 14.0 / 13.7 / 14.9 us, of 16384 25.8 / 20.3 / 16.9 / 17.3,
         // 64 of 16384 28.6 / 23.4 / 29.9 / 54.7, 100 of 131072 468 / 235 / 137 / 176.
         uint32_t cluster = 1;

@@ -7,7 +7,7 @@
 // (16 bits, g query heads to a kv head) that it reads for them, and scores_kernel
 // sums them for each token in the order of the heads.  The logits stay in L2; their
 // writes, the third launch and its dependent loads are what scores cost (48 requests of
-// 4096 tokens and fewer, 40 heads: 98 us with them, 86 without).
+// 4096 tokens and fewer, 40 heads: 97 us with them, 86 without).
 #include "paged_attention.cuh"
 
 using namespace lcpp;

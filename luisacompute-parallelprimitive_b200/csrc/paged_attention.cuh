@@ -7,25 +7,26 @@
 // m follows the maximum only when a logit passes it by 2^8: between, a tile costs
 // a vote instead of reductions and rescaling, and no term leaves its range.
 //
-// Work.  A unit is a request's tokens under one kv head, with up to 8 to 32
-// query heads on it, cut into tiles of 16 tokens.  All tiles of the call are
+// Work.  A unit is a request's tokens under one kv head, with up to 4 to 32 query
+// heads on it (see choose), cut into tiles of 16 tokens.  All tiles of the call are
 // numbered and every block takes an equal run of them, so a few long requests
 // fill the GPU as well as many short ones.  The lengths are on the device: each
 // block sums them itself.  A unit that a run covers whole is written out by its
 // block, the parts of the others by join_kernel, which starts early and waits.
 //
-// A warp works on its own: it takes every fourth tile of the run, copies the
-// tile's 16 keys, then its 16 values, into slots of a ring of its own with
+// A warp works on its own: of a block's four (two for 256 columns of 32 bits) it takes
+// every fourth (second) tile of the run, copies the tile's 16 keys, then its 16 values, into slots of a ring of its own with
 // cp.async, some slots ahead and across the borders of units, and needs the
 // block's other warps only where a unit ends.  Page ids are read four tiles before
 // the copies that need them.
 //
 // Bound by memory where contexts are long: every key and value is read once.  64
-// requests of 16384 tokens and fewer, 32 heads on 8 of 128 in bfloat16: 390 us, 6.6
-// TB/s (a copy reaches 6.5); 2 requests of 131072, 16 on 2 of 256 in float16: 78 us,
-// 5.5 TB/s; 301 of 1500 under a window of 1000, 7 of 80 in float32: 200 us, 6.0 TB/s.
+// requests of 16384 tokens and fewer, 32 heads on 8 of 128 in bfloat16: 382 to 405 us by
+// machine, 6.4 to 6.8 TB/s (a copy reaches 6.5); 2 requests of 131072, 16 on 2 of 256 in
+// float16: 78 us, 5.5 TB/s.  301 of 1500 under a window of 1000, 7 of 80 in float32, reach
+// 5.3 TB/s (198 us): their slots hold 128 columns, so less is under way.
 // Short ones are a chain of latencies (lengths, page ids, keys, values, a part's end,
-// the join's launch): 1 request of 700 tokens takes 9.6 us.  Finer runs than equal
+// the join's launch): 1 request of 700 tokens takes 9.7 us.  Finer runs than equal
 // ones, and blocks that the hardware hands out in waves, measured slower.
 // The matrix products take 15 % of the tensor cores' time: mma.sync on tiles of 16
 // tokens, whose few heads would leave most of a larger instruction's columns empty.
@@ -1320,7 +1321,9 @@ inline Choice choose(uint32_t group, uint32_t dim, bool f32)
 {
     Choice c{};
     c.columns = dim <= 64 ? 64 : !f32 && dim <= 96 ? 96 : dim <= 128 ? 128 : (f32 || dim > 192) ? 256 : 192;
-    // what a warp's accumulators hold: 128 registers of them
+    // what a warp's accumulators hold: up to 128 registers of them in 16 bits, 32 in 32, where
+    // a lane's loads of its token's queries bound the time (larger groups read the cache once
+    // for each chunk of theirs)
     const uint32_t most = f32 ? (c.columns == 256 ? 4 : 8) : (c.columns <= 128 ? 32 : 16);
     c.chunks = (group + most - 1) / most;
     c.per_unit = (group + c.chunks - 1) / c.chunks;
